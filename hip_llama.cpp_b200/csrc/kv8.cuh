@@ -1,0 +1,57 @@
+// The cache in 8 bits: what its kernels share.  A block of positions and a head is [position][channel] bytes without gaps, so that 16 positions are one
+// contiguous run of 16 * dim bytes; all offsets are multiples of 16 bytes because channels are multiples of 16.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "hybrid_ops.cuh"
+#include "split_f16.cuh"
+
+namespace tha {
+
+// index of (block, layer, head): of its scale, and in units of block_size * width of its codes and open rows
+__device__ __forceinline__ size_t kv8_tile(const tha_kv8_t& kv, int block, int layer, int head) {
+  return ((size_t)block * kv.n_cache_layers + layer) * kv.kv_heads + head;
+}
+// block id of a slot's position, -1 where the table holds none that exists
+__device__ __forceinline__ int kv8_block(const tha_kv8_t& kv, int slot, int t) {
+  const int b = t / kv.block_size;
+  if (t < 0 || b >= kv.table_stride) return -1;
+  const int id = kv.table[(size_t)slot * kv.table_stride + b];
+  return (unsigned)id < (unsigned)kv.n_blocks ? id : -1;
+}
+// Piece `i` of the pieces that `of(seq)` counts for every sequence, in order; seq -1 behind the last.  A whole warp asks.
+struct Kv8Piece { int seq, at; };
+template <typename F>
+__device__ __forceinline__ Kv8Piece kv8_find(int n_seqs, int i, F of) {
+  const int lane = threadIdx.x & 31;
+  for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+    const int mine = s0 + lane < n_seqs ? of(s0 + lane) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(THA_FULL_MASK, upto, o); if (lane >= o) upto += v; }
+    const unsigned past = __ballot_sync(THA_FULL_MASK, upto > i);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      return {s0 + l, i - __shfl_sync(THA_FULL_MASK, upto - mine, l)};
+    }
+    i -= __shfl_sync(THA_FULL_MASK, upto, 31);
+  }
+  return {-1, 0};
+}
+
+// four codes to fp32
+template <int FMT>
+__device__ __forceinline__ float4 kv8_decode4(uint32_t w) {
+  if (FMT == THA_KV8_INT8)
+    return make_float4((float)(int8_t)(w & 0xFFu), (float)(int8_t)(w >> 8 & 0xFFu), (float)(int8_t)(w >> 16 & 0xFFu), (float)(int8_t)(w >> 24));
+  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+  const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// host side: kv8_rows.cu
+int kv8_check(const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const char* who);
+int kv8_refuse(const char* who, const char* why);
+
+}  // namespace tha

@@ -1,0 +1,480 @@
+// Softmax attention over the cache in 8 bits (include/tha_hybrid.h, tha_hyb_kv8_attn): single rows, and portions of few (position, head) pairs.
+//
+// The bytes of the cache bound a decoded token, so a byte goes from memory to the tensor cores with as little as possible in between.  Every int8 and e4m3 code is an fp16
+// number, so codes are one operand as they are; the other operand, q or the softmax weights, is fp32 and becomes two fp16, hi + lo 2^-11, that carry 22 bits of it
+// (split_f16.cuh).  mma.m16n8k16 has 16 rows: eight (position, query head) pairs of one key/value head, hi in rows 0 .. 7, lo in rows 8 .. 15, so that one instruction makes
+// both products and a thread finds a pair's two sums in its own registers.  The scores' layout is the one the weights enter the second product with:
+// nothing of them is exchanged.
+//
+// A block takes eight pairs of one key/value head and a run of tiles of 32 keys, its warps every fourth tile.  A warp's tiles come through a ring in shared memory of its own
+// (cp.async).  Channels of K and the order of channels in V's column groups are free, as long as both operands agree, and chosen so that
+// a lane reads 16 bytes at a time and the eight lanes of a shared-memory phase meet 32 different banks (16-byte pieces of a row are stored at piece ^ (row mod 8)).
+// V's scale belongs to a block of keys, the accumulator to all of them: a weight is multiplied by scale / (largest scale of the run's blocks, rounded up to a
+// power of two) ahead of the split.  Weights have the factor 2^15, so that the 22 bits reach down to 2^-28 of the largest.
+#include "kv8.cuh"
+
+namespace tha {
+
+constexpr int K8_WARPS = 4, K8_THREADS = 32 * K8_WARPS, K8_PAIRS = 8, K8_KEYS = 32, K8_SEG = 256, K8_MAX_SPLITS = 64;
+constexpr float K8_UP = 15.0f;   // weights: 2^(score log2(e) - maximum + 15)
+
+template <int DT>
+struct Kv8Ring {
+  static constexpr int TILE = K8_KEYS * DT;                 // bytes of a tile's K, and of its V
+  static constexpr int STAGES = DT == 128 ? 3 : 4;
+  static constexpr int WARP = STAGES * 2 * TILE;
+  static constexpr int BYTES = K8_WARPS * WARP;
+};
+// byte offset of 16-byte piece c of row r of a tile with DT-byte rows
+template <int DT>
+__device__ __forceinline__ int k8_piece(int r, int c) { return r * DT + ((DT == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); }
+
+__device__ __forceinline__ void k8_copy16(uint32_t dst, const void* src, bool there) {   // not there: zeros, src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void k8_await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float k8_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void k8_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Bytes 0 and 2 of w as fp16.  int8: a byte with its sign flipped is code + 128; in the low half of 0x6400 = 1024.0 that is 1024 + 128 + code exactly.
+__device__ __forceinline__ uint32_t k8_bytes02(uint32_t w) {
+  const uint32_t u = (w & 0x00FF00FFu) ^ 0x64806480u;
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ uint32_t k8_e4m3x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return (uint32_t)h.x | (uint32_t)h.y << 16;
+}
+// The channels of a word of K that go to the two registers of the B operand: (0, 2) and (1, 3), or (0, 1) and (2, 3) -- what is cheapest to take apart
+template <int FMT>
+__device__ __forceinline__ void k8_keys(uint32_t w, uint32_t& b0, uint32_t& b1) {
+  if (FMT == THA_KV8_INT8) { b0 = k8_bytes02(w); b1 = k8_bytes02(w >> 8); }
+  else { b0 = k8_e4m3x2(w & 0xFFFFu); b1 = k8_e4m3x2(w >> 16); }
+}
+// byte i of x and of y as fp16
+template <int FMT, int I>
+__device__ __forceinline__ uint32_t k8_values(uint32_t x, uint32_t y) {
+  if (FMT == THA_KV8_INT8) return k8_bytes02(__byte_perm(x, y, I | I << 4 | (4 + I) << 8 | (4 + I) << 12));
+  return k8_e4m3x2(__byte_perm(x, y, I | (4 + I) << 4));
+}
+
+// Tiles of eight pairs of sequence s.
+__device__ __forceinline__ int k8_tiles_of(const tha_rows_t& rows, int s, int gsize) {
+  return ((rows.seq_first[s + 1] - rows.seq_first[s]) * gsize + K8_PAIRS - 1) / K8_PAIRS;
+}
+// The factor of a (query, head)'s accumulator with m the maximum (times log2(e)) and l the sum: 1 / (l + exp(sink - m)) times the head's gate; 0 where nothing was seen.
+__device__ __forceinline__ float k8_final(const tha_attn_t& a, int h, float m, float l, const float* gate_row) {
+  if (!(m > -INFINITY)) return m != m ? m : 0.f;            // a NaN stays one
+  float f;
+  if (a.sink) {
+    const float sk = a.sink[h] * 1.4426950408889634f, M = fmaxf(m, sk), e = exp2f(m - M);
+    f = e / (l * e + exp2f(sk - M));
+  } else {
+    f = 1.0f / l;
+  }
+  if (gate_row) f *= hyb_sigmoid(gate_row[h]);
+  return f;
+}
+__device__ __forceinline__ void k8_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void k8_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// grid (tiles of pairs * splits, kv_heads).  Partial results of a split: sums and maxima [split][row * heads + head][2], then accumulators [..][vdim].
+template <int DT, int FMT, bool MORE, typename T>
+__global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, const float* q, T* out, int splits, int run,
+                                                                 float* partial, const float* gate, long long ldg) {
+  using Ring = Kv8Ring<DT>;
+  constexpr float LOG2E = 1.4426950408889634f;
+  constexpr int KS = DT / 16;                               // k steps of the scores
+  constexpr int NV = DT / 8;                                // column groups of the accumulator
+  extern __shared__ __align__(128) unsigned char k8_ring[];
+  __shared__ int s_id[2 * K8_SEG];                          // per 16 keys of a segment's tiles: block id, the scales
+  __shared__ float s_ks[2 * K8_SEG], s_vs[2 * K8_SEG];
+  __shared__ float s_red[33];
+  __shared__ float s_ml[K8_WARPS][K8_PAIRS][2];
+  const int D = a.dim, E = a.vdim, gsize = a.heads / a.kv_heads, B = kv.block_size, layer = a.cache_layer;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  // channels past the head's are zeros that no copy touches
+  for (int i = threadIdx.x; i < Ring::BYTES / 16; i += K8_THREADS) reinterpret_cast<uint4*>(k8_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+  hyb_pdl_enter();
+  const int kvh = blockIdx.y, sp = blockIdx.x % splits;
+  int seq, tile;
+  {
+    const int i = blockIdx.x / splits, per = (gsize + K8_PAIRS - 1) / K8_PAIRS;
+    if (rows.max_seq_rows == 1) {
+      seq = i / per; tile = i - seq * per;
+    } else {
+      const Kv8Piece pc = kv8_find(rows.n_seqs, i, [&](int s) { return k8_tiles_of(rows, s, gsize); });
+      seq = pc.seq; tile = pc.at;
+    }
+  }
+  if (seq < 0) return;
+  const int r0 = rows.seq_first[seq], n_rows = rows.seq_first[seq + 1] - r0, slot = rows.seq_slot[seq];
+  const int pairs = min(K8_PAIRS, n_rows * gsize - tile * K8_PAIRS);
+  if (pairs < 1) return;
+  const int pr = tile * K8_PAIRS + min(g, pairs - 1), pp = pr / gsize, head = kvh * gsize + (pr - pp * gsize);   // this lane's pair (behind the last: the last again)
+  const int p_seq = rows.pos[r0];
+  const int p_first = p_seq + (tile * K8_PAIRS) / gsize, p_last = p_seq + (tile * K8_PAIRS + pairs - 1) / gsize, pos = p_seq + pp;
+  const int key_lo = a.chunk > 0 ? (p_first / a.chunk) * a.chunk : 0, last_lo = a.chunk > 0 ? (p_last / a.chunk) * a.chunk : 0;
+  const int my_lo = a.chunk > 0 ? (pos / a.chunk) * a.chunk : 0;
+  HybTiles tiles = {0, 0, 0, 0};
+  if (p_seq >= 0) tiles = hyb_attn_tiles(a, key_lo, p_first, p_last);
+  const int ti0 = min(sp * run, tiles.n), ti1 = sp == splits - 1 ? tiles.n : min(ti0 + run, tiles.n);
+  auto tile_key = [&](int ti) { return ti < tiles.n_a ? tiles.begin + 32 * ti : tiles.resume + 32 * (ti - tiles.n_a); };
+
+  // q: the lane's channels of its pair are those it reads of a key, DT / 4
+  uint32_t qf[KS][4];
+  float fac;
+  {
+    const float* qr = q + ((size_t)(r0 + pp) * a.heads + head) * D;
+    float v[KS][4], top = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const int c = (DT == 128 ? 2 * t + (s >> 2) : t) * 16 + (s & 3) * 4;
+      const float4 x = c < D && p_seq >= 0 ? *reinterpret_cast<const float4*>(qr + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[s][0] = x.x; v[s][1] = x.y; v[s][2] = x.z; v[s][3] = x.w;
+#pragma unroll
+      for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(v[s][i]));
+    }
+    top = fmaxf(top, __shfl_xor_sync(THA_FULL_MASK, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(THA_FULL_MASK, top, 2));
+    float inverse;
+    const float up = split_scale<100>(top, 14, &inverse);
+    constexpr int X = FMT == THA_KV8_INT8 ? 2 : 1, Y = FMT == THA_KV8_INT8 ? 1 : 2;   // k8_keys
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      split_f16x2(make_float2(v[s][0], v[s][X]), up, qf[s][0], qf[s][1]);
+      split_f16x2(make_float2(v[s][Y], v[s][3]), up, qf[s][2], qf[s][3]);
+    }
+    fac = inverse * a.scale * (a.head_scale ? a.head_scale[head] : 1.0f);
+    if (!MORE) fac *= LOG2E;
+  }
+
+  float acc[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  float m = -INFINITY, l = 0.f, ref = 0.f;                  // l: this lane's keys only
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(k8_ring) + warp * Ring::WARP;
+  const uint8_t *kpool = static_cast<const uint8_t*>(kv.k_pool), *vpool = static_cast<const uint8_t*>(kv.v_pool);
+
+  for (int s0 = ti0; s0 < ti1; s0 += K8_SEG) {
+    const int s1 = min(s0 + K8_SEG, ti1);
+    __syncthreads();
+    float top = 0.f;
+    for (int e = threadIdx.x; e < 2 * (s1 - s0); e += K8_THREADS) {
+      const int key = tile_key(s0 + (e >> 1)) + 16 * (e & 1);
+      const int id = key <= p_last ? kv8_block(kv, slot, key) : -1;
+      s_id[e] = id;
+      const size_t at = id >= 0 ? kv8_tile(kv, id, layer, kvh) : 0;
+      s_ks[e] = id >= 0 ? kv.k_scale[at] : 0.f;
+      s_vs[e] = id >= 0 ? kv.v_scale[at] : 0.f;
+      top = fmaxf(top, s_vs[e]);
+    }
+    top = block_max(top, s_red);                            // its barriers publish the table as well
+    float down = 1.0f;
+    if (top > ref) {                                        // up to the next power of two: what is there changes units exactly
+      const float to = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u));
+      const float corr = ref / to;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) acc[i][x] *= corr;
+      ref = to;
+    }
+    if (ref > 0.f) down = 1.0f / ref;
+
+    auto fetch = [&](int ti, int stage) {                   // every lane's share of a tile; nothing behind the segment's last
+      if (ti >= s1) return;
+      const int e = 2 * (ti - s0), key = tile_key(ti);
+      const uint32_t dst = ring + stage * 2 * Ring::TILE;
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const int id = s_id[e + hf];
+        const size_t row = (id >= 0 ? kv8_tile(kv, id, layer, kvh) * B + (key + 16 * hf) % B : 0);
+        const uint8_t *ks = kpool + row * D, *vs = vpool + row * E;
+#pragma unroll
+        for (int i = 0; i < DT / 32; i++) {                 // 16 rows of DT / 16 pieces, 32 at a time
+          const int x = 32 * i + lane, r = x / (DT / 16), c = x % (DT / 16);
+          if (16 * c < D) k8_copy16(dst + k8_piece<DT>(16 * hf + r, c), ks + r * D + 16 * c, id >= 0);
+          if (16 * c < E) k8_copy16(dst + Ring::TILE + k8_piece<DT>(16 * hf + r, c), vs + r * E + 16 * c, id >= 0);
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < Ring::STAGES - 1; i++) { fetch(s0 + warp + i * K8_WARPS, i); k8_commit(); }
+    int stage = 0;
+    for (int ti = s0 + warp; ti < s1; ti += K8_WARPS) {
+      fetch(ti + (Ring::STAGES - 1) * K8_WARPS, stage == 0 ? Ring::STAGES - 1 : stage - 1);
+      k8_commit();
+      k8_await<Ring::STAGES - 1>();
+      __syncwarp();
+      const unsigned char* st = k8_ring + warp * Ring::WARP + stage * 2 * Ring::TILE;
+      const int e = 2 * (ti - s0), kt = tile_key(ti);
+      // scores
+      float sc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+#pragma unroll
+        for (int pcs = 0; pcs < DT / 64; pcs++) {
+          const uint4 w = *reinterpret_cast<const uint4*>(st + k8_piece<DT>(8 * j + g, DT == 128 ? 2 * t + pcs : t));
+          uint32_t b0, b1;
+          k8_keys<FMT>(w.x, b0, b1); k8_mma(sc[j], qf[4 * pcs], b0, b1);
+          k8_keys<FMT>(w.y, b0, b1); k8_mma(sc[j], qf[4 * pcs + 1], b0, b1);
+          k8_keys<FMT>(w.z, b0, b1); k8_mma(sc[j], qf[4 * pcs + 2], b0, b1);
+          k8_keys<FMT>(w.w, b0, b1); k8_mma(sc[j], qf[4 * pcs + 3], b0, b1);
+        }
+      }
+      const float f0 = fac * s_ks[e], f1 = fac * s_ks[e + 1];
+      const bool there0 = s_id[e] >= 0, there1 = s_id[e + 1] >= 0;
+      const bool whole = there0 && there1 && kt + 31 <= p_first && kt >= last_lo && (a.window <= 0 || p_last - kt < a.window || kt + 32 <= a.keep_first);
+      float x[8], top_x = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          float v = fmaf(sc[j][2 + i], SPLIT_DOWN, sc[j][i]) * (j < 2 ? f0 : f1);
+          if (MORE) {
+            if (a.softcap > 0.f) v = hyb_softcap(v, a.softcap);
+            if (a.rel) v += hyb_attn_rel(a, head, pos - (kt + 8 * j + 2 * t + i));
+            v *= LOG2E;
+          }
+          if (!whole && !((j < 2 ? there0 : there1) && hyb_attn_sees(a, kt + 8 * j + 2 * t + i, pos, my_lo))) v = -INFINITY;
+          x[2 * j + i] = v;
+          top_x = fmaxf(top_x, v);
+        }
+      top_x = fmaxf(top_x, __shfl_xor_sync(THA_FULL_MASK, top_x, 1));
+      top_x = fmaxf(top_x, __shfl_xor_sync(THA_FULL_MASK, top_x, 2));
+      const bool grow = top_x > m;
+      if (__any_sync(THA_FULL_MASK, grow)) {
+        const float to = grow ? top_x : m, corr = m > -INFINITY ? k8_ex2(m - to) : grow ? 0.f : 1.f;
+        m = to;
+        l *= corr;
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+          for (int y = 0; y < 4; y++) acc[i][y] *= corr;
+      }
+      const float shift = m > -INFINITY ? K8_UP - m : 0.f;   // nothing seen so far: weights are 2^-inf
+      const float v0 = s_vs[e] * down, v1 = s_vs[e + 1] * down;
+      uint32_t pf[2][4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float w0 = k8_ex2(x[2 * j] + shift), w1 = k8_ex2(x[2 * j + 1] + shift);
+        l += w0 + w1;
+        split_f16x2(f32x2_mul(make_float2(w0, w1), j < 2 ? make_float2(v0, v0) : make_float2(v1, v1)), 1.0f, pf[j >> 1][2 * (j & 1)], pf[j >> 1][2 * (j & 1) + 1]);
+      }
+      // weights x values: 16 keys at a time
+      const unsigned char* sv = st + Ring::TILE;
+#pragma unroll
+      for (int kk = 0; kk < 2; kk++) {
+        const int k0 = 16 * kk + 2 * t;
+        if (DT == 128) {
+          const uint4 wa = *reinterpret_cast<const uint4*>(sv + k8_piece<DT>(k0, g)), wb = *reinterpret_cast<const uint4*>(sv + k8_piece<DT>(k0 + 1, g));
+          const uint4 wc = *reinterpret_cast<const uint4*>(sv + k8_piece<DT>(k0 + 8, g)), wd = *reinterpret_cast<const uint4*>(sv + k8_piece<DT>(k0 + 9, g));
+          const uint32_t A[4] = {wa.x, wa.y, wa.z, wa.w}, Bw[4] = {wb.x, wb.y, wb.z, wb.w}, C[4] = {wc.x, wc.y, wc.z, wc.w}, Dw[4] = {wd.x, wd.y, wd.z, wd.w};
+#pragma unroll
+          for (int w = 0; w < NV / 4; w++) {
+            k8_mma(acc[4 * w], pf[kk], k8_values<FMT, 0>(A[w], Bw[w]), k8_values<FMT, 0>(C[w], Dw[w]));
+            k8_mma(acc[4 * w + 1], pf[kk], k8_values<FMT, 1>(A[w], Bw[w]), k8_values<FMT, 1>(C[w], Dw[w]));
+            k8_mma(acc[4 * w + 2], pf[kk], k8_values<FMT, 2>(A[w], Bw[w]), k8_values<FMT, 2>(C[w], Dw[w]));
+            k8_mma(acc[4 * w + 3], pf[kk], k8_values<FMT, 3>(A[w], Bw[w]), k8_values<FMT, 3>(C[w], Dw[w]));
+          }
+        } else {
+          auto two = [&](int r) { return *reinterpret_cast<const uint2*>(sv + k8_piece<DT>(r, g >> 1) + 8 * (g & 1)); };
+          const uint2 wa = two(k0), wb = two(k0 + 1), wc = two(k0 + 8), wd = two(k0 + 9);
+          const uint32_t A[2] = {wa.x, wa.y}, Bw[2] = {wb.x, wb.y}, C[2] = {wc.x, wc.y}, Dw[2] = {wd.x, wd.y};
+#pragma unroll
+          for (int w = 0; w < NV / 4; w++) {
+            k8_mma(acc[4 * w], pf[kk], k8_values<FMT, 0>(A[w], Bw[w]), k8_values<FMT, 0>(C[w], Dw[w]));
+            k8_mma(acc[4 * w + 1], pf[kk], k8_values<FMT, 1>(A[w], Bw[w]), k8_values<FMT, 1>(C[w], Dw[w]));
+            k8_mma(acc[4 * w + 2], pf[kk], k8_values<FMT, 2>(A[w], Bw[w]), k8_values<FMT, 2>(C[w], Dw[w]));
+            k8_mma(acc[4 * w + 3], pf[kk], k8_values<FMT, 3>(A[w], Bw[w]), k8_values<FMT, 3>(C[w], Dw[w]));
+          }
+        }
+      }
+      __syncwarp();                                          // the stage has been read
+      stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
+    }
+    k8_await<0>();
+  }
+
+  // the warps meet: accumulators [warp][pair][DT] over the ring
+  l += __shfl_xor_sync(THA_FULL_MASK, l, 1);
+  l += __shfl_xor_sync(THA_FULL_MASK, l, 2);
+  __syncthreads();
+  float* s_acc = reinterpret_cast<float*>(k8_ring);
+  if (t == 0) { s_ml[warp][g][0] = l == l ? m : l; s_ml[warp][g][1] = l; }   // a NaN among the scores shows in the sum alone
+#pragma unroll
+  for (int i = 0; i < NV; i++)
+#pragma unroll
+    for (int x = 0; x < 2; x++)                              // column 2 t + x of group i is channel (2 t + x) * DT / 8 + i
+      s_acc[(warp * K8_PAIRS + g) * DT + (2 * t + x) * (DT / 8) + i] = fmaf(acc[i][2 + x], SPLIT_DOWN, acc[i][x]);
+  __syncthreads();
+  for (int w = warp; w < pairs; w += K8_WARPS) {
+    const int pr2 = tile * K8_PAIRS + w, pp2 = pr2 / gsize, h2 = kvh * gsize + (pr2 - pp2 * gsize), r = r0 + pp2;
+    float M = -INFINITY, L = 0.f, f[K8_WARPS];
+#pragma unroll
+    for (int x = 0; x < K8_WARPS; x++) M = s_ml[x][w][0] > M || s_ml[x][w][0] != s_ml[x][w][0] ? s_ml[x][w][0] : M;
+#pragma unroll
+    for (int x = 0; x < K8_WARPS; x++) {
+      f[x] = s_ml[x][w][0] > -INFINITY ? exp2f(s_ml[x][w][0] - M) : 0.f;
+      L += f[x] * s_ml[x][w][1];
+    }
+    L *= exp2f(-K8_UP);
+    float scale = ref * exp2f(-K8_UP);
+    const size_t at = (size_t)r * a.heads + h2, all = (size_t)rows.n_rows * a.heads;
+    float* pd = splits > 1 ? partial + 2 * all * splits + ((size_t)sp * all + at) * E : nullptr;
+    if (!pd) scale *= k8_final(a, h2, M, L, gate ? gate + (size_t)r * ldg : nullptr);
+    else if (lane == 0) { float* ml = partial + 2 * ((size_t)sp * all + at); ml[0] = M; ml[1] = L; }
+    for (int c = lane; c < E; c += 32) {
+      float o = 0.f;
+#pragma unroll
+      for (int x = 0; x < K8_WARPS; x++) o += f[x] * s_acc[(x * K8_PAIRS + w) * DT + c];
+      if (pd) pd[c] = o * scale;
+      else if (a.out_f32) reinterpret_cast<float*>(out)[at * E + c] = o * scale;
+      else k8_store(out + at * E + c, o * scale);
+    }
+  }
+}
+
+// The parts of a (row, head) in order.  grid (rows * heads)
+template <typename T>
+__global__ void __launch_bounds__(128) kv8_merge_kernel(T* out, const float* partial, tha_rows_t rows, int splits, tha_attn_t a, const float* gate, long long ldg) {
+  hyb_pdl_enter();
+  __shared__ float s_w[K8_MAX_SPLITS];
+  __shared__ float s_f;
+  const size_t at = blockIdx.x, all = (size_t)rows.n_rows * a.heads;
+  const int E = a.vdim;
+  if (threadIdx.x < 32) {
+    float m[2], l[2], M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int s = threadIdx.x + 32 * i;
+      const float2 ml = s < splits ? *reinterpret_cast<const float2*>(partial + 2 * ((size_t)s * all + at)) : make_float2(-INFINITY, 0.f);
+      m[i] = ml.x; l[i] = ml.y;
+      M = fmaxf(M, m[i]);
+    }
+    const bool nan = __any_sync(THA_FULL_MASK, m[0] != m[0] || m[1] != m[1]);
+    M = warp_max(M);
+    float L = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float w = m[i] > -INFINITY ? exp2f(m[i] - M) : 0.f;
+      s_w[threadIdx.x + 32 * i] = w;
+      L += w * l[i];
+    }
+    L = warp_sum(L);
+    const int row = (int)(at / a.heads), h = (int)(at - (size_t)row * a.heads);
+    const float f = k8_final(a, h, nan ? NAN : M, L, gate ? gate + (size_t)row * ldg : nullptr);
+    if (threadIdx.x == 0) s_f = f;
+  }
+  __syncthreads();
+  const float* p = partial + 2 * all * splits + at * E;
+  for (int c = threadIdx.x; c < E; c += blockDim.x) {
+    float o = 0.f;
+    for (int s = 0; s < splits; s++)
+      if (s_w[s] > 0.f) o = fmaf(p[(size_t)s * all * E + c], s_w[s], o);
+    o *= s_f;
+    if (a.out_f32) reinterpret_cast<float*>(out)[at * E + c] = o;
+    else k8_store(out + at * E + c, o);
+  }
+}
+
+// Keys that the row of the longest context sees at most, as tiles of 32.
+static int k8_most_tiles(const tha_attn_t* a, const tha_rows_t* rows) {
+  const long long seen = rows->max_pos + 1ll;
+  long long keys = a->chunk > 0 ? (long long)a->chunk + rows->max_seq_rows : seen;
+  if (a->window > 0 && (long long)a->window + a->keep_first + rows->max_seq_rows + 64 < keys) keys = (long long)a->window + a->keep_first + rows->max_seq_rows + 64;
+  if (keys > seen) keys = seen;
+  return (int)((keys + 31) / 32) + 1;
+}
+static int k8_pair_tiles(const tha_attn_t* a, const tha_rows_t* rows) {
+  const int gsize = a->heads / a->kv_heads;
+  if (rows->max_seq_rows == 1) return rows->n_seqs * ceil_div(gsize, K8_PAIRS);
+  return (int)(((long long)rows->n_rows * gsize) / K8_PAIRS) + rows->n_seqs;
+}
+// Parts of a context: enough blocks for each SM to have several, of at least 8 tiles (two a warp).
+static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows) {
+  const int most = k8_most_tiles(a, rows);
+  const long long blocks = (long long)k8_pair_tiles(a, rows) * a->kv_heads;
+  long long s = (4 * 148 + blocks - 1) / blocks;
+  if (s > most / 8) s = most / 8;
+  return s < 1 ? 1 : s > K8_MAX_SPLITS ? K8_MAX_SPLITS : (int)s;
+}
+
+template <int DT, int FMT, bool MORE, typename T>
+static int k8_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int splits, float* partial,
+                     const float* gate, long long ldg) {
+  auto k = kv8_attn_kernel<DT, FMT, MORE, T>;
+  THA_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8Ring<DT>::BYTES));
+  const int run = ceil_div(k8_most_tiles(a, rows), splits);
+  THA_CUDA_OK(launch(k, dim3((unsigned)k8_pair_tiles(a, rows) * splits, a->kv_heads), dim3(K8_THREADS), Kv8Ring<DT>::BYTES, s, pdl_enabled() != 0, *a, *rows, *kv, q, out,
+                     splits, run, partial, gate, ldg));
+  if (splits > 1)
+    THA_CUDA_OK(launch(kv8_merge_kernel<T>, dim3((unsigned)rows->n_rows * a->heads), dim3(128), 0, s, pdl_enabled() != 0, out, (const float*)partial, *rows, splits, *a, gate, ldg));
+  return THA_STATUS_SUCCESS;
+}
+template <int DT, typename T>
+static int k8_form(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int splits, float* partial,
+                   const float* gate, long long ldg) {
+  const bool more = a->softcap > 0.f || a->rel;
+  if (kv->format == THA_KV8_INT8)
+    return more ? k8_launch<DT, THA_KV8_INT8, true>(s, a, rows, kv, q, out, splits, partial, gate, ldg)
+                : k8_launch<DT, THA_KV8_INT8, false>(s, a, rows, kv, q, out, splits, partial, gate, ldg);
+  return more ? k8_launch<DT, THA_KV8_E4M3, true>(s, a, rows, kv, q, out, splits, partial, gate, ldg)
+              : k8_launch<DT, THA_KV8_E4M3, false>(s, a, rows, kv, q, out, splits, partial, gate, ldg);
+}
+static size_t k8_scratch(const tha_attn_t* a, const tha_rows_t* rows, int splits) {
+  return splits > 1 ? (size_t)splits * rows->n_rows * a->heads * (a->vdim + 2) : 0;
+}
+static int k8_check(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const char* who) {
+  THA_TRY_RC(kv8_check(rows, kv, a->cache_layer, who));
+  if (a->kv_heads != kv->kv_heads || a->dim != kv->dim || a->vdim != kv->vdim) return kv8_refuse(who, "heads or channels are not the cache's");
+  if (a->heads < 1 || a->heads % a->kv_heads) return kv8_refuse(who, "query heads are a multiple of the key/value heads");
+  if (a->window < 0 || a->keep_first < 0 || a->chunk < 0) return kv8_refuse(who, "a mask's extent is below 0");
+  if (a->rel && a->rel_n < 1) return kv8_refuse(who, "distance biases without an extent");
+  if (a->values_in_keys || a->v_share > 1 || a->diff) {
+    kv8_refuse(who, "values_in_keys, v_share and diff are not for this cache");
+    return THA_STATUS_NOT_SUPPORTED;
+  }
+  if ((long long)rows->n_rows * a->heads > 1ll << 30) return kv8_refuse(who, "too many rows");
+  return THA_STATUS_SUCCESS;
+}
+
+}  // namespace tha
+
+using namespace tha;
+
+extern "C" size_t tha_hyb_kv8_attn_scratch(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv) {
+  if (rows->n_rows < 1 || k8_check(a, rows, kv, "tha_hyb_kv8_attn_scratch") != THA_STATUS_SUCCESS) return 0;
+  return k8_scratch(a, rows, k8_splits(a, rows));
+}
+
+extern "C" int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,
+                                size_t scratch_floats, const float* proj, long long ldp) {
+  if (rows->n_rows < 1) return THA_STATUS_SUCCESS;
+  THA_TRY_RC(k8_check(a, rows, kv, "tha_hyb_kv8_attn"));
+  if (dtype != THA_DT_BF16 && dtype != THA_DT_F32) return kv8_refuse("tha_hyb_kv8_attn", "unknown dtype");
+  if (!q || !out || !aligned16(q)) return kv8_refuse("tha_hyb_kv8_attn", "q on a 16-byte boundary and a result are needed");
+  if (scratch && !aligned16(scratch)) return kv8_refuse("tha_hyb_kv8_attn", "scratch on a 16-byte boundary");
+  const float* gate = a->head_gate && proj ? proj + a->o_g : nullptr;
+  int splits = scratch ? k8_splits(a, rows) : 1;
+  while (splits > 1 && k8_scratch(a, rows, splits) > scratch_floats) splits--;
+  cudaStream_t s = (cudaStream_t)stream;
+  const bool wide = a->dim > 64 || a->vdim > 64;
+  if (dtype == THA_DT_BF16) {
+    auto o = (__nv_bfloat16*)out;
+    return wide ? k8_form<128>(s, a, rows, kv, q, o, splits, scratch, gate, ldp) : k8_form<64>(s, a, rows, kv, q, o, splits, scratch, gate, ldp);
+  }
+  auto o = (float*)out;
+  return wide ? k8_form<128>(s, a, rows, kv, q, o, splits, scratch, gate, ldp) : k8_form<64>(s, a, rows, kv, q, o, splits, scratch, gate, ldp);
+}

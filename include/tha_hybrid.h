@@ -627,6 +627,55 @@ int tha_hyb_diff_combine(void* stream, int dtype, const tha_attn_t* a, const flo
 int tha_hyb_hgrn_scan(void* stream, int dtype, const tha_hgrn_t* g, const tha_rows_t* rows, const tha_state_store_t* st, float* proj,
                       long long ldp, float* decay, float* o_raw, void* out, float* seg_scratch, size_t seg_scratch_floats);
 
+/* ---- a cache in 8 bits ------------------------------------------------------------------------------------------- */
+#define THA_KV8_INT8 0 /* two's complement -127 .. 127 */
+#define THA_KV8_E4M3 1 /* 8-bit floating point, 4 bits of exponent, 3 of mantissa, up to 448 */
+
+/* Cache rows as bytes with one scale for each block of positions and key/value head: a quarter of the bytes of tha_kv_t's fp32 rows.  Blocks are found
+ * through a table as there.  A block's scale is the largest |x| of its rows over the format's largest number (127, 448) as fp32, at least 2^-126 unless all rows are 0; a
+ * value's code is the format's number nearest to the real quotient x / scale, ties to even, and stands for code * scale.  Infinities do not enter the scale and get
+ * the largest code of their sign, NaN gets 0: the cache holds finite numbers only.  Rows of a slot's last block, while it is not full, are also kept
+ * in fp32 (k_open, v_open), and its codes are made anew whenever rows join it: a code is one rounding of its value under the scale of all rows that are
+ * there, however the rows were cut into calls.
+ * The table's ids are checked on the device: a block whose id is not below n_blocks is not written, reads as zeros, and its keys are not seen. */
+typedef struct {
+  void* k_pool;         /* codes [block][cache layer][kv head][position in block][dim] */
+  void* v_pool;         /* codes [block][cache layer][kv head][position in block][vdim] */
+  float* k_scale;       /* [block][cache layer][kv head] */
+  float* v_scale;
+  float* k_open;        /* [slot][cache layer][kv head][position in block][dim]: rows of the slot's last block */
+  float* v_open;
+  const int* table;     /* [slot][table_stride] block ids */
+  int table_stride;     /* blocks per slot */
+  int block_size;       /* positions per block: 16, 32, 64 or 128 */
+  int n_blocks, n_cache_layers;
+  int kv_heads, dim, vdim; /* dim, vdim: multiples of 16 up to 128 */
+  int format;           /* THA_KV8_* */
+} tha_kv8_t;
+
+/* In the calls below the rows of a sequence are at consecutive positions; a sequence of one row at a negative position is idle. */
+
+/* Rows enter the cache: row r's heads are kv_heads * dim values at k + r * ldk and kv_heads * vdim at v + r * ldv (dtype-typed, pitches in elements).  The first
+ * row of a sequence is at the position behind the slot's last one, or at any earlier one of the same block, or at the start of a block: rows of its block ahead of it are those of
+ * k_open, v_open.  What the slot held from that position on is gone.  A step brings at most one sequence of a slot, and no two of its sequences write one block.  Idle sequences write nothing. */
+int tha_hyb_kv8_write(void* stream, int dtype, const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const void* k, long long ldk, const void* v,
+                      long long ldv);
+/* Cache rows as the values they stand for, rounded once to dtype: k_out [n_rows, ldk], v_out (either NULL: not wanted); pitches in elements.  Idle rows read as zeros. */
+int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, void* k_out, long long ldk, void* v_out,
+                     long long ldv);
+/* tha_hyb_attn_gated over such a cache: every row attends to the visible keys as the cache holds them, which for rows of a block that is not full are their codes
+ * under its present scale.  a: heads, kv_heads, dim, vdim, scale, chunk, cache_layer, window, keep_first, sink, head_scale, softcap, rel, head_gate and out_f32 as there
+ * (values_in_keys, v_share and diff are refused); q fp32 [n_rows, heads * dim]; out dtype-typed [n_rows, heads * vdim].  Idle rows get zeros.
+ * Codes are exact in fp16; q and the weights enter the products as two fp16 that carry 22 bits of them (a value 2^28 below the largest of its row of q, a
+ * weighted value 2^28 below the row's largest weight times the largest scale of V's blocks that the row sees, still has them).  Rows of prompts with dtype
+ * THA_DT_BF16 may use one fp16 of 11 bits instead.  Sums and softmax are fp32.
+ * scratch (nullable, 16-byte aligned): room for partial results where long contexts are cut along the keys (n * n_rows * heads * (vdim + 2) floats for n parts; as
+ * many as fit, 64 at most); calls that may run at the same time need scratch of their own. */
+int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,
+                     size_t scratch_floats, const float* proj, long long ldp);
+/* floats of scratch with which such a call is cut as it pleases (0: it needs none) */
+size_t tha_hyb_kv8_attn_scratch(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,161 @@
+"""The cache in 8 bits without a GPU: the binding's structs against the header, the oracle's roundings against torch's, and what the calls refuse (before any launch)."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_oracle as O
+from pkgload import load_pkg
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+K = load_pkg("kv8")
+A = 1 << 20                                                       # an aligned address that no refused call looks at
+
+
+def test_structs_match_the_header(tmp_path):
+    src, want = ['#include <stdio.h>', '#include "tha_hybrid.h"', "int main(void) {"], []
+    for s in K.STRUCTS:
+        src.append('printf("%%zu\\n", sizeof(%s));' % s.__name__)
+        want.append(C.sizeof(s))
+        for f, _ in s._fields_:
+            src.append('printf("%%zu\\n", offsetof(%s, %s));' % (s.__name__, f))
+            want.append(getattr(s, f).offset)
+    (tmp_path / "a.c").write_text("\n".join(src + ["return 0; }"]))
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "a"), str(tmp_path / "a.c")])
+    assert [int(x) for x in subprocess.check_output([str(tmp_path / "a")]).split()] == want
+
+
+def test_every_declared_call_is_exported():
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "tha_hybrid.h")).read(), flags=re.S)
+    names = set(re.findall(r"\b(tha_hyb_kv8_[a-z0-9_]+)\s*\(", text))
+    assert names == {"tha_hyb_kv8_write", "tha_hyb_kv8_read", "tha_hyb_kv8_attn", "tha_hyb_kv8_attn_scratch"}
+    assert all(hasattr(K.lib().c, n) for n in names)
+
+
+def test_the_oracle_rounds_as_the_formats_do():
+    y = np.concatenate([np.linspace(-448, 448, 20001), O.levels("e4m3"), -O.levels("e4m3"), (O.levels("e4m3")[1:] + O.levels("e4m3")[:-1]) / 2])
+    got = torch.from_numpy(y).float().to(torch.float8_e4m3fn).float().numpy()
+    assert np.array_equal(O.nearest(y.astype(np.float32).astype(np.float64), "e4m3"), got.astype(np.float64))
+    y = np.concatenate([np.linspace(-127, 127, 5001), np.arange(-126.5, 127, 1)])
+    assert np.array_equal(O.nearest(y, "int8"), np.rint(y))
+    codes = np.arange(256, dtype=np.uint8)
+    assert np.array_equal(O.numbers(codes, "int8"), codes.view(np.int8).astype(np.float64))
+    of = torch.from_numpy(codes).view(torch.float8_e4m3fn).float().numpy().astype(np.float64)
+    assert np.array_equal(O.numbers(codes, "e4m3"), of, equal_nan=True)
+
+
+def rows(**more):
+    return K.RowsStruct(**{**dict(n_rows=3, n_seqs=2, pos=A, row_seq=A, seq_first=A, seq_slot=A, max_seq_rows=2, max_pos=40), **more})
+
+
+def cache(**more):
+    return K.Kv8Struct(**{**dict(k_pool=A, v_pool=A, k_scale=A, v_scale=A, k_open=A, v_open=A, table=A, table_stride=4, block_size=16, n_blocks=9, n_cache_layers=2,
+                                 kv_heads=2, dim=64, vdim=64, format=0), **more})
+
+
+def attn(**more):
+    return K.AttnStruct(**{**dict(heads=4, kv_heads=2, dim=64, vdim=64, scale=0.125), **more})
+
+
+REFUSED_ROWS = [dict(pos=None), dict(row_seq=None), dict(seq_first=None), dict(seq_slot=None), dict(n_seqs=0), dict(n_seqs=4), dict(max_seq_rows=0), dict(max_seq_rows=4),
+                dict(max_pos=64)]
+REFUSED_CACHE = [dict(k_pool=None), dict(v_pool=None), dict(k_scale=None), dict(v_scale=None), dict(table=None), dict(format=2), dict(format=-1), dict(block_size=8),
+                 dict(block_size=48), dict(block_size=256), dict(dim=0), dict(dim=24), dict(dim=144), dict(vdim=8), dict(vdim=136), dict(kv_heads=0), dict(kv_heads=65536),
+                 dict(n_cache_layers=0), dict(n_cache_layers=1), dict(n_blocks=0), dict(table_stride=0), dict(table_stride=2), dict(k_pool=A + 8), dict(v_pool=A + 1)]
+
+
+def status(call, *args):
+    got = call(*args)
+    return got, K.lib().c.tha_last_error().decode()
+
+
+def calls(r, c, layer=1, dtype=1):
+    """(name, status, text) of the three calls with these descriptions."""
+    f = K.lib().c
+    return [("write",) + status(f.tha_hyb_kv8_write, None, dtype, r, c, layer, A, 128, A, 128),
+            ("read",) + status(f.tha_hyb_kv8_read, None, dtype, r, c, layer, A, 128, A, 128),
+            ("attn",) + status(f.tha_hyb_kv8_attn, None, dtype, attn(cache_layer=layer, kv_heads=c.kv_heads, heads=2 * c.kv_heads, dim=c.dim, vdim=c.vdim), r, c, A, A, None, 0,
+                               None, 0)]
+
+
+@pytest.mark.parametrize("bad", REFUSED_ROWS, ids=str)
+def test_rows_that_are_refused(bad):
+    for name, got, text in calls(rows(**bad), cache()):
+        assert got == 2 and "tha_hyb_kv8_" + name in text
+
+
+@pytest.mark.parametrize("bad", REFUSED_CACHE, ids=str)
+def test_caches_that_are_refused(bad):
+    for name, got, text in calls(rows(), cache(**bad)):
+        assert got == 2 and "tha_hyb_kv8_" + name in text
+
+
+def test_layers_and_types_that_are_refused():
+    for r, c, layer, dtype in ((rows(), cache(), 2, 1), (rows(), cache(), -1, 1), (rows(), cache(), 0, 2), (rows(), cache(), 0, -1)):
+        assert all(got == 2 for _, got, _ in calls(r, c, layer, dtype))
+
+
+def test_operands_that_are_refused():
+    f, r, c = K.lib().c, rows(), cache()
+    for k, ldk, v, ldv in ((None, 128, A, 128), (A, 128, None, 128), (A, 127, A, 128), (A, 128, A, 64)):
+        assert f.tha_hyb_kv8_write(None, 1, r, c, 0, k, ldk, v, ldv) == 2
+    for more in (dict(k_open=None), dict(v_open=None), dict(k_open=A + 4), dict(v_open=A + 8)):
+        assert f.tha_hyb_kv8_write(None, 1, r, cache(**more), 0, A, 128, A, 128) == 2
+    for k, ldk, v, ldv in ((A, 127, A, 128), (A, 128, A, 100), (A, 1, None, 0)):
+        assert f.tha_hyb_kv8_read(None, 1, r, c, 0, k, ldk, v, ldv) == 2
+    for q, out, scratch in ((None, A, None), (A, None, None), (A + 4, A, None), (A, A, A + 8)):
+        assert f.tha_hyb_kv8_attn(None, 1, attn(), r, c, q, out, scratch, 1 << 20, None, 0) == 2
+
+
+@pytest.mark.parametrize("bad,code", [(dict(heads=3), 2), (dict(heads=0), 2), (dict(kv_heads=4), 2), (dict(dim=32), 2), (dict(vdim=32), 2), (dict(window=-1), 2),
+                                      (dict(keep_first=-1), 2), (dict(chunk=-1), 2), (dict(rel=A), 2), (dict(cache_layer=2), 2), (dict(values_in_keys=1), 7),
+                                      (dict(v_share=2), 7), (dict(diff=1), 7)], ids=str)
+def test_attention_that_is_refused(bad, code):
+    f = K.lib().c
+    assert f.tha_hyb_kv8_attn(None, 1, attn(**bad), rows(), cache(), A, A, None, 0, None, 0) == code
+    assert f.tha_hyb_kv8_attn_scratch(attn(**bad), rows(), cache()) == 0
+
+
+def test_no_rows_are_no_work():
+    f, r = K.lib().c, rows(n_rows=0)
+    assert f.tha_hyb_kv8_write(None, 1, r, cache(), 0, A, 128, A, 128) == 0
+    assert f.tha_hyb_kv8_read(None, 1, r, cache(), 0, A, 128, A, 128) == 0
+    assert f.tha_hyb_kv8_attn(None, 1, attn(), r, cache(), A, A, None, 0, None, 0) == 0
+    assert f.tha_hyb_kv8_read(None, 1, rows(), cache(), 0, None, 0, None, 0) == 0
+
+
+def small(device="cpu", **more):
+    return K.Kv8Cache.empty(**{**dict(blocks=4, layers=1, kv_heads=2, block_size=16, dim=32, slots=2, table_stride=2, device=device), **more})
+
+
+def test_the_binding_refuses_what_the_library_cannot_see():
+    z = torch.zeros
+    pool, scale, rows_, table = z(4, 1, 2, 16, 32, dtype=torch.int8), z(4, 1, 2), z(2, 1, 2, 16, 32), z(2, 2, dtype=torch.int32)
+    good = [pool, pool.clone(), scale, scale.clone(), rows_, rows_.clone(), table]
+    K.Kv8Cache(*good)
+    K.Kv8Cache(*good[:4], None, None, table)
+    for i, bad in ((0, pool.float()), (1, pool.view(torch.float8_e4m3fn)), (1, pool[:3]), (0, pool.transpose(2, 3)), (2, scale[:3]), (3, scale.double()), (4, None),
+                   (4, rows_[:1]), (5, rows_.half()), (6, table.long()), (6, table[0]), (6, z(2, 4, dtype=torch.int32)[:, ::2])):
+        with pytest.raises(ValueError):
+            K.Kv8Cache(*good[:i], bad, *good[i + 1:])
+    with pytest.raises(ValueError):
+        K.Rows.of([], "cpu")
+    for portion in ((0, 0, 0), (0, -1, 2)):
+        with pytest.raises(ValueError):
+            K.Rows.of([portion], "cpu")
+    ints = z(3, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        K.Rows(ints, ints[:2], ints, ints[:2], 2, 0)
+    with pytest.raises(ValueError):
+        K.Rows(ints, ints, ints[:2], ints[:2], 2, 0)
+    with pytest.raises(ValueError):
+        K.Attention(4, 2, 32, scale=1.0, sink=z(3))
+    with pytest.raises(ValueError):
+        K.Attention(4, 2, 32, scale=1.0, rel=z(2, 8))
+    r = K.Rows.of([(0, 0, 3), (1, 5, 1), (1, -1, 1)], "cpu")
+    assert r.n == 5 and r.c.max_seq_rows == 3 and r.c.max_pos == 5 and r.slots == (0, 1, True)
+    assert not K.Rows.of([(0, 0, 3), (0, 5, 1)], "cpu").slots[2]
