@@ -50,8 +50,44 @@ __device__ __forceinline__ float4 kv8_decode4(uint32_t w) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
+__device__ __forceinline__ float k8_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Bytes 0 and 2 of w as fp16.  int8: a byte with its sign flipped is code + 128; in the low half of 0x6400 = 1024.0 that is 1024 + 128 + code exactly.
+__device__ __forceinline__ uint32_t k8_bytes02(uint32_t w) {
+  const uint32_t u = (w & 0x00FF00FFu) ^ 0x64806480u;
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ uint32_t k8_e4m3x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return (uint32_t)h.x | (uint32_t)h.y << 16;
+}
+
+// The factor of a (query, head)'s accumulator with m the maximum (times log2(e)) and l the sum: 1 / (l + exp(sink - m)) times the head's gate; 0 where nothing was seen.
+__device__ __forceinline__ float k8_final(const tha_attn_t& a, int h, float m, float l, const float* gate_row) {
+  if (!(m > -INFINITY)) return m != m ? m : 0.f;            // a NaN stays one
+  float f;
+  if (a.sink) {
+    const float sk = a.sink[h] * 1.4426950408889634f, M = fmaxf(m, sk), e = exp2f(m - M);
+    f = e / (l * e + exp2f(sk - M));
+  } else {
+    f = 1.0f / l;
+  }
+  if (gate_row) f *= hyb_sigmoid(gate_row[h]);
+  return f;
+}
+__device__ __forceinline__ void k8_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void k8_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
 // host side: kv8_rows.cu
 int kv8_check(const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const char* who);
 int kv8_refuse(const char* who, const char* why);
+// kv8_attn_tc.cu: sequences of at least min_rows rows; THA_STATUS_NOT_SUPPORTED (nothing launched): the caller takes another form
+int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles);
+int kv8_attn_tc_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int min_rows, int splits,
+                       float* partial, const float* gate, long long ldg);
 
 }  // namespace tha

@@ -35,24 +35,9 @@ __device__ __forceinline__ void k8_copy16(uint32_t dst, const void* src, bool th
 __device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void k8_await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float k8_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void k8_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// Bytes 0 and 2 of w as fp16.  int8: a byte with its sign flipped is code + 128; in the low half of 0x6400 = 1024.0 that is 1024 + 128 + code exactly.
-__device__ __forceinline__ uint32_t k8_bytes02(uint32_t w) {
-  const uint32_t u = (w & 0x00FF00FFu) ^ 0x64806480u;
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-__device__ __forceinline__ uint32_t k8_e4m3x2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return (uint32_t)h.x | (uint32_t)h.y << 16;
 }
 // The channels of a word of K that go to the two registers of the B operand: (0, 2) and (1, 3), or (0, 1) and (2, 3) -- what is cheapest to take apart
 template <int FMT>
@@ -67,29 +52,14 @@ __device__ __forceinline__ uint32_t k8_values(uint32_t x, uint32_t y) {
   return k8_e4m3x2(__byte_perm(x, y, I | (4 + I) << 4));
 }
 
-// Tiles of eight pairs of sequence s.
-__device__ __forceinline__ int k8_tiles_of(const tha_rows_t& rows, int s, int gsize) {
-  return ((rows.seq_first[s + 1] - rows.seq_first[s]) * gsize + K8_PAIRS - 1) / K8_PAIRS;
+// Tiles of eight pairs of sequence s: none where it has more than `most` rows.
+__device__ __forceinline__ int k8_tiles_of(const tha_rows_t& rows, int s, int gsize, int most) {
+  const int n = rows.seq_first[s + 1] - rows.seq_first[s];
+  return n <= most ? (n * gsize + K8_PAIRS - 1) / K8_PAIRS : 0;
 }
-// The factor of a (query, head)'s accumulator with m the maximum (times log2(e)) and l the sum: 1 / (l + exp(sink - m)) times the head's gate; 0 where nothing was seen.
-__device__ __forceinline__ float k8_final(const tha_attn_t& a, int h, float m, float l, const float* gate_row) {
-  if (!(m > -INFINITY)) return m != m ? m : 0.f;            // a NaN stays one
-  float f;
-  if (a.sink) {
-    const float sk = a.sink[h] * 1.4426950408889634f, M = fmaxf(m, sk), e = exp2f(m - M);
-    f = e / (l * e + exp2f(sk - M));
-  } else {
-    f = 1.0f / l;
-  }
-  if (gate_row) f *= hyb_sigmoid(gate_row[h]);
-  return f;
-}
-__device__ __forceinline__ void k8_store(float* p, float v) { *p = v; }
-__device__ __forceinline__ void k8_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
 // grid (tiles of pairs * splits, kv_heads).  Partial results of a split: sums and maxima [split][row * heads + head][2], then accumulators [..][vdim].
 template <int DT, int FMT, bool MORE, typename T>
-__global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, const float* q, T* out, int splits, int run,
+__global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, const float* q, T* out, int most_rows, int splits, int run,
                                                                  float* partial, const float* gate, long long ldg) {
   using Ring = Kv8Ring<DT>;
   constexpr float LOG2E = 1.4426950408889634f;
@@ -112,7 +82,7 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     if (rows.max_seq_rows == 1) {
       seq = i / per; tile = i - seq * per;
     } else {
-      const Kv8Piece pc = kv8_find(rows.n_seqs, i, [&](int s) { return k8_tiles_of(rows, s, gsize); });
+      const Kv8Piece pc = kv8_find(rows.n_seqs, i, [&](int s) { return k8_tiles_of(rows, s, gsize, most_rows); });
       seq = pc.seq; tile = pc.at;
     }
   }
@@ -165,8 +135,31 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(k8_ring) + warp * Ring::WARP;
   const uint8_t *kpool = static_cast<const uint8_t*>(kv.k_pool), *vpool = static_cast<const uint8_t*>(kv.v_pool);
 
+  // The tensor cores cut off what their fp32 sums cannot hold: an accumulator sums a segment's tiles, 128 sums a warp, and the segments' are added here.
+  float seg_total[2 * NV], m_total = -INFINITY, ref_total = 0.f;
+  float* total = seg_total;
+  asm volatile("" : "+l"(total));                           // local memory: few contexts have a second segment
+  auto add_segment = [&]() {
+    const float f = m_total > -INFINITY ? k8_ex2(m_total - m) * (ref > 0.f ? ref_total / ref : 0.f) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        acc[i][x] = fmaf(acc[i][2 + x], SPLIT_DOWN, acc[i][x]);
+        if (f != 0.f) acc[i][x] = fmaf(f, total[2 * i + x], acc[i][x]);
+        acc[i][2 + x] = 0.f;
+      }
+  };
   for (int s0 = ti0; s0 < ti1; s0 += K8_SEG) {
     const int s1 = min(s0 + K8_SEG, ti1);
+    if (s0 > ti0) {
+      add_segment();
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) { total[2 * i + x] = acc[i][x]; acc[i][x] = 0.f; }
+      m_total = m; ref_total = ref;
+    }
     __syncthreads();
     float top = 0.f;
     for (int e = threadIdx.x; e < 2 * (s1 - s0); e += K8_THREADS) {
@@ -307,6 +300,8 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     k8_await<0>();
   }
 
+  add_segment();
+
   // the warps meet: accumulators [warp][pair][DT] over the ring
   l += __shfl_xor_sync(THA_FULL_MASK, l, 1);
   l += __shfl_xor_sync(THA_FULL_MASK, l, 2);
@@ -317,7 +312,7 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
   for (int i = 0; i < NV; i++)
 #pragma unroll
     for (int x = 0; x < 2; x++)                              // column 2 t + x of group i is channel (2 t + x) * DT / 8 + i
-      s_acc[(warp * K8_PAIRS + g) * DT + (2 * t + x) * (DT / 8) + i] = fmaf(acc[i][2 + x], SPLIT_DOWN, acc[i][x]);
+      s_acc[(warp * K8_PAIRS + g) * DT + (2 * t + x) * (DT / 8) + i] = acc[i][x];
   __syncthreads();
   for (int w = warp; w < pairs; w += K8_WARPS) {
     const int pr2 = tile * K8_PAIRS + w, pp2 = pr2 / gsize, h2 = kvh * gsize + (pr2 - pp2 * gsize), r = r0 + pp2;
@@ -346,14 +341,18 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
   }
 }
 
-// The parts of a (row, head) in order.  grid (rows * heads)
+// The parts of a (row, head) in order, of sequences of least .. most rows.  grid (rows * heads)
 template <typename T>
-__global__ void __launch_bounds__(128) kv8_merge_kernel(T* out, const float* partial, tha_rows_t rows, int splits, tha_attn_t a, const float* gate, long long ldg) {
+__global__ void __launch_bounds__(128) kv8_merge_kernel(T* out, const float* partial, tha_rows_t rows, int least, int most, int splits, tha_attn_t a, const float* gate, long long ldg) {
   hyb_pdl_enter();
   __shared__ float s_w[K8_MAX_SPLITS];
   __shared__ float s_f;
   const size_t at = blockIdx.x, all = (size_t)rows.n_rows * a.heads;
   const int E = a.vdim;
+  {
+    const int seq = rows.row_seq[blockIdx.x / a.heads], n = rows.seq_first[seq + 1] - rows.seq_first[seq];
+    if (n < least || n > most) return;
+  }
   if (threadIdx.x < 32) {
     float m[2], l[2], M = -INFINITY;
 #pragma unroll
@@ -397,44 +396,79 @@ static int k8_most_tiles(const tha_attn_t* a, const tha_rows_t* rows) {
   if (keys > seen) keys = seen;
   return (int)((keys + 31) / 32) + 1;
 }
-static int k8_pair_tiles(const tha_attn_t* a, const tha_rows_t* rows) {
+// Pair tiles of the sequences of up to `most` rows, at most.
+static int k8_pair_tiles(const tha_attn_t* a, const tha_rows_t* rows, int most) {
   const int gsize = a->heads / a->kv_heads;
   if (rows->max_seq_rows == 1) return rows->n_seqs * ceil_div(gsize, K8_PAIRS);
-  return (int)(((long long)rows->n_rows * gsize) / K8_PAIRS) + rows->n_seqs;
+  const long long by_rows = (long long)rows->n_rows * gsize / K8_PAIRS + rows->n_seqs;
+  const long long by_seqs = (long long)rows->n_seqs * (((long long)(most < rows->max_seq_rows ? most : rows->max_seq_rows) * gsize + K8_PAIRS - 1) / K8_PAIRS);
+  return (int)(by_rows < by_seqs ? by_rows : by_seqs);
 }
 // Parts of a context: enough blocks for each SM to have several, of at least 8 tiles (two a warp).
-static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows) {
+static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows) {
   const int most = k8_most_tiles(a, rows);
-  const long long blocks = (long long)k8_pair_tiles(a, rows) * a->kv_heads;
+  const long long blocks = (long long)k8_pair_tiles(a, rows, most_rows) * a->kv_heads;
   long long s = (4 * 148 + blocks - 1) / blocks;
   if (s > most / 8) s = most / 8;
   return s < 1 ? 1 : s > K8_MAX_SPLITS ? K8_MAX_SPLITS : (int)s;
 }
 
+template <typename T>
+static int k8_merge(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, T* out, int least, int most, int splits, const float* partial, const float* gate, long long ldg) {
+  if (splits > 1)
+    THA_CUDA_OK(launch(kv8_merge_kernel<T>, dim3((unsigned)rows->n_rows * a->heads), dim3(128), 0, s, pdl_enabled() != 0, out, partial, *rows, least, most, splits, *a, gate, ldg));
+  return THA_STATUS_SUCCESS;
+}
 template <int DT, int FMT, bool MORE, typename T>
-static int k8_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int splits, float* partial,
+static int k8_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int most_rows, int splits, float* partial,
                      const float* gate, long long ldg) {
   auto k = kv8_attn_kernel<DT, FMT, MORE, T>;
   THA_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8Ring<DT>::BYTES));
   const int run = ceil_div(k8_most_tiles(a, rows), splits);
-  THA_CUDA_OK(launch(k, dim3((unsigned)k8_pair_tiles(a, rows) * splits, a->kv_heads), dim3(K8_THREADS), Kv8Ring<DT>::BYTES, s, pdl_enabled() != 0, *a, *rows, *kv, q, out,
-                     splits, run, partial, gate, ldg));
-  if (splits > 1)
-    THA_CUDA_OK(launch(kv8_merge_kernel<T>, dim3((unsigned)rows->n_rows * a->heads), dim3(128), 0, s, pdl_enabled() != 0, out, (const float*)partial, *rows, splits, *a, gate, ldg));
+  THA_CUDA_OK(launch(k, dim3((unsigned)k8_pair_tiles(a, rows, most_rows) * splits, a->kv_heads), dim3(K8_THREADS), Kv8Ring<DT>::BYTES, s, pdl_enabled() != 0, *a, *rows, *kv, q,
+                     out, most_rows, splits, run, partial, gate, ldg));
   return THA_STATUS_SUCCESS;
 }
 template <int DT, typename T>
-static int k8_form(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int splits, float* partial,
+static int k8_form(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int most_rows, int splits, float* partial,
                    const float* gate, long long ldg) {
   const bool more = a->softcap > 0.f || a->rel;
   if (kv->format == THA_KV8_INT8)
-    return more ? k8_launch<DT, THA_KV8_INT8, true>(s, a, rows, kv, q, out, splits, partial, gate, ldg)
-                : k8_launch<DT, THA_KV8_INT8, false>(s, a, rows, kv, q, out, splits, partial, gate, ldg);
-  return more ? k8_launch<DT, THA_KV8_E4M3, true>(s, a, rows, kv, q, out, splits, partial, gate, ldg)
-              : k8_launch<DT, THA_KV8_E4M3, false>(s, a, rows, kv, q, out, splits, partial, gate, ldg);
+    return more ? k8_launch<DT, THA_KV8_INT8, true>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
+                : k8_launch<DT, THA_KV8_INT8, false>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
+  return more ? k8_launch<DT, THA_KV8_E4M3, true>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
+              : k8_launch<DT, THA_KV8_E4M3, false>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
 }
-static size_t k8_scratch(const tha_attn_t* a, const tha_rows_t* rows, int splits) {
-  return splits > 1 ? (size_t)splits * rows->n_rows * a->heads * (a->vdim + 2) : 0;
+// Which sequences take which form: by their own rows alone.  short_rows: up to so many take kv8_attn_kernel; has_short, has_long: whether the step may hold any.
+struct Kv8Forms { int short_rows; bool has_short, has_long; };
+constexpr int K8_LONG_PAIRS = 128;
+static Kv8Forms k8_forms(const tha_attn_t* a, const tha_rows_t* rows) {
+  const int gsize = a->heads / a->kv_heads;
+  Kv8Forms f = {gsize > 256 ? 0x7FFFFFFF : ceil_div(K8_LONG_PAIRS, gsize), true, false};
+  if (f.short_rows < 1) f.short_rows = 1;
+  f.has_long = rows->max_seq_rows > f.short_rows;
+  f.has_short = !(f.has_long && (long long)rows->n_seqs * rows->max_seq_rows == rows->n_rows);   // all sequences are as long as the longest
+  return f;
+}
+template <typename T>
+static int k8_attend(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, float* scratch, size_t room,
+                     const float* gate, long long ldg) {
+  const Kv8Forms f = k8_forms(a, rows);
+  const size_t one = (size_t)rows->n_rows * a->heads * (a->vdim + 2);
+  auto fit = [&](int splits) { return !scratch ? 1 : (size_t)splits * one <= room ? splits : room / one < 2 ? 1 : (int)(room / one); };
+  int short_rows = f.short_rows;
+  if (f.has_long) {
+    const int splits = fit(kv8_attn_tc_splits(a, rows, k8_most_tiles(a, rows)));
+    const int st = kv8_attn_tc_launch(s, dtype, a, rows, kv, q, out, short_rows + 1, splits, scratch, gate, ldg);
+    if (st == THA_STATUS_SUCCESS) THA_TRY_RC(k8_merge(s, a, rows, out, short_rows + 1, 0x7FFFFFFF, splits, scratch, gate, ldg));
+    else if (st != THA_STATUS_NOT_SUPPORTED) return st;
+    else short_rows = 0x7FFFFFFF;
+    if (st == THA_STATUS_SUCCESS && !f.has_short) return THA_STATUS_SUCCESS;
+  }
+  const int splits = fit(k8_splits(a, rows, short_rows));
+  if (a->dim > 64 || a->vdim > 64) THA_TRY_RC((k8_form<128>(s, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg)));
+  else THA_TRY_RC((k8_form<64>(s, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg)));
+  return k8_merge(s, a, rows, out, 0, short_rows, splits, scratch, gate, ldg);
 }
 static int k8_check(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const char* who) {
   THA_TRY_RC(kv8_check(rows, kv, a->cache_layer, who));
@@ -456,7 +490,10 @@ using namespace tha;
 
 extern "C" size_t tha_hyb_kv8_attn_scratch(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv) {
   if (rows->n_rows < 1 || k8_check(a, rows, kv, "tha_hyb_kv8_attn_scratch") != THA_STATUS_SUCCESS) return 0;
-  return k8_scratch(a, rows, k8_splits(a, rows));
+  const Kv8Forms f = k8_forms(a, rows);
+  const int longs = f.has_long ? kv8_attn_tc_splits(a, rows, k8_most_tiles(a, rows)) : 1, shorts = f.has_short ? k8_splits(a, rows, f.short_rows) : 1;
+  const int most = longs > shorts ? longs : shorts;
+  return most > 1 ? (size_t)most * rows->n_rows * a->heads * (a->vdim + 2) : 0;
 }
 
 extern "C" int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,
@@ -467,14 +504,7 @@ extern "C" int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, co
   if (!q || !out || !aligned16(q)) return kv8_refuse("tha_hyb_kv8_attn", "q on a 16-byte boundary and a result are needed");
   if (scratch && !aligned16(scratch)) return kv8_refuse("tha_hyb_kv8_attn", "scratch on a 16-byte boundary");
   const float* gate = a->head_gate && proj ? proj + a->o_g : nullptr;
-  int splits = scratch ? k8_splits(a, rows) : 1;
-  while (splits > 1 && k8_scratch(a, rows, splits) > scratch_floats) splits--;
   cudaStream_t s = (cudaStream_t)stream;
-  const bool wide = a->dim > 64 || a->vdim > 64;
-  if (dtype == THA_DT_BF16) {
-    auto o = (__nv_bfloat16*)out;
-    return wide ? k8_form<128>(s, a, rows, kv, q, o, splits, scratch, gate, ldp) : k8_form<64>(s, a, rows, kv, q, o, splits, scratch, gate, ldp);
-  }
-  auto o = (float*)out;
-  return wide ? k8_form<128>(s, a, rows, kv, q, o, splits, scratch, gate, ldp) : k8_form<64>(s, a, rows, kv, q, o, splits, scratch, gate, ldp);
+  if (dtype == THA_DT_BF16) return k8_attend(s, dtype, a, rows, kv, q, (__nv_bfloat16*)out, scratch, scratch_floats, gate, ldp);
+  return k8_attend(s, dtype, a, rows, kv, q, (float*)out, scratch, scratch_floats, gate, ldp);
 }

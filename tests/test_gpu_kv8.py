@@ -3,7 +3,8 @@
 Tolerances.  Codes, scales and kept rows are equal to the bit.  Values read back: code * scale rounded once (2^-24 of the value in fp32), bf16 once more (2^-8).
 Attention in fp32, relative to the norm of the result, for q and keys of order one, scale dim^-1/2: a score is a sum of up to 128 products with sum |q k| scale of about 0.64 * 128^1/2 =
 7, off by 2^-22 of that (q in two fp16) and 2^-23 (fp32 sums), 2.5e-6 if all errors agree; its rounding beside the maximum and the factor 2^15, |x| < 32, adds 2^-24 * 32 = 1.9e-6; the
-weight 2^-22 (ex2) + 2^-22 (two fp16), the sums 2^-22: 0.7e-6.  Together 5.1e-6, and 6e-6 is asked for.  A bf16 result is off by half a step more, 2^-8 of each value."""
+weight 2^-22 (ex2) + 2^-22 (two fp16), the sums 2^-22: 0.7e-6.  Together 5.1e-6, and 6e-6 is asked for.  (Sums of the tensor cores are cut off, not rounded: 128 of them in a row, each
+2^-24 of what is there, on the average half of it and of the end's value, are 128 * 2^-26 = 1.9e-6; they and the scores' errors do not agree.)  A bf16 result is off by half a step more, 2^-8 of each value."""
 import numpy as np
 import pytest
 import torch
@@ -319,6 +320,83 @@ def test_a_query_that_is_not_a_number():
         assert bool(torch.isfinite(out[0]).all()) and bool(torch.isnan(out[1]).all())
 
 
+def test_a_query_of_a_portion_that_is_not_a_number():
+    m = filled(32, 2, 128, 128, "int8", (700,))
+    q = torch.randn(300, 512, device="cuda")
+    q[123, 130] = float("nan")
+    q[7, 400] = float("inf")
+    for dtype in (torch.float32, torch.bfloat16):
+        out = m.cache.attend(K.Attention(4, 2, 128, scale=0.1), K.Rows.of([(0, 400, 300)]), q, layer=LAYER, dtype=dtype).view(300, 4, 128)
+        bad = torch.zeros(300, 4, dtype=torch.bool, device="cuda")
+        bad[123, 1] = bad[7, 3] = True
+        assert bool((~torch.isfinite(out)).all(-1)[bad].all()) and bool(torch.isfinite(out)[~bad].all())
+
+
+LONG = [("int8", 16, 8, 2, 128, 128, [(0, 1500, 300)], {}), ("e4m3", 64, 4, 1, 128, 128, [(0, 3000, 150)], dict(window=1000, keep_first=40)),
+        ("int8", 16, 4, 4, 64, 64, [(0, 100, 129), (1, 0, 128), (2, 2000, 400)], {}), ("int8", 32, 5, 1, 96, 80, [(0, 900, 260), (1, 17, 3), (2, 3, 1), (3, 40, 90)], dict(sink=True)),
+        ("e4m3", 128, 16, 1, 128, 64, [(0, 2500, 77), (1, 30, 60)], dict(chunk=700)), ("int8", 16, 3, 1, 16, 128, [(0, 0, 600)], dict(softcap=5.0)),
+        ("e4m3", 16, 6, 2, 112, 48, [(0, 1000, 200)], dict(rel=300)), ("int8", 16, 2, 2, 128, 128, [(i, 7 * i, 130 + i % 3) for i in range(40)], {})]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{c[4]}-{c[5]}-{len(c[6])}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lead", [0, 1])
+def test_prompt_portions(case, dtype, lead):
+    """Portions for the tensor-core form, behind contexts that are cut and beside short ones; with lead 1 the result is on no 16-byte boundary."""
+    fmt, block, heads, kv_heads, dim, vdim, parts, mask = case
+    m = filled(block, kv_heads, dim, vdim, fmt, [p + n for _, p, n in parts])
+    rng = np.random.default_rng(3)
+    a = dict(mask, heads=heads, scale=dim ** -0.5)
+    if a.get("sink"):
+        a["sink"] = rng.standard_normal(heads).astype(np.float32)
+    if a.get("rel"):
+        a["rel"] = rng.standard_normal((heads, a["rel"])).astype(np.float32)
+    out, want = attend(m, a, parts, dtype)
+    close(out, want)
+    if lead:
+        room = torch.full((out.numel() + 1,), 9.0, device="cuda", dtype=dtype)
+        dev = lambda x: None if x is None else torch.from_numpy(x).cuda()  # noqa: E731
+        at = K.Attention(heads, kv_heads, dim, vdim, scale=a["scale"], chunk=a.get("chunk", 0), window=a.get("window", 0), keep_first=a.get("keep_first", 0),
+                         sink=dev(a.get("sink")), softcap=a.get("softcap", 0.0), rel=dev(a.get("rel")))
+        q = torch.randn(out.shape[0], heads * dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+        m.cache.attend(at, K.Rows.of(parts), q, layer=LAYER, out=room[1:].view(out.shape))
+        close(room[1:].view(out.shape), want)
+        assert float(room[0]) == 9.0
+
+
+def test_blocks_that_do_not_exist_under_a_portion():
+    m = filled(16, 2, 128, 128, "int8", (900,))
+    bad = m.cache.table.clone()
+    for b in (0, 9, 30, 50):
+        bad[0, b] = -7 if b & 1 else m.cache.k_pool.shape[0]
+    m.cache.table.copy_(bad)
+    q = torch.randn(400, 512, device="cuda")
+    out = m.cache.attend(K.Attention(4, 2, 128, scale=0.1), K.Rows.of([(0, 500, 400)]), q, layer=LAYER)
+    absent = np.isin(np.arange(900) // 16, (0, 9, 30, 50))
+    want = O.attend(dict(scale=0.1), q.double().cpu().numpy().reshape(400, 4, 128), m.values("k", 0, 900), m.values("v", 0, 900), 500, absent)
+    assert rel(out, want.reshape(400, -1)) < F32_TOL
+
+
+@pytest.mark.parametrize("scratch", [0, 1, 2, 3, 16])
+def test_parts_of_a_portions_context_meet(scratch):
+    m = filled(16, 1, 128, 128, "int8", (4000,))
+    parts, heads = [(0, 3900, 100)], 2
+    out, want = attend(m, dict(heads=heads, scale=128 ** -0.5), parts, torch.float32)
+    close(out, want)
+    r, at = K.Rows.of(parts), K.Attention(heads, 1, 128, scale=128 ** -0.5)
+    at.c.cache_layer = LAYER
+    q = torch.randn(100, heads * 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    floats = scratch * 100 * heads * 130
+    room = torch.full((floats + 512,), 3.25, device="cuda")
+    got = torch.full_like(out, float("nan"))
+    lib = K.lib()
+    lib.check(lib.c.tha_hyb_kv8_attn(torch.cuda.current_stream().cuda_stream, 1, at.ref, r.ref, m.cache.ref, q.data_ptr(), got.data_ptr(), room.data_ptr() if floats else None,
+                                     floats, None, 0))
+    torch.cuda.synchronize()
+    assert bool((room[floats:] == 3.25).all())
+    close(got, want)
+
+
 @pytest.mark.parametrize("scratch", [0, 1, 2, 7, 63, 1000])
 def test_parts_of_a_context_meet(scratch):
     """With any room for partial results, and nothing behind the room."""
@@ -342,8 +420,8 @@ def test_parts_of_a_context_meet(scratch):
 
 def test_a_very_long_context():
     """Offsets of a pool beyond 2^31 bytes, and a table of more blocks than a block of threads holds at once."""
-    n, H, D = 70000, 1, 128
-    m = Mirror(1, n, H, 16, D, D, "int8", spare=0)
+    n, D = 70000, 128
+    assert n > 2 * 8192
     big = K.Kv8Cache.empty(blocks=180000, layers=LAYERS, kv_heads=2, block_size=16, dim=D, slots=1, table_stride=-(-n // 16))   # 2.2e9 bytes a pool
     ids = torch.arange(179999, 179999 - big.table.shape[1], -1, dtype=torch.int32)
     big.table[0] = ids.cuda()
@@ -358,6 +436,23 @@ def test_a_very_long_context():
     s = torch.einsum("hd,thd->ht", q.double().view(2, D), kb.double().view(n, 2, D)) * D ** -0.5
     want = torch.einsum("ht,the->he", torch.softmax(s, -1), vb.double().view(n, 2, D)).reshape(1, -1)
     assert rel(out, want.cpu().numpy()) < F32_TOL
+    # without room for parts: one block of threads and all keys
+    at.c.cache_layer = LAYER
+    lib, r = K.lib(), K.Rows.of([(0, n - 1, 1)])
+    out.fill_(float("nan"))
+    lib.check(lib.c.tha_hyb_kv8_attn(torch.cuda.current_stream().cuda_stream, 1, at.ref, r.ref, big.ref, q.data_ptr(), out.data_ptr(), None, 0, None, 0))
+    assert rel(out, want.cpu().numpy()) < F32_TOL
+    # a portion, its parts and without
+    q = torch.randn(130, 2 * D, device="cuda")
+    r = K.Rows.of([(0, n - 130, 130)])
+    hidden = torch.arange(n, device="cuda")[None] > torch.arange(n - 130, n, device="cuda")[:, None]
+    s = torch.einsum("rhd,thd->hrt", q.double().view(130, 2, D), kb.double().view(n, 2, D)) * D ** -0.5
+    want = torch.einsum("hrt,the->rhe", torch.softmax(s.masked_fill(hidden, float("-inf")), -1), vb.double().view(n, 2, D)).reshape(130, -1).cpu().numpy()
+    out = big.attend(at, r, q, layer=LAYER)
+    assert rel(out, want) < F32_TOL
+    out.fill_(float("nan"))
+    lib.check(lib.c.tha_hyb_kv8_attn(torch.cuda.current_stream().cuda_stream, 1, at.ref, r.ref, big.ref, q.data_ptr(), out.data_ptr(), None, 0, None, 0))
+    assert rel(out, want) < F32_TOL
 
 
 def test_other_streams_and_graphs():
