@@ -39,6 +39,14 @@ __device__ __forceinline__ Kv8Piece kv8_find(int n_seqs, int i, F of) {
   return {-1, 0};
 }
 
+// hyb_attn_sees for the 32 keys from kt on, as bits: a query at `pos` whose chunk begins at `first`
+__device__ __forceinline__ uint32_t kv8_sees32(const tha_attn_t& a, int kt, int pos, int first) {
+  auto below = [&](int t) { const int n = t - kt; return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };   // keys kt .. t - 1
+  uint32_t seen = ~below(first);
+  if (a.window > 0) seen &= ~below(pos - a.window + 1) | below(a.keep_first);
+  return seen & below(pos + 1);
+}
+
 // four codes to fp32
 template <int FMT>
 __device__ __forceinline__ float4 kv8_decode4(uint32_t w) {

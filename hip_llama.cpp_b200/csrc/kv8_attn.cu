@@ -229,6 +229,13 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
       const float f0 = fac * s_ks[e], f1 = fac * s_ks[e + 1];
       const bool there0 = s_id[e] >= 0, there1 = s_id[e + 1] >= 0;
       const bool whole = there0 && there1 && kt + 31 <= p_first && kt >= last_lo && (a.window <= 0 || p_last - kt < a.window || kt + 32 <= a.keep_first);
+      uint32_t seen = 0xFFFFFFFFu;
+      if (!whole) {
+        seen = kv8_sees32(a, kt, pos, my_lo);
+        if (!there0) seen &= 0xFFFF0000u;
+        if (!there1) seen &= 0xFFFFu;
+      }
+      seen >>= 2 * t;                                        // bits 8 j, 8 j + 1 are this lane's
       float x[8], top_x = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; j++)
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
             if (a.rel) v += hyb_attn_rel(a, head, pos - (kt + 8 * j + 2 * t + i));
             v *= LOG2E;
           }
-          if (!whole && !((j < 2 ? there0 : there1) && hyb_attn_sees(a, kt + 8 * j + 2 * t + i, pos, my_lo))) v = -INFINITY;
+          if (!(seen >> (8 * j + i) & 1u)) v = -INFINITY;
           x[2 * j + i] = v;
           top_x = fmaxf(top_x, v);
         }

@@ -138,27 +138,38 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_attn_tc_kernel(tha_attn_t a
     return;
   }
 
-  // q: warp w takes rows w, w + 16, ..; pairs past the block's positions are zeros.  A negative factor of the scores goes into q.
-  for (int pr = warp; pr < 2 * KT_ROWS; pr += KT_THREADS / 32) {
-    const int pp = pr / gsize, h = g * gsize + (pr - pp * gsize), c = 4 * lane;
-    const bool ok = pp < AP && r0 + pp < r_end;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ok && c < D) v = *reinterpret_cast<const float4*>(q + ((size_t)(r0 + pp) * a.heads + h) * D + c);
-    const float top = warp_max(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-    float inverse;
-    const float up = split_scale<100>(top, 14, &inverse);
-    const float f = ok ? a.scale * (a.head_scale ? a.head_scale[h] : 1.0f) : 0.f;
-    if (lane == 0) s_fac[pr] = inverse * fabsf(f) * (MORE ? 1.0f : LOG2E);
-    if (c < DT) {
-      const float s = f < 0.f ? -up : up;
-      if (FMT == THA_KV8_INT8) { const float y = v.y; v.y = v.z; v.z = y; }
-      v.x *= s; v.y *= s; v.z *= s; v.w *= s;
-      const uint2 hi = make_uint2(f16x2_of(make_float2(v.x, v.y)), f16x2_of(make_float2(v.z, v.w)));
-      unsigned char* dst = Qs + (pr / KT_ROWS) * (SPLIT ? 2 : 1) * Q_PART + (c >> 6) * (KT_ROWS * 128) + (pr % KT_ROWS) * 128 + ((((c & 63) >> 3) ^ (pr & 7)) << 4) + ((c & 7) << 1);
-      *reinterpret_cast<uint2*>(dst) = hi;
-      if (SPLIT) {   // what is left, in the same units: both parts go into one accumulator
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-        *reinterpret_cast<uint2*>(dst + Q_PART) = make_uint2(f16x2_of(make_float2(v.x - x.x, v.y - x.y)), f16x2_of(make_float2(v.z - y.x, v.w - y.y)));
+  // q: warp w takes rows w, w + 16, .., eight on their way at a time; pairs past the block's positions are zeros.  A negative factor of the scores goes into q.
+#pragma unroll 1
+  for (int b0 = warp; b0 < 2 * KT_ROWS; b0 += 8 * (KT_THREADS / 32)) {
+    const int c = 4 * lane;
+    float4 rows4[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int pr = b0 + i * (KT_THREADS / 32), pp = pr / gsize, h = g * gsize + (pr - pp * gsize);
+      rows4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (pp < AP && r0 + pp < r_end && c < D) rows4[i] = *reinterpret_cast<const float4*>(q + ((size_t)(r0 + pp) * a.heads + h) * D + c);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int pr = b0 + i * (KT_THREADS / 32), pp = pr / gsize, h = g * gsize + (pr - pp * gsize);
+      const bool ok = pp < AP && r0 + pp < r_end;
+      float4 v = rows4[i];
+      const float top = warp_max(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+      float inverse;
+      const float up = split_scale<100>(top, 14, &inverse);
+      const float f = ok ? a.scale * (a.head_scale ? a.head_scale[h] : 1.0f) : 0.f;
+      if (lane == 0) s_fac[pr] = inverse * fabsf(f) * (MORE ? 1.0f : LOG2E);
+      if (c < DT) {
+        const float s = f < 0.f ? -up : up;
+        if (FMT == THA_KV8_INT8) { const float y = v.y; v.y = v.z; v.z = y; }
+        v.x *= s; v.y *= s; v.z *= s; v.w *= s;
+        const uint2 hi = make_uint2(f16x2_of(make_float2(v.x, v.y)), f16x2_of(make_float2(v.z, v.w)));
+        unsigned char* dst = Qs + (pr / KT_ROWS) * (SPLIT ? 2 : 1) * Q_PART + (c >> 6) * (KT_ROWS * 128) + (pr % KT_ROWS) * 128 + ((((c & 63) >> 3) ^ (pr & 7)) << 4) + ((c & 7) << 1);
+        *reinterpret_cast<uint2*>(dst) = hi;
+        if (SPLIT) {   // what is left, in the same units: both parts go into one accumulator
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+          *reinterpret_cast<uint2*>(dst + Q_PART) = make_uint2(f16x2_of(make_float2(v.x - x.x, v.y - x.y)), f16x2_of(make_float2(v.z - y.x, v.w - y.y)));
+        }
       }
     }
   }
@@ -229,9 +240,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_attn_tc_kernel(tha_attn_t a
         const bool whole = there && kt + 31 <= p_first && kt >= last_first && (a.window <= 0 || p_last - kt < a.window || kt + 32 <= a.keep_first) && ks[2 * hf] >= 0.f &&
                            ks[2 * hf + 1] >= 0.f;
         if (!whole) {
+          uint32_t seen = row_ok && there ? kv8_sees32(a, kt, pos, first) : 0u;
+          if (ks[2 * hf] < 0.f) seen &= 0xFFFF0000u;
+          if (ks[2 * hf + 1] < 0.f) seen &= 0xFFFFu;
 #pragma unroll
-          for (int i = 0; i < 32; i++)
-            if (!(row_ok && there && ks[2 * hf + (i >> 4)] >= 0.f && hyb_attn_sees(a, kt + i, pos, first))) sr[32 * hf + i] = 0xFF800000u;
+          for (int i = 0; i < 32; i++) sr[32 * hf + i] = seen >> i & 1u ? sr[32 * hf + i] : 0xFF800000u;
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -421,12 +434,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv8_attn_tc_kernel(tha_attn_t a
     auto scores = [&](int jl, int w) {
       const uint32_t d = tmem + (uint32_t)(w * 2 * KT_KEYS + (jl & 1) * KT_KEYS), k = kv_addr + (uint32_t)((jl % STAGES) * KV_STAGE);
 #pragma unroll
-      for (int s = 0; s < DT / 16; s++) {
-        if (s >= k_steps) break;
-        const uint32_t at = (uint32_t)(w * (SPLIT ? 2 : 1) * Q_PART + (s >> 2) * KT_ROWS * 128);
-        const uint64_t bd = tc_smem_desc(k + (uint32_t)((s >> 2) * KT_KEYS * 128)) + (uint64_t)(2 * (s & 3));
-        tc_mma_f16(d, tc_smem_desc(q_addr + at) + (uint64_t)(2 * (s & 3)), bd, id_s, (uint32_t)(s != 0));
-        if (SPLIT) tc_mma_f16(d, tc_smem_desc(q_addr + at + Q_PART) + (uint64_t)(2 * (s & 3)), bd, id_s, 1u);
+      for (int part = SPLIT ? 1 : 0; part >= 0; part--) {   // what is small first: sums are cut off at the size of what is there
+#pragma unroll
+        for (int s = 0; s < DT / 16; s++) {
+          if (s >= k_steps) break;
+          const uint64_t ad = tc_smem_desc(q_addr + (uint32_t)((w * (SPLIT ? 2 : 1) + part) * Q_PART + (s >> 2) * KT_ROWS * 128)) + (uint64_t)(2 * (s & 3));
+          const uint64_t bd = tc_smem_desc(k + (uint32_t)((s >> 2) * KT_KEYS * 128)) + (uint64_t)(2 * (s & 3));
+          tc_mma_f16(d, ad, bd, id_s, (uint32_t)(s != 0 || (SPLIT && part == 0)));
+        }
       }
       tc_commit(&s_full[w][jl & 1]);
     };
