@@ -90,12 +90,17 @@ __device__ __forceinline__ float k8_final(const tha_attn_t& a, int h, float m, f
 __device__ __forceinline__ void k8_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void k8_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// Partial results of `splits` parts of `all` (row, head)s: maxima and sums [part][all][2], rounded up to 16 bytes, then accumulators [part][all][E]
+__host__ __device__ __forceinline__ size_t k8_sums_floats(int splits, size_t all) { return (2 * all * splits + 3) & ~(size_t)3; }
+__host__ __device__ __forceinline__ size_t k8_partial_floats(int splits, size_t all, int E) { return k8_sums_floats(splits, all) + all * splits * E; }
+
 // host side: kv8_rows.cu
 int kv8_check(const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const char* who);
 int kv8_refuse(const char* who, const char* why);
 // kv8_attn_tc.cu: sequences of at least min_rows rows; THA_STATUS_NOT_SUPPORTED (nothing launched): the caller takes another form
-int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles);
-int kv8_attn_tc_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int min_rows, int splits,
-                       float* partial, const float* gate, long long ldg);
+int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int most_tiles);
+size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles);
+int kv8_attn_tc_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int min_rows, int most_tiles,
+                       int splits, void* staged, float* partial, const float* gate, long long ldg);
 
 }  // namespace tha

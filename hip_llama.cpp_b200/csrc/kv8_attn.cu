@@ -72,8 +72,6 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
   __shared__ float s_ml[K8_WARPS][K8_PAIRS][2];
   const int D = a.dim, E = a.vdim, gsize = a.heads / a.kv_heads, B = kv.block_size, layer = a.cache_layer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  // channels past the head's are zeros that no copy touches
-  for (int i = threadIdx.x; i < Ring::BYTES / 16; i += K8_THREADS) reinterpret_cast<uint4*>(k8_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   hyb_pdl_enter();
   const int kvh = blockIdx.y, sp = blockIdx.x % splits;
   int seq, tile;
@@ -87,6 +85,8 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     }
   }
   if (seq < 0) return;
+  if (D < DT || E < DT)                                     // channels past the head's are zeros that no copy touches
+    for (int i = threadIdx.x; i < Ring::BYTES / 16; i += K8_THREADS) reinterpret_cast<uint4*>(k8_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   const int r0 = rows.seq_first[seq], n_rows = rows.seq_first[seq + 1] - r0, slot = rows.seq_slot[seq];
   const int pairs = min(K8_PAIRS, n_rows * gsize - tile * K8_PAIRS);
   if (pairs < 1) return;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     L *= exp2f(-K8_UP);
     float scale = ref * exp2f(-K8_UP);
     const size_t at = (size_t)r * a.heads + h2, all = (size_t)rows.n_rows * a.heads;
-    float* pd = splits > 1 ? partial + 2 * all * splits + ((size_t)sp * all + at) * E : nullptr;
+    float* pd = splits > 1 ? partial + k8_sums_floats(splits, all) + ((size_t)sp * all + at) * E : nullptr;
     if (!pd) scale *= k8_final(a, h2, M, L, gate ? gate + (size_t)r * ldg : nullptr);
     else if (lane == 0) { float* ml = partial + 2 * ((size_t)sp * all + at); ml[0] = M; ml[1] = L; }
     for (int c = lane; c < E; c += 32) {
@@ -348,50 +348,58 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
   }
 }
 
-// The parts of a (row, head) in order, of sequences of least .. most rows.  grid (rows * heads)
-template <typename T>
+// The parts of a (row, head), of sequences of least .. most rows, four channels a lane.  WARPS 1: a warp has them all, in order; 4: a block, every fourth to a warp (many parts of few rows:
+// one after the other they took 12 us).  grid (rows * heads * WARPS / 4)
+template <int WARPS, typename T>
 __global__ void __launch_bounds__(128) kv8_merge_kernel(T* out, const float* partial, tha_rows_t rows, int least, int most, int splits, tha_attn_t a, const float* gate, long long ldg) {
   hyb_pdl_enter();
-  __shared__ float s_w[K8_MAX_SPLITS];
-  __shared__ float s_f;
-  const size_t at = blockIdx.x, all = (size_t)rows.n_rows * a.heads;
-  const int E = a.vdim;
-  {
-    const int seq = rows.row_seq[blockIdx.x / a.heads], n = rows.seq_first[seq + 1] - rows.seq_first[seq];
-    if (n < least || n > most) return;
-  }
-  if (threadIdx.x < 32) {
-    float m[2], l[2], M = -INFINITY;
+  __shared__ float4 s_o[WARPS][32];
+  const int warp = threadIdx.x >> 5, w0 = WARPS == 1 ? 0 : warp;
+  const size_t at = (size_t)blockIdx.x * (4 / WARPS) + (WARPS == 1 ? warp : 0), all = (size_t)rows.n_rows * a.heads;
+  if (at >= all) return;
+  const int E = a.vdim, lane = threadIdx.x & 31, row = (int)(at / a.heads), h = (int)(at - (size_t)row * a.heads);
+  const int seq = rows.row_seq[row], n = rows.seq_first[seq + 1] - rows.seq_first[seq];
+  if (n < least || n > most) return;
+  static_assert(K8_MAX_SPLITS == 64, "two parts a lane");
+  float m[2], l[2], w[2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int s = threadIdx.x + 32 * i;
-      const float2 ml = s < splits ? *reinterpret_cast<const float2*>(partial + 2 * ((size_t)s * all + at)) : make_float2(-INFINITY, 0.f);
-      m[i] = ml.x; l[i] = ml.y;
-      M = fmaxf(M, m[i]);
-    }
-    const bool nan = __any_sync(THA_FULL_MASK, m[0] != m[0] || m[1] != m[1]);
-    M = warp_max(M);
-    float L = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const float w = m[i] > -INFINITY ? exp2f(m[i] - M) : 0.f;
-      s_w[threadIdx.x + 32 * i] = w;
-      L += w * l[i];
-    }
-    L = warp_sum(L);
-    const int row = (int)(at / a.heads), h = (int)(at - (size_t)row * a.heads);
-    const float f = k8_final(a, h, nan ? NAN : M, L, gate ? gate + (size_t)row * ldg : nullptr);
-    if (threadIdx.x == 0) s_f = f;
+  for (int i = 0; i < 2; i++) {
+    const int s = lane + 32 * i;
+    const float2 ml = s < splits ? *reinterpret_cast<const float2*>(partial + 2 * ((size_t)s * all + at)) : make_float2(-INFINITY, 0.f);
+    m[i] = ml.x; l[i] = ml.y;
   }
-  __syncthreads();
-  const float* p = partial + 2 * all * splits + at * E;
-  for (int c = threadIdx.x; c < E; c += blockDim.x) {
-    float o = 0.f;
-    for (int s = 0; s < splits; s++)
-      if (s_w[s] > 0.f) o = fmaf(p[(size_t)s * all * E + c], s_w[s], o);
-    o *= s_f;
-    if (a.out_f32) reinterpret_cast<float*>(out)[at * E + c] = o;
-    else k8_store(out + at * E + c, o);
+  const float* p = partial + k8_sums_floats(splits, all) + at * E + 4 * lane;
+  const bool mine = 4 * lane < E, nan = __any_sync(THA_FULL_MASK, m[0] != m[0] || m[1] != m[1]);
+  const float M = warp_max(fmaxf(m[0], m[1]));
+#pragma unroll
+  for (int i = 0; i < 2; i++) w[i] = m[i] > -INFINITY ? exp2f(m[i] - M) : 0.f;
+  const float L = warp_sum(w[0] * l[0] + w[1] * l[1]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = w0; s < splits; s += WARPS) {
+    const float ws = __shfl_sync(THA_FULL_MASK, s < 32 ? w[0] : w[1], s & 31);
+    if (ws > 0.f && mine) {                                 // parts that saw nothing hold nothing
+      const float4 v = *reinterpret_cast<const float4*>(p + (size_t)s * all * E);
+      o.x = fmaf(v.x, ws, o.x); o.y = fmaf(v.y, ws, o.y); o.z = fmaf(v.z, ws, o.z); o.w = fmaf(v.w, ws, o.w);
+    }
+  }
+  if (WARPS > 1) {                                          // the whole block is one (row, head): it comes here as one
+    s_o[w0][lane] = o;
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int i = 1; i < WARPS; i++) {
+      const float4 v = s_o[i][lane];
+      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+    }
+  }
+  if (!mine) return;
+  const float f = k8_final(a, h, nan ? NAN : M, L, gate ? gate + (size_t)row * ldg : nullptr);
+  const float v[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (a.out_f32) reinterpret_cast<float*>(out)[at * E + 4 * lane + i] = v[i];
+    else k8_store(out + at * E + 4 * lane + i, v[i]);
   }
 }
 
@@ -422,8 +430,11 @@ static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows)
 
 template <typename T>
 static int k8_merge(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, T* out, int least, int most, int splits, const float* partial, const float* gate, long long ldg) {
-  if (splits > 1)
-    THA_CUDA_OK(launch(kv8_merge_kernel<T>, dim3((unsigned)rows->n_rows * a->heads), dim3(128), 0, s, pdl_enabled() != 0, out, partial, *rows, least, most, splits, *a, gate, ldg));
+  const unsigned all = (unsigned)rows->n_rows * a->heads;
+  if (splits > 8)
+    THA_CUDA_OK(launch(kv8_merge_kernel<4, T>, dim3(all), dim3(128), 0, s, pdl_enabled() != 0, out, partial, *rows, least, most, splits, *a, gate, ldg));
+  else if (splits > 1)
+    THA_CUDA_OK(launch(kv8_merge_kernel<1, T>, dim3((all + 3) / 4), dim3(128), 0, s, pdl_enabled() != 0, out, partial, *rows, least, most, splits, *a, gate, ldg));
   return THA_STATUS_SUCCESS;
 }
 template <int DT, int FMT, bool MORE, typename T>
@@ -451,7 +462,7 @@ struct Kv8Forms { int short_rows; bool has_short, has_long; };
 constexpr int K8_LONG_PAIRS = 128;
 static Kv8Forms k8_forms(const tha_attn_t* a, const tha_rows_t* rows) {
   const int gsize = a->heads / a->kv_heads;
-  Kv8Forms f = {gsize > 256 ? 0x7FFFFFFF : ceil_div(K8_LONG_PAIRS, gsize), true, false};
+  Kv8Forms f = {gsize > 128 ? 0x7FFFFFFF : ceil_div(K8_LONG_PAIRS, gsize), true, false};
   if (f.short_rows < 1) f.short_rows = 1;
   f.has_long = rows->max_seq_rows > f.short_rows;
   f.has_short = !(f.has_long && (long long)rows->n_seqs * rows->max_seq_rows == rows->n_rows);   // all sequences are as long as the longest
@@ -461,18 +472,29 @@ template <typename T>
 static int k8_attend(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, float* scratch, size_t room,
                      const float* gate, long long ldg) {
   const Kv8Forms f = k8_forms(a, rows);
-  const size_t one = (size_t)rows->n_rows * a->heads * (a->vdim + 2);
-  auto fit = [&](int splits) { return !scratch ? 1 : (size_t)splits * one <= room ? splits : room / one < 2 ? 1 : (int)(room / one); };
+  const size_t all = (size_t)rows->n_rows * a->heads;
+  auto fit = [&](int splits, size_t room) {
+    while (splits > 1 && k8_partial_floats(splits, all, a->vdim) > room) splits--;
+    return splits;
+  };
   int short_rows = f.short_rows;
   if (f.has_long) {
-    const int splits = fit(kv8_attn_tc_splits(a, rows, k8_most_tiles(a, rows)));
-    const int st = kv8_attn_tc_launch(s, dtype, a, rows, kv, q, out, short_rows + 1, splits, scratch, gate, ldg);
-    if (st == THA_STATUS_SUCCESS) THA_TRY_RC(k8_merge(s, a, rows, out, short_rows + 1, 0x7FFFFFFF, splits, scratch, gate, ldg));
-    else if (st != THA_STATUS_NOT_SUPPORTED) return st;
-    else short_rows = 0x7FFFFFFF;
-    if (st == THA_STATUS_SUCCESS && !f.has_short) return THA_STATUS_SUCCESS;
+    // tiles in fp16 first, partial results behind them
+    const int most = k8_most_tiles(a, rows);
+    const size_t stage = kv8_attn_tc_stage_bytes(a, rows, most) / sizeof(float);
+    int st = THA_STATUS_NOT_SUPPORTED;
+    if (scratch && stage && stage <= room) {
+      const int splits = fit(kv8_attn_tc_splits(a, rows, dtype, most), room - stage);
+      st = kv8_attn_tc_launch(s, dtype, a, rows, kv, q, out, short_rows + 1, most, splits, scratch, scratch + stage, gate, ldg);
+      if (st == THA_STATUS_SUCCESS) {
+        THA_TRY_RC(k8_merge(s, a, rows, out, short_rows + 1, 0x7FFFFFFF, splits, scratch + stage, gate, ldg));
+        if (!f.has_short) return THA_STATUS_SUCCESS;
+      }
+    }
+    if (st == THA_STATUS_NOT_SUPPORTED) short_rows = 0x7FFFFFFF;
+    else if (st != THA_STATUS_SUCCESS) return st;
   }
-  const int splits = fit(k8_splits(a, rows, short_rows));
+  const int splits = scratch ? fit(k8_splits(a, rows, short_rows), room) : 1;
   if (a->dim > 64 || a->vdim > 64) THA_TRY_RC((k8_form<128>(s, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg)));
   else THA_TRY_RC((k8_form<64>(s, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg)));
   return k8_merge(s, a, rows, out, 0, short_rows, splits, scratch, gate, ldg);
@@ -495,12 +517,23 @@ static int k8_check(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t
 
 using namespace tha;
 
-extern "C" size_t tha_hyb_kv8_attn_scratch(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv) {
+extern "C" size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv) {
   if (rows->n_rows < 1 || k8_check(a, rows, kv, "tha_hyb_kv8_attn_scratch") != THA_STATUS_SUCCESS) return 0;
   const Kv8Forms f = k8_forms(a, rows);
-  const int longs = f.has_long ? kv8_attn_tc_splits(a, rows, k8_most_tiles(a, rows)) : 1, shorts = f.has_short ? k8_splits(a, rows, f.short_rows) : 1;
-  const int most = longs > shorts ? longs : shorts;
-  return most > 1 ? (size_t)most * rows->n_rows * a->heads * (a->vdim + 2) : 0;
+  const size_t all = (size_t)rows->n_rows * a->heads;
+  const int most = k8_most_tiles(a, rows);
+  const size_t stage = f.has_long ? kv8_attn_tc_stage_bytes(a, rows, most) / sizeof(float) : 0;
+  size_t need = 0;
+  if (f.has_short || !stage) {
+    const int splits = k8_splits(a, rows, stage ? f.short_rows : 0x7FFFFFFF);
+    if (splits > 1) need = k8_partial_floats(splits, all, a->vdim);
+  }
+  if (stage) {
+    const int splits = kv8_attn_tc_splits(a, rows, dtype, most);
+    const size_t with = stage + (splits > 1 ? k8_partial_floats(splits, all, a->vdim) : 0);
+    if (with > need) need = with;
+  }
+  return need;
 }
 
 extern "C" int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,

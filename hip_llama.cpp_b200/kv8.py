@@ -49,7 +49,7 @@ def lib():
         c.tha_hyb_kv8_write.argtypes = [P, I, R, K, I, P, L, P, L]
         c.tha_hyb_kv8_read.argtypes = [P, I, R, K, I, P, L, P, L]
         c.tha_hyb_kv8_attn.argtypes = [P, I, A, R, K, P, P, P, C.c_size_t, P, L]
-        c.tha_hyb_kv8_attn_scratch.argtypes = [A, R, K]
+        c.tha_hyb_kv8_attn_scratch.argtypes = [I, A, R, K]
         c.tha_hyb_kv8_attn_scratch.restype = C.c_size_t
     return _lib
 
@@ -217,7 +217,7 @@ class Kv8Cache:
                 raise ValueError("head_gate reads its columns from proj [rows, columns]")
             gate, ldg = self._rows("proj", proj, rows.n, proj.shape[1], (torch.float32,))
         c = self.lib.c
-        need = c.tha_hyb_kv8_attn_scratch(attn.ref, rows.ref, self.ref)
+        need = c.tha_hyb_kv8_attn_scratch(DTYPES[out.dtype], attn.ref, rows.ref, self.ref)
         scratch = torch.empty(need, dtype=torch.float32, device=self.device) if need else None
         self.lib.check(c.tha_hyb_kv8_attn(stream, DTYPES[out.dtype], attn.ref, rows.ref, self.ref, q.data_ptr(), out.data_ptr(), scratch.data_ptr() if need else None, need,
                                           gate, ldg), "tha_hyb_kv8_attn")

@@ -666,15 +666,16 @@ int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_
 /* tha_hyb_attn_gated over such a cache: every row attends to the visible keys as the cache holds them, which for rows of a block that is not full are their codes
  * under its present scale.  a: heads, kv_heads, dim, vdim, scale, chunk, cache_layer, window, keep_first, sink, head_scale, softcap, rel, head_gate and out_f32 as there
  * (values_in_keys, v_share and diff are refused); q fp32 [n_rows, heads * dim]; out dtype-typed [n_rows, heads * vdim].  Idle rows get zeros.
- * Codes are exact in fp16; q and the weights enter the products as two fp16 that carry 22 bits of them (a value 2^28 below the largest of its row of q, a
- * weighted value 2^28 below the row's largest weight times the largest scale of V's blocks that the row sees, still has them).  Rows of prompts with dtype
- * THA_DT_BF16 may use one fp16 of 11 bits instead.  Sums and softmax are fp32.
- * scratch (nullable, 16-byte aligned): room for partial results where long contexts are cut along the keys (n * n_rows * heads * (vdim + 2) floats for n parts; as
- * many as fit, 64 at most); calls that may run at the same time need scratch of their own. */
+ * Codes are exact in fp16; q and the weights enter the products as two fp16: q with 22 bits of each value, or 2^-28 of the largest of its row of a head; a weight times its value's
+ * scale with 22 bits, or 2^-32 of the largest of the row (2^-34 where V's scales differ).  Rows of longer portions with dtype THA_DT_BF16 use one fp16 of 11 bits instead.  Sums and softmax are
+ * fp32.
+ * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones, and for
+ * partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may
+ * run at the same time need scratch of their own. */
 int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,
                      size_t scratch_floats, const float* proj, long long ldp);
-/* floats of scratch with which such a call is cut as it pleases (0: it needs none) */
-size_t tha_hyb_kv8_attn_scratch(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv);
+/* floats of scratch for such a call (0: it needs none, or would be refused) */
+size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv);
 
 #ifdef __cplusplus
 }

@@ -377,19 +377,20 @@ def test_blocks_that_do_not_exist_under_a_portion():
     assert rel(out, want.reshape(400, -1)) < F32_TOL
 
 
-@pytest.mark.parametrize("scratch", [0, 1, 2, 3, 16])
-def test_parts_of_a_portions_context_meet(scratch):
-    m = filled(16, 1, 128, 128, "int8", (4000,))
-    parts, heads = [(0, 3900, 100)], 2
+@pytest.mark.parametrize("share", [0.0, 0.01, 0.5, 0.95, 0.99, 1.0, 1.5])
+@pytest.mark.parametrize("parts", [[(0, 3900, 100)], [(0, 3900, 100), (1, 20, 90), (1, 30, 1), (0, 1000, 70)]], ids=["one", "four"])
+def test_parts_of_a_portions_context_meet(share, parts):
+    """With less room than the call would like, and nothing behind the room."""
+    m = filled(16, 1, 128, 128, "int8", (4000, 111))
+    heads, n = 2, sum(x[2] for x in parts)
     out, want = attend(m, dict(heads=heads, scale=128 ** -0.5), parts, torch.float32)
     close(out, want)
-    r, at = K.Rows.of(parts), K.Attention(heads, 1, 128, scale=128 ** -0.5)
+    r, at, lib = K.Rows.of(parts), K.Attention(heads, 1, 128, scale=128 ** -0.5), K.lib()
     at.c.cache_layer = LAYER
-    q = torch.randn(100, heads * 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
-    floats = scratch * 100 * heads * 130
+    q = torch.randn(n, heads * 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    floats = int(share * lib.c.tha_hyb_kv8_attn_scratch(1, at.ref, r.ref, m.cache.ref))
     room = torch.full((floats + 512,), 3.25, device="cuda")
     got = torch.full_like(out, float("nan"))
-    lib = K.lib()
     lib.check(lib.c.tha_hyb_kv8_attn(torch.cuda.current_stream().cuda_stream, 1, at.ref, r.ref, m.cache.ref, q.data_ptr(), got.data_ptr(), room.data_ptr() if floats else None,
                                      floats, None, 0))
     torch.cuda.synchronize()

@@ -117,7 +117,7 @@ def test_operands_that_are_refused():
 def test_attention_that_is_refused(bad, code):
     f = K.lib().c
     assert f.tha_hyb_kv8_attn(None, 1, attn(**bad), rows(), cache(), A, A, None, 0, None, 0) == code
-    assert f.tha_hyb_kv8_attn_scratch(attn(**bad), rows(), cache()) == 0
+    assert f.tha_hyb_kv8_attn_scratch(1, attn(**bad), rows(), cache()) == 0
 
 
 def test_no_rows_are_no_work():
