@@ -63,6 +63,17 @@ __device__ __forceinline__ float k8_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float k8_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 k8_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 // Bytes 0 and 2 of w as fp16.  int8: a byte with its sign flipped is code + 128; in the low half of 0x6400 = 1024.0 that is 1024 + 128 + code exactly.
 __device__ __forceinline__ uint32_t k8_bytes02(uint32_t w) {
   const uint32_t u = (w & 0x00FF00FFu) ^ 0x64806480u;

@@ -21,7 +21,7 @@ constexpr float K8_UP = 15.0f;   // weights: 2^(score log2(e) - maximum + 15)
 template <int DT>
 struct Kv8Ring {
   static constexpr int TILE = K8_KEYS * DT;                 // bytes of a tile's K, and of its V
-  static constexpr int STAGES = DT == 128 ? 3 : 4;
+  static constexpr int STAGES = DT == 128 ? 2 : 4;
   static constexpr int WARP = STAGES * 2 * TILE;
   static constexpr int BYTES = K8_WARPS * WARP;
 };
@@ -35,9 +35,9 @@ __device__ __forceinline__ void k8_copy16(uint32_t dst, const void* src, bool th
 __device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void k8_await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void k8_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void k8_mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 // The channels of a word of K that go to the two registers of the B operand: (0, 2) and (1, 3), or (0, 1) and (2, 3) -- what is cheapest to take apart
 template <int FMT>
@@ -58,19 +58,21 @@ __device__ __forceinline__ int k8_tiles_of(const tha_rows_t& rows, int s, int gs
   return n <= most ? (n * gsize + K8_PAIRS - 1) / K8_PAIRS : 0;
 }
 // grid (tiles of pairs * splits, kv_heads).  Partial results of a split: sums and maxima [split][row * heads + head][2], then accumulators [..][vdim].
-template <int DT, int FMT, bool MORE, typename T>
-__global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, const float* q, T* out, int most_rows, int splits, int run,
+// FULL: heads have DT channels, keys and values alike.
+template <int DT, int FMT, bool MORE, bool FULL>
+__global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, const float* q, void* out, int out_bf16, int most_rows, int splits, int run,
                                                                  float* partial, const float* gate, long long ldg) {
   using Ring = Kv8Ring<DT>;
   constexpr float LOG2E = 1.4426950408889634f;
   constexpr int KS = DT / 16;                               // k steps of the scores
   constexpr int NV = DT / 8;                                // column groups of the accumulator
   extern __shared__ __align__(128) unsigned char k8_ring[];
-  __shared__ int s_id[2 * K8_SEG];                          // per 16 keys of a segment's tiles: block id, the scales
+  __shared__ uint4 s_q[KS][32];                             // q as the A operand of every step, a lane's registers together
+  __shared__ int s_tile[2 * K8_SEG];                        // per 16 keys of a segment's tiles: (block, layer, head), -1 where they do not exist, and the scales
   __shared__ float s_ks[2 * K8_SEG], s_vs[2 * K8_SEG];
-  __shared__ float s_red[33];
+  __shared__ float s_top[K8_WARPS];
   __shared__ float s_ml[K8_WARPS][K8_PAIRS][2];
-  const int D = a.dim, E = a.vdim, gsize = a.heads / a.kv_heads, B = kv.block_size, layer = a.cache_layer;
+  const int D = FULL ? DT : a.dim, E = FULL ? DT : a.vdim, gsize = a.heads / a.kv_heads, B = kv.block_size, layer = a.cache_layer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   hyb_pdl_enter();
   const int kvh = blockIdx.y, sp = blockIdx.x % splits;
@@ -85,13 +87,16 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     }
   }
   if (seq < 0) return;
-  if (D < DT || E < DT)                                     // channels past the head's are zeros that no copy touches
-    for (int i = threadIdx.x; i < Ring::BYTES / 16; i += K8_THREADS) reinterpret_cast<uint4*>(k8_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
-  const int r0 = rows.seq_first[seq], n_rows = rows.seq_first[seq + 1] - r0, slot = rows.seq_slot[seq];
+  // What a block waits for ahead of its first tile is a chain of loads: positions, block ids, codes.  With every sequence a row the first row of one is its number, and the
+  // scales and q's parts are made while the first codes are on their way.
+  const bool singles = rows.max_seq_rows == 1;
+  const int r0 = singles ? seq : rows.seq_first[seq], n_rows = singles ? 1 : rows.seq_first[seq + 1] - r0, slot = rows.seq_slot[seq];
   const int pairs = min(K8_PAIRS, n_rows * gsize - tile * K8_PAIRS);
   if (pairs < 1) return;
   const int pr = tile * K8_PAIRS + min(g, pairs - 1), pp = pr / gsize, head = kvh * gsize + (pr - pp * gsize);   // this lane's pair (behind the last: the last again)
   const int p_seq = rows.pos[r0];
+  if (!FULL)                                                // channels past the head's are zeros that no copy touches
+    for (int i = threadIdx.x; i < Ring::BYTES / 16; i += K8_THREADS) reinterpret_cast<uint4*>(k8_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   const int p_first = p_seq + (tile * K8_PAIRS) / gsize, p_last = p_seq + (tile * K8_PAIRS + pairs - 1) / gsize, pos = p_seq + pp;
   const int key_lo = a.chunk > 0 ? (p_first / a.chunk) * a.chunk : 0, last_lo = a.chunk > 0 ? (p_last / a.chunk) * a.chunk : 0;
   const int my_lo = a.chunk > 0 ? (pos / a.chunk) * a.chunk : 0;
@@ -100,40 +105,48 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
   const int ti0 = min(sp * run, tiles.n), ti1 = sp == splits - 1 ? tiles.n : min(ti0 + run, tiles.n);
   auto tile_key = [&](int ti) { return ti < tiles.n_a ? tiles.begin + 32 * ti : tiles.resume + 32 * (ti - tiles.n_a); };
 
-  // q: the lane's channels of its pair are those it reads of a key, DT / 4
-  uint32_t qf[KS][4];
-  float fac;
-  {
+  // q's parts as operands, and the factor of its scores: a lane's channels of its pair are those it reads of a key
+  float fac = 0.f;
+  auto make_q = [&]() {
     const float* qr = q + ((size_t)(r0 + pp) * a.heads + head) * D;
     float v[KS][4], top = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       const int c = (DT == 128 ? 2 * t + (s >> 2) : t) * 16 + (s & 3) * 4;
-      const float4 x = c < D && p_seq >= 0 ? *reinterpret_cast<const float4*>(qr + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x = c < D ? *reinterpret_cast<const float4*>(qr + c) : make_float4(0.f, 0.f, 0.f, 0.f);
       v[s][0] = x.x; v[s][1] = x.y; v[s][2] = x.z; v[s][3] = x.w;
+    }
+#pragma unroll
+    for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(v[s][i]));
-    }
     top = fmaxf(top, __shfl_xor_sync(THA_FULL_MASK, top, 1));
     top = fmaxf(top, __shfl_xor_sync(THA_FULL_MASK, top, 2));
     float inverse;
     const float up = split_scale<100>(top, 14, &inverse);
     constexpr int X = FMT == THA_KV8_INT8 ? 2 : 1, Y = FMT == THA_KV8_INT8 ? 1 : 2;   // k8_keys
+    if (warp == 0) {                                        // all warps have the same
 #pragma unroll
-    for (int s = 0; s < KS; s++) {
-      split_f16x2(make_float2(v[s][0], v[s][X]), up, qf[s][0], qf[s][1]);
-      split_f16x2(make_float2(v[s][Y], v[s][3]), up, qf[s][2], qf[s][3]);
+      for (int s = 0; s < KS; s++) {
+        uint4 f;
+        split_f16x2(make_float2(v[s][0], v[s][X]), up, f.x, f.y);
+        split_f16x2(make_float2(v[s][Y], v[s][3]), up, f.z, f.w);
+        s_q[s][lane] = f;
+      }
     }
-    fac = inverse * a.scale * (a.head_scale ? a.head_scale[head] : 1.0f);
-    if (!MORE) fac *= LOG2E;
-  }
+    fac = inverse * a.scale * (a.head_scale ? a.head_scale[head] : 1.0f) * (MORE ? 1.0f : LOG2E);
+  };
 
   float acc[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   float m = -INFINITY, l = 0.f, ref = 0.f;                  // l: this lane's keys only
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(k8_ring) + warp * Ring::WARP;
-  const uint8_t *kpool = static_cast<const uint8_t*>(kv.k_pool), *vpool = static_cast<const uint8_t*>(kv.v_pool);
+  const int lane_r = lane / (DT / 16), lane_c = lane % (DT / 16);   // the row and piece of 512 bytes of a tile that this lane copies
+  const uint32_t lane_to = (uint32_t)k8_piece<DT>(lane_r, lane_c);
+  const bool k_there = 16 * lane_c < D, v_there = 16 * lane_c < E;
+  const size_t k_tile = (size_t)B * D, v_tile = (size_t)B * E;
+  const uint8_t *kpool = static_cast<const uint8_t*>(kv.k_pool) + lane_r * D + 16 * lane_c, *vpool = static_cast<const uint8_t*>(kv.v_pool) + lane_r * E + 16 * lane_c;
 
   // The tensor cores cut off what their fp32 sums cannot hold: an accumulator sums a segment's tiles, 128 sums a warp, and the segments' are added here.
   float seg_total[2 * NV], m_total = -INFINITY, ref_total = 0.f;
@@ -161,17 +174,46 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
       m_total = m; ref_total = ref;
     }
     __syncthreads();
-    float top = 0.f;
     for (int e = threadIdx.x; e < 2 * (s1 - s0); e += K8_THREADS) {
       const int key = tile_key(s0 + (e >> 1)) + 16 * (e & 1);
       const int id = key <= p_last ? kv8_block(kv, slot, key) : -1;
-      s_id[e] = id;
-      const size_t at = id >= 0 ? kv8_tile(kv, id, layer, kvh) : 0;
-      s_ks[e] = id >= 0 ? kv.k_scale[at] : 0.f;
-      s_vs[e] = id >= 0 ? kv.v_scale[at] : 0.f;
-      top = fmaxf(top, s_vs[e]);
+      s_tile[e] = id >= 0 ? (int)kv8_tile(kv, id, layer, kvh) : -1;   // a tile has 256 bytes at least: they are below 2^31 in any memory
     }
-    top = block_max(top, s_red);                            // its barriers publish the table as well
+    __syncthreads();
+    auto fetch = [&](int ti, int stage) {                   // every lane's share of a tile; nothing behind the segment's last
+      if (ti >= s1) return;
+      const int e = 2 * (ti - s0), in_block = tile_key(ti) & (B - 1);
+      const uint32_t dst = ring + stage * 2 * Ring::TILE;
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const int tile = s_tile[e + hf], row = (in_block + 16 * hf) & (B - 1);
+        const bool there = tile >= 0;
+        const uint8_t *ks = kpool + (there ? (size_t)(unsigned)tile * k_tile + row * D : 0), *vs = vpool + (there ? (size_t)(unsigned)tile * v_tile + row * E : 0);
+#pragma unroll
+        for (int i = 0; i < DT / 32; i++) {                 // rows lane_r, lane_r + STEP, ..: the piece's place turns with the row
+          constexpr int STEP = 512 / DT;
+          const int turn = DT == 128 ? (i & 1) * 64 : (i & 1) * 0;
+          const uint32_t to = dst + (16 * hf + STEP * i) * DT + (lane_to ^ turn);
+          if (FULL || k_there) k8_copy16(to, ks + STEP * i * D, there);
+          if (FULL || v_there) k8_copy16(to + Ring::TILE, vs + STEP * i * E, there);
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < Ring::STAGES - 1; i++) { fetch(s0 + warp + i * K8_WARPS, i); k8_commit(); }
+    float top = 0.f;
+    for (int e = threadIdx.x; e < 2 * (s1 - s0); e += K8_THREADS) {
+      const int at = s_tile[e];
+      s_ks[e] = at >= 0 ? kv.k_scale[at] : 0.f;
+      const float vs = at >= 0 ? kv.v_scale[at] : 0.f;
+      s_vs[e] = vs;
+      top = fmaxf(top, vs);
+    }
+    top = warp_max(top);
+    if (lane == 0) s_top[warp] = top;
+    if (s0 == ti0) make_q();
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
     float down = 1.0f;
     if (top > ref) {                                        // up to the next power of two: what is there changes units exactly
       const float to = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u));
@@ -184,25 +226,6 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     }
     if (ref > 0.f) down = 1.0f / ref;
 
-    auto fetch = [&](int ti, int stage) {                   // every lane's share of a tile; nothing behind the segment's last
-      if (ti >= s1) return;
-      const int e = 2 * (ti - s0), key = tile_key(ti);
-      const uint32_t dst = ring + stage * 2 * Ring::TILE;
-#pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        const int id = s_id[e + hf];
-        const size_t row = (id >= 0 ? kv8_tile(kv, id, layer, kvh) * B + (key + 16 * hf) % B : 0);
-        const uint8_t *ks = kpool + row * D, *vs = vpool + row * E;
-#pragma unroll
-        for (int i = 0; i < DT / 32; i++) {                 // 16 rows of DT / 16 pieces, 32 at a time
-          const int x = 32 * i + lane, r = x / (DT / 16), c = x % (DT / 16);
-          if (16 * c < D) k8_copy16(dst + k8_piece<DT>(16 * hf + r, c), ks + r * D + 16 * c, id >= 0);
-          if (16 * c < E) k8_copy16(dst + Ring::TILE + k8_piece<DT>(16 * hf + r, c), vs + r * E + 16 * c, id >= 0);
-        }
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < Ring::STAGES - 1; i++) { fetch(s0 + warp + i * K8_WARPS, i); k8_commit(); }
     int stage = 0;
     for (int ti = s0 + warp; ti < s1; ti += K8_WARPS) {
       fetch(ti + (Ring::STAGES - 1) * K8_WARPS, stage == 0 ? Ring::STAGES - 1 : stage - 1);
@@ -211,46 +234,53 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
       __syncwarp();
       const unsigned char* st = k8_ring + warp * Ring::WARP + stage * 2 * Ring::TILE;
       const int e = 2 * (ti - s0), kt = tile_key(ti);
-      // scores
+      // scores: 16 bytes of each of the lane's four keys at a time, q of a step read once for them
       float sc[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      for (int j = 0; j < 4; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
 #pragma unroll
-        for (int pcs = 0; pcs < DT / 64; pcs++) {
-          const uint4 w = *reinterpret_cast<const uint4*>(st + k8_piece<DT>(8 * j + g, DT == 128 ? 2 * t + pcs : t));
-          uint32_t b0, b1;
-          k8_keys<FMT>(w.x, b0, b1); k8_mma(sc[j], qf[4 * pcs], b0, b1);
-          k8_keys<FMT>(w.y, b0, b1); k8_mma(sc[j], qf[4 * pcs + 1], b0, b1);
-          k8_keys<FMT>(w.z, b0, b1); k8_mma(sc[j], qf[4 * pcs + 2], b0, b1);
-          k8_keys<FMT>(w.w, b0, b1); k8_mma(sc[j], qf[4 * pcs + 3], b0, b1);
+      for (int pcs = 0; pcs < DT / 64; pcs++) {
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = *reinterpret_cast<const uint4*>(st + k8_piece<DT>(8 * j + g, DT == 128 ? 2 * t + pcs : t));
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const uint4 qf = s_q[4 * pcs + x][lane];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint32_t b0, b1;
+            k8_keys<FMT>(x == 0 ? w[j].x : x == 1 ? w[j].y : x == 2 ? w[j].z : w[j].w, b0, b1);
+            k8_mma(sc[j], qf, b0, b1);
+          }
         }
       }
       const float f0 = fac * s_ks[e], f1 = fac * s_ks[e + 1];
-      const bool there0 = s_id[e] >= 0, there1 = s_id[e + 1] >= 0;
+      const bool there0 = s_tile[e] >= 0, there1 = s_tile[e + 1] >= 0;
       const bool whole = there0 && there1 && kt + 31 <= p_first && kt >= last_lo && (a.window <= 0 || p_last - kt < a.window || kt + 32 <= a.keep_first);
-      uint32_t seen = 0xFFFFFFFFu;
+      float2 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float f = j < 2 ? f0 : f1;
+        x[j] = f32x2_mul(f32x2_fma(make_float2(sc[j][2], sc[j][3]), make_float2(SPLIT_DOWN, SPLIT_DOWN), make_float2(sc[j][0], sc[j][1])), make_float2(f, f));
+        if (MORE) {
+          const int key = kt + 8 * j + 2 * t;
+          if (a.softcap > 0.f) { x[j].x = hyb_softcap(x[j].x, a.softcap); x[j].y = hyb_softcap(x[j].y, a.softcap); }
+          if (a.rel) { x[j].x += hyb_attn_rel(a, head, pos - key); x[j].y += hyb_attn_rel(a, head, pos - key - 1); }
+          x[j].x *= LOG2E; x[j].y *= LOG2E;
+        }
+      }
       if (!whole) {
-        seen = kv8_sees32(a, kt, pos, my_lo);
+        uint32_t seen = kv8_sees32(a, kt, pos, my_lo);
         if (!there0) seen &= 0xFFFF0000u;
         if (!there1) seen &= 0xFFFFu;
-      }
-      seen >>= 2 * t;                                        // bits 8 j, 8 j + 1 are this lane's
-      float x[8], top_x = -INFINITY;
+        seen >>= 2 * t;                                      // bits 8 j, 8 j + 1 are this lane's
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          float v = fmaf(sc[j][2 + i], SPLIT_DOWN, sc[j][i]) * (j < 2 ? f0 : f1);
-          if (MORE) {
-            if (a.softcap > 0.f) v = hyb_softcap(v, a.softcap);
-            if (a.rel) v += hyb_attn_rel(a, head, pos - (kt + 8 * j + 2 * t + i));
-            v *= LOG2E;
-          }
-          if (!(seen >> (8 * j + i) & 1u)) v = -INFINITY;
-          x[2 * j + i] = v;
-          top_x = fmaxf(top_x, v);
+        for (int j = 0; j < 4; j++) {
+          if (!(seen >> (8 * j) & 1u)) x[j].x = -INFINITY;
+          if (!(seen >> (8 * j + 1) & 1u)) x[j].y = -INFINITY;
         }
+      }
+      float top_x = k8_max3(k8_max3(x[0].x, x[0].y, x[1].x), k8_max3(x[1].y, x[2].x, x[2].y), fmaxf(x[3].x, x[3].y));
       top_x = fmaxf(top_x, __shfl_xor_sync(THA_FULL_MASK, top_x, 1));
       top_x = fmaxf(top_x, __shfl_xor_sync(THA_FULL_MASK, top_x, 2));
       const bool grow = top_x > m;
@@ -265,13 +295,15 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
       }
       const float shift = m > -INFINITY ? K8_UP - m : 0.f;   // nothing seen so far: weights are 2^-inf
       const float v0 = s_vs[e] * down, v1 = s_vs[e + 1] * down;
-      uint32_t pf[2][4];
+      uint4 pf[2];
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float w0 = k8_ex2(x[2 * j] + shift), w1 = k8_ex2(x[2 * j + 1] + shift);
-        l += w0 + w1;
-        split_f16x2(f32x2_mul(make_float2(w0, w1), j < 2 ? make_float2(v0, v0) : make_float2(v1, v1)), 1.0f, pf[j >> 1][2 * (j & 1)], pf[j >> 1][2 * (j & 1) + 1]);
+        const float2 y = k8_add2(x[j], make_float2(shift, shift)), w = make_float2(k8_ex2(y.x), k8_ex2(y.y));
+        sum = k8_add2(sum, w);
+        split_f16x2(f32x2_mul(w, j < 2 ? make_float2(v0, v0) : make_float2(v1, v1)), 1.0f, j & 1 ? pf[j >> 1].z : pf[j >> 1].x, j & 1 ? pf[j >> 1].w : pf[j >> 1].y);
       }
+      l += sum.x + sum.y;
       // weights x values: 16 keys at a time
       const unsigned char* sv = st + Ring::TILE;
 #pragma unroll
@@ -309,17 +341,17 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
 
   add_segment();
 
-  // the warps meet: accumulators [warp][pair][DT] over the ring
+  // The warps meet: accumulators over the ring, [warp][column group][pair][8 columns], the groups two words apart in the banks: neither a warp's pairs of columns nor a pair's
+  // channels meet in one.  (As [pair][channel] all 32 lanes met in a bank, and a block took 5 us beside its keys.)
+  constexpr int GROUP = 8 * K8_PAIRS + 2;
   l += __shfl_xor_sync(THA_FULL_MASK, l, 1);
   l += __shfl_xor_sync(THA_FULL_MASK, l, 2);
   __syncthreads();
   float* s_acc = reinterpret_cast<float*>(k8_ring);
   if (t == 0) { s_ml[warp][g][0] = l == l ? m : l; s_ml[warp][g][1] = l; }   // a NaN among the scores shows in the sum alone
 #pragma unroll
-  for (int i = 0; i < NV; i++)
-#pragma unroll
-    for (int x = 0; x < 2; x++)                              // column 2 t + x of group i is channel (2 t + x) * DT / 8 + i
-      s_acc[(warp * K8_PAIRS + g) * DT + (2 * t + x) * (DT / 8) + i] = acc[i][x];
+  for (int i = 0; i < NV; i++)                               // columns 2 t, 2 t + 1 of group i are channels 2 t * DT / 8 + i, (2 t + 1) * DT / 8 + i
+    *reinterpret_cast<float2*>(s_acc + (warp * NV + i) * GROUP + g * 8 + 2 * t) = make_float2(acc[i][0], acc[i][1]);
   __syncthreads();
   for (int w = warp; w < pairs; w += K8_WARPS) {
     const int pr2 = tile * K8_PAIRS + w, pp2 = pr2 / gsize, h2 = kvh * gsize + (pr2 - pp2 * gsize), r = r0 + pp2;
@@ -340,10 +372,10 @@ __global__ void __launch_bounds__(K8_THREADS, 2) kv8_attn_kernel(tha_attn_t a, t
     for (int c = lane; c < E; c += 32) {
       float o = 0.f;
 #pragma unroll
-      for (int x = 0; x < K8_WARPS; x++) o += f[x] * s_acc[(x * K8_PAIRS + w) * DT + c];
+      for (int x = 0; x < K8_WARPS; x++) o += f[x] * s_acc[(x * NV + c % NV) * GROUP + w * 8 + c / NV];
       if (pd) pd[c] = o * scale;
-      else if (a.out_f32) reinterpret_cast<float*>(out)[at * E + c] = o * scale;
-      else k8_store(out + at * E + c, o * scale);
+      else if (out_bf16) reinterpret_cast<__nv_bfloat16*>(out)[at * E + c] = __float2bfloat16_rn(o * scale);
+      else reinterpret_cast<float*>(out)[at * E + c] = o * scale;
     }
   }
 }
@@ -419,13 +451,30 @@ static int k8_pair_tiles(const tha_attn_t* a, const tha_rows_t* rows, int most) 
   const long long by_seqs = (long long)rows->n_seqs * (((long long)(most < rows->max_seq_rows ? most : rows->max_seq_rows) * gsize + K8_PAIRS - 1) / K8_PAIRS);
   return (int)(by_rows < by_seqs ? by_rows : by_seqs);
 }
-// Parts of a context: enough blocks for each SM to have several, of at least 8 tiles (two a warp).
+// Parts of a context.  444 blocks run at once, three on an SM; a block takes the time of six tiles of 32 keys (4 us) beside its own, the meeting of the parts as much.  One context:
+// rounds of whole parts.  Several: their lengths are between nothing and the longest, blocks follow one another as they end, and the last of them is the tail.  us with 1 / 2 / 4 / 6 /
+// 10 / 20 parts, heads of 128: 64 contexts up to 2048 of 32 heads 125 / 136 / 162 / 192; 16 up to 8192 of 8 heads (3 parts: 69) 56 (4) / 50 / 51 / 59; one of 131072 of 8 heads with 18 /
+// 37 / 55 / 64 parts 145 / 83 / 63 / 74.
 static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows) {
+  constexpr int SLOTS = 3 * 148;
+  constexpr float BESIDE = 6.f;
   const int most = k8_most_tiles(a, rows);
   const long long blocks = (long long)k8_pair_tiles(a, rows, most_rows) * a->kv_heads;
-  long long s = (4 * 148 + blocks - 1) / blocks;
-  if (s > most / 8) s = most / 8;
-  return s < 1 ? 1 : s > K8_MAX_SPLITS ? K8_MAX_SPLITS : (int)s;
+  int best = 1;
+  float least = 0.f;
+  for (int s = 1; s <= K8_MAX_SPLITS && (s == 1 || s * 4 <= most); s++) {   // a tile for each warp at least
+    const float run = (float)ceil_div(most, s) + BESIDE;
+    float cost;
+    if (rows->n_seqs == 1) {
+      cost = (float)((blocks * s + SLOTS - 1) / SLOTS) * run;
+    } else {
+      cost = (float)blocks * (0.5f * most + BESIDE * s) / SLOTS + 0.5f * run;
+      if (cost < run) cost = run;
+    }
+    if (s > 1) cost += BESIDE;
+    if (s == 1 || cost < least) { least = cost; best = s; }
+  }
+  return best;
 }
 
 template <typename T>
@@ -437,25 +486,24 @@ static int k8_merge(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows,
     THA_CUDA_OK(launch(kv8_merge_kernel<1, T>, dim3((all + 3) / 4), dim3(128), 0, s, pdl_enabled() != 0, out, partial, *rows, least, most, splits, *a, gate, ldg));
   return THA_STATUS_SUCCESS;
 }
-template <int DT, int FMT, bool MORE, typename T>
-static int k8_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int most_rows, int splits, float* partial,
-                     const float* gate, long long ldg) {
-  auto k = kv8_attn_kernel<DT, FMT, MORE, T>;
+template <int DT, int FMT, bool MORE, bool FULL>
+static int k8_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int most_rows, int splits,
+                     float* partial, const float* gate, long long ldg) {
+  auto k = kv8_attn_kernel<DT, FMT, MORE, FULL>;
   THA_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8Ring<DT>::BYTES));
   const int run = ceil_div(k8_most_tiles(a, rows), splits);
   THA_CUDA_OK(launch(k, dim3((unsigned)k8_pair_tiles(a, rows, most_rows) * splits, a->kv_heads), dim3(K8_THREADS), Kv8Ring<DT>::BYTES, s, pdl_enabled() != 0, *a, *rows, *kv, q,
-                     out, most_rows, splits, run, partial, gate, ldg));
+                     out, (int)(dtype == THA_DT_BF16 && !a->out_f32), most_rows, splits, run, partial, gate, ldg));
   return THA_STATUS_SUCCESS;
 }
-template <int DT, typename T>
-static int k8_form(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int most_rows, int splits, float* partial,
-                   const float* gate, long long ldg) {
-  const bool more = a->softcap > 0.f || a->rel;
-  if (kv->format == THA_KV8_INT8)
-    return more ? k8_launch<DT, THA_KV8_INT8, true>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
-                : k8_launch<DT, THA_KV8_INT8, false>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
-  return more ? k8_launch<DT, THA_KV8_E4M3, true>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
-              : k8_launch<DT, THA_KV8_E4M3, false>(s, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
+template <int DT, int FMT>
+static int k8_form(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int most_rows, int splits,
+                   float* partial, const float* gate, long long ldg) {
+  const bool more = a->softcap > 0.f || a->rel, full = a->dim == DT && a->vdim == DT;
+  if (more) return full ? k8_launch<DT, FMT, true, true>(s, dtype, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
+                        : k8_launch<DT, FMT, true, false>(s, dtype, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
+  return full ? k8_launch<DT, FMT, false, true>(s, dtype, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
+              : k8_launch<DT, FMT, false, false>(s, dtype, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
 }
 // Which sequences take which form: by their own rows alone.  short_rows: up to so many take kv8_attn_kernel; has_short, has_long: whether the step may hold any.
 struct Kv8Forms { int short_rows; bool has_short, has_long; };
@@ -495,8 +543,11 @@ static int k8_attend(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_r
     else if (st != THA_STATUS_SUCCESS) return st;
   }
   const int splits = scratch ? fit(k8_splits(a, rows, short_rows), room) : 1;
-  if (a->dim > 64 || a->vdim > 64) THA_TRY_RC((k8_form<128>(s, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg)));
-  else THA_TRY_RC((k8_form<64>(s, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg)));
+  const bool wide = a->dim > 64 || a->vdim > 64;
+  if (kv->format == THA_KV8_INT8)
+    THA_TRY_RC((wide ? k8_form<128, THA_KV8_INT8> : k8_form<64, THA_KV8_INT8>)(s, dtype, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg));
+  else
+    THA_TRY_RC((wide ? k8_form<128, THA_KV8_E4M3> : k8_form<64, THA_KV8_E4M3>)(s, dtype, a, rows, kv, q, out, short_rows, splits, scratch, gate, ldg));
   return k8_merge(s, a, rows, out, 0, short_rows, splits, scratch, gate, ldg);
 }
 static int k8_check(const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const char* who) {

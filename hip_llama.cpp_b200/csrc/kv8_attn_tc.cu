@@ -70,17 +70,6 @@ __device__ __forceinline__ bool kt_any_of_pair(bool mine, int bar) {
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((unsigned)mine), "r"(bar) : "memory");
   return any != 0;
 }
-__device__ __forceinline__ float kt_max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-__device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 // kind::f16, fp16 x fp16 -> fp32, M = 128; b_mn: the B operand's N runs along its rows
 __device__ __forceinline__ uint32_t kt_idesc(int n, int b_mn) {
   return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -412,9 +401,9 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int y = 0; y < 5; y++)
-            top[5 * i + y] = kt_max3(__uint_as_float(x[16 * i + 3 * y]), __uint_as_float(x[16 * i + 3 * y + 1]), __uint_as_float(x[16 * i + 3 * y + 2]));
-        const float m0 = kt_max3(kt_max3(top[0], top[1], top[2]), fmaxf(top[3], top[4]), __uint_as_float(x[15]));
-        const float m1 = kt_max3(kt_max3(top[5], top[6], top[7]), fmaxf(top[8], top[9]), __uint_as_float(x[31]));
+            top[5 * i + y] = k8_max3(__uint_as_float(x[16 * i + 3 * y]), __uint_as_float(x[16 * i + 3 * y + 1]), __uint_as_float(x[16 * i + 3 * y + 2]));
+        const float m0 = k8_max3(k8_max3(top[0], top[1], top[2]), fmaxf(top[3], top[4]), __uint_as_float(x[15]));
+        const float m1 = k8_max3(k8_max3(top[5], top[6], top[7]), fmaxf(top[8], top[9]), __uint_as_float(x[31]));
         mx = MORE ? fmaxf(m0, m1) : fmaxf(m0 * f0, m1 * f1);
       }
       bool grow = mx > m + KT_SLACK || (m == -INFINITY && mx > -INFINITY);
@@ -452,10 +441,10 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
       for (int i = 0; i < 16; i++) {
         float2 y = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
         const float f = i < 8 ? f0 : f1, vr = i < 8 ? vr0 : vr1;
-        if (MORE) y = kt_add2(y, make_float2(shift, shift));
+        if (MORE) y = k8_add2(y, make_float2(shift, shift));
         else y = f32x2_fma(y, make_float2(f, f), make_float2(shift, shift));
         const float2 p = make_float2(k8_ex2(y.x), k8_ex2(y.y));
-        sum = kt_add2(sum, p);
+        sum = k8_add2(sum, p);
         const float2 z = f32x2_mul(p, make_float2(vr, vr));
         hi[i] = f16x2_of(z);
         if (SPLIT) {
