@@ -38,6 +38,8 @@ Kv8Struct = _struct("tha_kv8_t", [("k_pool v_pool k_scale v_scale k_open v_open 
                                   ("table_stride block_size n_blocks n_cache_layers kv_heads dim vdim format", I)])
 STRUCTS = (RowsStruct, AttnStruct, Kv8Struct)
 
+# the number of the current stream of a device; the public call makes an object around it first, 3.3 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _lib = None
 
 
@@ -112,11 +114,12 @@ class Attention:
         self.device = next((t.device for t in self._keep if t is not None), None)
         if any(t is not None and t.device != self.device for t in self._keep):
             raise ValueError("sink, head_scale and rel are on different devices")
+        vdim = dim if vdim is None else vdim
         at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        self.c = AttnStruct(heads=heads, kv_heads=kv_heads, dim=dim, vdim=dim if vdim is None else vdim, rot=-1, scale=scale, chunk=chunk, window=window,
-                            keep_first=keep_first, sink=at(sink), head_scale=at(head_scale), softcap=softcap, rel=at(rel),
-                            rel_n=0 if rel is None else rel.shape[1], head_gate=int(head_gate), o_g=gate_column)
+        self.c = AttnStruct(heads=heads, kv_heads=kv_heads, dim=dim, vdim=vdim, rot=-1, scale=scale, chunk=chunk, window=window, keep_first=keep_first, sink=at(sink),
+                            head_scale=at(head_scale), softcap=softcap, rel=at(rel), rel_n=0 if rel is None else rel.shape[1], head_gate=int(head_gate), o_g=gate_column)
         self.ref = C.byref(self.c)
+        self.heads, self.q_width, self.out_width, self.layer, self.gate = heads, heads * dim, heads * vdim, 0, gate_column if head_gate else None
 
 
 class Kv8Cache:
@@ -147,7 +150,8 @@ class Kv8Cache:
         at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         self.c = Kv8Struct(at(k_pool), at(v_pool), at(k_scale), at(v_scale), at(k_open), at(v_open), at(table), table.shape[1], size, blocks, layers, heads, dim, vdim,
                            FORMATS[k_pool.dtype])
-        self.ref, self.lib = C.byref(self.c), lib()
+        self.ref, self.lib, self.slots = C.byref(self.c), lib(), table.shape[0]
+        self.calls = self.lib.c
 
     @classmethod
     def empty(cls, *, blocks: int, layers: int, kv_heads: int, block_size: int, dim: int, vdim: int | None = None, slots: int, table_stride: int,
@@ -161,64 +165,74 @@ class Kv8Cache:
     def _stream(self, rows):
         if rows.device != self.device:
             raise ValueError(f"the rows are described on {rows.device}, the cache is on {self.device}")
-        if rows.slots is not None and (rows.slots[0] < 0 or rows.slots[1] >= self.table.shape[0]):
-            raise ValueError(f"slots {rows.slots[0]} .. {rows.slots[1]} of a cache of {self.table.shape[0]}")
+        if rows.slots is not None and (rows.slots[0] < 0 or rows.slots[1] >= self.slots):
+            raise ValueError(f"slots {rows.slots[0]} .. {rows.slots[1]} of a cache of {self.slots}")
         if torch.cuda.current_device() != self.device.index:
             raise ValueError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(self.device.index)
 
-    def _rows(self, name, t, n, width, dtypes):
-        if t.device != self.device or t.dtype not in dtypes or t.dim() != 2 or t.shape[0] != n or t.shape[1] != width or (n and t.stride(1) != 1) or (n > 1 and t.stride(0) < width):
+    def _pitch(self, name, t, n, width, dtypes):
+        """The row pitch of t [n, width], whose columns are neighbours."""
+        s = t.stride()
+        if t.shape != (n, width) or t.dtype not in dtypes or t.device != self.device or (n and s[1] != 1) or (n > 1 and s[0] < width):
             raise ValueError(f"{name}: [{n}, {width}] on {self.device} of {' or '.join(str(d) for d in dtypes)} with neighbouring columns is needed, "
-                             f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-        return t.data_ptr(), t.stride(0) if n > 1 else max(width, t.stride(0))
+                             f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {s}")
+        return s[0] if n > 1 else max(width, s[0])
+
+    def _check(self, status, name):
+        if status:
+            self.lib.check(status, name)
 
     def write(self, rows: Rows, k, v, layer: int = 0) -> None:
         """Rows enter the cache (tha_hyb_kv8_write): k [rows, kv heads * dim], v [rows, kv heads * vdim] in fp32 or bf16, rows any pitch apart."""
         stream = self._stream(rows)
         if rows.slots is not None and not rows.slots[2]:
             raise ValueError("a step writes at most one portion of a slot")
-        kp, ldk = self._rows("k", k, rows.n, self.kw, DTYPES)
-        vp, ldv = self._rows("v", v, rows.n, self.vw, (k.dtype,))
-        self.lib.check(self.lib.c.tha_hyb_kv8_write(stream, DTYPES[k.dtype], rows.ref, self.ref, layer, kp, ldk, vp, ldv), "tha_hyb_kv8_write")
+        kind = k.dtype
+        ldk, ldv = self._pitch("k", k, rows.n, self.kw, DTYPES), self._pitch("v", v, rows.n, self.vw, (kind,))
+        self._check(self.calls.tha_hyb_kv8_write(stream, DTYPES[kind], rows.ref, self.ref, layer, k.data_ptr(), ldk, v.data_ptr(), ldv), "tha_hyb_kv8_write")
 
     def read(self, rows: Rows, layer: int = 0, dtype=torch.float32, k_out=None, v_out=None):
         """The values of cached rows (tha_hyb_kv8_read) as (k, v); into k_out, v_out where given."""
-        stream = self._stream(rows)
+        stream, n, ldk, ldv = self._stream(rows), rows.n, self.kw, self.vw
+        if k_out is not None:
+            ldk, dtype = self._pitch("k_out", k_out, n, ldk, DTYPES), k_out.dtype
+        if v_out is not None:
+            dtype = dtype if k_out is not None else v_out.dtype
+            ldv = self._pitch("v_out", v_out, n, ldv, (dtype,))
+        if dtype not in DTYPES:
+            raise ValueError(f"values are read as float32 or bfloat16, not {dtype}")
         if k_out is None:
-            k_out = torch.empty(rows.n, self.kw, dtype=dtype, device=self.device)
+            k_out = torch.empty((n, ldk), dtype=dtype, device=self.device)
         if v_out is None:
-            v_out = torch.empty(rows.n, self.vw, dtype=dtype, device=self.device)
-        kp, ldk = self._rows("k_out", k_out, rows.n, self.kw, DTYPES)
-        vp, ldv = self._rows("v_out", v_out, rows.n, self.vw, (k_out.dtype,))
-        self.lib.check(self.lib.c.tha_hyb_kv8_read(stream, DTYPES[k_out.dtype], rows.ref, self.ref, layer, kp, ldk, vp, ldv), "tha_hyb_kv8_read")
+            v_out = torch.empty((n, ldv), dtype=dtype, device=self.device)
+        self._check(self.calls.tha_hyb_kv8_read(stream, DTYPES[dtype], rows.ref, self.ref, layer, k_out.data_ptr(), ldk, v_out.data_ptr(), ldv), "tha_hyb_kv8_read")
         return k_out, v_out
 
     def attend(self, attn: Attention, rows: Rows, q, layer: int = 0, dtype=torch.float32, out=None, proj=None):
         """Attention of every row over its visible keys (tha_hyb_kv8_attn): q fp32 [rows, heads * dim] -> [rows, heads * vdim] of `dtype`.  proj: what head_gate reads."""
-        stream = self._stream(rows)
-        a = attn.c
+        stream, n = self._stream(rows), rows.n
         if attn.device is not None and attn.device != self.device:
             raise ValueError(f"the attention's tensors are on {attn.device}, the cache is on {self.device}")
-        if layer != a.cache_layer:
-            a.cache_layer = layer
-        self._rows("q", q, rows.n, a.heads * a.dim, (torch.float32,))
-        if not q.is_contiguous():
-            raise ValueError("q has rows without gaps")
+        if attn.layer != layer:
+            attn.c.cache_layer = attn.layer = layer
+        if q.shape != (n, attn.q_width) or q.dtype != torch.float32 or q.device != self.device or not q.is_contiguous():
+            raise ValueError(f"q: contiguous float32 [{n}, {attn.q_width}] on {self.device} is needed, got {tuple(q.shape)} {q.dtype} on {q.device}, strides {q.stride()}")
         if out is None:
-            out = torch.empty(rows.n, a.heads * a.vdim, dtype=dtype, device=self.device)
-        else:
-            self._rows("out", out, rows.n, a.heads * a.vdim, DTYPES)
-            if not out.is_contiguous():
-                raise ValueError("out has rows without gaps")
+            if dtype not in DTYPES:
+                raise ValueError(f"results are float32 or bfloat16, not {dtype}")
+            out = torch.empty((n, attn.out_width), dtype=dtype, device=self.device)
+        elif out.shape != (n, attn.out_width) or out.dtype not in DTYPES or out.device != self.device or not out.is_contiguous():
+            raise ValueError(f"out: contiguous [{n}, {attn.out_width}] float32 or bfloat16 on {self.device} is needed, got {tuple(out.shape)} {out.dtype} on {out.device}")
         gate, ldg = None, 0
-        if a.head_gate:
-            if proj is None or proj.dim() != 2 or a.o_g < 0 or a.o_g + a.heads > proj.shape[1]:
+        if attn.gate is not None:
+            if proj is None or proj.dim() != 2 or attn.gate < 0 or attn.gate + attn.heads > proj.shape[1]:
                 raise ValueError("head_gate reads its columns from proj [rows, columns]")
-            gate, ldg = self._rows("proj", proj, rows.n, proj.shape[1], (torch.float32,))
-        c = self.lib.c
-        need = c.tha_hyb_kv8_attn_scratch(DTYPES[out.dtype], attn.ref, rows.ref, self.ref)
-        scratch = torch.empty(need, dtype=torch.float32, device=self.device) if need else None
-        self.lib.check(c.tha_hyb_kv8_attn(stream, DTYPES[out.dtype], attn.ref, rows.ref, self.ref, q.data_ptr(), out.data_ptr(), scratch.data_ptr() if need else None, need,
-                                          gate, ldg), "tha_hyb_kv8_attn")
+            gate, ldg = proj.data_ptr(), self._pitch("proj", proj, n, proj.shape[1], (torch.float32,))
+        kind, room = DTYPES[out.dtype], None
+        need = self.calls.tha_hyb_kv8_attn_scratch(kind, attn.ref, rows.ref, self.ref)
+        if need:
+            scratch = torch.empty(need, dtype=torch.float32, device=self.device)
+            room = scratch.data_ptr()
+        self._check(self.calls.tha_hyb_kv8_attn(stream, kind, attn.ref, rows.ref, self.ref, q.data_ptr(), out.data_ptr(), room, need, gate, ldg), "tha_hyb_kv8_attn")
         return out
