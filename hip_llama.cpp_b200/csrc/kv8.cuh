@@ -12,9 +12,11 @@ namespace tha {
 __device__ __forceinline__ size_t kv8_tile(const tha_kv8_t& kv, int block, int layer, int head) {
   return ((size_t)block * kv.n_cache_layers + layer) * kv.kv_heads + head;
 }
+// log2 of a block size
+__device__ __forceinline__ int kv8_shift(int block_size) { return 31 - __clz(block_size); }
 // block id of a slot's position, -1 where the table holds none that exists
 __device__ __forceinline__ int kv8_block(const tha_kv8_t& kv, int slot, int t) {
-  const int b = t / kv.block_size;
+  const int b = t >> kv8_shift(kv.block_size);
   if (t < 0 || b >= kv.table_stride) return -1;
   const int id = kv.table[(size_t)slot * kv.table_stride + b];
   return (unsigned)id < (unsigned)kv.n_blocks ? id : -1;

@@ -3,6 +3,9 @@
 // A code is the format's number nearest to the real quotient x / scale.  The usual way is y = x * (1 / scale), off by 2^-22 of itself at most, and rounding
 // y; only where y is that near to a border between two numbers the quotient itself is asked for, rounded towards zero with its last bit set where it is not exact ("round to
 // odd"), from which a second rounding to fewer bits gives what one rounding of the real quotient gives.
+//
+// Both directions are bound by memory, and are a chain of three or four loads (rows, block ids, values) ahead of it: a block of threads finds its rows once for several heads or rows, and
+// then has all its values on their way at once.
 #include <stdio.h>
 
 #include "kv8.cuh"
@@ -35,18 +38,27 @@ __device__ __forceinline__ float quotient_to_odd(float x, float s) {
   const float y = __fdiv_rz(x, s);
   return fmaf(-y, s, x) != 0.f ? __uint_as_float(__float_as_uint(y) | 1u) : y;
 }
+// odd: a value of the tile is an infinity or NaN
 template <int FMT>
-__device__ __forceinline__ uint32_t kv8_encode4(float4 x, float s, float inv) {
+__device__ __forceinline__ uint32_t kv8_encode4(float4 x, float s, float inv, bool odd) {
   constexpr float MOST = FMT == THA_KV8_INT8 ? 127.f : 448.f;
-  float v[4] = {x.x, x.y, x.z, x.w}, y[4];
-  bool close = false;
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  float y[4];
+  bool close = odd;
+  if (FMT == THA_KV8_INT8) {
+    constexpr float MAGIC = 12582912.f;                     // 1.5 * 2^23: what is added to it is rounded to an integer, which the sum's low bits hold
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    y[i] = v[i] * inv;
-    y[i] = y[i] == y[i] ? fminf(fmaxf(y[i], -MOST), MOST) : 0.f;      // infinities, and NaN
-    if (FMT == THA_KV8_INT8) {
-      close |= fabsf(fabsf(y[i] - rintf(y[i])) - 0.5f) < 1e-4f;        // 127 * 2^-22 = 3e-5
-    } else {
+    for (int i = 0; i < 4; i++) {
+      const float r = fmaf(v[i], inv, MAGIC);
+      close |= fabsf(fmaf(v[i], inv, MAGIC - r)) > 0.4999f; // 127 * 2^-22 = 3e-5
+      w[i] = __float_as_uint(r);
+    }
+    if (!close) return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      y[i] = v[i] * inv;
       // a border is where bit 19 begins what is cut off, from 2^-6 upwards; below, steps are 2^-9 all the way, and few values are there
       const uint32_t b = __float_as_uint(y[i]);
       close |= (fabsf(y[i]) < 0.015625f && y[i] != 0.f) || ((b & 0xFFFFFu) - 0x80000u + 16u) < 33u;
@@ -54,8 +66,10 @@ __device__ __forceinline__ uint32_t kv8_encode4(float4 x, float s, float inv) {
   }
   if (close) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (fabsf(v[i]) < INFINITY && s > 0.f) y[i] = fminf(fmaxf(quotient_to_odd(v[i], s), -MOST), MOST);
+    for (int i = 0; i < 4; i++) {
+      y[i] = fabsf(v[i]) < INFINITY ? (s > 0.f ? quotient_to_odd(v[i], s) : 0.f) : v[i] == v[i] ? (s > 0.f ? copysignf(MOST, v[i]) : 0.f) : 0.f;
+      y[i] = fminf(fmaxf(y[i], -MOST), MOST);
+    }
   }
   if (FMT == THA_KV8_INT8) {
     uint32_t w = 0;
@@ -84,142 +98,221 @@ __device__ __forceinline__ int kv8_units(const tha_rows_t& rows, int s, int bloc
   if (n < 1) return 0;
   const int p0 = rows.pos[first];
   if (p0 < 0) return 0;
-  const int blocks = (p0 + n - 1) / block_size - p0 / block_size + 1;
+  const int sh = kv8_shift(block_size), blocks = ((p0 + n - 1) >> sh) - (p0 >> sh) + 1;
   return blocks > 1 ? blocks - 1 : 1;
 }
 
-// One thread block: a block of the cache, one head, K or V; its rows in registers (N float4 a thread) between the maximum and the codes, so that they are read once.
-// grid (units, kv_heads, 2)
-template <typename T, int FMT, int N, bool VEC>
-__global__ void __launch_bounds__(256) kv8_write_kernel(tha_rows_t rows, tha_kv8_t kv, int layer, const T* k, long long ldk, const T* v, long long ldv) {
+// A warp: 8 rows of a block of the cache, one head, K or V; their values in registers (up to 8 float4 a lane) between the maximum and the codes, so that they are read once.  The
+// block_size / 8 warps of a tile are neighbours and tell each other their maxima.  A thread block takes `each` units in turn, so that what it looks up for the first serves the others.
+// Prompts of 37, 1042 and 2048 rows, 32 heads of 128, fp32: a thread block a tile, with the quotients and positions made value by value, 68 us, like this 47 (behind cold caches;
+// 128 MB are 20).
+// grid (units / each, groups of 16 / (block_size / 8) heads, 2)
+constexpr int KW_WARPS = 16, KW_ROWS = 8;
+// FULL: heads of 128 channels, a row a warp's float4.
+template <typename T, int FMT, bool VEC, bool FULL>
+__global__ void __launch_bounds__(32 * KW_WARPS, 2) kv8_write_kernel(tha_rows_t rows, tha_kv8_t kv, int layer, int each, const T* k, long long ldk, const T* v, long long ldv) {
   hyb_pdl_enter();
   constexpr float MOST = FMT == THA_KV8_INT8 ? 127.f : 448.f;
-  __shared__ float red[33];
-  const int B = kv.block_size, h = blockIdx.y;
-  const bool is_v = blockIdx.z != 0;
-  const int W = is_v ? kv.vdim : kv.dim, w4 = W / 4;
-  int seq = blockIdx.x, unit = 0;
-  if (rows.max_seq_rows > 1) {
-    const Kv8Piece pc = kv8_find(rows.n_seqs, (int)blockIdx.x, [&](int s) { return kv8_units(rows, s, B); });
-    seq = pc.seq; unit = pc.at;
-  }
-  if (seq < 0) return;
-  const int r0 = rows.seq_first[seq], n = rows.seq_first[seq + 1] - r0, slot = rows.seq_slot[seq];
-  const int p0 = n > 0 ? rows.pos[r0] : -1;
-  if (p0 < 0) return;
-  const int p_end = p0 + n, first = p0 / B, last = (p_end - 1) / B;
-  const size_t open_at = kv8_tile(kv, slot, layer, h) * (size_t)B * W;
-  float* open = (is_v ? kv.v_open : kv.k_open) + open_at;
-  const T* src = is_v ? v + (long long)r0 * ldv + (long long)h * W : k + (long long)r0 * ldk + (long long)h * W;
+  constexpr int N = KW_ROWS;                                 // float4 a lane
+  __shared__ float s_top[2][KW_WARPS];                       // two tiles in turn: one barrier a tile
+  __shared__ int s_odd[2][KW_WARPS];
+  const int B = kv.block_size, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sh = kv8_shift(B), per = B / KW_ROWS, part = warp & (per - 1);
+  const int h = (blockIdx.y * KW_WARPS + warp) >> (sh - 3);
+  const bool is_v = blockIdx.z != 0, live = h < kv.kv_heads;
+  static_assert(KW_ROWS == 8, "block_size / 8 warps");
+  const int W = FULL ? 128 : is_v ? kv.vdim : kv.dim, w4 = W >> 2;
   const long long ld = is_v ? ldv : ldk;
   uint8_t* pool = static_cast<uint8_t*>(is_v ? kv.v_pool : kv.k_pool);
   float* scales = is_v ? kv.v_scale : kv.k_scale;
-
-  auto make = [&](int b) {
-    const int id = kv8_block(kv, slot, b * B);
+  // float4 lane + 32 i of the warp's rows: its row and column, one after the other
+  const int in0 = lane / w4, c0 = lane - in0 * w4, rows_on = 32 / w4, c_on = 32 - rows_on * w4;
+  auto next = [&](int& in, int& c) {
+    if (FULL) { in++; return; }
+    in += rows_on; c += c_on;
+    if (c >= w4) { c -= w4; in++; }
+  };
+  int turn = 0;
+  // of the present sequence
+  int p0 = 0, p_end = 0, slot = 0;
+  float* open = nullptr;
+  const T* src = nullptr;
+  auto make = [&](int b) {                                   // the whole thread block: one sequence, one block of positions
+    const int id = kv8_block(kv, slot, b << sh), t0 = (b << sh) + KW_ROWS * part;   // the warp's first position
     float4 x[N];
     float top = 0.f;
+    int in = in0, c = c0;
+    const T* from = src + (long long)(t0 - p0) * ld;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int e = threadIdx.x + i * blockDim.x, row = e / w4, c = 4 * (e - row * w4), t = b * B + row;
+      const int t = t0 + in;
       x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < B && t < p_end) {
-        if (t < p0) x[i] = *reinterpret_cast<const float4*>(open + (size_t)row * W + c);
-        else x[i] = kv8_row4<VEC>(src + (long long)(t - p0) * ld + c);
+      if (live && (FULL || in < KW_ROWS) && t < p_end) {
+        if (t < p0) x[i] = *reinterpret_cast<const float4*>(open + (KW_ROWS * part + in) * W + 4 * c);
+        else x[i] = kv8_row4<VEC>(from + in * ld + 4 * c);
+      }
+      next(in, c);
+    }
+    float2 none = make_float2(0.f, 0.f);                     // 0 times what is finite
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      top = k8_max3(top, k8_max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
+      none = f32x2_fma(make_float2(x[i].x, x[i].y), make_float2(0.f, 0.f), none);
+      none = f32x2_fma(make_float2(x[i].z, x[i].w), make_float2(0.f, 0.f), none);
+    }
+    const bool odd_here = none.x != 0.f || none.y != 0.f;    // true for NaN
+    if (odd_here) {
+      top = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float m[4] = {fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z), fabsf(x[i].w)};
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, m[j] < INFINITY ? m[j] : 0.f);   // false for NaN too
       }
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const float m[4] = {fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z), fabsf(x[i].w)};
-#pragma unroll
-      for (int j = 0; j < 4; j++) top = fmaxf(top, m[j] < INFINITY ? m[j] : 0.f);      // false for NaN too
-    }
-    top = block_max(top, red);
+    top = warp_max(top);
+    bool odd = __any_sync(THA_FULL_MASK, odd_here);
+    if (lane == 0) { s_top[turn][warp] = top; s_odd[turn][warp] = odd; }
+    __syncthreads();                                         // and the open rows of this block have been read
+    for (int i = 0; i < per; i++) { top = fmaxf(top, s_top[turn][warp - part + i]); odd |= s_odd[turn][warp - part + i] != 0; }
+    turn ^= 1;
     const float s = top > 0.f ? fmaxf(__fdiv_rn(top, MOST), 1.17549435e-38f) : 0.f, inv = s > 0.f ? __fdividef(1.0f, s) : 0.f;
-    const bool open_block = (b + 1) * B > p_end;
-    const size_t tile = id >= 0 ? kv8_tile(kv, id, layer, h) : 0;
-    if (id >= 0 && threadIdx.x == 0) scales[tile] = s;
+    const bool open_block = ((b + 1) << sh) > p_end;
+    const size_t tile = id >= 0 && live ? kv8_tile(kv, id, layer, h) : 0;
+    if (id >= 0 && live && part == 0 && lane == 0) scales[tile] = s;
+    uint8_t* codes = pool + (tile * B + KW_ROWS * part) * W;
+    in = in0; c = c0;
+    asm volatile("" : "+r"(in), "+r"(c));                    // counted anew: rows and columns kept from above are registers that the values need
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int e = threadIdx.x + i * blockDim.x, row = e / w4, c = 4 * (e - row * w4), t = b * B + row;
-      if (row >= B) continue;
-      if (id >= 0) *reinterpret_cast<uint32_t*>(pool + tile * (size_t)B * W + (size_t)row * W + c) = kv8_encode4<FMT>(x[i], s, inv);
-      if (open_block && t >= p0 && t < p_end) *reinterpret_cast<float4*>(open + (size_t)row * W + c) = x[i];
+      const int t = t0 + in;
+      if (live && (FULL || in < KW_ROWS)) {
+        if (id >= 0) *reinterpret_cast<uint32_t*>(codes + in * W + 4 * c) = kv8_encode4<FMT>(x[i], s, inv, odd);
+        if (open_block && t >= p0 && t < p_end) *reinterpret_cast<float4*>(open + (KW_ROWS * part + in) * W + 4 * c) = x[i];
+      }
+      next(in, c);
     }
   };
-  make(first + unit);
-  if (unit == 0 && last > first) {
-    __syncthreads();                                       // the open rows of the first block have been read
-    make(last);
+  int seq = -1, unit = 0, units = 0;
+  for (int u = 0; u < each; u++) {
+    const int i = blockIdx.x * each + u;
+    if (seq >= 0 && unit + 1 < units) {
+      unit++;
+    } else {
+      if (rows.max_seq_rows > 1) {
+        const Kv8Piece pc = kv8_find(rows.n_seqs, i, [&](int s) { return kv8_units(rows, s, B); });
+        seq = pc.seq; unit = pc.at;
+      } else {                                               // every sequence is a row: a unit
+        seq = i < rows.n_seqs ? i : -1; unit = 0;
+      }
+      if (seq < 0) return;
+      const int r0 = rows.max_seq_rows > 1 ? rows.seq_first[seq] : seq, n = rows.max_seq_rows > 1 ? rows.seq_first[seq + 1] - r0 : 1;
+      slot = rows.seq_slot[seq];
+      p0 = rows.pos[r0];
+      p_end = p0 + n;
+      units = p0 >= 0 ? ((p_end - 1) >> sh) - (p0 >> sh) : 0;
+      open = (is_v ? kv.v_open : kv.k_open) + (live ? kv8_tile(kv, slot, layer, h) * (size_t)B * W : 0);
+      src = (is_v ? v : k) + (long long)r0 * ld + (live ? (long long)h * W : 0);
+    }
+    if (p0 < 0) continue;
+    make((p0 >> sh) + unit);
+    // The thread block of a sequence's first block also makes its last one, because it reads the slot's open rows (behind make's barrier they have been read) and the last one
+    // replaces them.
+    if (unit == 0 && units > 0) make((p_end - 1) >> sh);
   }
 }
 
 // V codes a thread: 16 bytes of result
 template <typename T> struct Kv8Out;
 template <> struct Kv8Out<float> {
-  static constexpr int V = 4;
+  using Word = uint32_t;
   template <int FMT>
-  static __device__ __forceinline__ void put(float* dst, const uint8_t* src, float s) {
-    const float4 x = kv8_decode4<FMT>(*reinterpret_cast<const uint32_t*>(src));
-    *reinterpret_cast<float4*>(dst) = make_float4(x.x * s, x.y * s, x.z * s, x.w * s);
+  static __device__ __forceinline__ uint4 make(uint32_t w, float s) {
+    const float4 x = kv8_decode4<FMT>(w);
+    return make_uint4(__float_as_uint(x.x * s), __float_as_uint(x.y * s), __float_as_uint(x.z * s), __float_as_uint(x.w * s));
   }
 };
 template <> struct Kv8Out<__nv_bfloat16> {
-  static constexpr int V = 8;
+  using Word = uint2;
   template <int FMT>
-  static __device__ __forceinline__ void put(__nv_bfloat16* dst, const uint8_t* src, float s) {
-    const uint2 w = *reinterpret_cast<const uint2*>(src);
+  static __device__ __forceinline__ uint4 make(uint2 w, float s) {
     const float4 a = kv8_decode4<FMT>(w.x), b = kv8_decode4<FMT>(w.y);
     const __nv_bfloat162 p[4] = {__floats2bfloat162_rn(a.x * s, a.y * s), __floats2bfloat162_rn(a.z * s, a.w * s), __floats2bfloat162_rn(b.x * s, b.y * s),
                                  __floats2bfloat162_rn(b.z * s, b.w * s)};
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(p);
+    return *reinterpret_cast<const uint4*>(p);
   }
 };
 
-// grid (rows, 2): a row's heads, K or V
+// grid (groups of R rows, 2): the rows' heads, K or V.  Eight words of codes of a thread are on their way at once.  8 contexts of 301 .. 2048 rows, 32 heads of 128, bf16: a thread
+// block a row 63 us, 8 rows 42.
+constexpr int KR_ROWS = 8;
 template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(256) kv8_read_kernel(tha_rows_t rows, tha_kv8_t kv, int layer, T* k, long long ldk, T* v, long long ldv) {
+__global__ void __launch_bounds__(256) kv8_read_kernel(tha_rows_t rows, tha_kv8_t kv, int layer, int R, T* k, long long ldk, T* v, long long ldv) {
   hyb_pdl_enter();
-  constexpr int V = Kv8Out<T>::V;
+  using Word = typename Kv8Out<T>::Word;
+  constexpr int V = 16 / (int)sizeof(T), DEEP = 8;
   const bool is_v = blockIdx.y != 0;
   T* out = is_v ? v : k;
   if (!out) return;
-  const int r = blockIdx.x, W = is_v ? kv.vdim : kv.dim, wv = W / V, B = kv.block_size;
-  out += (long long)r * (is_v ? ldv : ldk);
-  const int t = rows.pos[r], slot = rows.seq_slot[rows.row_seq[r]];
-  const int id = t >= 0 ? kv8_block(kv, slot, t) : -1;
-  const size_t tile = id >= 0 ? kv8_tile(kv, id, layer, 0) : 0;
-  const uint8_t* pool = static_cast<const uint8_t*>(is_v ? kv.v_pool : kv.k_pool) + (tile * B + (id >= 0 ? t % B : 0)) * W;
-  const float* scales = (is_v ? kv.v_scale : kv.k_scale) + tile;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < kv.kv_heads * wv; e += blockDim.x) {
-    const int h = e / wv, c = V * (e - h * wv);
-    alignas(16) T x[V] = {};
-    if (id >= 0) Kv8Out<T>::template put<FMT>(x, pool + (size_t)h * B * W + c, scales[h]);
-    T* dst = out + (size_t)h * W + c;
-    if (VEC) {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
-    } else {
+  __shared__ long long s_at[KR_ROWS];                        // of the row's tile of head 0, -1: it has none
+  __shared__ int s_in[KR_ROWS];
+  const int W = is_v ? kv.vdim : kv.dim, wv = W / V, B = kv.block_size, r0 = blockIdx.x * R, here = min(R, rows.n_rows - r0), words = kv.kv_heads * wv;
+  const long long ld = is_v ? ldv : ldk;
+  if (threadIdx.x < here) {
+    const int r = r0 + threadIdx.x, t = rows.pos[r], id = t >= 0 ? kv8_block(kv, rows.seq_slot[rows.row_seq[r]], t) : -1;
+    s_at[threadIdx.x] = id >= 0 ? (long long)kv8_tile(kv, id, layer, 0) : -1;
+    s_in[threadIdx.x] = t >= 0 ? t & (B - 1) : 0;
+  }
+  __syncthreads();
+  const uint8_t* pool = static_cast<const uint8_t*>(is_v ? kv.v_pool : kv.k_pool);
+  const float* scales = is_v ? kv.v_scale : kv.k_scale;
+  // x / wv for x < 2^22: words of a row are below 65536 * 32
+  const unsigned inverse = (unsigned)((0x100000000ull + wv - 1) / (unsigned)wv);
+  int row = threadIdx.x / words, x = threadIdx.x - row * words;   // of the word that is asked for next
+  auto next = [&](int& row, int& x) {
+    for (x += blockDim.x; x >= words; x -= words) row++;
+  };
+  while (row < here) {
+    Word w[DEEP];
+    float s[DEEP];
+    int put_row = row, put_x = x;
 #pragma unroll
-      for (int i = 0; i < V; i++) dst[i] = x[i];
+    for (int i = 0; i < DEEP; i++) {
+      const int h = (int)__umulhi((unsigned)x, inverse), c = V * (x - h * wv);
+      const long long at = row < here ? s_at[row] : -1;
+      w[i] = {};
+      s[i] = 0.f;
+      if (at >= 0) {
+        w[i] = __ldg(reinterpret_cast<const Word*>(pool + (((size_t)at + h) * B + s_in[row]) * W + c));
+        s[i] = __ldg(scales + at + h);
+      }
+      next(row, x);
+    }
+#pragma unroll
+    for (int i = 0; i < DEEP; i++) {
+      if (put_row >= here) break;
+      const uint4 y = Kv8Out<T>::template make<FMT>(w[i], s[i]);
+      T* dst = out + (long long)(r0 + put_row) * ld + V * put_x;   // heads follow one another
+      if (VEC) {
+        *reinterpret_cast<uint4*>(dst) = y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) dst[j] = reinterpret_cast<const T*>(&y)[j];
+      }
+      next(put_row, put_x);
     }
   }
 }
 
 template <typename T, int FMT, bool VEC>
 static int write_launch(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* kv, int layer, const T* k, long long ldk, const T* v, long long ldv) {
-  const int most = kv->block_size * (kv->dim > kv->vdim ? kv->dim : kv->vdim) / 4;       // float4 of a block and head: 64 .. 4096
-  const int threads = most > 1024 ? 256 : 128, per = ceil_div(most, threads);
   const int units = rows->max_seq_rows == 1 ? rows->n_seqs : rows->n_rows / kv->block_size + rows->n_seqs;
-  const dim3 grid(units, kv->kv_heads, 2);
+  const int groups = ceil_div(kv->kv_heads, KW_WARPS * KW_ROWS / kv->block_size);
+  const int each = units * groups >= 4 * 2 * 148 ? 4 : units * groups >= 2 * 2 * 148 ? 2 : 1;   // two rounds of two blocks on every SM, K and V
   auto go = [&](auto kernel) -> int {
-    THA_CUDA_OK(launch(kernel, grid, dim3(threads), 0, s, pdl_enabled() != 0, *rows, *kv, layer, k, ldk, v, ldv));
+    THA_CUDA_OK(launch(kernel, dim3(ceil_div(units, each), groups, 2), dim3(32 * KW_WARPS), 0, s, pdl_enabled() != 0, *rows, *kv, layer, each, k, ldk, v, ldv));
     return THA_STATUS_SUCCESS;
   };
-  if (per <= 2) return go(kv8_write_kernel<T, FMT, 2, VEC>);
-  if (per <= 4) return go(kv8_write_kernel<T, FMT, 4, VEC>);
-  if (per <= 8) return go(kv8_write_kernel<T, FMT, 8, VEC>);
-  return go(kv8_write_kernel<T, FMT, 16, VEC>);
+  return kv->dim == 128 && kv->vdim == 128 ? go(kv8_write_kernel<T, FMT, VEC, true>) : go(kv8_write_kernel<T, FMT, VEC, false>);
 }
 template <typename T>
 static int write_form(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* kv, int layer, const T* k, long long ldk, const T* v, long long ldv) {
@@ -230,11 +323,13 @@ static int write_form(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* k
 }
 template <typename T>
 static int read_form(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* kv, int layer, T* k, long long ldk, T* v, long long ldv) {
-  const bool vec = ((k ? ldk : 0) | (v ? ldv : 0)) % Kv8Out<T>::V == 0 && aligned16(k) && aligned16(v);
-  const int most = kv->kv_heads * (kv->dim > kv->vdim ? kv->dim : kv->vdim) / Kv8Out<T>::V;
-  const dim3 grid(rows->n_rows, 2), block(most > 128 ? 256 : most > 64 ? 128 : 64);
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vec = ((k ? ldk : 0) | (v ? ldv : 0)) % V == 0 && aligned16(k) && aligned16(v);
+  const int R = rows->n_rows > 2 * 148 * KR_ROWS ? KR_ROWS : 1;   // blocks for every SM first: 700 rows of 4 heads 8.1 us one by one, 9.5 in pairs
+  const int words = R * kv->kv_heads * (kv->dim > kv->vdim ? kv->dim : kv->vdim) / V;
+  const dim3 grid(ceil_div(rows->n_rows, R), 2), block(words > 128 ? 256 : words > 64 ? 128 : 64);
   auto go = [&](auto kernel) -> int {
-    THA_CUDA_OK(launch(kernel, grid, block, 0, s, pdl_enabled() != 0, *rows, *kv, layer, k, ldk, v, ldv));
+    THA_CUDA_OK(launch(kernel, grid, block, 0, s, pdl_enabled() != 0, *rows, *kv, layer, R, k, ldk, v, ldv));
     return THA_STATUS_SUCCESS;
   };
   if (kv->format == THA_KV8_INT8) return vec ? go(kv8_read_kernel<T, THA_KV8_INT8, true>) : go(kv8_read_kernel<T, THA_KV8_INT8, false>);
