@@ -11,6 +11,8 @@
 // a lane reads 16 bytes at a time and the eight lanes of a shared-memory phase meet 32 different banks (16-byte pieces of a row are stored at piece ^ (row mod 8)).
 // V's scale belongs to a block of keys, the accumulator to all of them: a weight is multiplied by scale / (largest scale of the run's blocks, rounded up to a
 // power of two) ahead of the split.  Weights have the factor 2^15, so that the 22 bits reach down to 2^-28 of the largest.
+#include <math.h>
+
 #include "kv8.cuh"
 
 namespace tha {
@@ -505,21 +507,38 @@ static int k8_form(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_row
   return full ? k8_launch<DT, FMT, false, true>(s, dtype, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg)
               : k8_launch<DT, FMT, false, false>(s, dtype, a, rows, kv, q, out, most_rows, splits, partial, gate, ldg);
 }
-// Which sequences take which form: by their own rows alone.  short_rows: up to so many take kv8_attn_kernel; has_short, has_long: whether the step may hold any.
+// Which sequences take which form.  short_rows: up to so many rows take kv8_attn_kernel; has_short, has_long: whether the step may hold any.
 struct Kv8Forms { int short_rows; bool has_short, has_long; };
-constexpr int K8_LONG_PAIRS = 128;
-static Kv8Forms k8_forms(const tha_attn_t* a, const tha_rows_t* rows) {
+// The two forms' times, in us, for n_seqs sequences of n rows that see `keys` keys at most, from what both were measured to take.  kv8_attn_kernel: 8, and 0.75 (heads up to 64 channels:
+// 0.44) for a tile of 32 keys of one of 444 blocks, six of them beside its keys.  kv8_attn_tc_kernel: 21, 1.6 for 10000 staged keys of a head, and for a tile of 64 keys of a block on one of 148
+// SMs 0.6 (128 pairs, bf16 results), 2.4 (256 pairs, fp32), with 64 channels 0.48 and 0.81 (128 pairs).  Model / measured, short and long: 32 heads of 128, 128 rows 16 / 16 and 22 / 16,
+// 1024 rows 161 / 150 and 37 / 35, 128 rows behind 4000 keys 125 / 127 and 49 / 58; 16 on 4, 64 rows behind 4000 keys 37 / 38 and 28 / 28; 256 rows 19 / 19 and 22 / 14.
+static bool k8_long_pays(const tha_attn_t* a, const tha_rows_t* rows, int dtype, long long keys, int n) {
   const int gsize = a->heads / a->kv_heads;
-  Kv8Forms f = {gsize > 128 ? 0x7FFFFFFF : ceil_div(K8_LONG_PAIRS, gsize), true, false};
-  if (f.short_rows < 1) f.short_rows = 1;
-  f.has_long = rows->max_seq_rows > f.short_rows;
+  const bool wide = a->dim > 64 || a->vdim > 64, exact = dtype == THA_DT_F32;
+  const float seqs = (float)rows->n_seqs, pairs = (float)n * gsize, seen = keys > n ? (float)keys - 0.5f * n : 0.5f * keys;
+  const float blocks = ceilf(pairs / K8_PAIRS) * a->kv_heads * seqs;
+  const float as_short = 8.f + (wide ? 0.75f : 0.44f) * blocks * (seen / 32.f + 6.f) / 444.f;
+  const float tiles = ceilf(pairs / (wide && exact ? 256.f : 128.f)) * a->kv_heads * seqs * seen / 64.f;
+  const float as_long = 21.f + 1.6e-4f * (wide ? 1.f : 0.5f) * keys * a->kv_heads * seqs + (wide ? (exact ? 2.4f : 0.6f) : (exact ? 0.81f : 0.48f)) * tiles / 148.f;
+  return as_long < as_short;
+}
+static Kv8Forms k8_forms(const tha_attn_t* a, const tha_rows_t* rows, int dtype) {
+  Kv8Forms f = {0x7FFFFFFF, true, false};
+  if (a->heads / a->kv_heads > 128 || rows->max_seq_rows < 2) return f;
+  const long long keys = 32ll * k8_most_tiles(a, rows);
+  for (int n = 2;; n = n + n / 4 + 1) {
+    if (n > rows->max_seq_rows) n = rows->max_seq_rows;
+    if (k8_long_pays(a, rows, dtype, keys, n)) { f.short_rows = n - 1; f.has_long = true; break; }
+    if (n == rows->max_seq_rows) break;
+  }
   f.has_short = !(f.has_long && (long long)rows->n_seqs * rows->max_seq_rows == rows->n_rows);   // all sequences are as long as the longest
   return f;
 }
 template <typename T>
 static int k8_attend(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, float* scratch, size_t room,
                      const float* gate, long long ldg) {
-  const Kv8Forms f = k8_forms(a, rows);
+  const Kv8Forms f = k8_forms(a, rows, dtype);
   const size_t all = (size_t)rows->n_rows * a->heads;
   auto fit = [&](int splits, size_t room) {
     while (splits > 1 && k8_partial_floats(splits, all, a->vdim) > room) splits--;
@@ -570,7 +589,7 @@ using namespace tha;
 
 extern "C" size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv) {
   if (rows->n_rows < 1 || k8_check(a, rows, kv, "tha_hyb_kv8_attn_scratch") != THA_STATUS_SUCCESS) return 0;
-  const Kv8Forms f = k8_forms(a, rows);
+  const Kv8Forms f = k8_forms(a, rows, dtype);
   const size_t all = (size_t)rows->n_rows * a->heads;
   const int most = k8_most_tiles(a, rows);
   const size_t stage = f.has_long ? kv8_attn_tc_stage_bytes(a, rows, most) / sizeof(float) : 0;

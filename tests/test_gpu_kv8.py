@@ -280,33 +280,57 @@ def test_masks_and_options(mask, fmt, heads, kv_heads, dim, vdim, block, parts):
     close(out, want)
 
 
+@pytest.mark.parametrize("mask", MASKS, ids=lambda m: "-".join(f"{k}{'' if v is True else v}" for k, v in m.items()))
+@pytest.mark.parametrize("fmt,heads,kv_heads,dim,vdim,block,dtype", [("int8", 12, 4, 128, 128, 16, torch.float32), ("e4m3", 20, 4, 64, 48, 64, torch.float32),
+                                                                     ("e4m3", 16, 4, 112, 128, 32, torch.bfloat16)])
+def test_masks_and_options_of_prompts(mask, fmt, heads, kv_heads, dim, vdim, block, dtype):
+    parts = [(0, 300, 700), (1, 0, 40)]
+    m = filled(block, kv_heads, dim, vdim, fmt, (1000, 40))
+    rng = np.random.default_rng(3)
+    a = dict(mask, heads=heads, scale=dim ** -0.5)
+    if a.get("sink"):
+        a["sink"] = rng.standard_normal(heads).astype(np.float32)
+    if a.get("head_scale"):
+        a["head_scale"] = rng.uniform(-1.5, 1.5, heads).astype(np.float32)
+    if a.get("rel"):
+        a["rel"] = rng.standard_normal((heads, a["rel"])).astype(np.float32)
+    gate = rng.standard_normal((740, heads)).astype(np.float32) if a.pop("gate", None) else None
+    assert takes_tiles(a, m, parts, dtype) or a.get("window", 10000) < 100 or a.get("chunk", 10000) < 100    # few keys: no tiles pay
+    out, want = attend(m, a, parts, dtype, gate=gate)
+    close(out, want)
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
-@pytest.mark.parametrize("parts", [[(0, 1299, 1)], [(0, 1200, 100)]], ids=["single", "portion"])
+@pytest.mark.parametrize("parts", [[(0, 1299, 1)], [(0, 700, 600)]], ids=["single", "portion"])
 def test_blocks_of_very_different_scales(fmt, parts):
     """Values of blocks 2^20 apart: what is small beside the largest block's is off by less than 2^-28 of a weight times the largest scale's values."""
     m = Mirror(1, 1300, 2, 16, 64, 64, fmt)
     k, v = (torch.from_numpy(m.rng.standard_normal((1300, 128)).astype(np.float32)).cuda() for _ in range(2))
     up = torch.exp2(torch.from_numpy(m.rng.integers(-20, 1, 82).repeat(16)[:1300].astype(np.float32))).cuda()
     m.write([(0, 0, 1300)], k * 0.3, v * up[:, None])
-    out, want = attend(m, dict(heads=4, scale=0.125), parts, torch.float32)
+    assert takes_tiles(dict(heads=32, scale=0.125), m, parts, torch.float32) == (parts[0][2] > 1)
+    out, want = attend(m, dict(heads=32, scale=0.125), parts, torch.float32)
     close(out, want)
     # ... and alone under a window that hides the others
     m.write([(0, 0, 1300)], k * 0.3, v * 2.0 ** -100)
-    out, want = attend(m, dict(heads=4, scale=0.125, window=40), parts, torch.float32)
+    out, want = attend(m, dict(heads=32, scale=0.125, window=140), parts, torch.float32)
     close(out, want)
 
 
-@pytest.mark.parametrize("parts", [[(0, 299, 1)], [(0, 200, 100)]], ids=["single", "portion"])
+@pytest.mark.parametrize("parts", [[(0, 299, 1)], [(0, 200, 100)], [(0, 0, 1600)]], ids=["single", "portion", "prompt"])
 def test_keys_of_zeros_and_scores_far_apart(parts):
     """A cache of zeros gives zeros; scores hundreds apart leave one key."""
-    m = Mirror(1, 300, 1, 16, 64, 64, "int8")
-    z = torch.zeros(300, 64, device="cuda")
-    m.write([(0, 0, 300)], z, z)
-    out, want = attend(m, dict(heads=2, scale=0.125), parts, torch.float32)
+    n = parts[0][1] + parts[0][2]
+    m = Mirror(1, n, 1, 16, 64, 64, "int8")
+    z = torch.zeros(n, 64, device="cuda")
+    m.write([(0, 0, n)], z, z)
+    a = dict(heads=8, scale=0.125)
+    assert takes_tiles(a, m, parts, torch.float32) == (n == 1600)
+    out, want = attend(m, a, parts, torch.float32)
     assert bool((out == 0).all())
-    k, v = (torch.from_numpy(m.rng.standard_normal((300, 64)).astype(np.float32)).cuda() for _ in range(2))
-    m.write([(0, 0, 300)], k, v)
-    out, want = attend(m, dict(heads=2, scale=0.125), parts, torch.float32, scale_q=200.0)
+    k, v = (torch.from_numpy(m.rng.standard_normal((n, 64)).astype(np.float32)).cuda() for _ in range(2))
+    m.write([(0, 0, n)], k, v)
+    out, want = attend(m, a, parts, torch.float32, scale_q=200.0)
     # scores of order 200 * 8 / 8: errors 200 times those of the head comment
     close(out, want, 200 * F32_TOL)
 
@@ -321,21 +345,32 @@ def test_a_query_that_is_not_a_number():
 
 
 def test_a_query_of_a_portion_that_is_not_a_number():
-    m = filled(32, 2, 128, 128, "int8", (700,))
-    q = torch.randn(300, 512, device="cuda")
+    m = filled(32, 4, 128, 128, "int8", (900,))
+    q = torch.randn(500, 16 * 128, device="cuda")
     q[123, 130] = float("nan")
     q[7, 400] = float("inf")
     for dtype in (torch.float32, torch.bfloat16):
-        out = m.cache.attend(K.Attention(4, 2, 128, scale=0.1), K.Rows.of([(0, 400, 300)]), q, layer=LAYER, dtype=dtype).view(300, 4, 128)
-        bad = torch.zeros(300, 4, dtype=torch.bool, device="cuda")
+        assert takes_tiles(dict(heads=16, scale=0.1), m, [(0, 400, 500)], dtype)
+        out = m.cache.attend(K.Attention(16, 4, 128, scale=0.1), K.Rows.of([(0, 400, 500)]), q, layer=LAYER, dtype=dtype).view(500, 16, 128)
+        bad = torch.zeros(500, 16, dtype=torch.bool, device="cuda")
         bad[123, 1] = bad[7, 3] = True
         assert bool((~torch.isfinite(out)).all(-1)[bad].all()) and bool(torch.isfinite(out)[~bad].all())
 
 
-LONG = [("int8", 16, 8, 2, 128, 128, [(0, 1500, 300)], {}), ("e4m3", 64, 4, 1, 128, 128, [(0, 3000, 150)], dict(window=1000, keep_first=40)),
-        ("int8", 16, 4, 4, 64, 64, [(0, 100, 129), (1, 0, 128), (2, 2000, 400)], {}), ("int8", 32, 5, 1, 96, 80, [(0, 900, 260), (1, 17, 3), (2, 3, 1), (3, 40, 90)], dict(sink=True)),
-        ("e4m3", 128, 16, 1, 128, 64, [(0, 2500, 77), (1, 30, 60)], dict(chunk=700)), ("int8", 16, 3, 1, 16, 128, [(0, 0, 600)], dict(softcap=5.0)),
-        ("e4m3", 16, 6, 2, 112, 48, [(0, 1000, 200)], dict(rel=300)), ("int8", 16, 2, 2, 128, 128, [(i, 7 * i, 130 + i % 3) for i in range(40)], {})]
+def takes_tiles(a, m, parts, dtype):
+    """Whether the step's portions go to the tensor-core form of prompts: it stages the visible keys and values in fp16, which is most of the scratch that it asks for."""
+    lib, r = K.lib(), K.Rows.of(parts)
+    at = K.Attention(a["heads"], m.H, m.dim, m.vdim, scale=a["scale"], chunk=a.get("chunk", 0), window=a.get("window", 0), keep_first=a.get("keep_first", 0))
+    floats = lib.c.tha_hyb_kv8_attn_scratch(K.DTYPES[dtype], at.ref, r.ref, m.cache.ref)
+    keys = min(max(p + n for _, p, n in parts), a.get("window") or 1 << 30, a.get("chunk") or 1 << 30)
+    return floats >= keys * m.H * (128 if max(m.dim, m.vdim) > 64 else 64)
+
+
+LONG = [("int8", 16, 16, 4, 128, 128, [(0, 1500, 300)], {}), ("e4m3", 64, 16, 4, 128, 128, [(0, 3000, 250)], dict(window=1000, keep_first=40)),
+        ("int8", 16, 8, 8, 64, 64, [(0, 100, 450), (1, 0, 520), (2, 2000, 400)], {}), ("int8", 32, 20, 4, 96, 80, [(0, 900, 460), (1, 17, 3), (2, 3, 1), (3, 40, 90)], dict(sink=True)),
+        ("e4m3", 128, 32, 2, 128, 64, [(0, 2500, 177), (1, 30, 60)], dict(chunk=700)), ("int8", 16, 12, 4, 16, 128, [(0, 0, 900)], dict(softcap=5.0)),
+        ("e4m3", 16, 12, 4, 112, 48, [(0, 1000, 500)], dict(rel=300)), ("int8", 16, 4, 4, 128, 128, [(i, 7 * i, 230 + i % 3) for i in range(40)], {}),
+        ("e4m3", 32, 128, 1, 64, 16, [(0, 2000, 300)], {}), ("int8", 64, 5, 5, 48, 64, [(0, 0, 1300), (1, -1, 1)], dict(window=300))]
 
 
 @pytest.mark.parametrize("case", LONG, ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{c[4]}-{c[5]}-{len(c[6])}")
@@ -344,13 +379,14 @@ LONG = [("int8", 16, 8, 2, 128, 128, [(0, 1500, 300)], {}), ("e4m3", 64, 4, 1, 1
 def test_prompt_portions(case, dtype, lead):
     """Portions for the tensor-core form, behind contexts that are cut and beside short ones; with lead 1 the result is on no 16-byte boundary."""
     fmt, block, heads, kv_heads, dim, vdim, parts, mask = case
-    m = filled(block, kv_heads, dim, vdim, fmt, [p + n for _, p, n in parts])
+    m = filled(block, kv_heads, dim, vdim, fmt, [max(1, p + n) for _, p, n in parts])
     rng = np.random.default_rng(3)
     a = dict(mask, heads=heads, scale=dim ** -0.5)
     if a.get("sink"):
         a["sink"] = rng.standard_normal(heads).astype(np.float32)
     if a.get("rel"):
         a["rel"] = rng.standard_normal((heads, a["rel"])).astype(np.float32)
+    assert takes_tiles(a, m, parts, dtype)
     out, want = attend(m, a, parts, dtype)
     close(out, want)
     if lead:
@@ -364,25 +400,28 @@ def test_prompt_portions(case, dtype, lead):
         assert float(room[0]) == 9.0
 
 
-def test_blocks_that_do_not_exist_under_a_portion():
-    m = filled(16, 2, 128, 128, "int8", (900,))
+@pytest.mark.parametrize("rows", [30, 600])
+def test_blocks_that_do_not_exist_under_a_portion(rows):
+    m = filled(16, 4, 128, 128, "int8", (900,))
     bad = m.cache.table.clone()
     for b in (0, 9, 30, 50):
         bad[0, b] = -7 if b & 1 else m.cache.k_pool.shape[0]
     m.cache.table.copy_(bad)
-    q = torch.randn(400, 512, device="cuda")
-    out = m.cache.attend(K.Attention(4, 2, 128, scale=0.1), K.Rows.of([(0, 500, 400)]), q, layer=LAYER)
+    q, p0 = torch.randn(rows, 16 * 128, device="cuda"), 900 - rows
+    assert takes_tiles(dict(heads=16, scale=0.1), m, [(0, p0, rows)], torch.float32) == (rows == 600)
+    out = m.cache.attend(K.Attention(16, 4, 128, scale=0.1), K.Rows.of([(0, p0, rows)]), q, layer=LAYER)
     absent = np.isin(np.arange(900) // 16, (0, 9, 30, 50))
-    want = O.attend(dict(scale=0.1), q.double().cpu().numpy().reshape(400, 4, 128), m.values("k", 0, 900), m.values("v", 0, 900), 500, absent)
-    assert rel(out, want.reshape(400, -1)) < F32_TOL
+    want = O.attend(dict(scale=0.1), q.double().cpu().numpy().reshape(rows, 16, 128), m.values("k", 0, 900), m.values("v", 0, 900), p0, absent)
+    assert rel(out, want.reshape(rows, -1)) < F32_TOL
 
 
 @pytest.mark.parametrize("share", [0.0, 0.01, 0.5, 0.95, 0.99, 1.0, 1.5])
-@pytest.mark.parametrize("parts", [[(0, 3900, 100)], [(0, 3900, 100), (1, 20, 90), (1, 30, 1), (0, 1000, 70)]], ids=["one", "four"])
+@pytest.mark.parametrize("parts", [[(0, 3700, 300)], [(0, 3700, 300), (1, 20, 90), (1, 30, 1), (0, 1000, 270)]], ids=["one", "four"])
 def test_parts_of_a_portions_context_meet(share, parts):
     """With less room than the call would like, and nothing behind the room."""
     m = filled(16, 1, 128, 128, "int8", (4000, 111))
-    heads, n = 2, sum(x[2] for x in parts)
+    heads, n = 8, sum(x[2] for x in parts)
+    assert takes_tiles(dict(heads=heads, scale=128 ** -0.5), m, parts, torch.float32)
     out, want = attend(m, dict(heads=heads, scale=128 ** -0.5), parts, torch.float32)
     close(out, want)
     r, at, lib = K.Rows.of(parts), K.Attention(heads, 1, 128, scale=128 ** -0.5), K.lib()
@@ -443,9 +482,10 @@ def test_a_very_long_context():
     out.fill_(float("nan"))
     lib.check(lib.c.tha_hyb_kv8_attn(torch.cuda.current_stream().cuda_stream, 1, at.ref, r.ref, big.ref, q.data_ptr(), out.data_ptr(), None, 0, None, 0))
     assert rel(out, want.cpu().numpy()) < F32_TOL
-    # a portion, its parts and without
+    # a portion, with tiles and parts, and without
     q = torch.randn(130, 2 * D, device="cuda")
     r = K.Rows.of([(0, n - 130, 130)])
+    assert lib.c.tha_hyb_kv8_attn_scratch(1, at.ref, r.ref, big.ref) > n * 2 * 128
     hidden = torch.arange(n, device="cuda")[None] > torch.arange(n - 130, n, device="cuda")[:, None]
     s = torch.einsum("rhd,thd->hrt", q.double().view(130, 2, D), kb.double().view(n, 2, D)) * D ** -0.5
     want = torch.einsum("hrt,the->rhe", torch.softmax(s.masked_fill(hidden, float("-inf")), -1), vb.double().view(n, 2, D)).reshape(130, -1).cpu().numpy()
