@@ -11,6 +11,10 @@
 // a lane reads 16 bytes at a time and the eight lanes of a shared-memory phase meet 32 different banks (16-byte pieces of a row are stored at piece ^ (row mod 8)).
 // V's scale belongs to a block of keys, the accumulator to all of them: a weight is multiplied by scale / (largest scale of the run's blocks, rounded up to a
 // power of two) ahead of the split.  Weights have the factor 2^15, so that the 22 bits reach down to 2^-28 of the largest.
+//
+// Bound: the cache's bytes where nothing else is; here the instructions that turn them into fp16 pairs (int8: five for four codes of K, six of V) and the chain of a tile, which
+// three blocks on an SM (168 registers, a ring of two tiles a warp) hide better than two (217 registers, three tiles: 168 us where these take 146).  One context of 131072 keys, 8
+// heads of 128: 63 us, 4.2 of 6.55 TB/s; 64 contexts of 3 to 2047 keys, 32 heads: 125 us, 4.3 TB/s; 16 of 501 to 8190, 8 heads, e4m3: 50 us, 2.9 TB/s (the longest are the tail).
 #include <math.h>
 
 #include "kv8.cuh"
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
 #pragma unroll
         for (int i = 0; i < DT / 32; i++) {                 // rows lane_r, lane_r + STEP, ..: the piece's place turns with the row
           constexpr int STEP = 512 / DT;
-          const int turn = DT == 128 ? (i & 1) * 64 : (i & 1) * 0;
+          const int turn = DT == 128 ? (i & 1) * 64 : 0;
           const uint32_t to = dst + (16 * hf + STEP * i) * DT + (lane_to ^ turn);
           if (FULL || k_there) k8_copy16(to, ks + STEP * i * D, there);
           if (FULL || v_there) k8_copy16(to + Ring::TILE, vs + STEP * i * E, there);
@@ -462,6 +466,10 @@ static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows)
   constexpr float BESIDE = 6.f;
   const int most = k8_most_tiles(a, rows);
   const long long blocks = (long long)k8_pair_tiles(a, rows, most_rows) * a->kv_heads;
+  // kv8_merge_kernel passes every row of the step: 2700 (row, head) a tile's time.  Rows of longer sequences, which it leaves as they are, count here: two prompts of 777 and 2048
+  // rows, 32 heads, whose step may hold short portions but does not, took 115 us with such a pass and take 91 without.
+  const long long rows_short = (long long)rows->n_seqs * (most_rows < rows->max_seq_rows ? most_rows : rows->max_seq_rows);
+  const float passed = rows->n_rows > rows_short ? (float)(rows->n_rows - rows_short) * a->heads / 2700.f : 0.f;
   int best = 1;
   float least = 0.f;
   for (int s = 1; s <= K8_MAX_SPLITS && (s == 1 || s * 4 <= most); s++) {   // a tile for each warp at least
@@ -473,7 +481,7 @@ static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows)
       cost = (float)blocks * (0.5f * most + BESIDE * s) / SLOTS + 0.5f * run;
       if (cost < run) cost = run;
     }
-    if (s > 1) cost += BESIDE;
+    if (s > 1) cost += BESIDE + passed;
     if (s == 1 || cost < least) { least = cost; best = s; }
   }
   return best;

@@ -120,6 +120,16 @@ def test_attention_that_is_refused(bad, code):
     assert f.tha_hyb_kv8_attn_scratch(1, attn(**bad), rows(), cache()) == 0
 
 
+def test_a_step_of_prompts_is_not_cut_for_the_short_portions_it_might_hold():
+    """Room for the visible keys as fp16 and nothing for partial results: a step of prompts would pass all of its rows once more."""
+    big = dict(kv_heads=32, dim=128, vdim=128)
+    r, c = rows(n_rows=2825, max_seq_rows=2048, max_pos=2047), cache(**big, table_stride=128, n_blocks=257)
+    a = attn(heads=32, **big)
+    parts = 2 * (2048 // 32 + 2)                                  # of 32 keys, K and V, fp16; one more percent for their scales
+    need = 4 * K.lib().c.tha_hyb_kv8_attn_scratch(1, a, r, c)
+    assert 2 * 2048 * 32 * 2 * 128 * 2 <= need <= parts * 32 * 32 * 2 * 128 * 2 * 1.01
+
+
 def test_no_rows_are_no_work():
     f, r = K.lib().c, rows(n_rows=0)
     assert f.tha_hyb_kv8_write(None, 1, r, cache(), 0, A, 128, A, 128) == 0
