@@ -1,5 +1,5 @@
-// Softmax attention of prompt portions over the cache in 8 bits on the 5th-generation tensor cores (tcgen05 + TMEM): sequences whose (position, head) pairs fill
-// tiles of 256.  kv8_attn.cu keeps single rows and short portions.
+// Softmax attention of prompt portions over the cache in 8 bits on the 5th-generation tensor cores (tcgen05 + TMEM).  kv8_attn.cu keeps single rows and the portions that take longer
+// here (k8_long_pays).
 //
 // Codes are fp16 numbers.  A step's visible keys and values are turned into fp16 once (kv8_stage_kernel), without scales, into scratch that holds tiles as they will lie in shared
 // memory, from where bulk copies fetch them: warps of the block that did it themselves, tile by tile and again for every 256 rows, took half of the SM's issue slots (8000
@@ -16,6 +16,10 @@
 // The accumulator stays in TMEM.  The tensor cores cut off what their fp32 sums cannot hold, so that an error grows with the number of sums: 100 rows behind 3900 keys were 8.6e-6
 // off with two fp16 an operand.  SPLIT therefore adds the accumulators of runs of 8 tiles (64 sums) in fp32, in local memory.  It is rescaled only where a row's maximum has grown
 // by more than 2^8 since its reference was taken (weights are at most 2^15 then: fp16 holds them), or V's scales outgrow theirs.
+//
+// Bound: the tensor cores' shared-memory operand and the softmax together, 2100 cycles for 256 rows of a tile where the products alone are 1320 (a score product of 128 x 64 x 16 reads 6 KB of
+// shared memory in 50 cycles, one of weights x values takes 65).  Two bf16 prompts of 777 and 2048 rows, 32 heads of 128: 91 us with 10 to 20 of staging, 430 TFLOP/s of the visible
+// pairs; one fp32 prompt of 1024 (twice the products): 58 us.
 #include "gemm_tc.h"
 #include "kv8.cuh"
 #include "tc_common.cuh"
@@ -29,7 +33,7 @@ __host__ __device__ constexpr int kt_groups(bool split, int DT) { return split &
 __host__ __device__ constexpr int kt_threads(bool split, int DT) { return 32 * (9 * kt_groups(split, DT) + 1); }
 constexpr float KT_UP = 7.0f, KT_SLACK = 8.0f;
 constexpr int KT_RUN = 8;      // SPLIT: tiles that one accumulator sums
-constexpr long long KT_MOST_STAGED = 1ll << 30;
+constexpr long long KT_MOST_STAGED = 1ll << 30;   // bytes of scratch beyond which a step takes the form that needs none
 constexpr int KT_SCALES = 8;   // tiles whose scales are kept: K of tile j + 8 comes into a ring of four behind the scores of tile j + 4, those behind the weights of tile j + 2
 // Staged keys: 32 at a time (a part), per part and head [K, V][64 channels][key][128 bytes swizzled] and the scales of its two 16 keys: (K, K, V, V), K's below 0: they do not exist
 __host__ __device__ constexpr int kt_part(int DT) { return 2 * 32 * DT * 2; }
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         float corr = 1.f;
         if (grow) { corr = m > -INFINITY ? k8_ex2(m - mx) : 0.f; m = mx; shift = KT_UP - m; }
         l *= corr;
-        if (wider) {                                  // the next power of two and a factor of 4 more, so that this is rare
+        if (wider) {                                  // the next power of two and a factor of 4 more, so that this is rare; lo ends at 2^-25 / 2^7 ref, below 2^-29 of the scale
           const float to = __uint_as_float(min(((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u) + 0x1000000u, 0x7E800000u));
           corr *= ref / to;
           ref = to;

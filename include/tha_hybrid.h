@@ -637,7 +637,8 @@ int tha_hyb_hgrn_scan(void* stream, int dtype, const tha_hgrn_t* g, const tha_ro
  * the largest code of their sign, NaN gets 0: the cache holds finite numbers only.  Rows of a slot's last block, while it is not full, are also kept
  * in fp32 (k_open, v_open), and its codes are made anew whenever rows join it: a code is one rounding of its value under the scale of all rows that are
  * there, however the rows were cut into calls.
- * The table's ids are checked on the device: a block whose id is not below n_blocks is not written, reads as zeros, and its keys are not seen. */
+ * What fills the pools in another way than by tha_hyb_kv8_write writes whole blocks, and no e4m3 code of NaN.  The table's ids are checked on the
+ * device: a block whose id is not below n_blocks is not written, reads as zeros, and its keys are not seen. */
 typedef struct {
   void* k_pool;         /* codes [block][cache layer][kv head][position in block][dim] */
   void* v_pool;         /* codes [block][cache layer][kv head][position in block][vdim] */
@@ -666,9 +667,9 @@ int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_
 /* tha_hyb_attn_gated over such a cache: every row attends to the visible keys as the cache holds them, which for rows of a block that is not full are their codes
  * under its present scale.  a: heads, kv_heads, dim, vdim, scale, chunk, cache_layer, window, keep_first, sink, head_scale, softcap, rel, head_gate and out_f32 as there
  * (values_in_keys, v_share and diff are refused); q fp32 [n_rows, heads * dim]; out dtype-typed [n_rows, heads * vdim].  Idle rows get zeros.
- * Codes are exact in fp16; q and the weights enter the products as two fp16: q with 22 bits of each value, or 2^-28 of the largest of its row of a head; a weight times its value's
- * scale with 22 bits, or 2^-32 of the largest of the row (2^-34 where V's scales differ).  Rows of longer portions with dtype THA_DT_BF16 use one fp16 of 11 bits instead.  Sums and softmax are
- * fp32.
+ * Codes are exact in fp16; q and the weights, each times its value's scale, enter the products as two fp16.  A number of q is off by 2^-22 of itself or 2^-39 of the largest
+ * of its row of a head, whichever is more; a weight by 2^-22 of itself or 2^-29 of the row's largest weight times the largest scale.  Rows of longer portions with dtype
+ * THA_DT_BF16 use one fp16: 2^-11 of itself instead of 2^-22.  Sums and softmax are fp32.  Which portions are long goes by the step: heads, keys, rows.
  * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones, and for
  * partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may
  * run at the same time need scratch of their own. */

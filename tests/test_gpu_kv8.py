@@ -533,6 +533,16 @@ def test_other_streams_and_graphs():
             assert bool((got[0] == want[0]).all()) and all(bool((a == b).all()) for a, b in zip(got[1], want[1]))
 
 
+def test_a_step_of_idle_slots():
+    m = filled(16, 2, 64, 64, "int8", (30, 30))
+    before = m.cache.k_pool.clone()
+    r = K.Rows.of([(1, -1, 1), (0, -1, 1)])
+    m.cache.write(r, torch.ones(2, 128, device="cuda"), torch.ones(2, 128, device="cuda"), layer=LAYER)
+    k, v = m.cache.read(r, layer=LAYER)
+    out = m.cache.attend(K.Attention(4, 2, 64, scale=0.125, sink=torch.zeros(4, device="cuda")), r, torch.randn(2, 256, device="cuda"), layer=LAYER)
+    assert bool((m.cache.k_pool == before).all()) and bool((k == 0).all()) and bool((v == 0).all()) and bool((out == 0).all())
+
+
 def test_calls_side_by_side():
     """Attention of two steps on two streams at once over one cache."""
     m = filled(16, 2, 128, 128, "int8", (3000, 2900))
