@@ -533,6 +533,27 @@ def test_other_streams_and_graphs():
             assert bool((got[0] == want[0]).all()) and all(bool((a == b).all()) for a, b in zip(got[1], want[1]))
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("parts", [[(0, 110, 1), (1, 120, 1)], [(1, 100, 21), (0, 111, 1)], [(0, 96, 16), (1, 96, 25)]], ids=["single", "mixed", "portions"])
+def test_full_blocks_of_two_slots(fmt, parts):
+    """Two slots share a prefix of full blocks: each writes behind it, the prefix keeps its bytes, and both attend over it."""
+    m = Mirror(2, 160, 2, 16, 64, 64, fmt)
+    m.put([(0, 0, 96)])
+    m.table[1, :6] = m.table[0, :6]
+    m.cache.table.copy_(torch.from_numpy(m.table))
+    ids = torch.from_numpy(m.table[0, :6].astype(np.int64)).cuda()
+    before = [t.view(torch.int8)[ids].clone() for t in (m.cache.k_pool, m.cache.v_pool)] + [t[ids].clone() for t in (m.cache.k_scale, m.cache.v_scale)]
+    for slot in (0, 1):
+        m.rows[slot] = {side: m.rows[0][side][:96] for side in "kv"}
+    m.put([(0, 96, 16), (1, 96, 25)])
+    m.check()
+    for was, t in zip(before, (m.cache.k_pool.view(torch.int8), m.cache.v_pool.view(torch.int8), m.cache.k_scale, m.cache.v_scale)):
+        assert torch.equal(was, t[ids])
+    for dtype in (torch.float32, torch.bfloat16):
+        out, want = attend(m, dict(heads=8, scale=0.125), parts, dtype)
+        close(out, want)
+
+
 def test_a_step_of_idle_slots():
     m = filled(16, 2, 64, 64, "int8", (30, 30))
     before = m.cache.k_pool.clone()
