@@ -119,7 +119,17 @@ class Attention:
         self.c = AttnStruct(heads=heads, kv_heads=kv_heads, dim=dim, vdim=vdim, rot=-1, scale=scale, chunk=chunk, window=window, keep_first=keep_first, sink=at(sink),
                             head_scale=at(head_scale), softcap=softcap, rel=at(rel), rel_n=0 if rel is None else rel.shape[1], head_gate=int(head_gate), o_g=gate_column)
         self.ref = C.byref(self.c)
-        self.heads, self.q_width, self.out_width, self.layer, self.gate = heads, heads * dim, heads * vdim, 0, gate_column if head_gate else None
+        self.heads, self.q_width, self.out_width, self.gate = heads, heads * dim, heads * vdim, gate_column if head_gate else None
+        self._of = {}
+
+    def of(self, layer: int):
+        """The struct with this cache layer in it: one for each layer, written before anyone sees it, because other threads may be in calls with theirs."""
+        at = self._of.get(layer)
+        if at is None:
+            c = AttnStruct.from_buffer_copy(self.c)
+            c.cache_layer = layer
+            at = self._of.setdefault(layer, C.byref(c))         # a reference keeps its struct
+        return at
 
 
 class Kv8Cache:
@@ -214,8 +224,7 @@ class Kv8Cache:
         stream, n = self._stream(rows), rows.n
         if attn.device is not None and attn.device != self.device:
             raise ValueError(f"the attention's tensors are on {attn.device}, the cache is on {self.device}")
-        if attn.layer != layer:
-            attn.c.cache_layer = attn.layer = layer
+        of = attn.of(layer)
         if q.shape != (n, attn.q_width) or q.dtype != torch.float32 or q.device != self.device or not q.is_contiguous():
             raise ValueError(f"q: contiguous float32 [{n}, {attn.q_width}] on {self.device} is needed, got {tuple(q.shape)} {q.dtype} on {q.device}, strides {q.stride()}")
         if out is None:
@@ -230,9 +239,9 @@ class Kv8Cache:
                 raise ValueError("head_gate reads its columns from proj [rows, columns]")
             gate, ldg = proj.data_ptr(), self._pitch("proj", proj, n, proj.shape[1], (torch.float32,))
         kind, room = DTYPES[out.dtype], None
-        need = self.calls.tha_hyb_kv8_attn_scratch(kind, attn.ref, rows.ref, self.ref)
+        need = self.calls.tha_hyb_kv8_attn_scratch(kind, of, rows.ref, self.ref)
         if need:
             scratch = torch.empty(need, dtype=torch.float32, device=self.device)
             room = scratch.data_ptr()
-        self._check(self.calls.tha_hyb_kv8_attn(stream, kind, attn.ref, rows.ref, self.ref, q.data_ptr(), out.data_ptr(), room, need, gate, ldg), "tha_hyb_kv8_attn")
+        self._check(self.calls.tha_hyb_kv8_attn(stream, kind, of, rows.ref, self.ref, q.data_ptr(), out.data_ptr(), room, need, gate, ldg), "tha_hyb_kv8_attn")
         return out

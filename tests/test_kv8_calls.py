@@ -1,0 +1,50 @@
+"""What the binding of the cache in 8 bits hands to the library, with a recorder in the library's place: no GPU."""
+import threading
+import types
+
+import pytest
+import torch
+
+from pkgload import load_pkg
+
+K = load_pkg("kv8")
+
+
+def recorded(monkeypatch, **calls):
+    """A cache on the CPU whose calls go to `calls`."""
+    cache = K.Kv8Cache.empty(blocks=4, layers=3, kv_heads=2, block_size=16, dim=32, slots=2, table_stride=2, device="cpu")
+    monkeypatch.setattr(cache, "_stream", lambda rows: 0)
+    cache.calls = types.SimpleNamespace(**calls)
+    return cache
+
+
+@pytest.mark.parametrize("layers", [(0, 1), (2, 0), (1, 1)])
+def test_threads_share_an_attention(monkeypatch, layers):
+    """The library lets go of the interpreter in every call: both threads are in their first call before either makes its second."""
+    both, seen = threading.Barrier(2, timeout=30), {}
+
+    def scratch(kind, a, rows, kv):
+        both.wait()
+        seen.setdefault(threading.get_ident(), []).append(a._obj.cache_layer)
+        return 0
+
+    def attn(stream, kind, a, rows, kv, *rest):
+        both.wait()
+        seen[threading.get_ident()].append(a._obj.cache_layer)
+        return 0
+
+    cache = recorded(monkeypatch, tha_hyb_kv8_attn_scratch=scratch, tha_hyb_kv8_attn=attn)
+    at, rows, q = K.Attention(4, 2, 32, scale=1.0), K.Rows.of([(0, 0, 1)], "cpu"), torch.zeros(1, 128)
+    want = {}
+
+    def work(layer):
+        want[threading.get_ident()] = [layer] * 6
+        for _ in range(3):
+            cache.attend(at, rows, q, layer=layer)
+
+    threads = [threading.Thread(target=work, args=(layer,)) for layer in layers]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert seen == want
