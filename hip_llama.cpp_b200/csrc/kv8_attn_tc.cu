@@ -5,7 +5,8 @@
 // memory, from where bulk copies fetch them: warps of the block that did it themselves, tile by tile and again for every 256 rows, took half of the SM's issue slots (8000
 // instructions of 32 lanes a tile instead of 3500).  K's scale belongs to 16 or more neighbouring keys and multiplies their scores, V's multiplies their weights, relative to a power of two
 // that all of a row's weights share.  q is brought to [2^14, 2^15) by a power of two a row and rounded to one fp16 (bf16 results) or two (SPLIT: fp32 results, 22 bits; weights
-// likewise), each product fp32.
+// likewise), each product fp32.  A row's power of two is that of the scales that it sees itself: with one for the block's rows, a row lost as many bits as the scale of a block
+// hidden from it was larger.
 // A block takes 128 pairs of one key/value head (with two fp16 an operand and heads beyond 64 channels 256, two groups of 128 that share every tile) and a run of tiles of 64 keys.
 // Ten warps (nineteen):
 //   0 .. 7 (.. 15)   softmax of a group, a row for two threads of 32 keys each: scores out of TMEM, factor, mask, weights back into the same TMEM columns as the A operand of the
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
       kt_any_of_pair(false, pair_bar);
       if (!hv) { mine = join(mine, s_row[pr]); s_row[pr] = mine; }
       kt_any_of_pair(false, pair_bar);
-      return s_row[pr];                               // nothing writes it ahead of the pair's next barrier
+      return hv ? s_row[pr] : mine;                   // who joins reads it behind a barrier only, so that the other may write the next number at once
     };
     kt_any_of_pair(false, pair_bar);                  // both have read their factor
     for (int jl = 0; jl < n; jl++) {                  // to the end even where a wait has given up: the two warps meet at their barrier
@@ -374,8 +375,9 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
       const uint32_t at = t_s + (uint32_t)(b * KT_KEYS);
       uint32_t x[32];
       kt_ld32(at, x);
-      const float4 mine = s_scales[jl % KT_SCALES][hv], others = s_scales[jl % KT_SCALES][hv ^ 1];
+      const float4 mine = s_scales[jl % KT_SCALES][hv];
       const float2 ks = make_float2(mine.x, mine.y);
+      float vs0 = mine.z, vs1 = mine.w;               // of what this row sees: a weight of 0 under a scale far above the row's unit is no number
       const int ti = 2 * (j0 + jl) + hv;
       const bool there = ti < tiles.n;
       const int kt = part_key(there ? ti : tiles.n - 1);   // behind the last 32 their own keys again, as fetched
@@ -397,6 +399,8 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         if (ks.y < 0.f) seen &= 0xFFFFu;
 #pragma unroll
         for (int i = 0; i < 32; i++) x[i] = seen >> i & 1u ? x[i] : 0xFF800000u;
+        if (!(seen & 0xFFFFu)) vs0 = 0.f;
+        if (!(seen >> 16)) vs1 = 0.f;
       }
       float mx;
       {
@@ -411,15 +415,15 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         mx = MORE ? fmaxf(m0, m1) : fmaxf(m0 * f0, m1 * f1);
       }
       bool grow = mx > m + KT_SLACK || (m == -INFINITY && mx > -INFINITY);
-      const float vtop = fmaxf(fmaxf(mine.z, mine.w), fmaxf(others.z, others.w));
-      const bool wider = vtop > ref;                  // the same for the whole block
-      if (kt_any_of_pair(grow, pair_bar) || wider) {
+      float vtop = fmaxf(vs0, vs1);
+      if (kt_any_of_pair(grow || vtop > ref, pair_bar)) {
         mx = both(mx, [](float a, float b) { return fmaxf(a, b); });
+        vtop = both(vtop, [](float a, float b) { return fmaxf(a, b); });
         grow = mx > m + KT_SLACK || (m == -INFINITY && mx > -INFINITY);
         float corr = 1.f;
         if (grow) { corr = m > -INFINITY ? k8_ex2(m - mx) : 0.f; m = mx; shift = KT_UP - m; }
         l *= corr;
-        if (wider) {                                  // the next power of two and a factor of 4 more, so that this is rare; lo ends at 2^-25 / 2^7 ref, below 2^-29 of the scale
+        if (vtop > ref) {                             // the next power of two and a factor of 4 more, so that this is rare; lo ends at 2^-25 / 2^7 ref, below 2^-29 of the scale
           const float to = __uint_as_float(min(((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u) + 0x1000000u, 0x7E800000u));
           corr *= ref / to;
           ref = to;
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         }
       }
       float2 sum = make_float2(0.f, 0.f);
-      const float vr0 = mine.z * down, vr1 = mine.w * down;
+      const float vr0 = vs0 * down, vr1 = vs1 * down;
       uint32_t hi[16], lo[16];
 #pragma unroll
       for (int i = 0; i < 16; i++) {

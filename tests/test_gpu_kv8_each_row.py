@@ -1,0 +1,119 @@
+"""Attention over the cache in 8 bits, every (row, head, channel) by itself against float64: rows that see little stand beside rows that see much, and a norm over all of them shows the
+first alone.
+
+The bound of a result o_c = sum_j p_j v_jc: an error of eps in every score or weight moves it by eps * (sum_j p_j |v_jc| + |o_c|).
+eps, fp32 results: a score sums products of absolute sum T (its largest over the visible keys), q off by 2^-22, and dim / 16 sums of two operands cut off at 2^-23 of what is there; the score beside
+its maximum, X in units of ln 2 and 16 more, is rounded twice; tanh is off by 2^-22 of the cap; a weight by 3 * 2^-22; 128 sums in a row, each cut off at 2^-23.
+One fp16 an operand (bf16 results of long portions): 2^-11 of the products and of the weight more.
+On top, 2^-29 of the row's largest weight times the largest VISIBLE scale for every visible key (the header's statement, a scale's largest number being 128 or more of its steps), doubled
+for what the weights' sum takes of it; and the last rounding, 2^-24 or 2^-8 of the result."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_oracle as O
+import test_gpu_kv8 as T
+
+pytestmark = pytest.mark.gpu
+K, LAYER = T.K, T.LAYER
+
+
+def expected(a, q, keys, values, p0, eps_more=0.0):
+    """(results, bounds) [n, heads, vdim] of rows at p0 .. in float64."""
+    n, heads, dim = q.shape
+    group = heads // keys.shape[1]
+    t, p = np.arange(keys.shape[0])[None], np.arange(p0, p0 + n)[:, None]
+    vis = O.sees(a, t, p)
+    out, far = np.zeros((n, heads, values.shape[2])), np.zeros((n, heads, values.shape[2]))
+    for h in range(heads):
+        k, v = keys[:, h // group], values[:, h // group]
+        f = a["scale"] * (a["head_scale"][h] if a.get("head_scale") is not None else 1.0)
+        s = q[:, h] @ k.T * f
+        top = np.where(vis, np.abs(q[:, h]) @ np.abs(k).T * abs(f), 0).max(1)
+        cap = a.get("softcap") or 0.0
+        if cap:
+            s = cap * np.tanh(s / cap)
+        if a.get("rel") is not None:
+            s = s + a["rel"][h].astype(np.float64)[np.clip(p - t, 0, a["rel"].shape[1] - 1)]
+        s = np.where(vis, s, -np.inf)
+        sink = float(a["sink"][h]) if a.get("sink") is not None else -np.inf
+        m = np.maximum(s.max(1), sink)
+        w = np.exp(s - np.where(np.isfinite(m), m, 0.0)[:, None])
+        total = w.sum(1) + (np.exp(sink - m) if np.isfinite(sink) else 0.0)
+        w = w / np.where(total > 0, total, 1)[:, None]
+        o, size = w @ v, w @ np.abs(v)
+        x = np.where(vis & np.isfinite(s), np.abs(s), 0).max(1) if a.get("rel") is None else np.full(n, 64.0)
+        eps = top * (2.0 ** -22 + dim / 16 * 2.0 ** -22 + eps_more) + (1.45 * x + 16) * 2.0 ** -23 + cap * 2.0 ** -22 + 3 * 2.0 ** -22 + 128 * 2.0 ** -23 + eps_more
+        largest = np.where(vis, np.abs(v).max(1)[None], 0).max(1) * w.max(1) * vis.sum(1)
+        out[:, h] = o
+        far[:, h] = eps[:, None] * (size + np.abs(o)) + (2.0 ** -28 * largest)[:, None]
+    return out, far
+
+
+def check(m, a, parts, dtype, seed=5, tiles=None):
+    """The rows of `parts` over m's cache: no number further off than its bound."""
+    heads = a["heads"]
+    assert tiles is None or T.takes_tiles(a, m, parts, dtype) == tiles
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = sum(x[2] for x in parts)
+    q = torch.randn(n, heads * m.dim, device="cuda", generator=g)
+    dev = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda()  # noqa: E731
+    at = K.Attention(heads, m.H, m.dim, m.vdim, scale=a["scale"], chunk=a.get("chunk", 0), window=a.get("window", 0), keep_first=a.get("keep_first", 0), sink=dev(a.get("sink")),
+                     head_scale=dev(a.get("head_scale")), softcap=a.get("softcap", 0.0), rel=dev(a.get("rel")))
+    got = m.cache.attend(at, K.Rows.of(parts), q, layer=LAYER, dtype=dtype).double().cpu().numpy().reshape(n, heads, m.vdim)
+    qn, row, worst = q.double().cpu().numpy().reshape(n, heads, m.dim), 0, 0.0
+    for slot, p, c in parts:
+        if p >= 0:
+            want, far = expected(a, qn[row:row + c], m.values("k", slot, p + c), m.values("v", slot, p + c), p, 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
+            far = far + np.abs(want) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) + 1e-40
+            worst = max(worst, float((np.abs(got[row:row + c] - want) / far).max()))
+        else:
+            assert not got[row:row + c].any()
+        row += c
+    assert worst < 1.0
+    return got
+
+
+@pytest.mark.parametrize("case", T.LONG, ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{c[4]}-{c[5]}-{len(c[6])}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompts(case, dtype):
+    fmt, block, heads, kv_heads, dim, vdim, parts, mask = case
+    m = T.filled(block, kv_heads, dim, vdim, fmt, [max(1, p + n) for _, p, n in parts])
+    rng, a = np.random.default_rng(3), dict(mask, heads=heads, scale=dim ** -0.5)
+    if a.get("sink"):
+        a["sink"] = rng.standard_normal(heads).astype(np.float32)
+    if a.get("rel"):
+        a["rel"] = rng.standard_normal((heads, a["rel"])).astype(np.float32)
+    check(m, a, parts, dtype, tiles=True)
+
+
+@pytest.mark.parametrize("block,heads,kv_heads,dim,vdim,fmt", [(16, 4, 4, 64, 64, "int8"), (32, 8, 2, 128, 128, "e4m3"), (128, 20, 2, 96, 112, "int8")])
+@pytest.mark.parametrize("parts", [T.SINGLES, T.PORTIONS], ids=["singles", "portions"])
+@pytest.mark.parametrize("mask", [dict(), dict(window=33, keep_first=4), dict(chunk=50), dict(softcap=3.0)], ids=str)
+def test_few_rows(block, heads, kv_heads, dim, vdim, fmt, parts, mask):
+    m = T.filled(block, kv_heads, dim, vdim, fmt)
+    check(m, dict(mask, heads=heads, scale=dim ** -0.5), parts, torch.float32)
+
+
+def uneven(n, heads, dim, vdim, block, fmt, up, which):
+    """A context whose value blocks `which(block number)` are 2^up larger than the others."""
+    m = T.Mirror(1, n, heads, block, dim, vdim, fmt)
+    k = torch.from_numpy(m.rng.standard_normal((n, heads * dim)).astype(np.float32)).cuda()
+    v = m.rng.standard_normal((n, heads * vdim)).astype(np.float32)
+    v *= np.where(which(np.arange(n) // block), np.float32(2.0 ** up), np.float32(1))[:, None]
+    m.write([(0, 0, n)], k, torch.from_numpy(v).cuda())
+    return m
+
+
+HIDING = [(dict(), lambda b: b % 8 == 3), (dict(window=40), lambda b: b % 8 == 3), (dict(window=70, keep_first=5), lambda b: b % 16 == 5), (dict(chunk=48), lambda b: b % 3 == 2),
+          (dict(chunk=64, window=30, keep_first=200), lambda b: b % 4 == 1), (dict(softcap=5.0, window=33), lambda b: b % 8 == 1)]
+
+
+@pytest.mark.parametrize("mask,which", HIDING, ids=lambda x: str(x) if isinstance(x, dict) else "")
+@pytest.mark.parametrize("up", [13, 26, 60])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim,fmt", [(32, 8, 128, "int8"), (64, 16, 64, "e4m3")])
+def test_scales_of_keys_that_a_row_of_a_prompt_does_not_see(mask, which, up, dtype, heads, kv_heads, dim, fmt):
+    """Blocks of values far larger than the others, ahead of a row's window or chunk or behind the row itself, while rows of the same tile see them: they cost the row no bit."""
+    m = uneven(640, kv_heads, dim, dim, 16, fmt, up, which)
+    check(m, dict(mask, heads=heads, scale=dim ** -0.5), [(0, 0, 640)], dtype, tiles=None if "window" in mask or "chunk" in mask else True)
