@@ -9,8 +9,8 @@
 // A block takes eight pairs of one key/value head and a run of tiles of 32 keys, its warps every fourth tile.  A warp's tiles come through a ring in shared memory of its own
 // (cp.async).  Channels of K and the order of channels in V's column groups are free, as long as both operands agree, and chosen so that
 // a lane reads 16 bytes at a time and the eight lanes of a shared-memory phase meet 32 different banks (16-byte pieces of a row are stored at piece ^ (row mod 8)).
-// V's scale belongs to a block of keys, the accumulator to all of them: a weight is multiplied by scale / (largest scale of the run's blocks, rounded up to a
-// power of two) ahead of the split.  Weights have the factor 2^15, so that the 22 bits reach down to 2^-28 of the largest.
+// V's scale belongs to a block of keys, the accumulator to all of them: a weight is multiplied by scale / (largest scale that its pair and warp have seen, rounded up to a
+// power of two) ahead of the split; scales that a mask hides from a pair cost it nothing.  Weights have the factor 2^15, so that the 22 bits reach down to 2^-28 of the largest.
 //
 // Bound: the cache's bytes where nothing else is; here the instructions that turn them into fp16 pairs (int8: five for four codes of K, six of V) and the chain of a tile, which
 // three blocks on an SM (168 registers, a ring of two tiles a warp) hide better than two (217 registers, three tiles: 168 us where these take 146).  One context of 131072 keys, 8
@@ -76,8 +76,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
   __shared__ uint4 s_q[KS][32];                             // q as the A operand of every step, a lane's registers together
   __shared__ int s_tile[2 * K8_SEG];                        // per 16 keys of a segment's tiles: (block, layer, head), -1 where they do not exist, and the scales
   __shared__ float s_ks[2 * K8_SEG], s_vs[2 * K8_SEG];
-  __shared__ float s_top[K8_WARPS];
-  __shared__ float s_ml[K8_WARPS][K8_PAIRS][2];
+  __shared__ float s_ml[K8_WARPS][K8_PAIRS][3];             // maximum, sum, unit
   const int D = FULL ? DT : a.dim, E = FULL ? DT : a.vdim, gsize = a.heads / a.kv_heads, B = kv.block_size, layer = a.cache_layer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   hyb_pdl_enter();
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
   float acc[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-  float m = -INFINITY, l = 0.f, ref = 0.f;                  // l: this lane's keys only
+  float m = -INFINITY, l = 0.f, ref = 0.f, down = 0.f;      // l: this lane's keys only; ref: the unit of this lane's pair and its warp, 1 / down
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(k8_ring) + warp * Ring::WARP;
   const int lane_r = lane / (DT / 16), lane_c = lane % (DT / 16);   // the row and piece of 512 bytes of a tile that this lane copies
   const uint32_t lane_to = (uint32_t)k8_piece<DT>(lane_r, lane_c);
@@ -207,30 +206,13 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
     };
 #pragma unroll
     for (int i = 0; i < Ring::STAGES - 1; i++) { fetch(s0 + warp + i * K8_WARPS, i); k8_commit(); }
-    float top = 0.f;
     for (int e = threadIdx.x; e < 2 * (s1 - s0); e += K8_THREADS) {
       const int at = s_tile[e];
       s_ks[e] = at >= 0 ? kv.k_scale[at] : 0.f;
-      const float vs = at >= 0 ? kv.v_scale[at] : 0.f;
-      s_vs[e] = vs;
-      top = fmaxf(top, vs);
+      s_vs[e] = at >= 0 ? kv.v_scale[at] : 0.f;
     }
-    top = warp_max(top);
-    if (lane == 0) s_top[warp] = top;
     if (s0 == ti0) make_q();
     __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-    float down = 1.0f;
-    if (top > ref) {                                        // up to the next power of two: what is there changes units exactly
-      const float to = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u));
-      const float corr = ref / to;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int x = 0; x < 4; x++) acc[i][x] *= corr;
-      ref = to;
-    }
-    if (ref > 0.f) down = 1.0f / ref;
 
     int stage = 0;
     for (int ti = s0 + warp; ti < s1; ti += K8_WARPS) {
@@ -275,10 +257,13 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
           x[j].x *= LOG2E; x[j].y *= LOG2E;
         }
       }
+      float v0 = s_vs[e], v1 = s_vs[e + 1];                  // of what this lane's pair sees: a weight of 0 under a scale far above the pair's unit is no number
       if (!whole) {
         uint32_t seen = kv8_sees32(a, kt, pos, my_lo);
         if (!there0) seen &= 0xFFFF0000u;
         if (!there1) seen &= 0xFFFFu;
+        if (!(seen & 0xFFFFu)) v0 = 0.f;
+        if (!(seen >> 16)) v1 = 0.f;
         seen >>= 2 * t;                                      // bits 8 j, 8 j + 1 are this lane's
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -289,18 +274,26 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
       float top_x = k8_max3(k8_max3(x[0].x, x[0].y, x[1].x), k8_max3(x[1].y, x[2].x, x[2].y), fmaxf(x[3].x, x[3].y));
       top_x = fmaxf(top_x, __shfl_xor_sync(THA_FULL_MASK, top_x, 1));
       top_x = fmaxf(top_x, __shfl_xor_sync(THA_FULL_MASK, top_x, 2));
-      const bool grow = top_x > m;
-      if (__any_sync(THA_FULL_MASK, grow)) {
-        const float to = grow ? top_x : m, corr = m > -INFINITY ? k8_ex2(m - to) : grow ? 0.f : 1.f;
+      const float top_v = fmaxf(v0, v1);
+      const bool grow = top_x > m, wider = top_v > ref;
+      if (__any_sync(THA_FULL_MASK, grow || wider)) {
+        const float to = grow ? top_x : m;
+        float corr = m > -INFINITY ? k8_ex2(m - to) : grow ? 0.f : 1.f;
         m = to;
         l *= corr;
+        if (wider) {                                         // up to the next power of two: what is there changes units exactly
+          const float unit = __uint_as_float(min((__float_as_uint(top_v) + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u));
+          corr *= ref / unit;
+          ref = unit;
+          down = 1.0f / unit;
+        }
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
           for (int y = 0; y < 4; y++) acc[i][y] *= corr;
       }
       const float shift = m > -INFINITY ? K8_UP - m : 0.f;   // nothing seen so far: weights are 2^-inf
-      const float v0 = s_vs[e] * down, v1 = s_vs[e + 1] * down;
+      v0 *= down; v1 *= down;
       uint4 pf[2];
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -354,7 +347,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
   l += __shfl_xor_sync(THA_FULL_MASK, l, 2);
   __syncthreads();
   float* s_acc = reinterpret_cast<float*>(k8_ring);
-  if (t == 0) { s_ml[warp][g][0] = l == l ? m : l; s_ml[warp][g][1] = l; }   // a NaN among the scores shows in the sum alone
+  if (t == 0) { s_ml[warp][g][0] = l == l ? m : l; s_ml[warp][g][1] = l; s_ml[warp][g][2] = ref; }   // a NaN among the scores shows in the sum alone
 #pragma unroll
   for (int i = 0; i < NV; i++)                               // columns 2 t, 2 t + 1 of group i are channels 2 t * DT / 8 + i, (2 t + 1) * DT / 8 + i
     *reinterpret_cast<float2*>(s_acc + (warp * NV + i) * GROUP + g * 8 + 2 * t) = make_float2(acc[i][0], acc[i][1]);
@@ -370,18 +363,20 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
       L += f[x] * s_ml[x][w][1];
     }
     L *= exp2f(-K8_UP);
-    float scale = ref * exp2f(-K8_UP);
+    float scale = exp2f(-K8_UP);
     const size_t at = (size_t)r * a.heads + h2, all = (size_t)rows.n_rows * a.heads;
     float* pd = splits > 1 ? partial + k8_sums_floats(splits, all) + ((size_t)sp * all + at) * E : nullptr;
     if (!pd) scale *= k8_final(a, h2, M, L, gate ? gate + (size_t)r * ldg : nullptr);
     else if (lane == 0) { float* ml = partial + 2 * ((size_t)sp * all + at); ml[0] = M; ml[1] = L; }
+#pragma unroll
+    for (int x = 0; x < K8_WARPS; x++) f[x] *= scale;
     for (int c = lane; c < E; c += 32) {
       float o = 0.f;
 #pragma unroll
-      for (int x = 0; x < K8_WARPS; x++) o += f[x] * s_acc[(x * NV + c % NV) * GROUP + w * 8 + c / NV];
-      if (pd) pd[c] = o * scale;
-      else if (out_bf16) reinterpret_cast<__nv_bfloat16*>(out)[at * E + c] = __float2bfloat16_rn(o * scale);
-      else reinterpret_cast<float*>(out)[at * E + c] = o * scale;
+      for (int x = 0; x < K8_WARPS; x++) o += s_acc[(x * NV + c % NV) * GROUP + w * 8 + c / NV] * f[x] * s_ml[x][w][2];
+      if (pd) pd[c] = o;
+      else if (out_bf16) reinterpret_cast<__nv_bfloat16*>(out)[at * E + c] = __float2bfloat16_rn(o);
+      else reinterpret_cast<float*>(out)[at * E + c] = o;
     }
   }
 }

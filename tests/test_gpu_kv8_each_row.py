@@ -117,3 +117,12 @@ def test_scales_of_keys_that_a_row_of_a_prompt_does_not_see(mask, which, up, dty
     """Blocks of values far larger than the others, ahead of a row's window or chunk or behind the row itself, while rows of the same tile see them: they cost the row no bit."""
     m = uneven(640, kv_heads, dim, dim, 16, fmt, up, which)
     check(m, dict(mask, heads=heads, scale=dim ** -0.5), [(0, 0, 640)], dtype, tiles=None if "window" in mask or "chunk" in mask else True)
+
+
+@pytest.mark.parametrize("mask,which", HIDING, ids=lambda x: str(x) if isinstance(x, dict) else "")
+@pytest.mark.parametrize("up", [13, 40, 70])
+@pytest.mark.parametrize("parts", [[(0, p, 1) for p in (47, 80, 100, 127, 200, 255)], [(0, 30, 9), (0, 60, 40), (0, 120, 1)]], ids=["singles", "portions"])
+@pytest.mark.parametrize("heads,kv_heads,dim,fmt", [(4, 2, 128, "e4m3"), (3, 3, 64, "int8")])
+def test_scales_of_keys_that_one_of_few_rows_does_not_see(mask, which, up, parts, heads, kv_heads, dim, fmt):
+    m = uneven(256, kv_heads, dim, dim, 16, fmt, up, which)
+    check(m, dict(mask, heads=heads, scale=dim ** -0.5), parts, torch.float32)
