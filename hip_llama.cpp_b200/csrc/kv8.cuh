@@ -103,7 +103,7 @@ __device__ __forceinline__ float k8_final(const tha_attn_t& a, int h, float m, f
 __device__ __forceinline__ void k8_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void k8_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Partial results of `splits` parts of `all` (row, head)s: maxima and sums [part][all][2], rounded up to 16 bytes, then accumulators [part][all][E]
+// Partial results of `splits` parts of `all` (row, head)s: maxima and sums [part][all][2], rounded up to 16 bytes, then weighted means [part][all][E]
 __host__ __device__ __forceinline__ size_t k8_sums_floats(int splits, size_t all) { return (2 * all * splits + 3) & ~(size_t)3; }
 __host__ __device__ __forceinline__ size_t k8_partial_floats(int splits, size_t all, int E) { return k8_sums_floats(splits, all) + all * splits * E; }
 

@@ -63,7 +63,7 @@ __device__ __forceinline__ int k8_tiles_of(const tha_rows_t& rows, int s, int gs
   const int n = rows.seq_first[s + 1] - rows.seq_first[s];
   return n <= most ? (n * gsize + K8_PAIRS - 1) / K8_PAIRS : 0;
 }
-// grid (tiles of pairs * splits, kv_heads).  Partial results of a split: sums and maxima [split][row * heads + head][2], then accumulators [..][vdim].
+// grid (tiles of pairs * splits, kv_heads).  Partial results of a split: sums and maxima [split][row * heads + head][2], then weighted means [..][vdim].
 // FULL: heads have DT channels, keys and values alike.
 template <int DT, int FMT, bool MORE, bool FULL>
 __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, const float* q, void* out, int out_bf16, int most_rows, int splits, int run,
@@ -366,8 +366,8 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
     float scale = exp2f(-K8_UP);
     const size_t at = (size_t)r * a.heads + h2, all = (size_t)rows.n_rows * a.heads;
     float* pd = splits > 1 ? partial + k8_sums_floats(splits, all) + ((size_t)sp * all + at) * E : nullptr;
-    if (!pd) scale *= k8_final(a, h2, M, L, gate ? gate + (size_t)r * ldg : nullptr);
-    else if (lane == 0) { float* ml = partial + 2 * ((size_t)sp * all + at); ml[0] = M; ml[1] = L; }
+    scale *= pd ? (L > 0.f ? 1.0f / L : L) : k8_final(a, h2, M, L, gate ? gate + (size_t)r * ldg : nullptr);   // a part is a mean: sums of values beyond 2^118 are not finite
+    if (pd && lane == 0) { float* ml = partial + 2 * ((size_t)sp * all + at); ml[0] = M; ml[1] = L; }
 #pragma unroll
     for (int x = 0; x < K8_WARPS; x++) f[x] *= scale;
     for (int c = lane; c < E; c += 32) {
@@ -406,7 +406,9 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(T* out, const float* par
   const float M = warp_max(fmaxf(m[0], m[1]));
 #pragma unroll
   for (int i = 0; i < 2; i++) w[i] = m[i] > -INFINITY ? exp2f(m[i] - M) : 0.f;
-  const float L = warp_sum(w[0] * l[0] + w[1] * l[1]);
+  const float L = warp_sum(w[0] * l[0] + w[1] * l[1]), inv = L > 0.f ? 1.0f / L : 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; i++) w[i] *= l[i] * inv;           // of the parts' means
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int s = w0; s < splits; s += WARPS) {
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(T* out, const float* par
     }
   }
   if (!mine) return;
-  const float f = k8_final(a, h, nan ? NAN : M, L, gate ? gate + (size_t)row * ldg : nullptr);
+  const float f = k8_final(a, h, nan ? NAN : M, L, gate ? gate + (size_t)row * ldg : nullptr) * L;
   const float v[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
 #pragma unroll
   for (int i = 0; i < 4; i++) {

@@ -473,14 +473,14 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
     ok = __all_sync(THA_FULL_MASK, ok);
     l = both(l, [](float a, float b) { return a + b; });
     const size_t at = row_ok ? (size_t)(r0 + pp) * a.heads + h : 0;
-    float scale = ref * exp2f(-KT_UP);
+    float scale = exp2f(-KT_UP);                      // times ref, in this order: ref's smallest number times less is none that holds all bits
     l *= exp2f(-KT_UP);
     if (SPLIT && n > KT_RUN) add_run();
     if (l != l) m = l;                                // a NaN among the scores shows in the sum alone
     float* pd = splits > 1 ? partial + k8_sums_floats(splits, all) + ((size_t)sp * all + at) * E : nullptr;
     if (row_ok) {
-      if (!pd) scale *= k8_final(a, h, m, l, gate ? gate + (size_t)(r0 + pp) * ldg : nullptr);
-      else if (hv == 0) *reinterpret_cast<float2*>(partial + 2 * ((size_t)sp * all + at)) = make_float2(m, l);
+      scale *= pd ? (l > 0.f ? 1.0f / l : l) : k8_final(a, h, m, l, gate ? gate + (size_t)(r0 + pp) * ldg : nullptr);   // a part is a mean
+      if (pd && hv == 0) *reinterpret_cast<float2*>(partial + 2 * ((size_t)sp * all + at)) = make_float2(m, l);
     }
 #pragma unroll 1
     for (int c = 0; c < DT / 2 && hv * (DT / 2) + c < E; c += 16) {
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const int from = FMT == THA_KV8_INT8 && (i & 3) % 3 ? i ^ 3 : i;   // columns 1 and 2 of every four hold channels 2 and 1
-          v[i] = __uint_as_float(o[from]) * scale;
+          v[i] = __uint_as_float(o[from]) * scale * ref;
         }
         if (pd || sizeof(T) == 4 || a.out_f32) {
           float* dst = pd ? pd + col : reinterpret_cast<float*>(out) + at * E + col;

@@ -65,7 +65,7 @@ def check(m, a, parts, dtype, seed=5, tiles=None):
     for slot, p, c in parts:
         if p >= 0:
             want, far = expected(a, qn[row:row + c], m.values("k", slot, p + c), m.values("v", slot, p + c), p, 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
-            far = far + np.abs(want) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) + 1e-40
+            far = far + np.abs(want) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) + 1e-44
             worst = max(worst, float((np.abs(got[row:row + c] - want) / far).max()))
         else:
             assert not got[row:row + c].any()
@@ -126,3 +126,21 @@ def test_scales_of_keys_that_a_row_of_a_prompt_does_not_see(mask, which, up, dty
 def test_scales_of_keys_that_one_of_few_rows_does_not_see(mask, which, up, parts, heads, kv_heads, dim, fmt):
     m = uneven(256, kv_heads, dim, dim, 16, fmt, up, which)
     check(m, dict(mask, heads=heads, scale=dim ** -0.5), parts, torch.float32)
+
+
+@pytest.mark.parametrize("parts", [[(0, 599, 1)], [(0, 599, 1)] * 48, [(0, 560, 40)], [(0, 0, 600)]], ids=["single", "singles", "portion", "prompt"])
+@pytest.mark.parametrize("up", [-112, -124, 100, 124])
+def test_values_at_the_ends_of_fp32(parts, up):
+    """Values of 2^-124 under the smallest scales keep their bits, and means of values of 2^126 are finite."""
+    m = T.Mirror(1, 600, 4, 16, 128, 128, "int8")
+    k, v = (torch.from_numpy(m.rng.standard_normal((600, 512)).astype(np.float32)).cuda() for _ in range(2))
+    m.write([(0, 0, 600)], k, (1 + v.abs().clamp(max=4)) * 2.0 ** up)
+    check(m, dict(heads=16, scale=128 ** -0.5), parts, torch.float32)
+
+
+@pytest.mark.parametrize("up", [-124, 124])
+def test_parts_of_a_prompts_context_at_the_ends_of_fp32(up):
+    m = T.Mirror(1, 4000, 1, 16, 128, 128, "int8")
+    k, v = (torch.from_numpy(m.rng.standard_normal((4000, 128)).astype(np.float32)).cuda() for _ in range(2))
+    m.write([(0, 0, 4000)], k, (1 + v.abs().clamp(max=4)) * 2.0 ** up)
+    check(m, dict(heads=8, scale=128 ** -0.5), [(0, 3700, 300)], torch.float32, tiles=True)
