@@ -87,12 +87,17 @@ __device__ __forceinline__ uint32_t k8_e4m3x2(uint32_t two) {
   return (uint32_t)h.x | (uint32_t)h.y << 16;
 }
 
+// x log2(e), finite where x is: numbers from 2^127 on, as the type's lowest that stands for "not this key", would become infinities.  They are brought closer together there, in their
+// order, and stay further apart than any weight reaches.
+__device__ __forceinline__ float k8_log2_units(float x) {
+  return fabsf(x) > 0x1p127f && fabsf(x) < INFINITY ? fmaf(0.5f, x, copysignf(1.88539f * 0x1p126f, x)) : x * 1.4426950408889634f;   // 2^127 log2(e) = 2^126 + 1.88539 2^126
+}
 // The factor of a (query, head)'s accumulator with m the maximum (times log2(e)) and l the sum: 1 / (l + exp(sink - m)) times the head's gate; 0 where nothing was seen.
 __device__ __forceinline__ float k8_final(const tha_attn_t& a, int h, float m, float l, const float* gate_row) {
   if (!(m > -INFINITY)) return m != m ? m : 0.f;            // a NaN stays one
   float f;
   if (a.sink) {
-    const float sk = a.sink[h] * 1.4426950408889634f, M = fmaxf(m, sk), e = exp2f(m - M);
+    const float sk = k8_log2_units(a.sink[h]), M = fmaxf(m, sk), e = exp2f(m - M);
     f = e / (l * e + exp2f(sk - M));
   } else {
     f = 1.0f / l;

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
           const int key = kt + 8 * j + 2 * t;
           if (a.softcap > 0.f) { x[j].x = hyb_softcap(x[j].x, a.softcap); x[j].y = hyb_softcap(x[j].y, a.softcap); }
           if (a.rel) { x[j].x += hyb_attn_rel(a, head, pos - key); x[j].y += hyb_attn_rel(a, head, pos - key - 1); }
-          x[j].x *= LOG2E; x[j].y *= LOG2E;
+          x[j].x = k8_log2_units(x[j].x); x[j].y = k8_log2_units(x[j].y);
         }
       }
       float v0 = s_vs[e], v1 = s_vs[e + 1];                  // of what this lane's pair sees: a weight of 0 under a scale far above the pair's unit is no number
@@ -292,13 +292,15 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
 #pragma unroll
           for (int y = 0; y < 4; y++) acc[i][y] *= corr;
       }
-      const float shift = m > -INFINITY ? K8_UP - m : 0.f;   // nothing seen so far: weights are 2^-inf
+      const float shift = m > -INFINITY ? (MORE ? -m : K8_UP - m) : 0.f;   // nothing seen so far: weights are 2^-inf; MORE: next to a maximum of 2^127, 15 is nothing
       v0 *= down; v1 *= down;
       uint4 pf[2];
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float2 y = k8_add2(x[j], make_float2(shift, shift)), w = make_float2(k8_ex2(y.x), k8_ex2(y.y));
+        float2 y = k8_add2(x[j], make_float2(shift, shift));
+        if (MORE) y = k8_add2(y, make_float2(K8_UP, K8_UP));
+        const float2 w = make_float2(k8_ex2(y.x), k8_ex2(y.y));
         sum = k8_add2(sum, w);
         split_f16x2(f32x2_mul(w, j < 2 ? make_float2(v0, v0) : make_float2(v1, v1)), 1.0f, j & 1 ? pf[j >> 1].z : pf[j >> 1].x, j & 1 ? pf[j >> 1].w : pf[j >> 1].y);
       }

@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
           float y = __uint_as_float(x[i]) * (i < 16 ? f0 : f1);
           if (a.softcap > 0.f) y = hyb_softcap(y, a.softcap);
           if (a.rel && row_ok) y += hyb_attn_rel(a, h, pos - (kt + i));
-          x[i] = __float_as_uint(y * LOG2E);
+          x[i] = __float_as_uint(k8_log2_units(y));
         }
       }
       if (!whole) {
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         vtop = both(vtop, [](float a, float b) { return fmaxf(a, b); });
         grow = mx > m + KT_SLACK || (m == -INFINITY && mx > -INFINITY);
         float corr = 1.f;
-        if (grow) { corr = m > -INFINITY ? k8_ex2(m - mx) : 0.f; m = mx; shift = KT_UP - m; }
+        if (grow) { corr = m > -INFINITY ? k8_ex2(m - mx) : 0.f; m = mx; shift = MORE ? -m : KT_UP - m; }
         l *= corr;
         if (vtop > ref) {                             // the next power of two and a factor of 4 more, so that this is rare; lo ends at 2^-25 / 2^7 ref, below 2^-29 of the scale
           const float to = __uint_as_float(min(((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u) + 0x1000000u, 0x7E800000u));
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
       for (int i = 0; i < 16; i++) {
         float2 y = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
         const float f = i < 8 ? f0 : f1, vr = i < 8 ? vr0 : vr1;
-        if (MORE) y = k8_add2(y, make_float2(shift, shift));
+        if (MORE) y = k8_add2(k8_add2(y, make_float2(shift, shift)), make_float2(KT_UP, KT_UP));   // next to a maximum of 2^127, 7 is nothing
         else y = f32x2_fma(y, make_float2(f, f), make_float2(shift, shift));
         const float2 p = make_float2(k8_ex2(y.x), k8_ex2(y.y));
         sum = k8_add2(sum, p);

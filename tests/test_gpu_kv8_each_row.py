@@ -144,3 +144,32 @@ def test_parts_of_a_prompts_context_at_the_ends_of_fp32(up):
     k, v = (torch.from_numpy(m.rng.standard_normal((4000, 128)).astype(np.float32)).cuda() for _ in range(2))
     m.write([(0, 0, 4000)], k, (1 + v.abs().clamp(max=4)) * 2.0 ** up)
     check(m, dict(heads=8, scale=128 ** -0.5), [(0, 3700, 300)], torch.float32, tiles=True)
+
+
+LOW = float(np.finfo(np.float32).min)
+
+
+@pytest.mark.parametrize("parts", [[(0, 599, 1), (1, 3, 1)], [(0, 590, 10), (1, 0, 4)], [(0, 0, 600), (1, 0, 4)]], ids=["singles", "portions", "prompt"])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("sink", [False, True])
+def test_biases_of_the_lowest_number(parts, softcap, sink):
+    """A bias of the type's lowest number hides a key as long as another is seen; a row that has no other is a mean of what it sees, because the biases leave nothing of the scores.
+    -inf hides a key for good."""
+    m = T.filled(16, 4, 128, 128, "int8", (600, 4))
+    rel = np.zeros((16, 600), np.float32)
+    rel[0] = LOW
+    rel[1, 3:] = LOW
+    rel[2, :3] = LOW
+    rel[3] = -np.inf
+    rel[4, 1:] = -np.inf
+    rel[5, :] = -np.inf
+    rel[5, 7] = LOW
+    rel[6, :] = LOW
+    rel[6, 5] = 0.97 * LOW                                       # finite, below what log2(e) times it could be
+    a = dict(heads=16, scale=128 ** -0.5, rel=rel, softcap=softcap)
+    if sink:
+        a["sink"] = np.random.default_rng(1).standard_normal(16).astype(np.float32)
+    got = check(m, a, parts, torch.float32)
+    assert not got[:, 3].any()
+    if not sink:
+        assert np.abs(got[:, 0]).max(1).min() > 0
