@@ -287,9 +287,9 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         for (int i = 0; i < DT / 32; i++) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[u][i].x), fabsf(x[u][i].y)), fmaxf(fabsf(x[u][i].z), fabsf(x[u][i].w))));
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFu << (lane & 24), top, o));
-                float inverse;
+        float inverse;
         const float up = split_scale<100>(top, 14, &inverse);
-        const float f = ok[u] ? a.scale * (a.head_scale ? a.head_scale[h[u]] : 1.0f) : 0.f, s = f < 0.f ? -up : up;
+        const float f = ok[u] ? a.scale * (a.head_scale ? a.head_scale[h[u]] : 1.0f) : 0.f, s = f < 0.f ? -up : f == f ? up : f;   // no number stays none: below, the factor is held above 1e-30
         if (l8 == 0) s_row[pr] = inverse * fabsf(f) * (MORE ? 1.0f : LOG2E);
         unsigned char* row = Qs + (pr / KT_ROWS) * (SPLIT ? 2 : 1) * Q_PART + (pr % KT_ROWS) * 128;
 #pragma unroll

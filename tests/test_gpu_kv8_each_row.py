@@ -173,3 +173,17 @@ def test_biases_of_the_lowest_number(parts, softcap, sink):
     assert not got[:, 3].any()
     if not sink:
         assert np.abs(got[:, 0]).max(1).min() > 0
+
+
+def test_a_head_scale_that_is_not_a_number():
+    """... shows in the results of its head, in every form."""
+    m = T.filled(16, 4, 128, 128, "int8", (900,))
+    hs = torch.ones(16, device="cuda")
+    hs[5] = float("nan")
+    for dtype in (torch.float32, torch.bfloat16):
+        for parts, tiles in (([(0, 899, 1)], False), ([(0, 300, 600)], True)):
+            assert T.takes_tiles(dict(heads=16, scale=0.1), m, parts, dtype) == tiles
+            n = sum(p[2] for p in parts)
+            out = m.cache.attend(K.Attention(16, 4, 128, scale=0.1, head_scale=hs), K.Rows.of(parts), torch.randn(n, 2048, device="cuda"), layer=LAYER, dtype=dtype).view(n, 16, 128)
+            bad = torch.isnan(out)
+            assert bool(bad[:, 5].all()) and not bool(bad[:, torch.arange(16) != 5].any())
