@@ -117,7 +117,8 @@ int kv8_check(const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, cons
 int kv8_refuse(const char* who, const char* why);
 // kv8_attn_tc.cu: sequences of at least min_rows rows; THA_STATUS_NOT_SUPPORTED (nothing launched): the caller takes another form
 int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int most_tiles);
-size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles);
+size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles, int min_rows);
+int kv8_attn_tc_room_for(const tha_attn_t* a, int most_tiles);   // sequences whose visible keys may be staged at once
 int kv8_attn_tc_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int min_rows, int most_tiles,
                        int splits, void* staged, float* partial, const float* gate, long long ldg);
 

@@ -539,6 +539,11 @@ static Kv8Forms k8_forms(const tha_attn_t* a, const tha_rows_t* rows, int dtype)
     if (k8_long_pays(a, rows, dtype, keys, n)) { f.short_rows = n - 1; f.has_long = true; break; }
     if (n == rows->max_seq_rows) break;
   }
+  if (f.has_long) {   // all sequences that might be long have to find room: where they do not, the shorter of them are short
+    const int room = kv8_attn_tc_room_for(a, (int)(keys / 32));
+    if (rows->n_seqs > room && rows->n_rows / (f.short_rows + 1) > room) f.short_rows = rows->n_rows / (room + 1);
+    if (room < 1 || f.short_rows >= rows->max_seq_rows) { f.short_rows = 0x7FFFFFFF; f.has_long = false; }
+  }
   f.has_short = !(f.has_long && (long long)rows->n_seqs * rows->max_seq_rows == rows->n_rows);   // all sequences are as long as the longest
   return f;
 }
@@ -555,7 +560,7 @@ static int k8_attend(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_r
   if (f.has_long) {
     // tiles in fp16 first, partial results behind them
     const int most = k8_most_tiles(a, rows);
-    const size_t stage = kv8_attn_tc_stage_bytes(a, rows, most) / sizeof(float);
+    const size_t stage = kv8_attn_tc_stage_bytes(a, rows, most, short_rows + 1) / sizeof(float);
     int st = THA_STATUS_NOT_SUPPORTED;
     if (scratch && stage && stage <= room) {
       const int splits = fit(kv8_attn_tc_splits(a, rows, dtype, most), room - stage);
@@ -599,7 +604,7 @@ extern "C" size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const
   const Kv8Forms f = k8_forms(a, rows, dtype);
   const size_t all = (size_t)rows->n_rows * a->heads;
   const int most = k8_most_tiles(a, rows);
-  const size_t stage = f.has_long ? kv8_attn_tc_stage_bytes(a, rows, most) / sizeof(float) : 0;
+  const size_t stage = f.has_long ? kv8_attn_tc_stage_bytes(a, rows, most, f.short_rows + 1) / sizeof(float) : 0;
   size_t need = 0;
   if (f.has_short || !stage) {
     const int splits = k8_splits(a, rows, stage ? f.short_rows : 0x7FFFFFFF);

@@ -24,6 +24,7 @@
 #include "gemm_tc.h"
 #include "kv8.cuh"
 #include "tc_common.cuh"
+#include "workspace.h"
 
 namespace tha {
 
@@ -125,15 +126,13 @@ __device__ __forceinline__ int kt_stage_base(const tha_attn_t& a, const tha_rows
 // The staged part that holds `key`, one of those
 __device__ __forceinline__ int kt_part_of(const HybTiles& t, int key) { return key < t.begin + 32 * t.n_a ? (key - t.begin) >> 5 : t.n_a + ((key - t.resume) >> 5); }
 
-// grid (parts of all sequences, groups of KT_STAGE_HEADS heads), a thread: row t / 8 of a part, 16-byte piece t % 8, all heads' loads on their way at once
+// grid (parts of all sequences or fewer, groups of KT_STAGE_HEADS heads), a thread: row t / 8 of a part, 16-byte piece t % 8, all heads' loads on their way at once
 constexpr int KT_STAGE_HEADS = 4;
 template <int DT, int FMT>
-__global__ void __launch_bounds__(2 * DT) kv8_stage_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, int min_rows, unsigned char* staged, float4* scales) {
-  pdl_wait();
-  pdl_trigger();                     // behind the wait: the kernel behind this one reads q without another
+__device__ __forceinline__ bool kt_stage_part(const tha_attn_t& a, const tha_rows_t& rows, const tha_kv8_t& kv, int min_rows, int i, unsigned char* staged, float4* scales) {
   constexpr int PIECES = DT / 16;
-  const Kv8Piece pc = kv8_find(rows.n_seqs, (int)blockIdx.x, [&](int s) { return kt_seq(a, rows, s, min_rows).parts.n; });
-  if (pc.seq < 0) return;
+  const Kv8Piece pc = kv8_find(rows.n_seqs, i, [&](int s) { return kt_seq(a, rows, s, min_rows).parts.n; });
+  if (pc.seq < 0) return false;
   const KtSeq sq = kt_seq(a, rows, pc.seq, min_rows);
   const HybTiles& parts = sq.parts;
   const int slot = rows.seq_slot[pc.seq], last = sq.p0 + sq.n - 1, g0 = blockIdx.y * KT_STAGE_HEADS;
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(2 * DT) kv8_stage_kernel(tha_attn_t a, tha_row
 #pragma unroll
   for (int h = 0; h < KT_STAGE_HEADS; h++) {
     if (g0 + h >= kv.kv_heads) break;
-    const size_t at = (size_t)blockIdx.x * kv.kv_heads + g0 + h;
+    const size_t at = (size_t)i * kv.kv_heads + g0 + h;
     unsigned char* d = staged + at * kt_part(DT) + (x >> 2) * (32 * 128) + r * 128;
 #pragma unroll
     for (int side = 0; side < 2; side++) {
@@ -167,6 +166,19 @@ __global__ void __launch_bounds__(2 * DT) kv8_stage_kernel(tha_attn_t a, tha_row
       s[0] = id >= 0 ? kv.k_scale[tile] : -1.f;
       s[2] = id >= 0 ? kv.v_scale[tile] : 0.f;
     }
+  }
+  return true;
+}
+// TURNS: a block may have several parts.  Its 57 registers for 48 are a block less on an SM: two prompts, 24 us for 20.
+template <int DT, int FMT, bool TURNS>
+__global__ void __launch_bounds__(2 * DT) kv8_stage_kernel(tha_attn_t a, tha_rows_t rows, tha_kv8_t kv, int min_rows, int parts, unsigned char* staged, float4* scales) {
+  pdl_wait();
+  pdl_trigger();                     // behind the wait: the kernel behind this one reads q without another
+  if (!TURNS) {
+    kt_stage_part<DT, FMT>(a, rows, kv, min_rows, (int)blockIdx.x, staged, scales);
+  } else {
+    for (int i = blockIdx.x; i < parts; i += gridDim.x)
+      if (!kt_stage_part<DT, FMT>(a, rows, kv, min_rows, i, staged, scales)) return;
   }
 }
 __device__ __forceinline__ void kt_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -612,7 +624,11 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
 static int kt_positions(const tha_attn_t* a, int dtype) {
   return kt_groups(dtype == THA_DT_F32, a->dim > 64 || a->vdim > 64 ? 128 : 64) * KT_ROWS / (a->heads / a->kv_heads);
 }
-static long long kt_blocks(const tha_attn_t* a, const tha_rows_t* rows, int dtype) { return (long long)rows->n_rows / kt_positions(a, dtype) + rows->n_seqs; }
+// Sequences of at least min_rows rows that a step has at most.  (From the rows alone: the longest portion that a caller names may be one that no sequence has.)
+static long long kt_sequences(const tha_rows_t* rows, int min_rows) { return rows->n_rows / min_rows < rows->n_seqs ? rows->n_rows / min_rows : rows->n_seqs; }
+static long long kt_blocks(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int min_rows) {
+  return (long long)rows->n_rows / kt_positions(a, dtype) + kt_sequences(rows, min_rows);
+}
 
 // Parts of a context, most_tiles: of 32 keys.
 int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int most_tiles) {
@@ -623,12 +639,14 @@ int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, i
   return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
 
-// Parts that a step's sequences have at most, bytes of scratch for them (0: this form does not take the step): the parts, then their scales
-static long long kt_parts(const tha_rows_t* rows, int most_tiles) { return (long long)rows->n_seqs * most_tiles; }
-size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles) {
-  const long long parts = kt_parts(rows, most_tiles), bytes = parts * a->kv_heads * (kt_part(a->dim > 64 || a->vdim > 64 ? 128 : 64) + 16);
+// Parts that a step's sequences of this form have at most, bytes of scratch for them (0: this form does not take the step): the parts, then their scales
+static long long kt_part_bytes(const tha_attn_t* a) { return (long long)a->kv_heads * (kt_part(a->dim > 64 || a->vdim > 64 ? 128 : 64) + 16); }
+static long long kt_parts(const tha_rows_t* rows, int most_tiles, int min_rows) { return kt_sequences(rows, min_rows) * most_tiles; }
+size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles, int min_rows) {
+  const long long parts = kt_parts(rows, most_tiles, min_rows), bytes = parts * kt_part_bytes(a);
   return parts > 0x7FFFFFFFll || bytes > KT_MOST_STAGED ? 0 : (size_t)bytes;
 }
+int kv8_attn_tc_room_for(const tha_attn_t* a, int most_tiles) { return (int)(KT_MOST_STAGED / (kt_part_bytes(a) * most_tiles)); }
 
 template <int DT, int FMT, bool SPLIT, bool MORE, typename T>
 static int kt_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int min_rows, int most_tiles, int splits,
@@ -639,12 +657,16 @@ static int kt_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows
   const int st = gemm_tc_init(&flag);
   THA_CUDA_OK(cudaThreadExchangeStreamCaptureMode(&mode));
   THA_TRY_RC(st);
-  const long long parts = kt_parts(rows, most_tiles);
+  const long long parts = kt_parts(rows, most_tiles, min_rows);
   float4* scales = reinterpret_cast<float4*>(staged + (size_t)parts * a->kv_heads * kt_part(DT));
-  THA_CUDA_OK(launch(kv8_stage_kernel<DT, FMT>, dim3((unsigned)parts, ceil_div(a->kv_heads, KT_STAGE_HEADS)), dim3(32 * DT / 16), 0, s, pdl_enabled() != 0, *a, *rows, *kv, min_rows, staged, scales));
+  // A step of a prompt and many single rows has far fewer parts than it might: blocks for those of one sequence, or for sixteen on an SM, take all of them in turn.
+  const int groups = ceil_div(a->kv_heads, KT_STAGE_HEADS), at_once = ceil_div(16 * sm_budget(), groups);
+  const long long blocks = at_once > most_tiles ? at_once : most_tiles;
+  THA_CUDA_OK(launch(parts > blocks ? kv8_stage_kernel<DT, FMT, true> : kv8_stage_kernel<DT, FMT, false>, dim3((unsigned)(parts > blocks ? blocks : parts), groups), dim3(32 * DT / 16), 0, s,
+                     pdl_enabled() != 0, *a, *rows, *kv, min_rows, (int)parts, staged, scales));
   auto k = kv8_attn_tc_kernel<DT, FMT, SPLIT, MORE, T>;
   THA_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kt_smem(SPLIT, DT)));
-  THA_CUDA_OK(launch(k, dim3(a->kv_heads, (unsigned)(kt_blocks(a, rows, SPLIT ? THA_DT_F32 : THA_DT_BF16) * splits)), dim3(kt_threads(SPLIT, DT)), kt_smem(SPLIT, DT), s, pdl_enabled() != 0, *a, *rows,
+  THA_CUDA_OK(launch(k, dim3(a->kv_heads, (unsigned)(kt_blocks(a, rows, SPLIT ? THA_DT_F32 : THA_DT_BF16, min_rows) * splits)), dim3(kt_threads(SPLIT, DT)), kt_smem(SPLIT, DT), s, pdl_enabled() != 0, *a, *rows,
                      (const unsigned char*)staged, (const float4*)scales, q, out, kt_positions(a, SPLIT ? THA_DT_F32 : THA_DT_BF16), min_rows, splits, partial, gate, ldg, flag));
   return THA_STATUS_SUCCESS;
 }
@@ -662,7 +684,7 @@ static int kt_form(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, 
 // staged: as many bytes as kv8_attn_tc_stage_bytes says, on a 16-byte boundary
 int kv8_attn_tc_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, int min_rows, int most_tiles,
                        int splits, void* staged, float* partial, const float* gate, long long ldg) {
-  if (!aligned16(out) || kt_blocks(a, rows, dtype) * splits > 65535) return THA_STATUS_NOT_SUPPORTED;
+  if (!aligned16(out) || kt_blocks(a, rows, dtype, min_rows) * splits > 65535) return THA_STATUS_NOT_SUPPORTED;
   const bool wide = a->dim > 64 || a->vdim > 64;
   auto st = (unsigned char*)staged;
   if (dtype == THA_DT_BF16) {

@@ -670,8 +670,9 @@ int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_
  * Codes are exact in fp16; q and the weights, each times its value's scale, enter the products as two fp16.  A number of q is off by 2^-22 of itself or 2^-39 of the largest
  * of its row of a head, whichever is more; a weight by 2^-22 of itself or 2^-29 of the row's largest weight times the largest scale that the row sees.  Rows of longer portions with dtype
  * THA_DT_BF16 use one fp16: 2^-11 of itself instead of 2^-22.  Sums and softmax are fp32.  Which portions are long goes by the step: heads, keys, rows.
- * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones, and for
- * partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may
+ * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones (it goes by how many
+ * sequences of the step may be long at all, n_rows over the rows of a long one, each as far as the longest context; where that were more than 1 GiB, the shorter portions take the
+ * form of short ones, and all do behind a context that needs so much by itself), and for partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may
  * run at the same time need scratch of their own. */
 int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,
                      size_t scratch_floats, const float* proj, long long ldp);

@@ -50,7 +50,7 @@ def expected(a, q, keys, values, p0, eps_more=0.0):
     return out, far
 
 
-def check(m, a, parts, dtype, seed=5, tiles=None):
+def check(m, a, parts, dtype, seed=5, tiles=None, most=0):
     """The rows of `parts` over m's cache: no number further off than its bound."""
     heads = a["heads"]
     assert tiles is None or T.takes_tiles(a, m, parts, dtype) == tiles
@@ -60,7 +60,9 @@ def check(m, a, parts, dtype, seed=5, tiles=None):
     dev = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda()  # noqa: E731
     at = K.Attention(heads, m.H, m.dim, m.vdim, scale=a["scale"], chunk=a.get("chunk", 0), window=a.get("window", 0), keep_first=a.get("keep_first", 0), sink=dev(a.get("sink")),
                      head_scale=dev(a.get("head_scale")), softcap=a.get("softcap", 0.0), rel=dev(a.get("rel")))
-    got = m.cache.attend(at, K.Rows.of(parts), q, layer=LAYER, dtype=dtype).double().cpu().numpy().reshape(n, heads, m.vdim)
+    rows = K.Rows.of(parts)
+    rows.c.max_pos = max(rows.c.max_pos, most)                   # a step may be described by more than it has
+    got = m.cache.attend(at, rows, q, layer=LAYER, dtype=dtype).double().cpu().numpy().reshape(n, heads, m.vdim)
     qn, row, worst = q.double().cpu().numpy().reshape(n, heads, m.dim), 0, 0.0
     for slot, p, c in parts:
         if p >= 0:
@@ -85,6 +87,30 @@ def test_prompts(case, dtype):
     if a.get("rel"):
         a["rel"] = rng.standard_normal((heads, a["rel"])).astype(np.float32)
     check(m, a, parts, dtype, tiles=True)
+
+
+@pytest.mark.parametrize("most", [0, 2111, 15999])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("parts", [[(0, 1400, 700)] + [(i, 19, 1) for i in range(1, 41)],
+                                   [(i, 3, 1) for i in range(1, 20)] + [(0, 1200, 512), (41, 0, 30), (42, 50, 150), (43, 5, 8), (44, -1, 1), (45, 0, 260)] + [(i, 19, 1) for i in range(20, 41)]],
+                         ids=["one prompt", "several portions"])
+def test_prompts_beside_many_decoded_rows(parts, dtype, most):
+    """... in a step whose contexts may be far longer than room for all of them would allow: the longest portions take tiles, the others the other form, and every row is right."""
+    m = T.Mirror(1, 16, 32, 16, 128, 128, "int8", spare=400)
+    m.table, at = np.full((46, 1000), -1, np.int32), 0
+    for s, p, n in parts:
+        if p >= 0:
+            blocks = -(-(p + n) // 16)
+            m.table[s, :blocks] = np.arange(at, at + blocks)[::-1]
+            at += blocks
+    c = m.cache
+    m.cache = K.Kv8Cache(c.k_pool, c.v_pool, c.k_scale, c.v_scale, *(torch.zeros(46, T.LAYERS, 32, 16, 128, device="cuda") for _ in range(2)), torch.from_numpy(m.table).cuda())
+    m.rows = [{x: np.zeros((0, 32, 128), np.float32) for x in "kv"} for _ in range(46)]
+    parts_in = [(s, 0, p + n) for s, p, n in parts if p >= 0]
+    n = sum(x[2] for x in parts_in)
+    k, v = (torch.from_numpy(m.rng.standard_normal((n, 32 * 128)).astype(np.float32)).cuda() for _ in range(2))
+    m.write(parts_in, k, v)
+    check(m, dict(heads=32, scale=128 ** -0.5), parts, dtype, tiles=True, most=most)
 
 
 @pytest.mark.parametrize("block,heads,kv_heads,dim,vdim,fmt", [(16, 4, 4, 64, 64, "int8"), (32, 8, 2, 128, 128, "e4m3"), (128, 20, 2, 96, 112, "int8")])

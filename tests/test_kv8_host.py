@@ -169,3 +169,28 @@ def test_the_binding_refuses_what_the_library_cannot_see():
     r = K.Rows.of([(0, 0, 3), (1, 5, 1), (1, -1, 1)], "cpu")
     assert r.n == 5 and r.c.max_seq_rows == 3 and r.c.max_pos == 5 and r.slots == (0, 1, True)
     assert not K.Rows.of([(0, 0, 3), (0, 5, 1)], "cpu").slots[2]
+
+
+@pytest.mark.parametrize("beside", [0, 1, 15, 31, 63, 127])
+@pytest.mark.parametrize("most,rows_", [(2047, 1024), (4095, 1024), (8191, 512)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_a_prompt_beside_decoded_rows_keeps_its_form(beside, most, rows_, dtype):
+    """Room for the visible keys as fp16 goes by the sequences that may be long, not by all of the step's: with that for all, 31 rows at up to 2048 were too much, and none was asked for."""
+    big = dict(kv_heads=32, dim=128, vdim=128)
+    c = cache(**big, table_stride=512, n_blocks=9000)
+    r = rows(n_rows=rows_ + beside, n_seqs=1 + beside, max_seq_rows=rows_, max_pos=most)
+    need = 4 * K.lib().c.tha_hyb_kv8_attn_scratch(dtype, attn(heads=32, **big), r, c)
+    one = 2 * (most + 1) * 32 * 2 * 128                           # of the prompt's context in fp16
+    assert one <= need < (1 << 30) + (64 << 20)
+    # Portions of up to 29 rows are short ones: four blocks of eight of them take 4 * 32 * 0.75 us / 444 / 32 = 6.8 ns a key, staged ones at least 32 * 0.16 ns, and 32 * 0.6 us / 148 / 64
+    # for their tiles, 7.1 ns.  Portions of 30 rows or more are at most so many of the step.
+    assert need <= max(1, min(1 + beside, (rows_ + beside) // 30)) * one * 1.1 + (64 << 20)
+
+
+def test_portions_that_find_no_room_are_the_shorter_ones():
+    """With more sequences that may be long than find room, the long ones keep the form; a context that finds no room alone does not have it."""
+    big = dict(kv_heads=32, dim=128, vdim=128)
+    for most, n_seqs, n_rows, there in ((32767, 40, 4000, True), (32767, 1, 2048, True), (131071, 1, 2048, False)):
+        r = rows(n_rows=n_rows, n_seqs=n_seqs, max_seq_rows=2048, max_pos=most)
+        need = 4 * K.lib().c.tha_hyb_kv8_attn_scratch(0, attn(heads=32, **big), r, cache(**big, table_stride=8192, n_blocks=9000))
+        assert (need >= 2 * most * 32 * 2 * 128) == there and need < (1 << 30) + (128 << 20)
