@@ -483,6 +483,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
     if (ok) ok = tc_mbar_wait(&pv_done[w][(n - 1) & 1], (unsigned)((n - 1) >> 1) & 1u, abort_flag);
     kt_fence_after();
     ok = __all_sync(THA_FULL_MASK, ok);
+    if (!ok) l = NAN;                                 // a wait has given up: the row, whichever of its threads it was, is no number rather than left as it was
     l = both(l, [](float a, float b) { return a + b; });
     const size_t at = row_ok ? (size_t)(r0 + pp) * a.heads + h : 0;
     float scale = exp2f(-KT_UP);                      // times ref, in this order: ref's smallest number times less is none that holds all bits
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         tc_tmem_ld16(t_o + (uint32_t)c, o);
         kt_wait_ld();
       }
-      if (row_ok && ok) {
+      if (row_ok) {
         const int col = hv * (DT / 2) + c;
         float v[16];
 #pragma unroll

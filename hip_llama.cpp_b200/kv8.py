@@ -189,6 +189,13 @@ class Kv8Cache:
                              f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {s}")
         return s[0] if n > 1 else max(width, s[0])
 
+    def check_error(self) -> None:
+        """Waits for the current stream; raises if a kernel on the device gave up on a barrier since the last such question (attend's rows concerned are NaN then)."""
+        if self.device.type == "cuda":
+            torch.cuda.current_stream(self.device).synchronize()
+        if self.calls.tha_gemm_check_error():
+            raise cabi.ThaError("a kernel gave up on a barrier of its own")
+
     def _check(self, status, name):
         if status:
             self.lib.check(status, name)

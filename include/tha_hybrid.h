@@ -673,7 +673,9 @@ int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_
  * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones (it goes by how many
  * sequences of the step may be long at all, n_rows over the rows of a long one, each as far as the longest context; where that were more than 1 GiB, the shorter portions take the
  * form of short ones, and all do behind a context that needs so much by itself), and for partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may
- * run at the same time need scratch of their own. */
+ * run at the same time need scratch of their own.
+ * A kernel that gives up on a barrier of its own (after 17 s: a fault of its pipeline) ends with NaN in the rows concerned; tha_gemm_check_error (tha_b200.h) says so, once the stream has
+ * been waited for. */
 int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,
                      size_t scratch_floats, const float* proj, long long ldp);
 /* floats of scratch for such a call (0: it needs none, or would be refused) */

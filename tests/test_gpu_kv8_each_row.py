@@ -213,3 +213,10 @@ def test_a_head_scale_that_is_not_a_number():
             out = m.cache.attend(K.Attention(16, 4, 128, scale=0.1, head_scale=hs), K.Rows.of(parts), torch.randn(n, 2048, device="cuda"), layer=LAYER, dtype=dtype).view(n, 16, 128)
             bad = torch.isnan(out)
             assert bool(bad[:, 5].all()) and not bool(bad[:, torch.arange(16) != 5].any())
+
+
+def test_no_kernel_gave_up():
+    """After a prompt: the question that a host asks behind its stream."""
+    m = T.filled(16, 4, 128, 128, "int8", (900,))
+    check(m, dict(heads=16, scale=0.1), [(0, 300, 600)], torch.float32, tiles=True)
+    m.cache.check_error()

@@ -1,4 +1,6 @@
 """What the binding of the cache in 8 bits hands to the library, with a recorder in the library's place: no GPU."""
+import os
+import re
 import threading
 import types
 
@@ -48,3 +50,26 @@ def test_threads_share_an_attention(monkeypatch, layers):
     for t in threads:
         t.join(60)
     assert seen == want
+
+
+def test_a_kernel_that_gave_up_is_an_error(monkeypatch):
+    answers = [0, 1, 0]
+    cache = recorded(monkeypatch, tha_gemm_check_error=lambda: answers.pop(0))
+    cache.check_error()
+    with pytest.raises(K.cabi.ThaError):
+        cache.check_error()
+    cache.check_error()
+
+
+def test_a_wait_that_gives_up_shows_in_its_rows():
+    """No wait of the prompt kernel runs out in a sound pipeline, so this is read from its source: the outcome of a row's waits goes into its sum as NaN ahead of its two threads joining their
+    sums, from which maximum, factor and partial results follow; and no store of a result is left out where a wait gave up."""
+    src = os.path.join(os.path.dirname(K.__file__), "csrc", "kv8_attn_tc.cu")
+    text = re.sub(r"//[^\n]*", "", open(src).read())
+    kernel = text[text.index("kv8_attn_tc_kernel(tha_attn_t a"):]
+    softmax = kernel[kernel.index("if (warp < KT_SOFTMAX) {"):kernel.index("else if (warp == KT_LOAD)")]
+    waits = [m.start() for m in re.finditer(r"tc_mbar_wait", softmax)]
+    gave_up, joined = softmax.index("if (!ok) l = NAN;"), softmax.index("l = both(l,")
+    assert len(waits) >= 4 and max(waits) < gave_up < joined < softmax.index("if (l != l) m = l;") < softmax.index("k8_final(")
+    assert all("ok" in softmax[softmax.rindex("\n", 0, w):softmax.index("\n", w)] for w in waits)
+    assert not re.search(r"if \([^)]*\bok\b[^)]*\)", softmax[joined:])
