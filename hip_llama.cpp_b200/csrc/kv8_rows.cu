@@ -102,14 +102,26 @@ __device__ __forceinline__ int kv8_units(const tha_rows_t& rows, int s, int bloc
   return blocks > 1 ? blocks - 1 : 1;
 }
 
+constexpr int KW_WARPS = 16, KW_ROWS = 8;
+// `words` words of codes under the scale *s (NULL: there is no block) into open rows, as the values that they stand for: a warp, every lane those that it has in kv8_write_kernel.
+template <int FMT>
+__device__ __forceinline__ void kv8_back_from_codes(const uint8_t* codes, const float* scale, int words, float* open) {
+  const float s = scale ? *scale : 0.f;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < words; i += 32) {
+    const float4 x = kv8_decode4<FMT>(scale ? reinterpret_cast<const uint32_t*>(codes)[i] : 0u);
+    reinterpret_cast<float4*>(open)[i] = make_float4(x.x * s, x.y * s, x.z * s, x.w * s);
+  }
+}
+
 // A warp: 8 rows of a block of the cache, one head, K or V; their values in registers (up to 8 float4 a lane) between the maximum and the codes, so that they are read once.  The
 // block_size / 8 warps of a tile are neighbours and tell each other their maxima.  A thread block takes `each` units in turn, so that what it looks up for the first serves the others.
 // Prompts of 37, 1042 and 2048 rows, 32 heads of 128, fp32: a thread block a tile, with the quotients and positions made value by value, 68 us, like this 47 (behind cold caches;
 // 128 MB are 20).
 // grid (units / each, groups of 16 / (block_size / 8) heads, 2)
-constexpr int KW_WARPS = 16, KW_ROWS = 8;
-// FULL: heads of 128 channels, a row a warp's float4.
-template <typename T, int FMT, bool VEC, bool FULL>
+// FULL: heads of 128 channels, a row a warp's float4.  ENDS: what the open rows hold is known (tha_kv8_t.open_end) and kept: a load more ahead of the
+// first block's rows, three prompts 49 us for 47, single rows 0.6 us more; 4 us more where a long prompt's first rows come back from codes.
+template <typename T, int FMT, bool VEC, bool FULL, bool ENDS>
 __global__ void __launch_bounds__(32 * KW_WARPS, 2) kv8_write_kernel(tha_rows_t rows, tha_kv8_t kv, int layer, int each, const T* k, long long ldk, const T* v, long long ldv) {
   hyb_pdl_enter();
   constexpr float MOST = FMT == THA_KV8_INT8 ? 127.f : 448.f;
@@ -212,12 +224,24 @@ __global__ void __launch_bounds__(32 * KW_WARPS, 2) kv8_write_kernel(tha_rows_t 
       units = p0 >= 0 ? ((p_end - 1) >> sh) - (p0 >> sh) : 0;
       open = (is_v ? kv.v_open : kv.k_open) + (live ? kv8_tile(kv, slot, layer, h) * (size_t)B * W : 0);
       src = (is_v ? v : k) + (long long)r0 * ld + (live ? (long long)h * W : 0);
+      if (ENDS && p0 >= 0 && unit == 0 && live && (p0 & (B - 1))) {
+        // rows of the block ahead of p0 that the open rows do not hold (they are a later block's): from the codes
+        const int lead = p0 & (B - 1), e = kv.open_end[2 * kv8_tile(kv, slot, layer, h) + is_v];
+        if (e >= 0 && (e < p0 || e > p0 - lead + B)) {
+          const int id = kv8_block(kv, slot, p0);
+          const size_t tile = id >= 0 ? kv8_tile(kv, id, layer, h) : 0;
+          kv8_back_from_codes<FMT>(pool + (tile * B + KW_ROWS * part) * W, id >= 0 ? scales + tile : nullptr, min(max(lead - KW_ROWS * part, 0), KW_ROWS) * w4, open + KW_ROWS * part * W);
+        }
+      }
     }
     if (p0 < 0) continue;
     make((p0 >> sh) + unit);
     // The thread block of a sequence's first block also makes its last one, because it reads the slot's open rows (behind make's barrier they have been read) and the last one
     // replaces them.
     if (unit == 0 && units > 0) make((p_end - 1) >> sh);
+    // what the open rows hold now: the last block's, or, where that is full, the first's ahead of p0 as before.  All warps of the tile have read the number ahead of make's barrier.
+    if (ENDS && unit == 0 && live && part == 0 && lane == 0)
+      kv.open_end[2 * kv8_tile(kv, slot, layer, h) + is_v] = p_end & (B - 1) ? p_end : p0 & (B - 1) ? p0 : 0;
   }
 }
 
@@ -312,7 +336,9 @@ static int write_launch(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t*
     THA_CUDA_OK(launch(kernel, dim3(ceil_div(units, each), groups, 2), dim3(32 * KW_WARPS), 0, s, pdl_enabled() != 0, *rows, *kv, layer, each, k, ldk, v, ldv));
     return THA_STATUS_SUCCESS;
   };
-  return kv->dim == 128 && kv->vdim == 128 ? go(kv8_write_kernel<T, FMT, VEC, true>) : go(kv8_write_kernel<T, FMT, VEC, false>);
+  const bool full = kv->dim == 128 && kv->vdim == 128;
+  if (kv->open_end) return full ? go(kv8_write_kernel<T, FMT, VEC, true, true>) : go(kv8_write_kernel<T, FMT, VEC, false, true>);
+  return full ? go(kv8_write_kernel<T, FMT, VEC, true, false>) : go(kv8_write_kernel<T, FMT, VEC, false, false>);
 }
 template <typename T>
 static int write_form(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* kv, int layer, const T* k, long long ldk, const T* v, long long ldv) {

@@ -35,7 +35,7 @@ AttnStruct = _struct("tha_attn_t", [("heads kv_heads dim vdim rot unit_rms", I),
                                     ("conv_state_off", L), ("conv_b", P), ("v_is_k", I), ("q_norm k_norm", P), ("softcap", F), ("b_o", P), ("head_norm", I),
                                     ("rel", P), ("rel_n v_mix v_mix_layer", I), ("v_mix_lambda", F)])
 Kv8Struct = _struct("tha_kv8_t", [("k_pool v_pool k_scale v_scale k_open v_open table", P),
-                                  ("table_stride block_size n_blocks n_cache_layers kv_heads dim vdim format", I)])
+                                  ("table_stride block_size n_blocks n_cache_layers kv_heads dim vdim format", I), ("open_end", P)])
 STRUCTS = (RowsStruct, AttnStruct, Kv8Struct)
 
 # the number of the current stream of a device; the public call makes an object around it first, 3.3 us
@@ -134,9 +134,11 @@ class Attention:
 
 class Kv8Cache:
     """Pools of codes [blocks, layers, kv heads, block size, channels] (int8 or float8_e4m3fn), their scales [blocks, layers, kv heads], the fp32 rows of every slot's last
-    block [slots, layers, kv heads, block size, channels] and the block table [slots, blocks per slot] int32.  k_open, v_open None: a cache that is only read."""
+    block [slots, layers, kv heads, block size, channels] and the block table [slots, blocks per slot] int32.  k_open, v_open None: a cache that is only read.
+    open_end [slots, layers, kv heads, 2] int32, at first -1: with it a slot may be written again from any position, across a border of blocks too; `empty` makes one.  It says behind which
+    position the rows of k_open, v_open end: a host that fills those sets it, or -1."""
 
-    def __init__(self, k_pool, v_pool, k_scale, v_scale, k_open, v_open, table):
+    def __init__(self, k_pool, v_pool, k_scale, v_scale, k_open, v_open, table, open_end=None):
         if k_pool.dtype not in FORMATS or v_pool.dtype != k_pool.dtype:
             raise ValueError(f"pools of int8 or float8_e4m3fn are needed, got {k_pool.dtype} and {v_pool.dtype}")
         if k_pool.dim() != 5 or v_pool.dim() != 5 or k_pool.shape[:4] != v_pool.shape[:4] or not k_pool.is_contiguous() or not v_pool.is_contiguous():
@@ -155,11 +157,16 @@ class Kv8Cache:
                                ("k_open", k_open, table.shape[0] * layers * heads * size * dim), ("v_open", v_open, table.shape[0] * layers * heads * size * vdim)):
             if t is not None:
                 _floats(name, t, count, dev)
+        if open_end is not None:
+            _ints("open_end", open_end, 2 * table.shape[0] * layers * heads)
+            if open_end.device != dev:
+                raise ValueError(f"open_end is on {open_end.device}, k_pool on {dev}")
         self.k_pool, self.v_pool, self.k_scale, self.v_scale, self.k_open, self.v_open, self.table = k_pool, v_pool, k_scale, v_scale, k_open, v_open, table
+        self.open_end = open_end
         self.device, self.kw, self.vw = dev, heads * dim, heads * vdim
         at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         self.c = Kv8Struct(at(k_pool), at(v_pool), at(k_scale), at(v_scale), at(k_open), at(v_open), at(table), table.shape[1], size, blocks, layers, heads, dim, vdim,
-                           FORMATS[k_pool.dtype])
+                           FORMATS[k_pool.dtype], at(open_end))
         self.ref, self.lib, self.slots = C.byref(self.c), lib(), table.shape[0]
         self.calls = self.lib.c
 
@@ -170,7 +177,8 @@ class Kv8Cache:
         codes = lambda w: torch.zeros(blocks, layers, kv_heads, block_size, w, dtype=torch.int8, device=device).view(dtype)  # noqa: E731
         scale = lambda: torch.zeros(blocks, layers, kv_heads, device=device)  # noqa: E731
         rows = lambda w: torch.zeros(slots, layers, kv_heads, block_size, w, device=device)  # noqa: E731
-        return cls(codes(dim), codes(vdim), scale(), scale(), rows(dim), rows(vdim), torch.zeros(slots, table_stride, dtype=torch.int32, device=device))
+        return cls(codes(dim), codes(vdim), scale(), scale(), rows(dim), rows(vdim), torch.zeros(slots, table_stride, dtype=torch.int32, device=device),
+                   torch.full((slots, layers, kv_heads, 2), -1, dtype=torch.int32, device=device))
 
     def _stream(self, rows):
         if rows.device != self.device:

@@ -652,13 +652,16 @@ typedef struct {
   int n_blocks, n_cache_layers;
   int kv_heads, dim, vdim; /* dim, vdim: multiples of 16 up to 128 */
   int format;           /* THA_KV8_* */
+  int* open_end;        /* nullable, [slot][cache layer][kv head][K, V]: the position behind the rows that k_open (v_open) hold, kept by tha_hyb_kv8_write; -1: not known.  A host that
+                           fills k_open itself sets it, or -1 */
 } tha_kv8_t;
 
 /* In the calls below the rows of a sequence are at consecutive positions; a sequence of one row at a negative position is idle. */
 
 /* Rows enter the cache: row r's heads are kv_heads * dim values at k + r * ldk and kv_heads * vdim at v + r * ldv (dtype-typed, pitches in elements).  The first
  * row of a sequence is at the position behind the slot's last one, or at any earlier one of the same block, or at the start of a block: rows of its block ahead of it are those of
- * k_open, v_open.  What the slot held from that position on is gone.  A step brings at most one sequence of a slot, and no two of its sequences write one block.  Idle sequences write nothing. */
+ * k_open, v_open.  With open_end it may be at any earlier position: where k_open holds the rows of another block by then (tokens are dropped across a border of blocks), the rows ahead of
+ * it are the values that their codes stand for.  What the slot held from that position on is gone.  A step brings at most one sequence of a slot, and no two of its sequences write one block.  Idle sequences write nothing. */
 int tha_hyb_kv8_write(void* stream, int dtype, const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const void* k, long long ldk, const void* v,
                       long long ldv);
 /* Cache rows as the values they stand for, rounded once to dtype: k_out [n_rows, ldk], v_out (either NULL: not wanted); pitches in elements.  Idle rows read as zeros. */

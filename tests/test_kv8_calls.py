@@ -73,3 +73,14 @@ def test_a_wait_that_gives_up_shows_in_its_rows():
     assert len(waits) >= 4 and max(waits) < gave_up < joined < softmax.index("if (l != l) m = l;") < softmax.index("k8_final(")
     assert all("ok" in softmax[softmax.rindex("\n", 0, w):softmax.index("\n", w)] for w in waits)
     assert not re.search(r"if \([^)]*\bok\b[^)]*\)", softmax[joined:])
+
+
+def test_open_end_is_refused_where_it_does_not_fit():
+    good = K.Kv8Cache.empty(blocks=4, layers=3, kv_heads=2, block_size=16, dim=32, slots=2, table_stride=2, device="cpu")
+    assert bool((good.open_end == -1).all()) and good.c.open_end == good.open_end.data_ptr()
+    parts = (good.k_pool, good.v_pool, good.k_scale, good.v_scale, good.k_open, good.v_open, good.table)
+    assert K.Kv8Cache(*parts).c.open_end is None
+    assert K.Kv8Cache(*parts, torch.zeros(2 * 3 * 2 * 2, dtype=torch.int32)).open_end is not None
+    for bad in (torch.zeros(2, 3, 2, 2), torch.zeros(2, 3, 2, dtype=torch.int32), torch.zeros(2, 3, 2, 4, dtype=torch.int32)[..., ::2]):
+        with pytest.raises(ValueError):
+            K.Kv8Cache(*parts, bad)
