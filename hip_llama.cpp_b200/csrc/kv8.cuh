@@ -115,6 +115,8 @@ __host__ __device__ __forceinline__ size_t k8_partial_floats(int splits, size_t 
 // host side: kv8_rows.cu
 int kv8_check(const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const char* who);
 int kv8_refuse(const char* who, const char* why);
+// whether every operand of the products is two fp16: portions with bf16 results take one, unless the caller asks for fp32 scores
+inline bool kv8_exact(const tha_attn_t* a, int dtype) { return dtype == THA_DT_F32 || a->fp32_scores; }
 // kv8_attn_tc.cu: sequences of at least min_rows rows; THA_STATUS_NOT_SUPPORTED (nothing launched): the caller takes another form
 int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int most_tiles);
 size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int most_tiles, int min_rows);

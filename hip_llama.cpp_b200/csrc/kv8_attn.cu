@@ -518,11 +518,11 @@ static int k8_form(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_row
 struct Kv8Forms { int short_rows; bool has_short, has_long; };
 // The two forms' times, in us, for n_seqs sequences of n rows that see `keys` keys at most, from what both were measured to take.  kv8_attn_kernel: 8, and 0.75 (heads up to 64 channels:
 // 0.44) for a tile of 32 keys of one of 444 blocks, six of them beside its keys.  kv8_attn_tc_kernel: 21, 1.6 for 10000 staged keys of a head, and for a tile of 64 keys of a block on one of 148
-// SMs 0.6 (128 pairs, bf16 results), 2.4 (256 pairs, fp32), with 64 channels 0.48 and 0.81 (128 pairs).  Model / measured, short and long: 32 heads of 128, 128 rows 16 / 16 and 22 / 16,
+// SMs 0.6 (128 pairs, one fp16 an operand), 2.4 (256 pairs, two), with 64 channels 0.48 and 0.81 (128 pairs).  Model / measured, short and long: 32 heads of 128, 128 rows 16 / 16 and 22 / 16,
 // 1024 rows 161 / 150 and 37 / 35, 128 rows behind 4000 keys 125 / 127 and 49 / 58; 16 on 4, 64 rows behind 4000 keys 37 / 38 and 28 / 28; 256 rows 19 / 19 and 22 / 14.
 static bool k8_long_pays(const tha_attn_t* a, const tha_rows_t* rows, int dtype, long long keys, int n) {
   const int gsize = a->heads / a->kv_heads;
-  const bool wide = a->dim > 64 || a->vdim > 64, exact = dtype == THA_DT_F32;
+  const bool wide = a->dim > 64 || a->vdim > 64, exact = kv8_exact(a, dtype);
   const float seqs = (float)rows->n_seqs, pairs = (float)n * gsize, seen = keys > n ? (float)keys - 0.5f * n : 0.5f * keys;
   const float blocks = ceilf(pairs / K8_PAIRS) * a->kv_heads * seqs;
   const float as_short = 8.f + (wide ? 0.75f : 0.44f) * blocks * (seen / 32.f + 6.f) / 444.f;

@@ -4,7 +4,7 @@
 // Codes are fp16 numbers.  A step's visible keys and values are turned into fp16 once (kv8_stage_kernel), without scales, into scratch that holds tiles as they will lie in shared
 // memory, from where bulk copies fetch them: warps of the block that did it themselves, tile by tile and again for every 256 rows, took half of the SM's issue slots (8000
 // instructions of 32 lanes a tile instead of 3500).  K's scale belongs to 16 or more neighbouring keys and multiplies their scores, V's multiplies their weights, relative to a power of two
-// that all of a row's weights share.  q is brought to [2^14, 2^15) by a power of two a row and rounded to one fp16 (bf16 results) or two (SPLIT: fp32 results, 22 bits; weights
+// that all of a row's weights share.  q is brought to [2^14, 2^15) by a power of two a row and rounded to one fp16 (bf16 results) or two (SPLIT: fp32 results or fp32 scores asked for, 22 bits; weights
 // likewise), each product fp32.  A row's power of two is that of the scales that it sees itself: with one for the block's rows, a row lost as many bits as the scale of a block
 // hidden from it was larger.
 // A block takes 128 pairs of one key/value head (with two fp16 an operand and heads beyond 64 channels 256, two groups of 128 that share every tile) and a run of tiles of 64 keys.
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
 }
 
 static int kt_positions(const tha_attn_t* a, int dtype) {
-  return kt_groups(dtype == THA_DT_F32, a->dim > 64 || a->vdim > 64 ? 128 : 64) * KT_ROWS / (a->heads / a->kv_heads);
+  return kt_groups(kv8_exact(a, dtype), a->dim > 64 || a->vdim > 64 ? 128 : 64) * KT_ROWS / (a->heads / a->kv_heads);
 }
 // Sequences of at least min_rows rows that a step has at most.  (From the rows alone: the longest portion that a caller names may be one that no sequence has.)
 static long long kt_sequences(const tha_rows_t* rows, int min_rows) { return rows->n_rows / min_rows < rows->n_seqs ? rows->n_rows / min_rows : rows->n_seqs; }
@@ -633,7 +633,7 @@ static long long kt_blocks(const tha_attn_t* a, const tha_rows_t* rows, int dtyp
 
 // Parts of a context, most_tiles: of 32 keys.
 int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int most_tiles) {
-  const int each = 3 - kt_groups(dtype == THA_DT_F32, a->dim > 64 || a->vdim > 64 ? 128 : 64);   // blocks an SM
+  const int each = 3 - kt_groups(kv8_exact(a, dtype), a->dim > 64 || a->vdim > 64 ? 128 : 64);   // blocks an SM
   const long long blocks = (long long)ceil_div(rows->n_rows, kt_positions(a, dtype)) * a->kv_heads;
   long long s = each * 148 / blocks;
   if (s > most_tiles / 16) s = most_tiles / 16;       // eight tiles each at least
@@ -650,7 +650,7 @@ size_t kv8_attn_tc_stage_bytes(const tha_attn_t* a, const tha_rows_t* rows, int 
 int kv8_attn_tc_room_for(const tha_attn_t* a, int most_tiles) { return (int)(KT_MOST_STAGED / (kt_part_bytes(a) * most_tiles)); }
 
 template <int DT, int FMT, bool SPLIT, bool MORE, typename T>
-static int kt_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int min_rows, int most_tiles, int splits,
+static int kt_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int min_rows, int most_tiles, int splits,
                      unsigned char* staged, float* partial, const float* gate, long long ldg) {
   int* flag = nullptr;                               // allocated by a device's first call, which a capture allows in this mode
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
@@ -667,19 +667,19 @@ static int kt_launch(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows
                      pdl_enabled() != 0, *a, *rows, *kv, min_rows, (int)parts, staged, scales));
   auto k = kv8_attn_tc_kernel<DT, FMT, SPLIT, MORE, T>;
   THA_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kt_smem(SPLIT, DT)));
-  THA_CUDA_OK(launch(k, dim3(a->kv_heads, (unsigned)(kt_blocks(a, rows, SPLIT ? THA_DT_F32 : THA_DT_BF16, min_rows) * splits)), dim3(kt_threads(SPLIT, DT)), kt_smem(SPLIT, DT), s, pdl_enabled() != 0, *a, *rows,
-                     (const unsigned char*)staged, (const float4*)scales, q, out, kt_positions(a, SPLIT ? THA_DT_F32 : THA_DT_BF16), min_rows, splits, partial, gate, ldg, flag));
+  THA_CUDA_OK(launch(k, dim3(a->kv_heads, (unsigned)(kt_blocks(a, rows, dtype, min_rows) * splits)), dim3(kt_threads(SPLIT, DT)), kt_smem(SPLIT, DT), s, pdl_enabled() != 0, *a, *rows,
+                     (const unsigned char*)staged, (const float4*)scales, q, out, kt_positions(a, dtype), min_rows, splits, partial, gate, ldg, flag));
   return THA_STATUS_SUCCESS;
 }
 template <int DT, bool SPLIT, typename T>
-static int kt_form(cudaStream_t s, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int min_rows, int most_tiles, int splits,
+static int kt_form(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, T* out, int min_rows, int most_tiles, int splits,
                    unsigned char* staged, float* partial, const float* gate, long long ldg) {
   const bool more = a->softcap > 0.f || a->rel;
   if (kv->format == THA_KV8_INT8)
-    return more ? kt_launch<DT, THA_KV8_INT8, SPLIT, true>(s, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg)
-                : kt_launch<DT, THA_KV8_INT8, SPLIT, false>(s, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg);
-  return more ? kt_launch<DT, THA_KV8_E4M3, SPLIT, true>(s, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg)
-              : kt_launch<DT, THA_KV8_E4M3, SPLIT, false>(s, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg);
+    return more ? kt_launch<DT, THA_KV8_INT8, SPLIT, true>(s, dtype, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg)
+                : kt_launch<DT, THA_KV8_INT8, SPLIT, false>(s, dtype, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg);
+  return more ? kt_launch<DT, THA_KV8_E4M3, SPLIT, true>(s, dtype, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg)
+              : kt_launch<DT, THA_KV8_E4M3, SPLIT, false>(s, dtype, a, rows, kv, q, out, min_rows, most_tiles, splits, staged, partial, gate, ldg);
 }
 
 // staged: as many bytes as kv8_attn_tc_stage_bytes says, on a 16-byte boundary
@@ -690,12 +690,14 @@ int kv8_attn_tc_launch(cudaStream_t s, int dtype, const tha_attn_t* a, const tha
   auto st = (unsigned char*)staged;
   if (dtype == THA_DT_BF16) {
     auto o = (__nv_bfloat16*)out;
-    return wide ? kt_form<128, false>(s, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg)
-                : kt_form<64, false>(s, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg);
+    if (kv8_exact(a, dtype)) return wide ? kt_form<128, true>(s, dtype, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg)
+                                         : kt_form<64, true>(s, dtype, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg);
+    return wide ? kt_form<128, false>(s, dtype, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg)
+                : kt_form<64, false>(s, dtype, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg);
   }
   auto o = (float*)out;
-  return wide ? kt_form<128, true>(s, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg)
-              : kt_form<64, true>(s, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg);
+  return wide ? kt_form<128, true>(s, dtype, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg)
+              : kt_form<64, true>(s, dtype, a, rows, kv, q, o, min_rows, most_tiles, splits, st, partial, gate, ldg);
 }
 
 }  // namespace tha

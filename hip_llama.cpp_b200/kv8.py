@@ -99,10 +99,11 @@ class Rows:
 
 class Attention:
     """The attention of a layer as far as a call over a cache goes (tha_attn_t, whose comments say what each argument does).  sink, head_scale: [heads], rel: [heads, n],
-    fp32 on the device.  head_gate: sigmoid of column gate_column + h of `proj` scales head h's result."""
+    fp32 on the device.  head_gate: sigmoid of column gate_column + h of `proj` scales head h's result.  fp32_scores: q and the
+    softmax weights keep 22 bits in long portions with bf16 results too, as they do everywhere else."""
 
     def __init__(self, heads: int, kv_heads: int, dim: int, vdim: int | None = None, *, scale: float, chunk: int = 0, window: int = 0, keep_first: int = 0, sink=None,
-                 head_scale=None, softcap: float = 0.0, rel=None, head_gate: bool = False, gate_column: int = 0):
+                 head_scale=None, softcap: float = 0.0, rel=None, head_gate: bool = False, gate_column: int = 0, fp32_scores: bool = False):
         for name, t, count in (("sink", sink, heads), ("head_scale", head_scale, heads)):
             if t is not None:
                 _floats(name, t, count, t.device)
@@ -117,7 +118,8 @@ class Attention:
         vdim = dim if vdim is None else vdim
         at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         self.c = AttnStruct(heads=heads, kv_heads=kv_heads, dim=dim, vdim=vdim, rot=-1, scale=scale, chunk=chunk, window=window, keep_first=keep_first, sink=at(sink),
-                            head_scale=at(head_scale), softcap=softcap, rel=at(rel), rel_n=0 if rel is None else rel.shape[1], head_gate=int(head_gate), o_g=gate_column)
+                            head_scale=at(head_scale), softcap=softcap, rel=at(rel), rel_n=0 if rel is None else rel.shape[1], head_gate=int(head_gate), o_g=gate_column,
+                            fp32_scores=int(fp32_scores))
         self.ref = C.byref(self.c)
         self.heads, self.q_width, self.out_width, self.gate = heads, heads * dim, heads * vdim, gate_column if head_gate else None
         self._of = {}

@@ -668,11 +668,11 @@ int tha_hyb_kv8_write(void* stream, int dtype, const tha_rows_t* rows, const tha
 int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, void* k_out, long long ldk, void* v_out,
                      long long ldv);
 /* tha_hyb_attn_gated over such a cache: every row attends to the visible keys as the cache holds them, which for rows of a block that is not full are their codes
- * under its present scale.  a: heads, kv_heads, dim, vdim, scale, chunk, cache_layer, window, keep_first, sink, head_scale, softcap, rel, head_gate and out_f32 as there
+ * under its present scale.  a: heads, kv_heads, dim, vdim, scale, chunk, cache_layer, window, keep_first, sink, head_scale, softcap, rel, head_gate, fp32_scores and out_f32 as there
  * (values_in_keys, v_share and diff are refused); q fp32 [n_rows, heads * dim]; out dtype-typed [n_rows, heads * vdim].  Idle rows get zeros.
  * Codes are exact in fp16; q and the weights, each times its value's scale, enter the products as two fp16.  A number of q is off by 2^-22 of itself or 2^-39 of the largest
  * of its row of a head, whichever is more; a weight by 2^-22 of itself or 2^-29 of the row's largest weight times the largest scale that the row sees.  Rows of longer portions with dtype
- * THA_DT_BF16 use one fp16: 2^-11 of itself instead of 2^-22.  Sums and softmax are fp32.  Which portions are long goes by the step: heads, keys, rows.
+ * THA_DT_BF16 use one fp16, 2^-11 of itself instead of 2^-22, unless fp32_scores asks for two.  Sums and softmax are fp32.  Which portions are long goes by the step: heads, keys, rows.
  * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones (it goes by how many
  * sequences of the step may be long at all, n_rows over the rows of a long one, each as far as the longest context; where that were more than 1 GiB, the shorter portions take the
  * form of short ones, and all do behind a context that needs so much by itself), and for partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may

@@ -50,7 +50,7 @@ def expected(a, q, keys, values, p0, eps_more=0.0):
     return out, far
 
 
-def check(m, a, parts, dtype, seed=5, tiles=None, most=0):
+def check(m, a, parts, dtype, seed=5, tiles=None, most=0, fp32_scores=False):
     """The rows of `parts` over m's cache: no number further off than its bound."""
     heads = a["heads"]
     assert tiles is None or T.takes_tiles(a, m, parts, dtype) == tiles
@@ -59,14 +59,14 @@ def check(m, a, parts, dtype, seed=5, tiles=None, most=0):
     q = torch.randn(n, heads * m.dim, device="cuda", generator=g)
     dev = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda()  # noqa: E731
     at = K.Attention(heads, m.H, m.dim, m.vdim, scale=a["scale"], chunk=a.get("chunk", 0), window=a.get("window", 0), keep_first=a.get("keep_first", 0), sink=dev(a.get("sink")),
-                     head_scale=dev(a.get("head_scale")), softcap=a.get("softcap", 0.0), rel=dev(a.get("rel")))
+                     head_scale=dev(a.get("head_scale")), softcap=a.get("softcap", 0.0), rel=dev(a.get("rel")), **({"fp32_scores": True} if fp32_scores else {}))
     rows = K.Rows.of(parts)
     rows.c.max_pos = max(rows.c.max_pos, most)                   # a step may be described by more than it has
     got = m.cache.attend(at, rows, q, layer=LAYER, dtype=dtype).double().cpu().numpy().reshape(n, heads, m.vdim)
     qn, row, worst = q.double().cpu().numpy().reshape(n, heads, m.dim), 0, 0.0
     for slot, p, c in parts:
         if p >= 0:
-            want, far = expected(a, qn[row:row + c], m.values("k", slot, p + c), m.values("v", slot, p + c), p, 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
+            want, far = expected(a, qn[row:row + c], m.values("k", slot, p + c), m.values("v", slot, p + c), p, 2.0 ** -11 if dtype == torch.bfloat16 and not fp32_scores else 0.0)
             far = far + np.abs(want) * (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) + 1e-44
             worst = max(worst, float((np.abs(got[row:row + c] - want) / far).max()))
         else:
@@ -220,3 +220,12 @@ def test_no_kernel_gave_up():
     m = T.filled(16, 4, 128, 128, "int8", (900,))
     check(m, dict(heads=16, scale=0.1), [(0, 300, 600)], torch.float32, tiles=True)
     m.cache.check_error()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim,fmt,mask", [(16, 4, 128, 128, "int8", dict()), (20, 4, 64, 48, "e4m3", dict(window=400, keep_first=4)), (12, 4, 112, 128, "e4m3", dict(softcap=5.0)),
+                                                              (8, 8, 64, 64, "int8", dict())])
+@pytest.mark.parametrize("parts", [[(0, 0, 700), (1, 0, 40), (2, 100, 1)], [(0, 2500, 200)]], ids=["prompt", "behind"])
+def test_fp32_scores_with_bf16_results(heads, kv_heads, dim, vdim, fmt, mask, parts):
+    """A caller that asks for fp32 scores gets the bounds of fp32 results and the last rounding, however long a portion is."""
+    m = T.filled(16, kv_heads, dim, vdim, fmt, [p + n for _, p, n in parts])
+    check(m, dict(mask, heads=heads, scale=dim ** -0.5), parts, torch.bfloat16, tiles=None if mask else True, fp32_scores=True)
