@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include "kv8.cuh"
+#include "workspace.h"
 
 namespace tha {
 
@@ -456,12 +457,12 @@ static int k8_pair_tiles(const tha_attn_t* a, const tha_rows_t* rows, int most) 
   const long long by_seqs = (long long)rows->n_seqs * (((long long)(most < rows->max_seq_rows ? most : rows->max_seq_rows) * gsize + K8_PAIRS - 1) / K8_PAIRS);
   return (int)(by_rows < by_seqs ? by_rows : by_seqs);
 }
-// Parts of a context.  444 blocks run at once, three on an SM; a block takes the time of six tiles of 32 keys (4 us) beside its own, the meeting of the parts as much.  One context:
+// Parts of a context.  Three blocks run at once on an SM, 444 on 148; a block takes the time of six tiles of 32 keys (4 us) beside its own, the meeting of the parts as much.  One context:
 // rounds of whole parts.  Several: their lengths are between nothing and the longest, blocks follow one another as they end, and the last of them is the tail.  us with 1 / 2 / 4 / 6 /
 // 10 / 20 parts, heads of 128: 64 contexts up to 2048 of 32 heads 125 / 136 / 162 / 192; 16 up to 8192 of 8 heads (3 parts: 69) 56 (4) / 50 / 51 / 59; one of 131072 of 8 heads with 18 /
 // 37 / 55 / 64 parts 145 / 83 / 63 / 74.
 static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows) {
-  constexpr int SLOTS = 3 * 148;
+  const int SLOTS = 3 * sm_budget();
   constexpr float BESIDE = 6.f;
   const int most = k8_most_tiles(a, rows);
   const long long blocks = (long long)k8_pair_tiles(a, rows, most_rows) * a->kv_heads;
@@ -516,18 +517,22 @@ static int k8_form(cudaStream_t s, int dtype, const tha_attn_t* a, const tha_row
 }
 // Which sequences take which form.  short_rows: up to so many rows take kv8_attn_kernel; has_short, has_long: whether the step may hold any.
 struct Kv8Forms { int short_rows; bool has_short, has_long; };
-// The two forms' times, in us, for n_seqs sequences of n rows that see `keys` keys at most, from what both were measured to take.  kv8_attn_kernel: 8, and 0.75 (heads up to 64 channels:
-// 0.44) for a tile of 32 keys of one of 444 blocks, six of them beside its keys.  kv8_attn_tc_kernel: 21, 1.6 for 10000 staged keys of a head, and for a tile of 64 keys of a block on one of 148
-// SMs 0.6 (128 pairs, one fp16 an operand), 2.4 (256 pairs, two), with 64 channels 0.48 and 0.81 (128 pairs).  Model / measured, short and long: 32 heads of 128, 128 rows 16 / 16 and 22 / 16,
-// 1024 rows 161 / 150 and 37 / 35, 128 rows behind 4000 keys 125 / 127 and 49 / 58; 16 on 4, 64 rows behind 4000 keys 37 / 38 and 28 / 28; 256 rows 19 / 19 and 22 / 14.
+// The two forms' times, in us, for n_seqs sequences of n rows that see `keys` keys at most, as both were measured over 1136 steps of 1 to 16 portions of 4 to 512 rows behind 0 to 70000 keys,
+// 2 to 64 heads on 1 to 32, 64 and 128 channels, both result types.  kv8_attn_kernel: 14.5, and 0.72 (heads up to 64 channels: 0.41) for a tile of 32 keys of one of 444 blocks, six of them
+// beside its keys.  kv8_attn_tc_kernel: 17, 1.45 for 10000 staged keys of a head, 8 where contexts are cut, and for a tile of 64 keys of a block on one of 148 SMs 1.0 (128 pairs, one fp16 an
+// operand) or 3.1 (256 pairs, two), but 0.5 or 1.2 for each of a block's own tiles at least; with 64 channels 0.64 and 1.15 (128 pairs).  What is chosen so is 0.6 % slower than the faster
+// form on the geometric mean, more than 10 % for 33 of the 1136, 48 % at worst (12 heads of 64, 256 rows, fp32: 38 for 26).  Model / measured, short and long: 32 heads of 128, 128 rows 22 / 22
+// and 18 / 17, 512 rows 64 / 65 and 23 / 28, 128 rows behind 4000 keys 126 / 140 and 58 / 60; 16 on 4, 64 rows behind 4000 keys 42 / 46 and 31 / 34; 256 rows 24 / 24 and 18 / 20.
 static bool k8_long_pays(const tha_attn_t* a, const tha_rows_t* rows, int dtype, long long keys, int n) {
   const int gsize = a->heads / a->kv_heads;
   const bool wide = a->dim > 64 || a->vdim > 64, exact = kv8_exact(a, dtype);
-  const float seqs = (float)rows->n_seqs, pairs = (float)n * gsize, seen = keys > n ? (float)keys - 0.5f * n : 0.5f * keys;
-  const float blocks = ceilf(pairs / K8_PAIRS) * a->kv_heads * seqs;
-  const float as_short = 8.f + (wide ? 0.75f : 0.44f) * blocks * (seen / 32.f + 6.f) / 444.f;
-  const float tiles = ceilf(pairs / (wide && exact ? 256.f : 128.f)) * a->kv_heads * seqs * seen / 64.f;
-  const float as_long = 21.f + 1.6e-4f * (wide ? 1.f : 0.5f) * keys * a->kv_heads * seqs + (wide ? (exact ? 2.4f : 0.6f) : (exact ? 0.81f : 0.48f)) * tiles / 148.f;
+  const float seqs = (float)rows->n_seqs, pairs = (float)n * gsize, seen = keys > n ? (float)keys - 0.5f * n : 0.5f * keys, sms = (float)sm_budget();
+  const float as_short = 14.5f + (wide ? 0.72f : 0.41f) * ceilf(pairs / K8_PAIRS) * a->kv_heads * seqs * (seen / 32.f + 6.f) / (3.f * sms);
+  const float blocks = ceilf(pairs / (wide && exact ? 256.f : 128.f)) * a->kv_heads * seqs;
+  float cut = floorf((wide && exact ? 1.f : 2.f) * sms / blocks);   // kv8_attn_tc_splits
+  cut = fmaxf(1.f, fminf(fminf(cut, (float)(keys / (32 * 16))), 16.f));
+  const float tiles = (wide ? (exact ? 3.1f : 1.0f) : (exact ? 1.15f : 0.64f)) * blocks * (seen / 64.f) / sms, alone = wide ? (exact ? 1.2f : 0.5f) * ceilf(seen / 64.f / cut) : 0.f;
+  const float as_long = 17.f + 1.45e-4f * (wide ? 1.f : 0.5f) * keys * a->kv_heads * seqs + (cut > 1.f ? 8.f : 0.f) + fmaxf(tiles, alone);
   return as_long < as_short;
 }
 static Kv8Forms k8_forms(const tha_attn_t* a, const tha_rows_t* rows, int dtype) {

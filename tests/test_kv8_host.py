@@ -182,8 +182,8 @@ def test_a_prompt_beside_decoded_rows_keeps_its_form(beside, most, rows_, dtype)
     need = 4 * K.lib().c.tha_hyb_kv8_attn_scratch(dtype, attn(heads=32, **big), r, c)
     one = 2 * (most + 1) * 32 * 2 * 128                           # of the prompt's context in fp16
     assert one <= need < (1 << 30) + (64 << 20)
-    # Portions of up to 29 rows are short ones: four blocks of eight of them take 4 * 32 * 0.75 us / 444 / 32 = 6.8 ns a key, staged ones at least 32 * 0.16 ns, and 32 * 0.6 us / 148 / 64
-    # for their tiles, 7.1 ns.  Portions of 30 rows or more are at most so many of the step.
+    # Portions of up to 29 rows are short ones: four blocks of eight of them take 4 * 32 * 0.72 us / 444 / 32 = 6.5 ns a key, staged ones at least 32 * 0.145 ns, and 32 * 1.0 us / 148 / 64
+    # for their tiles, 8.0 ns.  Portions of 30 rows or more are at most so many of the step.
     assert need <= max(1, min(1 + beside, (rows_ + beside) // 30)) * one * 1.1 + (64 << 20)
 
 
@@ -194,3 +194,20 @@ def test_portions_that_find_no_room_are_the_shorter_ones():
         r = rows(n_rows=n_rows, n_seqs=n_seqs, max_seq_rows=2048, max_pos=most)
         need = 4 * K.lib().c.tha_hyb_kv8_attn_scratch(0, attn(heads=32, **big), r, cache(**big, table_stride=8192, n_blocks=9000))
         assert (need >= 2 * most * 32 * 2 * 128) == there and need < (1 << 30) + (128 << 20)
+
+
+FASTER = [  # heads, kv heads, channels, fp32 results, sequences, first position, rows; us as short portions, us as long ones
+    (16, 4, 128, 0, 1, 0, 256, 23.6, 19.5), (32, 32, 128, 0, 4, 0, 64, 29.7, 17.4), (32, 8, 128, 0, 16, 0, 16, 27.6, 17.4), (12, 12, 64, 0, 16, 0, 64, 27.6, 17.4), (64, 8, 64, 0, 1, 0, 128, 22.5, 15.4),
+    (32, 32, 128, 1, 4, 0, 64, 29.7, 21.5), (32, 8, 128, 1, 1, 1000, 64, 27.6, 48.1), (16, 4, 128, 1, 1, 1000, 128, 29.7, 48.1), (8, 1, 128, 1, 1, 16000, 32, 44.0, 60.4),
+    (8, 1, 128, 1, 16, 16000, 128, 1422.3, 312.4), (32, 32, 128, 0, 1, 4000, 128, 140.2, 60.4), (16, 4, 128, 0, 1, 4000, 64, 46.1, 33.8)]
+
+
+@pytest.mark.parametrize("case", FASTER, ids=str)
+def test_portions_take_the_form_that_was_measured_to_be_faster(case):
+    """... by a quarter or more.  Staged keys are most of the scratch that the form of long ones asks for."""
+    heads, kv_heads, dim, dtype, seqs, p, n, short, long = case
+    assert max(short, long) >= 1.2 * min(short, long)
+    shape = dict(kv_heads=kv_heads, dim=dim, vdim=dim)
+    r = rows(n_rows=seqs * n, n_seqs=seqs, max_seq_rows=n, max_pos=p + n - 1)
+    floats = K.lib().c.tha_hyb_kv8_attn_scratch(dtype, attn(heads=heads, **shape), r, cache(**shape, table_stride=2048, n_blocks=40000))
+    assert (floats >= seqs * (p + n) * kv_heads * dim) == (long < short)
