@@ -635,7 +635,7 @@ static long long kt_blocks(const tha_attn_t* a, const tha_rows_t* rows, int dtyp
 int kv8_attn_tc_splits(const tha_attn_t* a, const tha_rows_t* rows, int dtype, int most_tiles) {
   const int each = 3 - kt_groups(kv8_exact(a, dtype), a->dim > 64 || a->vdim > 64 ? 128 : 64);   // blocks an SM
   const long long blocks = (long long)ceil_div(rows->n_rows, kt_positions(a, dtype)) * a->kv_heads;
-  long long s = each * 148 / blocks;
+  long long s = each * sm_budget() / blocks;
   if (s > most_tiles / 16) s = most_tiles / 16;       // eight tiles each at least
   return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }

@@ -9,6 +9,7 @@
 #include <stdio.h>
 
 #include "kv8.cuh"
+#include "workspace.h"
 
 namespace tha {
 
@@ -331,7 +332,7 @@ template <typename T, int FMT, bool VEC>
 static int write_launch(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* kv, int layer, const T* k, long long ldk, const T* v, long long ldv) {
   const int units = rows->max_seq_rows == 1 ? rows->n_seqs : rows->n_rows / kv->block_size + rows->n_seqs;
   const int groups = ceil_div(kv->kv_heads, KW_WARPS * KW_ROWS / kv->block_size);
-  const int each = units * groups >= 4 * 2 * 148 ? 4 : units * groups >= 2 * 2 * 148 ? 2 : 1;   // two rounds of two blocks on every SM, K and V
+  const int sms = sm_budget(), each = units * groups >= 8 * sms ? 4 : units * groups >= 4 * sms ? 2 : 1;   // two rounds of two blocks on every SM, K and V
   auto go = [&](auto kernel) -> int {
     THA_CUDA_OK(launch(kernel, dim3(ceil_div(units, each), groups, 2), dim3(32 * KW_WARPS), 0, s, pdl_enabled() != 0, *rows, *kv, layer, each, k, ldk, v, ldv));
     return THA_STATUS_SUCCESS;
@@ -351,7 +352,7 @@ template <typename T>
 static int read_form(cudaStream_t s, const tha_rows_t* rows, const tha_kv8_t* kv, int layer, T* k, long long ldk, T* v, long long ldv) {
   constexpr int V = 16 / (int)sizeof(T);
   const bool vec = ((k ? ldk : 0) | (v ? ldv : 0)) % V == 0 && aligned16(k) && aligned16(v);
-  const int R = rows->n_rows > 2 * 148 * KR_ROWS ? KR_ROWS : 1;   // blocks for every SM first: 700 rows of 4 heads 8.1 us one by one, 9.5 in pairs
+  const int R = rows->n_rows > 2 * sm_budget() * KR_ROWS ? KR_ROWS : 1;   // blocks for every SM first: 700 rows of 4 heads 8.1 us one by one, 9.5 in pairs
   const int words = R * kv->kv_heads * (kv->dim > kv->vdim ? kv->dim : kv->vdim) / V;
   const dim3 grid(ceil_div(rows->n_rows, R), 2), block(words > 128 ? 256 : words > 64 ? 128 : 64);
   auto go = [&](auto kernel) -> int {
