@@ -229,3 +229,21 @@ def test_fp32_scores_with_bf16_results(heads, kv_heads, dim, vdim, fmt, mask, pa
     """A caller that asks for fp32 scores gets the bounds of fp32 results and the last rounding, however long a portion is."""
     m = T.filled(16, kv_heads, dim, vdim, fmt, [p + n for _, p, n in parts])
     check(m, dict(mask, heads=heads, scale=dim ** -0.5), parts, torch.bfloat16, tiles=None if mask else True, fp32_scores=True)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,fmt,parts", [(16, 4, 128, "int8", [(0, 0, 1000)]), (16, 4, 128, "e4m3", [(0, 1500, 500)]), (32, 8, 64, "int8", [(0, 800, 700)])])
+def test_bf16_results_of_prompts_are_little_more_than_their_rounding_off(heads, kv_heads, dim, fmt, parts):
+    """For every row over its heads, and for every head over its rows.  A number rounded to fp16 is off by 2^-11 / 3^1/2 of it or, its place in the binade taken in, 2.0e-4 (rms).  A score is
+    sum q k / dim^1/2 with q, k of order one: errors of q make 2.0e-4 of it; a weight's are as large, and results, sums of values that do not agree, are off by 2^1/2 times that of themselves,
+    2.8e-4; 4.5e-4 is allowed beside the rounding itself, which is what it is for the exact result.  A row's 1024 values or more have an rms within 15 %, a head's within 5 %.  (Weights of
+    three bits fewer: 1.6e-3 beside 1.65e-3.)"""
+    m = T.filled(16, kv_heads, dim, dim, fmt, [p + n for _, p, n in parts])
+    a, (slot, p, n) = dict(heads=heads, scale=dim ** -0.5), parts[0]
+    got = check(m, a, parts, torch.bfloat16, tiles=True)
+    q = torch.randn(n, heads * dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).double().cpu().numpy().reshape(n, heads, dim)
+    want, _ = expected(a, q, m.values("k", slot, p + n), m.values("v", slot, p + n), p)
+    rounded = torch.from_numpy(want).to(torch.bfloat16).double().numpy()
+    for axes, slack in (((1, 2), 1.15), ((0, 2), 1.05)):
+        size = np.sqrt((want ** 2).mean(axes))
+        off, least = np.sqrt(((got - want) ** 2).mean(axes)) / size, np.sqrt(((rounded - want) ** 2).mean(axes)) / size
+        assert (off < slack * np.sqrt(least ** 2 + 4.5e-4 ** 2)).all()
