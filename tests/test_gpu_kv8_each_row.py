@@ -247,3 +247,90 @@ def test_bf16_results_of_prompts_are_little_more_than_their_rounding_off(heads, 
         size = np.sqrt((want ** 2).mean(axes))
         off, least = np.sqrt(((got - want) ** 2).mean(axes)) / size, np.sqrt(((rounded - want) ** 2).mean(axes)) / size
         assert (off < slack * np.sqrt(least ** 2 + 4.5e-4 ** 2)).all()
+
+
+def prompt_of(m, heads, parts, dtype, seed):
+    """(call, result of an eager call) of a step over m's cache"""
+    n = sum(x[2] for x in parts)
+    at, rows = K.Attention(heads, m.H, m.dim, m.vdim, scale=m.dim ** -0.5), K.Rows.of(parts)
+    q = torch.randn(n, heads * m.dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+    return lambda: m.cache.attend(at, rows, q, layer=LAYER, dtype=dtype)
+
+
+PROMPTS = [(16, [(0, 0, 700), (1, 290, 10), (2, 900, 1)], torch.bfloat16), (16, [(0, 300, 600), (2, 0, 900)], torch.float32), (32, [(1, 299, 1), (0, 899, 1)], torch.float32),
+           (32, [(1, 0, 300)], torch.bfloat16)]
+
+
+def test_prompts_captured_and_replayed():
+    """Four steps, prompts, portions and single rows, each in a graph of its own: replayed in any order, with other calls between them, they give the eager calls' bits."""
+    m = T.filled(16, 4, 128, 128, "int8", (900, 300, 901))
+    calls = [prompt_of(m, h, parts, dt, i) for i, (h, parts, dt) in enumerate(PROMPTS)]
+    want = [c().clone() for c in calls]
+    torch.cuda.synchronize()
+    graphs = []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = c()
+        graphs.append((g, out))
+    for order in ((0, 1, 2, 3), (3, 1, 1, 0), (2, 0, 3, 1)):
+        for _, out in graphs:
+            out.fill_(float("nan"))
+        for i in order:
+            graphs[i][0].replay()
+            calls[3 - i]()
+        torch.cuda.synchronize()
+        for i in set(order):
+            assert torch.equal(graphs[i][1], want[i]), i
+    m.cache.check_error()
+
+
+def test_prompts_side_by_side():
+    """The same steps on four streams at once, again and again."""
+    m = T.filled(16, 4, 128, 128, "int8", (900, 300, 901))
+    calls = [prompt_of(m, h, parts, dt, i) for i, (h, parts, dt) in enumerate(PROMPTS)]
+    want = [c().clone() for c in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], []
+    for _ in range(15):
+        for i, (s, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                got.append((i, c()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i]) for i, out in got)
+    m.cache.check_error()
+
+
+def test_threads_with_layers_of_their_own():
+    """Two threads, one attention, two layers: each gets its layer's rows."""
+    import threading
+    c = K.Kv8Cache.empty(blocks=40, layers=3, kv_heads=2, block_size=16, dim=64, slots=1, table_stride=40)
+    c.table.copy_(torch.arange(40, dtype=torch.int32)[None])
+    rows, at, q = K.Rows.of([(0, 0, 300)]), K.Attention(8, 2, 64, scale=0.125), torch.randn(1, 512, device="cuda")
+    for layer in range(3):
+        c.write(rows, *(torch.randn(300, 128, device="cuda") for _ in "kv"), layer=layer)
+    one = K.Rows.of([(0, 299, 1)])
+    want = [c.attend(at, one, q, layer=layer) for layer in range(3)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(layer):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(200):
+                if not torch.equal(c.attend(at, one, q, layer=layer), want[layer]):
+                    bad.append(layer)
+
+    threads = [threading.Thread(target=work, args=(layer,)) for layer in (0, 1, 2, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not bad
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(130, 1), (384, 2), (1, 1), (7, 7)])
+@pytest.mark.parametrize("parts", [[(0, 199, 1), (1, 0, 1)], [(0, 50, 90), (1, 0, 1)]], ids=["singles", "portion"])
+def test_unusual_numbers_of_heads(heads, kv_heads, parts):
+    m = T.filled(16, kv_heads, 64, 128, "int8", (200, 1))
+    for dtype in (torch.float32, torch.bfloat16):
+        check(m, dict(heads=heads, scale=0.125), parts, dtype)
