@@ -13,8 +13,9 @@
 // power of two) ahead of the split; scales that a mask hides from a pair cost it nothing.  Weights have the factor 2^15, so that the 22 bits reach down to 2^-28 of the largest.
 //
 // Bound: the cache's bytes where nothing else is; here the instructions that turn them into fp16 pairs (int8: five for four codes of K, six of V) and the chain of a tile, which
-// three blocks on an SM (168 registers, a ring of two tiles a warp) hide better than two (217 registers, three tiles: 168 us where these take 146).  One context of 131072 keys, 8
-// heads of 128: 63 us, 4.2 of 6.55 TB/s; 64 contexts of 3 to 2047 keys, 32 heads: 125 us, 4.3 TB/s; 16 of 501 to 8190, 8 heads, e4m3: 50 us, 2.9 TB/s (the longest are the tail).
+// three blocks on an SM (168 registers at most, a ring of two tiles a warp) hide better than two (217 registers, three tiles: 15 % more on the 64 contexts below).  One context of 131072
+// keys, 8 heads of 128: 66 us, 4.1 of 6.55 TB/s; 64 contexts of 3 to 2047 keys, 32 heads: 131 us, 4.1 TB/s; 16 of 501 to 8190, 8 heads, e4m3: 52 us, 2.8 TB/s (the longest are the tail).
+// A unit for each pair, compared with every tile's scales, costs 1 % of that; one for a block's pairs let the scales of hidden keys take bits from a row.
 #include <math.h>
 
 #include "kv8.cuh"
@@ -458,8 +459,8 @@ static int k8_pair_tiles(const tha_attn_t* a, const tha_rows_t* rows, int most) 
   return (int)(by_rows < by_seqs ? by_rows : by_seqs);
 }
 // Parts of a context.  Three blocks run at once on an SM, 444 on 148; a block takes the time of six tiles of 32 keys (4 us) beside its own, the meeting of the parts as much.  One context:
-// rounds of whole parts.  Several: their lengths are between nothing and the longest, blocks follow one another as they end, and the last of them is the tail.  us with 1 / 2 / 4 / 6 /
-// 10 / 20 parts, heads of 128: 64 contexts up to 2048 of 32 heads 125 / 136 / 162 / 192; 16 up to 8192 of 8 heads (3 parts: 69) 56 (4) / 50 / 51 / 59; one of 131072 of 8 heads with 18 /
+// rounds of whole parts.  Several: their lengths are between nothing and the longest, blocks follow one another as they end, and the last of them is the tail.  us (of an
+// earlier state, 2 % less than now) with 1 / 2 / 4 / 6 / 10 / 20 parts, heads of 128: 64 contexts up to 2048 of 32 heads 125 / 136 / 162 / 192; 16 up to 8192 of 8 heads (3 parts: 69) 56 (4) / 50 / 51 / 59; one of 131072 of 8 heads with 18 /
 // 37 / 55 / 64 parts 145 / 83 / 63 / 74.
 static int k8_splits(const tha_attn_t* a, const tha_rows_t* rows, int most_rows) {
   const int SLOTS = 3 * sm_budget();

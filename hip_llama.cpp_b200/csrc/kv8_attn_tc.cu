@@ -19,8 +19,8 @@
 // by more than 2^8 since its reference was taken (weights are at most 2^15 then: fp16 holds them), or V's scales outgrow theirs.
 //
 // Bound: the tensor cores' shared-memory operand and the softmax together, 2100 cycles for 256 rows of a tile where the products alone are 1320 (a score product of 128 x 64 x 16 reads 6 KB of
-// shared memory in 50 cycles, one of weights x values takes 65).  Two bf16 prompts of 777 and 2048 rows, 32 heads of 128: 91 us with 10 to 20 of staging, 430 TFLOP/s of the visible
-// pairs; one fp32 prompt of 1024 (twice the products): 58 us.
+// shared memory in 50 cycles, one of weights x values takes 65).  Two bf16 prompts of 777 and 2048 rows, 32 heads of 128: 92 us with 10 to 20 of staging, 430 TFLOP/s of the visible
+// pairs; one fp32 prompt of 1024 (twice the products): 62 us.
 #include "gemm_tc.h"
 #include "kv8.cuh"
 #include "tc_common.cuh"

@@ -7,8 +7,8 @@
     out = cache.attend(Attention(32, 8, 128, scale=128 ** -0.5), rows, q, layer=0)   # [301, 32 * 128]
     k, v = cache.read(rows, layer=0)                             # the values that the codes stand for
 
-Calls go to the current stream of the cache's device, which has to be the current device.  Nothing synchronises.  Results and scratch are allocated by torch on
-that stream, so that calls on several streams, and captured ones, share nothing; a cache is written by one stream at a time.
+Calls go to the current stream of the cache's device, which has to be the current device, and do not wait for it; Rows.of copies from pageable host memory, check_error waits.  Results and
+scratch are allocated by torch on that stream, so that calls on several streams, from several threads, and captured ones, share nothing; a cache is written by one stream at a time.
 """
 from __future__ import annotations
 

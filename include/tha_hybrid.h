@@ -634,7 +634,7 @@ int tha_hyb_hgrn_scan(void* stream, int dtype, const tha_hgrn_t* g, const tha_ro
 /* Cache rows as bytes with one scale for each block of positions and key/value head: a quarter of the bytes of tha_kv_t's fp32 rows.  Blocks are found
  * through a table as there.  A block's scale is the largest |x| of its rows over the format's largest number (127, 448) as fp32, at least 2^-126 unless all rows are 0; a
  * value's code is the format's number nearest to the real quotient x / scale, ties to even, and stands for code * scale.  Infinities do not enter the scale and get
- * the largest code of their sign, NaN gets 0: the cache holds finite numbers only.  Rows of a slot's last block, while it is not full, are also kept
+ * the largest code of their sign (0 in a block without another number), NaN gets 0: the cache holds finite numbers only.  Rows of a slot's last block, while it is not full, are also kept
  * in fp32 (k_open, v_open), and its codes are made anew whenever rows join it: a code is one rounding of its value under the scale of all rows that are
  * there, however the rows were cut into calls.
  * What fills the pools in another way than by tha_hyb_kv8_write writes whole blocks, and no e4m3 code of NaN.  The table's ids are checked on the
@@ -656,15 +656,17 @@ typedef struct {
                            fills k_open itself sets it, or -1 */
 } tha_kv8_t;
 
-/* In the calls below the rows of a sequence are at consecutive positions; a sequence of one row at a negative position is idle. */
+/* In the calls below the rows of a sequence are at consecutive positions; a sequence of one row at a negative position is idle.  max_seq_rows and max_pos of the rows may be more than the
+ * step has (a captured step whose rows change), never less. */
 
 /* Rows enter the cache: row r's heads are kv_heads * dim values at k + r * ldk and kv_heads * vdim at v + r * ldv (dtype-typed, pitches in elements).  The first
  * row of a sequence is at the position behind the slot's last one, or at any earlier one of the same block, or at the start of a block: rows of its block ahead of it are those of
  * k_open, v_open.  With open_end it may be at any earlier position: where k_open holds the rows of another block by then (tokens are dropped across a border of blocks), the rows ahead of
- * it are the values that their codes stand for.  What the slot held from that position on is gone.  A step brings at most one sequence of a slot, and no two of its sequences write one block.  Idle sequences write nothing. */
+ * it are the values that their codes stand for.  What the slot held from that position on is gone.  A step brings at most one sequence of a slot, and no two of its sequences write one block; a full block that slots share is not
+ * written again.  Idle sequences write nothing. */
 int tha_hyb_kv8_write(void* stream, int dtype, const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, const void* k, long long ldk, const void* v,
                       long long ldv);
-/* Cache rows as the values they stand for, rounded once to dtype: k_out [n_rows, ldk], v_out (either NULL: not wanted); pitches in elements.  Idle rows read as zeros. */
+/* Cache rows as the values they stand for: code * scale rounded to fp32, and that to dtype: k_out [n_rows, ldk], v_out (either NULL: not wanted); pitches in elements.  Idle rows read as zeros. */
 int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_kv8_t* kv, int cache_layer, void* k_out, long long ldk, void* v_out,
                      long long ldv);
 /* tha_hyb_attn_gated over such a cache: every row attends to the visible keys as the cache holds them, which for rows of a block that is not full are their codes
@@ -673,10 +675,10 @@ int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_
  * Codes are exact in fp16; q and the weights, each times its value's scale, enter the products as two fp16.  A number of q is off by 2^-22 of itself or 2^-39 of the largest
  * of its row of a head, whichever is more; a weight by 2^-22 of itself or 2^-29 of the row's largest weight times the largest scale that the row sees.  Rows of longer portions with dtype
  * THA_DT_BF16 use one fp16, 2^-11 of itself instead of 2^-22, unless fp32_scores asks for two.  Sums and softmax are fp32.  Which portions are long goes by the step: heads, keys, rows.
- * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones (it goes by how many
- * sequences of the step may be long at all, n_rows over the rows of a long one, each as far as the longest context; where that were more than 1 GiB, the shorter portions take the
- * form of short ones, and all do behind a context that needs so much by itself), and for partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  Calls that may
- * run at the same time need scratch of their own.
+ * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones, and for
+ * partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  The room goes by how many
+ * sequences of the step may be long at all (n_rows over the rows of a long one), each as far as the longest context.  Where that were more than 1 GiB, the shorter portions take the form
+ * of short ones, and all do behind a context that needs so much by itself.  Calls that may run at the same time need scratch of their own.
  * A kernel that gives up on a barrier of its own (after 17 s: a fault of its pipeline) ends with NaN in the rows concerned; tha_gemm_check_error (tha_b200.h) says so, once the stream has
  * been waited for. */
 int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv, const float* q, void* out, float* scratch,

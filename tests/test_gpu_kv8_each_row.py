@@ -334,3 +334,30 @@ def test_unusual_numbers_of_heads(heads, kv_heads, parts):
     m = T.filled(16, kv_heads, 64, 128, "int8", (200, 1))
     for dtype in (torch.float32, torch.bfloat16):
         check(m, dict(heads=heads, scale=0.125), parts, dtype)
+
+
+@pytest.mark.parametrize("parts", [[(i, 40 * i + 7, 1) for i in range(6)], [(0, 3, 30), (1, 0, 5), (2, 100, 1)], [(0, 0, 400), (1, 0, 400), (2, 390, 7)]], ids=["singles", "portions", "prompts"])
+@pytest.mark.parametrize("fmt,dtype", [("int8", torch.float32), ("e4m3", torch.bfloat16)])
+def test_steps_described_by_more_than_they_have(parts, fmt, dtype):
+    """A longest portion and a largest position beyond the step's own, as a captured step whose rows change has them: written, read and attended to alike."""
+    n, got = sum(x[2] for x in parts), []
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v, q = (torch.randn(n, w, device="cuda", generator=g) for w in (128, 256, 512))
+    for more in (False, True):
+        big = K.Kv8Cache.empty(blocks=200, layers=T.LAYERS, kv_heads=2, block_size=32, dim=64, vdim=128, slots=len(parts), table_stride=30, dtype=T.DT[fmt])
+        big.table.copy_(torch.arange(30 * len(parts), dtype=torch.int32).view(len(parts), 30))
+        first = [(s, 0, p) for s, p, _ in parts if p]
+        if first:
+            gen = torch.Generator(device="cuda").manual_seed(1)
+            total = sum(x[2] for x in first)
+            big.write(K.Rows.of(first), *(torch.randn(total, w, device="cuda", generator=gen) for w in (128, 256)), layer=LAYER)
+        rows = K.Rows.of(parts)
+        if more:
+            rows.c.max_seq_rows, rows.c.max_pos = n, 900
+        big.write(rows, k, v, layer=LAYER)
+        back = big.read(rows, layer=LAYER, dtype=dtype)
+        got.append((*back, big.k_scale, big.v_scale, big.k_open, big.attend(K.Attention(8, 2, 64, 128, scale=0.125), rows, q, layer=LAYER, dtype=dtype)))
+    for x, y in list(zip(*got))[:5]:
+        assert torch.equal(x, y)
+    a, b = got[0][5].double(), got[1][5].double()              # the form may differ
+    assert float((a - b).norm() / a.norm()) < (2e-5 if dtype == torch.float32 else 2.0 ** -7)
