@@ -125,12 +125,12 @@ class Attention:
         self._of = {}
 
     def of(self, layer: int):
-        """The struct with this cache layer in it: one for each layer, written before anyone sees it, because other threads may be in calls with theirs."""
-        at = self._of.get(layer)
-        if at is None:
+        """The struct `c` with this cache layer in it: one for each layer, written before anyone sees it, because other threads may be in calls with theirs."""
+        now, (was, at) = bytes(self.c), self._of.get(layer, (None, None))
+        if was != now:
             c = AttnStruct.from_buffer_copy(self.c)
-            c.cache_layer = layer
-            at = self._of.setdefault(layer, C.byref(c))         # a reference keeps its struct
+            c.cache_layer, at = layer, C.byref(c)               # a reference keeps its struct
+            self._of[layer] = now, at
         return at
 
 

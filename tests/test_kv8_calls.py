@@ -52,6 +52,14 @@ def test_threads_share_an_attention(monkeypatch, layers):
     assert seen == want
 
 
+def test_changes_of_an_attention_reach_the_next_call():
+    at = K.Attention(4, 2, 32, scale=1.0)
+    first = at.of(1)
+    assert first is at.of(1) and first._obj.cache_layer == 1 and at.of(0)._obj.cache_layer == 0 and at.c.cache_layer == 0
+    at.c.window = 7
+    assert at.of(1)._obj.window == 7 and at.of(0)._obj.window == 7 and first._obj.window == 0
+
+
 def test_a_kernel_that_gave_up_is_an_error(monkeypatch):
     answers = [0, 1, 0]
     cache = recorded(monkeypatch, tha_gemm_check_error=lambda: answers.pop(0))
