@@ -43,25 +43,9 @@ __device__ __forceinline__ uint32_t ptc_bf16x2(float a, float b) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-__device__ __forceinline__ void ptc_tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
-        "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-}
 // kind::f16, bf16 x bf16 -> fp32, both K-major, M = 128, N = n
 __host__ __device__ constexpr uint32_t ptc_idesc(int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-__device__ __forceinline__ void ptc_tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
 // MN-major B, SWIZZLE_128B: blocks of 64 columns x 8 rows of K; K groups 1024 bytes apart, column blocks `block` bytes
 __device__ __forceinline__ uint64_t ptc_desc_mn(uint32_t saddr, uint32_t block) {
@@ -167,7 +151,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_cons
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       uint32_t s[32];
-      ptc_tmem_ld32(ts + (uint32_t)(32 * half), s);
+      tc_tmem_ld32(ts + (uint32_t)(32 * half), s);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       if (whole) {
 #pragma unroll
@@ -186,7 +170,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_cons
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       uint32_t s[32], w[16];
-      ptc_tmem_ld32(ts + (uint32_t)(32 * half), s);
+      tc_tmem_ld32(ts + (uint32_t)(32 * half), s);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
       for (int j = 0; j < 32; j += 2) {
@@ -200,7 +184,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_cons
         lsum += p1;
         w[j >> 1] = ptc_bf16x2(p0, p1);
       }
-      ptc_tmem_st16(ts + (uint32_t)(16 * half), w);
+      tc_tmem_st16(ts + (uint32_t)(16 * half), w);
     }
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     l_run = l_run * corr + lsum;
@@ -232,7 +216,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_cons
 #pragma unroll
     for (int c0 = 0; c0 < HH; c0 += 32) {
       uint32_t v[32];
-      ptc_tmem_ld32(tpv + (uint32_t)c0, v);
+      tc_tmem_ld32(tpv + (uint32_t)c0, v);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
       for (int j = 0; j < 32; j++) acc[c0 + j] = acc[c0 + j] * corr + __uint_as_float(v[j]);

@@ -79,12 +79,6 @@ __device__ __forceinline__ void x3_mma(uint32_t tmem_d, uint32_t tmem_a, uint64_
       "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(X3_IDESC), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void x3_tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
 constexpr int X3_SCALE_MOST = 115;       // powers of two of a row's scale at most
 
 __global__ void __launch_bounds__(X3_BOUND, 1)
@@ -324,8 +318,8 @@ gemm_f16x3_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant
               if (g >= 2 && ok) ok = tc_mbar_wait_warp(&aempty[sa], ((g >> 1) & 1u) ^ 1u, abort_flag);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            x3_tmem_st16(ta + (uint32_t)(16 * half), hi);
-            x3_tmem_st16(ta + (uint32_t)(32 + 16 * half), lo);
+            tc_tmem_st16(ta + (uint32_t)(16 * half), hi);
+            tc_tmem_st16(ta + (uint32_t)(32 + 16 * half), lo);
           }
           __syncwarp();
           if (lane == 0) tc_mbar_arrive(&wfree[sw]);  // every value has been read and converted

@@ -23,14 +23,6 @@ namespace tha {
 constexpr int AR_HEADS = 4, AR_MAXD = 128, AR_THREADS = 128;
 constexpr int AR_STAGES = 3;   // tiles of a run in flight
 
-// sixteen bytes from global to shared memory behind the thread's back; bytes 0: zeros, src is not read
-__device__ __forceinline__ void ar_copy16(void* dst, const float* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void ar_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void ar_await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <typename T, int GS>
 __global__ void __launch_bounds__(AR_THREADS) hyb_attn_row_kernel(tha_attn_t a, tha_rows_t rows, tha_kv_t kv, const float* q, T* __restrict__ out,
                                                                   int splits, float* __restrict__ partial, const float* gate, long long ldg, int early) {
@@ -74,8 +66,8 @@ __global__ void __launch_bounds__(AR_THREADS) hyb_attn_row_kernel(tha_attn_t a, 
       float* dst = st + (4 * j + kq) * (D + E) + c4;
 #pragma unroll
       for (int i = 0; i < NI; i++) {
-        if (32 * i < D) ar_copy16(dst + 32 * i, kp + 32 * i, vis ? 16 : 0);
-        if (32 * i < E) ar_copy16(dst + D + 32 * i, vp + 32 * i, vis ? 16 : 0);
+        if (32 * i < D) hyb_copy16((uint32_t)__cvta_generic_to_shared(dst + 32 * i), kp + 32 * i, vis ? 16 : 0);
+        if (32 * i < E) hyb_copy16((uint32_t)__cvta_generic_to_shared(dst + D + 32 * i), vp + 32 * i, vis ? 16 : 0);
       }
     }
   };
@@ -109,7 +101,7 @@ __global__ void __launch_bounds__(AR_THREADS) hyb_attn_row_kernel(tha_attn_t a, 
     for (int i = 0; i < AR_STAGES; i++)
       if (late[i]) fetch(ti0 + i, row[i], late[i]);
   }
-  ar_commit();
+  hyb_copies_end();
   float4 qv[GS][NI], acc[GS][NI];
   float m_run[GS], l_run[GS], hs[GS];
 #pragma unroll
@@ -133,8 +125,8 @@ __global__ void __launch_bounds__(AR_THREADS) hyb_attn_row_kernel(tha_attn_t a, 
 #pragma unroll
         for (int j = 0; j < 2; j++) bias[h][j] = hyb_attn_rel(a, g * gsize + min(h0 + h, gsize - 1), max(p - (kt + 4 * j + kq), 0));
     }
-    if (ti == ti0) ar_await<0>();                          // the first round of the ring is one group, then a group a tile
-    else if (ti >= ti0 + AR_STAGES) ar_await<AR_STAGES - 1>();
+    if (ti == ti0) hyb_copies_await<0>();                          // the first round of the ring is one group, then a group a tile
+    else if (ti >= ti0 + AR_STAGES) hyb_copies_await<AR_STAGES - 1>();
     __syncwarp();
     const float* st = ring + (size_t)((ti - ti0) % AR_STAGES) * 8 * (D + E);
     float s[GS][2];                                        // the scores of all heads, then their sums: nothing of one waits for another
@@ -187,7 +179,7 @@ __global__ void __launch_bounds__(AR_THREADS) hyb_attn_row_kernel(tha_attn_t a, 
     }
     __syncwarp();
     if (ti + AR_STAGES < ti_end) fetch(ti + AR_STAGES, row_of(ti + AR_STAGES), ~0u);
-    ar_commit();
+    hyb_copies_end();
   }
   // the four key groups of a warp, then the four warps
 #pragma unroll

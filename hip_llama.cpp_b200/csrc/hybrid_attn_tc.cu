@@ -39,33 +39,8 @@ __device__ __forceinline__ uint32_t at_bf16x2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float at_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // element (row r, column c) of a tile of 128-byte rows (64 bf16), SWIZZLE_128B
 __device__ __forceinline__ int at_off(int r, int c) { return r * 128 + (((c >> 3) ^ (r & 7)) << 4) + ((c & 7) << 1); }
-__device__ __forceinline__ void at_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
-        "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void at_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
-__device__ __forceinline__ void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void at_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void at_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 // kind::f16, bf16 x bf16 -> fp32, M = 128; b_mn: the B operand's N runs along its rows
 __host__ __device__ constexpr uint32_t at_idesc(int n, int b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -160,9 +135,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(&tmem_slot)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  at_fence_before();
+  tc_fence_before();
   __syncthreads();
-  at_fence_after();
+  tc_fence_after();
   const uint32_t tmem = tmem_slot;
   hyb_pdl_enter();
   auto release = [&]() {
@@ -243,13 +218,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
       const int b = j & 1;
       ok = tc_mbar_wait(&s_full[w][b], (unsigned)(j >> 1) & 1u, abort_flag);
       ok = __all_sync(THA_FULL_MASK, ok);
-      at_fence_after();
+      tc_fence_after();
       float t[AT_KEYS];
       float mx = -INFINITY;
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
         uint32_t s[32];
-        at_ld32(t_s + (uint32_t)(b * AT_KEYS + 32 * hf), s);
+        tc_tmem_ld32(t_s + (uint32_t)(b * AT_KEYS + 32 * hf), s);
         const int ti = 2 * j + hf;
         const bool there = ti < tiles.n;
         const int kt = half_key(there ? ti : tiles.n - 1);   // behind the last half its own keys again, as fetched: the biases end there
@@ -257,7 +232,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
         const bool whole = there && kt + 31 <= p_first && kt >= last_first && (a.window <= 0 || p_last - kt < a.window || kt + 32 <= a.keep_first);
         const bool near = REL && p_first - (kt + 31) < a.rel_n - 1;   // the same for the whole block
         const float* bias = REL ? Bs + hg * BP + pad + (p_first + min(pp, AP - 1) - kt) : nullptr;
-        at_wait_ld();
+        tc_wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; i++) {
           const float sv = __uint_as_float(s[i]);
@@ -278,18 +253,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
       const bool grow = mx > m;                       // also from -inf, where nothing was seen before
       if (__any_sync(THA_FULL_MASK, grow)) {
         const float to = grow ? -mx * LOG2E : shift;
-        const float corr = m > -INFINITY ? at_ex2(to - shift) : grow ? 0.f : 1.f;
+        const float corr = m > -INFINITY ? hyb_ex2(to - shift) : grow ? 0.f : 1.f;
         m = grow ? mx : m;
         shift = to;
         l *= corr;
         if (j > 0) {   // all products of earlier tiles are in the accumulator
           ok = __all_sync(THA_FULL_MASK, tc_mbar_wait(&pv_done[w][b ^ 1], (unsigned)((j - 1) >> 1) & 1u, abort_flag) && ok);
-          at_fence_after();
+          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < DT; c += 32) {
             uint32_t o[32];
-            at_ld32(t_o + (uint32_t)c, o);
-            at_wait_ld();
+            tc_tmem_ld32(t_o + (uint32_t)c, o);
+            tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
             tc_tmem_st32(t_o + (uint32_t)c, o);
@@ -302,7 +277,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float p0 = at_ex2(fmaf(t[2 * (c + i)], LOG2E, shift)), p1 = at_ex2(fmaf(t[2 * (c + i) + 1], LOG2E, shift));
+          const float p0 = hyb_ex2(fmaf(t[2 * (c + i)], LOG2E, shift)), p1 = hyb_ex2(fmaf(t[2 * (c + i) + 1], LOG2E, shift));
           hi[i] = at_bf16x2(p0, p1);
           const float h0 = __uint_as_float(hi[i] << 16), h1 = __uint_as_float(hi[i] & 0xFFFF0000u);
           if (EXACT) {   // hi + lo carry 16 mantissa bits of the fp32 weight; the sum adds the fp32 weights themselves
@@ -312,29 +287,29 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
             sum += h0 + h1;
           }
         }
-        at_st16(t_s + (uint32_t)(b * AT_KEYS + c), hi);
-        if (EXACT) at_st16(t_s + (uint32_t)(b * AT_KEYS + 32 + c), lo);
+        tc_tmem_st16(t_s + (uint32_t)(b * AT_KEYS + c), hi);
+        if (EXACT) tc_tmem_st16(t_s + (uint32_t)(b * AT_KEYS + 32 + c), lo);
       }
       l += sum;
-      at_wait_st();
-      at_fence_before();
+      tc_wait_st();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) tc_mbar_arrive(&p_full[w][b]);
     }
     if (ok) ok = tc_mbar_wait(&pv_done[w][(n - 1) & 1], (unsigned)((n - 1) >> 1) & 1u, abort_flag);
-    at_fence_after();
+    tc_fence_after();
     ok = __all_sync(THA_FULL_MASK, ok);
     float inv = 0.f;
     if (row_ok) {
       // all weights and their sum carry the factor 2^(m log2(e) + shift) of the rounded shift; the sink is weighed by m itself
-      const float f = m > -INFINITY ? at_ex2(-fmaf(m, LOG2E, shift)) : 1.f;
+      const float f = m > -INFINITY ? hyb_ex2(-fmaf(m, LOG2E, shift)) : 1.f;
       inv = f * hyb_attn_final_factor(a, h, m, l * f, gate ? gate + (size_t)(r0 + pp) * ldg : nullptr);
     }
 #pragma unroll
     for (int c = 0; c < DT; c += 32) {
       uint32_t o[32];
-      at_ld32(t_o + (uint32_t)c, o);
-      at_wait_ld();
+      tc_tmem_ld32(t_o + (uint32_t)c, o);
+      tc_wait_ld();
       if (row_ok && ok) {
         const size_t at = ((size_t)(r0 + pp) * a.heads + h) * DT + c;
         if (a.out_f32) {
@@ -354,7 +329,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
         }
       }
     }
-    at_fence_before();
+    tc_fence_before();
   } else if (warp == 8) {
     // ===== tiles: two halves of 32 keys, each a box of 64 channels at a time
     if (tc_elect()) {
@@ -392,20 +367,20 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
       tc_commit(&s_full[w][j & 1]);
     };
     ok = tc_mbar_wait(&kv_full[0], 0u, abort_flag);
-    at_fence_after();
+    tc_fence_after();
     if (ok) { scores(0, 0); scores(0, 1); }
     for (int j = 0; j < n && ok; j++) {
       if (j + 1 < n) {
         ok = tc_mbar_wait(&kv_full[(j + 1) % AT_STAGES], (unsigned)((j + 1) / AT_STAGES) & 1u, abort_flag);
         for (int w = 0; w < 2 && ok; w++) {
           if (j > 0) ok = tc_mbar_wait(&pv_done[w][(j + 1) & 1], (unsigned)((j - 1) >> 1) & 1u, abort_flag);   // the buffer's weights have been used
-          at_fence_after();
+          tc_fence_after();
           if (ok) scores(j + 1, w);
         }
       }
       for (int w = 0; w < 2 && ok; w++) {
         ok = tc_mbar_wait(&p_full[w][j & 1], (unsigned)(j >> 1) & 1u, abort_flag);
-        at_fence_after();
+        tc_fence_after();
         if (!ok) break;
         const uint32_t d = tmem + (uint32_t)(4 * AT_KEYS + w * DT), p = tmem + (uint32_t)(w * 2 * AT_KEYS + (j & 1) * AT_KEYS);
         const uint64_t vd = at_desc_mn(kv_addr + (uint32_t)((j % AT_STAGES) * KV_STAGE + K_STAGE), AT_KEYS * 128);
@@ -421,7 +396,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) hyb_attn_tc_kernel(const __grid
   }
   __syncwarp();
   __syncthreads();
-  at_fence_after();
+  tc_fence_after();
   release();
   if (threadIdx.x == 0 && abort_s && error_flag) *((volatile int*)error_flag) = 1;
 }

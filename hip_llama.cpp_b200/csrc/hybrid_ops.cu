@@ -713,11 +713,6 @@ __device__ __forceinline__ float attn_softcap_fast(float s, float cap, float two
   return cap - __fdividef(2.0f * cap, 1.0f + __expf(s * two_over_cap));
 }
 
-__device__ __forceinline__ float attn_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __host__ __device__ inline int attn_rel_pitch(int AP) { return (AP + 31 - 8 + 31) / 32 * 32 + 8; }   // 8 banks from one head to the next
 // bytes of one half of the double buffer: [32][D + 8] keys, [32][E + 8] values, [AG][pitch] biases
@@ -918,11 +913,11 @@ __global__ void __launch_bounds__(AM_THREADS, 1) hyb_attn_mma_kernel(tha_attn_t 
       const float m_new = fmaxf(m_run[x], mx);
       const float shift = m_new > -INFINITY ? -m_new * LOG2E : 0.f;   // nothing seen yet: every weight is 2^-inf = 0
       corr[x] = 1.f;
-      if (m_new > -INFINITY) { corr[x] = attn_ex2(shift - shift_run[x]); shift_run[x] = shift; }   // exactly 1 while the maximum stays
+      if (m_new > -INFINITY) { corr[x] = hyb_ex2(shift - shift_run[x]); shift_run[x] = shift; }   // exactly 1 while the maximum stays
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float p0 = attn_ex2(fmaf(sacc[j][2 * x], LOG2E, shift)), p1 = attn_ex2(fmaf(sacc[j][2 * x + 1], LOG2E, shift));
+        const float p0 = hyb_ex2(fmaf(sacc[j][2 * x], LOG2E, shift)), p1 = hyb_ex2(fmaf(sacc[j][2 * x + 1], LOG2E, shift));
         const __nv_bfloat162 pr = __floats2bfloat162_rn(p0, p1);
         if (EXACT) {   // hi + lo carry 16 mantissa bits of the fp32 weight; the sum adds the fp32 weights themselves
           sum += p0 + p1;
@@ -974,7 +969,7 @@ __global__ void __launch_bounds__(AM_THREADS, 1) hyb_attn_mma_kernel(tha_attn_t 
     if (m_run[x] > -INFINITY) {
       // the weights are 2^(s log2(e) + shift) with shift = -m log2(e) ROUNDED: all of them, and their sum, carry the factor 2^(m log2(e) + shift)
       // over e^(s - m) (up to 6e-8 |m|; the fma gives the exponent exactly).  It goes out here: the merge of the splits and the sink weigh the sums by m.
-      const float f = attn_ex2(-fmaf(m_run[x], LOG2E, shift_run[x]));
+      const float f = hyb_ex2(-fmaf(m_run[x], LOG2E, shift_run[x]));
       l_run[x] *= f;
 #pragma unroll
       for (int n = 0; n < AM_MAXD / 8; n++) { oacc[n][2 * x] *= f; oacc[n][2 * x + 1] *= f; }

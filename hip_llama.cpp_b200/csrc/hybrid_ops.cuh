@@ -79,6 +79,20 @@ __device__ __forceinline__ float row_sum(const HybRow<P>& r, int width, HybRowSu
   }
   return block_sum(s, sm.red);                        // its first barrier ends the reading of the row
 }
+// 2^x, off by 2 units of the last place at most
+__device__ __forceinline__ float hyb_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// sixteen bytes from global to shared memory behind the thread's back; bytes 0: zeros, src is not read
+__device__ __forceinline__ void hyb_copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// a group of copies ends; all but the last N groups have landed
+__device__ __forceinline__ void hyb_copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void hyb_copies_await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float hyb_softcap(float z, float cap) { return cap * tanhf(z / cap); }
 __device__ __forceinline__ float hyb_logsigmoid(float z) { return fminf(z, 0.f) - log1pf(expf(-fabsf(z))); }
 __device__ __forceinline__ float hyb_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }

@@ -60,11 +60,6 @@ __device__ __forceinline__ float4 kv8_decode4(uint32_t w) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-__device__ __forceinline__ float k8_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float k8_max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

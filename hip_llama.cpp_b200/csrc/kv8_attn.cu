@@ -37,12 +37,6 @@ struct Kv8Ring {
 template <int DT>
 __device__ __forceinline__ int k8_piece(int r, int c) { return r * DT + ((DT == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); }
 
-__device__ __forceinline__ void k8_copy16(uint32_t dst, const void* src, bool there) {   // not there: zeros, src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void k8_await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void k8_mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
@@ -160,7 +154,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
   float* total = seg_total;
   asm volatile("" : "+l"(total));                           // local memory: few contexts have a second segment
   auto add_segment = [&]() {
-    const float f = m_total > -INFINITY ? k8_ex2(m_total - m) * (ref > 0.f ? ref_total / ref : 0.f) : 0.f;
+    const float f = m_total > -INFINITY ? hyb_ex2(m_total - m) * (ref > 0.f ? ref_total / ref : 0.f) : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -201,13 +195,13 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
           constexpr int STEP = 512 / DT;
           const int turn = DT == 128 ? (i & 1) * 64 : 0;
           const uint32_t to = dst + (16 * hf + STEP * i) * DT + (lane_to ^ turn);
-          if (FULL || k_there) k8_copy16(to, ks + STEP * i * D, there);
-          if (FULL || v_there) k8_copy16(to + Ring::TILE, vs + STEP * i * E, there);
+          if (FULL || k_there) hyb_copy16(to, ks + STEP * i * D, there ? 16 : 0);
+          if (FULL || v_there) hyb_copy16(to + Ring::TILE, vs + STEP * i * E, there ? 16 : 0);
         }
       }
     };
 #pragma unroll
-    for (int i = 0; i < Ring::STAGES - 1; i++) { fetch(s0 + warp + i * K8_WARPS, i); k8_commit(); }
+    for (int i = 0; i < Ring::STAGES - 1; i++) { fetch(s0 + warp + i * K8_WARPS, i); hyb_copies_end(); }
     for (int e = threadIdx.x; e < 2 * (s1 - s0); e += K8_THREADS) {
       const int at = s_tile[e];
       s_ks[e] = at >= 0 ? kv.k_scale[at] : 0.f;
@@ -219,8 +213,8 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
     int stage = 0;
     for (int ti = s0 + warp; ti < s1; ti += K8_WARPS) {
       fetch(ti + (Ring::STAGES - 1) * K8_WARPS, stage == 0 ? Ring::STAGES - 1 : stage - 1);
-      k8_commit();
-      k8_await<Ring::STAGES - 1>();
+      hyb_copies_end();
+      hyb_copies_await<Ring::STAGES - 1>();
       __syncwarp();
       const unsigned char* st = k8_ring + warp * Ring::WARP + stage * 2 * Ring::TILE;
       const int e = 2 * (ti - s0), kt = tile_key(ti);
@@ -280,7 +274,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
       const bool grow = top_x > m, wider = top_v > ref;
       if (__any_sync(THA_FULL_MASK, grow || wider)) {
         const float to = grow ? top_x : m;
-        float corr = m > -INFINITY ? k8_ex2(m - to) : grow ? 0.f : 1.f;
+        float corr = m > -INFINITY ? hyb_ex2(m - to) : grow ? 0.f : 1.f;
         m = to;
         l *= corr;
         if (wider) {                                         // up to the next power of two: what is there changes units exactly
@@ -302,7 +296,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
       for (int j = 0; j < 4; j++) {
         float2 y = k8_add2(x[j], make_float2(shift, shift));
         if (MORE) y = k8_add2(y, make_float2(K8_UP, K8_UP));
-        const float2 w = make_float2(k8_ex2(y.x), k8_ex2(y.y));
+        const float2 w = make_float2(hyb_ex2(y.x), hyb_ex2(y.y));
         sum = k8_add2(sum, w);
         split_f16x2(f32x2_mul(w, j < 2 ? make_float2(v0, v0) : make_float2(v1, v1)), 1.0f, j & 1 ? pf[j >> 1].z : pf[j >> 1].x, j & 1 ? pf[j >> 1].w : pf[j >> 1].y);
       }
@@ -339,7 +333,7 @@ __global__ void __launch_bounds__(K8_THREADS, 3) kv8_attn_kernel(tha_attn_t a, t
       __syncwarp();                                          // the stage has been read
       stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
     }
-    k8_await<0>();
+    hyb_copies_await<0>();
   }
 
   add_segment();

@@ -43,33 +43,13 @@ __host__ __device__ constexpr int kt_part(int DT) { return 2 * 32 * DT * 2; }
 __host__ __device__ constexpr int kt_slots(bool split, int DT) { return DT == 64 ? 4 : split ? 3 : 2; }   // of the ring of K tiles, and of V's
 __host__ __device__ constexpr int kt_smem(bool split, int DT) { return (split ? 2 : 1) * kt_groups(split, DT) * KT_ROWS * DT * 2 + 2 * kt_slots(split, DT) * KT_KEYS * DT * 2 + 1024; }
 
-__device__ __forceinline__ void kt_ld32(uint32_t taddr, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
-        "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void kt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
-__device__ __forceinline__ void kt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// the same where other work stands between: what is loaded is not touched ahead of it
+// tc_wait_ld where other work stands between: what is loaded is not touched ahead of it
 __device__ __forceinline__ void kt_wait_ld32(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
                  "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
                  "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) : : "memory");
 }
-__device__ __forceinline__ void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void kt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void kt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 // whether any thread of the 64 that meet at a barrier says so
 __device__ __forceinline__ bool kt_any_of_pair(bool mine, int bar) {
   unsigned any;
@@ -219,9 +199,9 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(&tmem_slot)), "r"(256 * GROUPS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  kt_fence_before();
+  tc_fence_before();
   __syncthreads();
-  kt_fence_after();
+  tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_trigger();                     // the kernel ahead has waited for those before it (kv8_stage_kernel): only what it stages is waited for, by the warp that fetches it
   auto release = [&]() {
@@ -342,14 +322,14 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
     alignas(16) float total[SPLIT ? DT / 2 : 1];
     float m_total = -INFINITY, ref_total = 0.f;       // the sum of the runs before this one, in its own units
     auto add_run = [&]() {                            // the accumulator into the total, in the present units
-      const float f = m_total > -INFINITY ? k8_ex2(m_total - m) * (ref > 0.f ? ref_total / ref : 0.f) : 0.f;
+      const float f = m_total > -INFINITY ? hyb_ex2(m_total - m) * (ref > 0.f ? ref_total / ref : 0.f) : 0.f;
 #pragma unroll 1
       for (int c = 0; c < DT / 2; c += 32) {          // columns from E on hold nothing, and nothing reads them
         float4 t[8];
         uint32_t o[32];
 #pragma unroll
         for (int i = 0; i < 8; i++) t[i] = *reinterpret_cast<const float4*>(total + c + 4 * i);
-        kt_ld32(t_o + (uint32_t)c, o);
+        tc_tmem_ld32(t_o + (uint32_t)c, o);
         kt_wait_ld32(o);
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -375,7 +355,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
       const int b = jl & 1;
       auto earlier = [&]() {                          // the products of earlier tiles are in the accumulator
         if (jl) ok = ok && tc_mbar_wait_warp(&pv_done[w][b ^ 1], (unsigned)((jl - 1) >> 1) & 1u, abort_flag);
-        kt_fence_after();
+        tc_fence_after();
       };
       const bool new_run = SPLIT && jl && jl % KT_RUN == 0;
       if (new_run) {
@@ -383,10 +363,10 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         add_run();
       }
       ok = ok && tc_mbar_wait_warp(&s_full[w][b], (unsigned)(jl >> 1) & 1u, abort_flag);   // the scales were there before the issuer saw the tile
-      kt_fence_after();
+      tc_fence_after();
       const uint32_t at = t_s + (uint32_t)(b * KT_KEYS);
       uint32_t x[32];
-      kt_ld32(at, x);
+      tc_tmem_ld32(at, x);
       const float4 mine = s_scales[jl % KT_SCALES][hv];
       const float2 ks = make_float2(mine.x, mine.y);
       float vs0 = mine.z, vs1 = mine.w;               // of what this row sees: a weight of 0 under a scale far above the row's unit is no number
@@ -433,7 +413,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         vtop = both(vtop, [](float a, float b) { return fmaxf(a, b); });
         grow = mx > m + KT_SLACK || (m == -INFINITY && mx > -INFINITY);
         float corr = 1.f;
-        if (grow) { corr = m > -INFINITY ? k8_ex2(m - mx) : 0.f; m = mx; shift = MORE ? -m : KT_UP - m; }
+        if (grow) { corr = m > -INFINITY ? hyb_ex2(m - mx) : 0.f; m = mx; shift = MORE ? -m : KT_UP - m; }
         l *= corr;
         if (vtop > ref) {                             // the next power of two and a factor of 4 more, so that this is rare; lo ends at 2^-25 / 2^7 ref, below 2^-29 of the scale
           const float to = __uint_as_float(min(((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u) + 0x1000000u, 0x7E800000u));
@@ -447,10 +427,10 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
           for (int c = 0; c < DT / 2; c += 16) {
             uint32_t o[16];
             tc_tmem_ld16(t_o + (uint32_t)c, o);
-            kt_wait_ld();
+            tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            kt_st16(t_o + (uint32_t)c, o);
+            tc_tmem_st16(t_o + (uint32_t)c, o);
           }
         }
       }
@@ -463,7 +443,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         const float f = i < 8 ? f0 : f1, vr = i < 8 ? vr0 : vr1;
         if (MORE) y = k8_add2(k8_add2(y, make_float2(shift, shift)), make_float2(KT_UP, KT_UP));   // next to a maximum of 2^127, 7 is nothing
         else y = f32x2_fma(y, make_float2(f, f), make_float2(shift, shift));
-        const float2 p = make_float2(k8_ex2(y.x), k8_ex2(y.y));
+        const float2 p = make_float2(hyb_ex2(y.x), hyb_ex2(y.y));
         sum = k8_add2(sum, p);
         const float2 z = f32x2_mul(p, make_float2(vr, vr));
         hi[i] = f16x2_of(z);
@@ -472,16 +452,16 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
           lo[i] = f16x2_of(make_float2(z.x - u.x, z.y - u.y));
         }
       }
-      kt_st16(at, hi);                                // over the scores that they come from
-      if (SPLIT) kt_st16(at + 16u, lo);
+      tc_tmem_st16(at, hi);                                // over the scores that they come from
+      if (SPLIT) tc_tmem_st16(at + 16u, lo);
       l += sum.x + sum.y;
-      kt_wait_st();
-      kt_fence_before();
+      tc_wait_st();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) tc_mbar_arrive(&p_full[w][b]);
     }
     if (ok) ok = tc_mbar_wait(&pv_done[w][(n - 1) & 1], (unsigned)((n - 1) >> 1) & 1u, abort_flag);
-    kt_fence_after();
+    tc_fence_after();
     ok = __all_sync(THA_FULL_MASK, ok);
     if (!ok) l = NAN;                                 // a wait has given up: the row, whichever of its threads it was, is no number rather than left as it was
     l = both(l, [](float a, float b) { return a + b; });
@@ -503,7 +483,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         for (int i = 0; i < 16; i++) o[i] = __float_as_uint(total[c + i]);
       } else {
         tc_tmem_ld16(t_o + (uint32_t)c, o);
-        kt_wait_ld();
+        tc_wait_ld();
       }
       if (row_ok) {
         const int col = hv * (DT / 2) + c;
@@ -527,7 +507,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
         }
       }
     }
-    kt_fence_before();
+    tc_fence_before();
   } else if (warp == KT_LOAD) {
     // ===== tiles: two parts each, behind the last the last again
     const int stage0 = kt_stage_base(a, rows, seq, min_rows);
@@ -578,7 +558,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
     auto scores = [&](int b) {
       const bool ok = tc_mbar_wait(&full[0][k_at], k_turn, abort_flag);
       if (!ok) return false;
-      kt_fence_after();
+      tc_fence_after();
       const uint32_t kd = k_desc + (uint32_t)(k_at * (TILE >> 4));
 #pragma unroll
       for (int part = SPLIT ? 1 : 0; part >= 0; part--) {   // what is small first: sums are cut off at the size of what is there
@@ -602,7 +582,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
       const uint32_t vd = v_desc + (uint32_t)(v_at * (TILE >> 4)), p = t_s + (uint32_t)(b * KT_KEYS);
       ok = tc_mbar_wait(&full[1][v_at], v_turn, abort_flag) && tc_mbar_wait(&p_full[w][b], (unsigned)(jl >> 1) & 1u, abort_flag);
       if (!ok) break;
-      kt_fence_after();
+      tc_fence_after();
 #pragma unroll
       for (int x = 0; x < KT_KEYS / 16; x++) {
         const uint32_t px = p + (uint32_t)(32 * (x >> 1) + 8 * (x & 1));
@@ -617,7 +597,7 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
   }
   __syncwarp();
   __syncthreads();
-  kt_fence_after();
+  tc_fence_after();
   release();
   if (threadIdx.x == 0 && abort_s && error_flag) *((volatile int*)error_flag) = 1;
 }
