@@ -673,7 +673,7 @@ int tha_hyb_kv8_read(void* stream, int dtype, const tha_rows_t* rows, const tha_
  * under its present scale.  a: heads, kv_heads, dim, vdim, scale, chunk, cache_layer, window, keep_first, sink, head_scale, softcap, rel, head_gate, fp32_scores and out_f32 as there
  * (values_in_keys, v_share and diff are refused); q fp32 [n_rows, heads * dim]; out dtype-typed [n_rows, heads * vdim].  Idle rows get zeros.
  * Codes are exact in fp16; q and the weights, each times its value's scale, enter the products as two fp16.  A number of q is off by 2^-22 of itself or 2^-39 of the largest
- * of its row of a head, whichever is more; a weight by 2^-22 of itself or 2^-29 of the row's largest weight times the largest scale that the row sees.  Rows of longer portions with dtype
+ * of its row of a head, whichever is more; a weight by 2^-22 of itself or 2^-29 of the row's largest weight times the largest scale of a block of which the row sees a key.  Rows of longer portions with dtype
  * THA_DT_BF16 use one fp16, 2^-11 of itself instead of 2^-22, unless fp32_scores asks for two.  Sums and softmax are fp32.  Which portions are long goes by the step: heads, keys, rows.
  * scratch (nullable, 16-byte aligned): room for the visible keys and values of prompt portions as fp16, without which portions take the slower form of short ones, and for
  * partial results where long contexts are cut along the keys; tha_hyb_kv8_attn_scratch says with how much a call does as it pleases, with less it does what fits.  The room goes by how many
