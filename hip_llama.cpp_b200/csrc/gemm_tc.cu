@@ -405,6 +405,19 @@ int tc_map(const void* ptr, long long rows, int K, long long ld, int box_rows, C
   return THA_STATUS_SUCCESS;
 }
 
+int tc_map_of(CUtensorMap* out, CUtensorMapDataType type, const void* ptr, long long rows, long long cols, long long pitch, int box_rows, int box_cols) {
+  {
+    std::lock_guard<std::mutex> lk(g_tc_mu);
+    THA_TRY_RC(tc_get_encode());
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const CUresult r = g_encode(out, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_last_error("cuTensorMapEncodeTiled", cudaErrorInvalidValue); return THA_STATUS_EXECUTION_FAILED; }
+  return THA_STATUS_SUCCESS;
+}
+
 // Per-device error flag (allocated on first use; callers that capture graphs call this beforehand).
 int gemm_tc_init(int** flag_out) {
   int dev = 0;

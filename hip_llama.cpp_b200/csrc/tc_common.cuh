@@ -199,5 +199,7 @@ struct TcSmem {
 // Tensor map of a row-major [rows, K] fp32 matrix (elem_bytes = 1: int8) with boxes of box_rows x 128 bytes, SWIZZLE_128B;
 // cached by (pointer, shape) -- gemm_tc.cu.
 int tc_map(const void* ptr, long long rows, int K, long long ld, int box_rows, CUtensorMap* out, int elem_bytes = 4);
+// Tensor map of a row-major matrix of `type` [rows, cols], rows `pitch` bytes apart, with boxes of box_rows x box_cols, SWIZZLE_128B; kept nowhere.
+int tc_map_of(CUtensorMap* out, CUtensorMapDataType type, const void* ptr, long long rows, long long cols, long long pitch, int box_rows, int box_cols);
 
 }  // namespace tha

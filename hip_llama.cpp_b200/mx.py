@@ -1,0 +1,217 @@
+"""Python binding of the matrices in microscaled numbers (tha_mx_t and tha_hyb_mx_* in include/tha_hybrid.h): 4 and 8 bits a value under a power of two for each 32.
+
+    w = quantise(weight)                                         # [n, k] fp32 or bf16 -> 4 bits (e2m1)
+    a = add_norm(x, attention, norm, eps=1e-5)                   # x += attention; its norm in 8 bits (e4m3)
+    h = linear_act(a, gate, up)                                  # silu(a gate^T) * (a up^T) in 8 bits
+    y = linear(h, down, dtype=torch.bfloat16)                    # [rows, n]
+    w.read(torch.float32)                                        # the values that the codes stand for
+
+Calls go to the current stream of the tensors' device, which has to be the current device, and do not wait for it; results are allocated by torch on that stream.  Nothing is kept between calls.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import cabi
+
+I, F, P, L = C.c_int, C.c_float, C.c_void_p, C.c_longlong
+DTYPES = {torch.bfloat16: 0, torch.float32: 1}                  # THA_DT_*
+FORMATS = {"e2m1": 0, "e4m3": 1}                                # THA_MX_*
+CODES = {torch.uint8: "e2m1", torch.float8_e4m3fn: "e4m3"}      # what holds them
+ACTS = {"clamped": 0, "relu2": 1, "gelu": 2, "xielu": 3, "silu": 4}    # THA_ACT_*
+UNGATED = ("relu2", "xielu")
+BLOCK, TILE = 32, 128
+
+
+class MxStruct(C.Structure):
+    _fields_ = [("codes", P), ("scales", P), ("rows", I), ("cols", I), ("format", I)]
+
+
+MxStruct.__name__ = "tha_mx_t"
+STRUCTS = (MxStruct,)
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_lib = None
+
+
+def lib():
+    global _lib
+    if _lib is None:
+        _lib = cabi.lib()
+        c, M = _lib.c, C.POINTER(MxStruct)
+        c.tha_hyb_mx_quant.argtypes = [P, I, P, L, M]
+        c.tha_hyb_mx_read.argtypes = [P, I, M, P, L]
+        c.tha_hyb_mx_add_norm.argtypes = [P, I, P, P, L, P, P, F, F, M]
+        c.tha_hyb_mx_linear.argtypes = [P, I, P, L, M, M]
+        c.tha_hyb_mx_linear_act.argtypes = [P, I, M, M, M, F, F, M]
+        for name in ("tha_hyb_mx_codes_bytes", "tha_hyb_mx_scales_bytes"):
+            getattr(c, name).restype = C.c_size_t
+        c.tha_hyb_mx_codes_bytes.argtypes, c.tha_hyb_mx_scales_bytes.argtypes = [I, I, I], [I, I]
+    return _lib
+
+
+def padded(cols: int) -> int:
+    """The columns that a row of codes has room for."""
+    return -(-cols // TILE) * TILE
+
+
+def tiles(scales):
+    """Scale bytes [rows, blocks of 32] in the order in which a matrix keeps them, [row tiles, column tiles, 32, 4, 4]."""
+    rows, blocks = scales.shape
+    s = torch.nn.functional.pad(scales, (0, -blocks % 4, 0, -rows % TILE))
+    return s.view(-1, 4, 32, s.shape[1] // 4, 4).permute(0, 3, 2, 1, 4).contiguous()
+
+
+class Mx:
+    """A matrix of rows x cols microscaled numbers.  codes: uint8 [rows, padded(cols) / 2] (e2m1, two a byte, the first in the low half) or float8_e4m3fn [rows, padded(cols)], what is padding 0;
+    scales: uint8 in the order of `tiles`, 255: NaN."""
+
+    def __init__(self, codes, scales, rows: int, cols: int):
+        if codes.dtype not in CODES:
+            raise ValueError(f"codes are uint8 (e2m1, two a byte) or float8_e4m3fn, not {codes.dtype}")
+        if rows < 0 or not 1 <= cols <= 0x7fffff00 or rows > 0x7fffffff:
+            raise ValueError(f"a matrix has rows and at least one column, got {rows} x {cols}")
+        self.format = CODES[codes.dtype]
+        width, count = padded(cols) // (2 if self.format == "e2m1" else 1), -(-rows // TILE) * padded(cols) * TILE // BLOCK
+        if codes.shape != (rows, width) or not codes.is_contiguous() or codes.data_ptr() % 32:
+            raise ValueError(f"codes: contiguous [{rows}, {width}] on a 32-byte boundary is needed, got {tuple(codes.shape)}, strides {codes.stride()}")
+        if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.numel() != count or scales.device != codes.device or scales.data_ptr() % 16:
+            raise ValueError(f"scales: {count} contiguous bytes on {codes.device} and a 16-byte boundary are needed, got {tuple(scales.shape)} {scales.dtype} on {scales.device}")
+        self.codes, self.scales, self.rows, self.cols, self.device = codes, scales, rows, cols, codes.device
+        self.c = MxStruct(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[self.format])
+        self.ref, self.lib = C.byref(self.c), lib()
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, format: str = "e2m1", device="cuda"):
+        """Room for a matrix: what a call fills."""
+        _format(format)
+        width = padded(cols)
+        codes = (torch.empty(rows, width // 2, dtype=torch.uint8, device=device) if format == "e2m1" else torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device))
+        return cls(codes, torch.empty(-(-rows // TILE) * width * TILE // BLOCK, dtype=torch.uint8, device=device), rows, cols)
+
+    @classmethod
+    def of_rows(cls, codes, scales, cols: int):
+        """From codes and scale bytes row by row, as checkpoints have them: codes uint8 [rows, cols / 2 rounded up] or float8_e4m3fn [rows, cols], scales uint8 [rows, cols / 32 rounded up]."""
+        kind = CODES.get(codes.dtype)
+        width = -(-cols // 2) if kind == "e2m1" else cols
+        if kind is None or codes.dim() != 2 or codes.shape[1] != width or scales.dtype != torch.uint8 or scales.shape != (codes.shape[0], -(-cols // BLOCK)):
+            raise ValueError(f"codes [rows, {width}] and scales uint8 [rows, {-(-cols // BLOCK)}] are needed, got {tuple(codes.shape)} {codes.dtype}, {tuple(scales.shape)} {scales.dtype}")
+        c = codes.view(torch.uint8)
+        if kind == "e2m1" and cols % 2:
+            c = torch.cat([c[:, :-1], c[:, -1:] & 15], 1)        # the last byte's other half is padding
+        c = torch.nn.functional.pad(c, (0, padded(cols) // (2 if kind == "e2m1" else 1) - width)).contiguous()
+        return cls(c if kind == "e2m1" else c.view(torch.float8_e4m3fn), tiles(scales), codes.shape[0], cols)
+
+    def read(self, dtype=torch.float32, out=None):
+        """The values that the codes stand for (tha_hyb_mx_read), [rows, cols]."""
+        out = _result("out", out, self.rows, self.cols, dtype, self.device)
+        _call(self, "tha_hyb_mx_read", DTYPES[out.dtype], self.ref, out.data_ptr(), _pitch("out", out, self.rows, self.cols, self.device))
+        return out
+
+
+def _format(format):
+    if format not in FORMATS:
+        raise ValueError(f"a format is e2m1 or e4m3, not {format!r}")
+
+
+def _pitch(name, t, rows, cols, device):
+    """The row pitch of t [rows, cols], whose columns are neighbours."""
+    s = t.stride()
+    if t.shape != (rows, cols) or t.dtype not in DTYPES or t.device != device or (rows and cols > 1 and s[1] != 1) or (rows > 1 and s[0] < cols):
+        raise ValueError(f"{name}: [{rows}, {cols}] float32 or bfloat16 with neighbouring columns on {device} is needed, got {tuple(t.shape)} {t.dtype} on {t.device}, strides {s}")
+    return s[0] if rows > 1 else cols
+
+
+def _floats(name, t, shape, device):
+    if t.shape != shape or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous float32 {list(shape)} on {device} is needed, got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+
+
+def _result(name, out, rows, cols, dtype, device):
+    if out is None:
+        if dtype not in DTYPES:
+            raise ValueError(f"results are float32 or bfloat16, not {dtype}")
+        return torch.empty((rows, cols), dtype=dtype, device=device)
+    _pitch(name, out, rows, cols, device)
+    return out
+
+
+def _matrix(name, m, rows, cols, format, device):
+    """`m`, or room for a matrix in its place"""
+    if m is None:
+        return Mx.empty(rows, cols, format, device)
+    if (m.rows, m.cols, m.device) != (rows, cols, device):
+        raise ValueError(f"{name}: {rows} x {cols} on {device} is needed, got {m.rows} x {m.cols} on {m.device}")
+    return m
+
+
+def _call(on, name, *args):
+    """A call on the current stream of the device that `on` lies on."""
+    if torch.cuda.current_device() != on.device.index:
+        raise ValueError(f"the tensors are on {on.device}, the current device is cuda:{torch.cuda.current_device()}")
+    library = lib()
+    status = getattr(library.c, name)(_raw_stream(on.device.index), *args)
+    if status:
+        library.check(status, name)
+
+
+def check_error(device="cuda") -> None:
+    """Waits for the current stream of a device; raises if a kernel on it gave up on a barrier since the last such question (the results of that call are NaN where it was)."""
+    torch.cuda.current_stream(device).synchronize()
+    if lib().c.tha_gemm_check_error():
+        raise cabi.ThaError("a kernel gave up on a barrier of its own")
+
+
+def quantise(x, format: str = "e2m1", out: Mx | None = None) -> Mx:
+    """x [rows, cols], fp32 or bf16, rows any pitch apart, as microscaled numbers (tha_hyb_mx_quant)."""
+    _format(format)
+    if x.dim() != 2:
+        raise ValueError(f"x: [rows, columns] is needed, got {tuple(x.shape)}")
+    rows, cols = x.shape
+    ldx = _pitch("x", x, rows, cols, x.device)
+    out = _matrix("out", out, rows, cols, format, x.device)
+    _call(x, "tha_hyb_mx_quant", DTYPES[x.dtype], x.data_ptr(), ldx, out.ref)
+    return out
+
+
+def add_norm(x, left, weight, *, eps: float, w_offset: float = 0.0, format: str = "e4m3", x_out=None, out: Mx | None = None) -> Mx:
+    """x + left (fp32 [rows, cols] and fp32 or bf16 of any pitch; left None: x alone) into x_out (None: x itself); its root-mean-square norm, weighted with w_offset + weight,
+    as microscaled numbers (tha_hyb_mx_add_norm)."""
+    _format(format)
+    if x.dim() != 2:
+        raise ValueError(f"x: [rows, columns] is needed, got {tuple(x.shape)}")
+    rows, cols = x.shape
+    x_out = x if x_out is None else x_out
+    for name, t, shape in (("x", x, (rows, cols)), ("x_out", x_out, (rows, cols)), ("weight", weight, (cols,))):
+        _floats(name, t, shape, x.device)
+    ldl = 0 if left is None else _pitch("left", left, rows, cols, x.device)
+    out = _matrix("out", out, rows, cols, format, x.device)
+    _call(x, "tha_hyb_mx_add_norm", 1 if left is None else DTYPES[left.dtype], x.data_ptr(), None if left is None else left.data_ptr(), ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps,
+          out.ref)
+    return out
+
+
+def linear(a: Mx, w: Mx, dtype=torch.float32, out=None):
+    """a [rows, k] times w [n, k] transposed (tha_hyb_mx_linear): [rows, n], fp32 or bf16.  w is e2m1."""
+    if a.device != w.device:
+        raise ValueError(f"the rows are on {a.device}, the matrix is on {w.device}")
+    out = _result("out", out, a.rows, w.rows, dtype, a.device)
+    _call(a, "tha_hyb_mx_linear", DTYPES[out.dtype], out.data_ptr(), _pitch("out", out, a.rows, w.rows, a.device), a.ref, w.ref)
+    return out
+
+
+def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = "e4m3", limit: float = 0.0, alpha: float = 0.0, out: Mx | None = None) -> Mx:
+    """A feed-forward's input products and activation (tha_hyb_mx_linear_act): act(a gate^T, a up^T) [rows, n] as microscaled numbers.  act: silu, gelu, clamped (limit, alpha), or without a gate
+    (None) relu2, xielu (its two stored numbers as limit, alpha)."""
+    _format(format)
+    if act not in ACTS:
+        raise ValueError(f"act is one of {', '.join(ACTS)}, not {act!r}")
+    if (gate is None) != (act in UNGATED):
+        raise ValueError(f"{act} {'has no gate' if act in UNGATED else 'needs a gate'}")
+    if any(m is not None and m.device != a.device for m in (gate, up)):
+        raise ValueError(f"the rows are on {a.device}, a matrix is not")
+    out = _matrix("out", out, a.rows, up.rows, format, a.device)
+    _call(a, "tha_hyb_mx_linear_act", ACTS[act], a.ref, None if gate is None else gate.ref, up.ref, limit, alpha, out.ref)
+    return out

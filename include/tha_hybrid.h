@@ -686,6 +686,43 @@ int tha_hyb_kv8_attn(void* stream, int dtype, const tha_attn_t* a, const tha_row
 /* floats of scratch for such a call (0: it needs none, or would be refused) */
 size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t* rows, const tha_kv8_t* kv);
 
+/* ---- microscaled numbers: 4 and 8 bits under a scale for each 32 ---------------------------------------------------- */
+#define THA_MX_E2M1 0 /* 4-bit floating point: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives */
+#define THA_MX_E4M3 1 /* 8-bit floating point, 4 bits of exponent, 3 of mantissa, up to 448 */
+
+/* A matrix whose rows are cut into blocks of 32 values.  A block has one scale, the power of two 2^(c - 127) kept as the byte c: the smallest from 0 on at which no
+ * value of the block exceeds the format's largest number M (6, 448).  A value's code is the format's number nearest to value / scale, ties to even.  A block that holds a NaN or an infinity gets
+ * c = 255, which stands for NaN, and codes of 0: all of it reads as NaN.
+ * Rows are padded to P = cols rounded up to a multiple of 128.  codes [rows][P / 2 bytes (E2M1: two values a byte, the first in the low half) or P bytes (E4M3)], on a 32-byte boundary.
+ * scales: in tiles of 128 rows and 4 blocks, [rows rounded up to 128 / 128][P / 128][row % 32][row / 32 % 4][block % 4], 512 bytes a tile, on a 16-byte boundary: the order in which the
+ * tensor cores take them.  What is padding in a row has codes of 0 and scales other than 255 (0 from the calls below); scale bytes of rows behind the last one may hold
+ * anything and are not written. */
+typedef struct {
+  void* codes;
+  uint8_t* scales;
+  int rows, cols;
+  int format;           /* THA_MX_* */
+} tha_mx_t;
+/* bytes of the two arrays; 0: no such matrix */
+size_t tha_hyb_mx_codes_bytes(int format, int rows, int cols);
+size_t tha_hyb_mx_scales_bytes(int rows, int cols);
+
+/* The calls below write rows, cols and format as `out` gives them and fail when these do not fit the other arguments.  Inputs and results do not overlap, but for x and x_out.  No rows: nothing is done.
+ * No call needs scratch, and all may be captured. */
+/* out = x [out->rows, out->cols], dtype-typed, rows ldx elements apart */
+int tha_hyb_mx_quant(void* stream, int dtype, const void* x, long long ldx, const tha_mx_t* out);
+/* x (dtype-typed, rows ldx elements apart) = the values that m stands for, code * 2^(c - 127) rounded to dtype (exact but at the ends of its range) */
+int tha_hyb_mx_read(void* stream, int dtype, const tha_mx_t* m, void* x, long long ldx);
+/* A sublayer's result joins the residual stream, whose norm is quantised: x_out = x + left (fp32 [rows, cols] without gaps; x_out may be x; left dtype-typed, rows ldl elements
+ * apart, NULL: x_out = x), out = x_out / sqrt(mean(x_out^2) + eps) * (w_offset + w), w [cols].  What is quantised is the norm in 64 bits: a code is one rounding of the norm of x_out as stored. */
+int tha_hyb_mx_add_norm(void* stream, int dtype, const float* x, const void* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t* out);
+/* C[m, n] = sum_k A[m, k] W[n, k] (dtype-typed, rows ldc elements apart).  A in either format, W E2M1, as many columns.  Products are exact, sums fp32 on the tensor cores.
+ * A kernel that gives up on a barrier (a fault of its pipeline) says so through tha_gemm_check_error (tha_b200.h). */
+int tha_hyb_mx_linear(void* stream, int dtype, void* C, long long ldc, const tha_mx_t* A, const tha_mx_t* W);
+/* The input products of a feed-forward with its activation: out [A->rows, W_up->rows] = act of A . W_gate^T and A . W_up^T (THA_ACT_* but for THA_ACT_POLYNORM; W_gate NULL for the ungated ones;
+ * limit, alpha as in tha_hyb_ff_act), quantised from fp32 where the products are read out.  out->cols is W_up->rows. */
+int tha_hyb_mx_linear_act(void* stream, int act, const tha_mx_t* A, const tha_mx_t* W_gate, const tha_mx_t* W_up, float limit, float alpha, const tha_mx_t* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,237 @@
+"""Matrices in microscaled numbers: quantising, reading back, the norm that ends in them, products and a feed-forward's input products, against 64 bits (mx_oracle.py)."""
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as O
+from pkgload import load_pkg
+
+M = load_pkg("mx")
+pytestmark = pytest.mark.gpu
+FORMATS = ["e2m1", "e4m3"]
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def numbers(rows, cols, seed, spread=3.0):
+    """Values over several binades, with zeros, whole blocks of them, and values on the borders between codes"""
+    g = np.random.default_rng(seed)
+    x = g.standard_normal((rows, cols)) * np.exp2(g.uniform(-spread, spread, (rows, cols)))
+    x[g.random((rows, cols)) < 0.05] = 0.0
+    on_border = g.random((rows, cols)) < 0.2
+    x[on_border] = (g.integers(-24, 25, (rows, cols)) / 4.0)[on_border]
+    if cols >= 64:
+        x[:, 32:64][g.random(rows) < 0.3] = 0.0
+    return x
+
+
+def upload(x, dtype=torch.float32, wide=0, offset=0):
+    """x on the device, as columns of a wider array"""
+    t = torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda().to(dtype)
+    if not wide and not offset:
+        return t
+    room = torch.full((x.shape[0], x.shape[1] + wide + offset), 7.0, dtype=dtype, device="cuda")
+    room[:, offset:offset + x.shape[1]] = t
+    return room[:, offset:offset + x.shape[1]]
+
+
+def same_matrix(m, x):
+    """Codes and scales of m are those of x in 64 bits; padding holds codes of 0 and scales that are numbers."""
+    v, byte, code = O.quantise(x, m.format)
+    got, s = O.codes_of(m), O.scales_of(m)
+    assert np.array_equal(s[:, :byte.shape[1]], byte)
+    assert np.array_equal(got[:, :m.cols], code)
+    assert not got[:, m.cols:].any() and (s[:, byte.shape[1]:] == 0).all()
+    return v
+
+
+# ---- quantising and reading back --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,wide,offset", [(1, 1, 0, 0), (1, 768, 0, 0), (3, 31, 1, 0), (5, 33, 0, 3), (130, 256, 8, 0), (37, 257, 7, 1), (200, 1000, 0, 0), (129, 383, 1, 0),
+                                                   (2, 5000, 24, 8)])
+def test_quantise(fmt, dtype, rows, cols, wide, offset):
+    x = upload(numbers(rows, cols, rows + cols), dtype, wide, offset)
+    m = M.quantise(x, fmt)
+    v = same_matrix(m, x.double().cpu().numpy())
+    for out in DTYPES:
+        assert torch.equal(m.read(out).double().cpu(), torch.from_numpy(v))      # few bits under a power of two: exact in either
+    room = torch.full((rows, cols + 5), 9.0, device="cuda")
+    m.read(out=room[:, 2:2 + cols])
+    assert torch.equal(room[:, 2:2 + cols].double().cpu(), torch.from_numpy(v)) and (room[:, :2] == 9).all() and (room[:, 2 + cols:] == 9).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_every_binade_and_border(fmt):
+    """Scales from the smallest power to the largest numbers of fp32; values just at, below and above the border of a scale and of codes"""
+    most = O.MOST[fmt]
+    rows = []
+    for e in list(range(-149, 128, 3)) + [-127, -126, -125, 126, 127]:
+        top = np.float32(np.ldexp(1.0, e))
+        rows.append(np.float32(np.linspace(-1, 1, 32)) * top)
+    edge = (O.levels(fmt)[1:] + O.levels(fmt)[:-1]) / 2
+    for e in (-100, 0, 60):
+        for s in (np.nextafter(np.float32(most), np.float32(0)), np.float32(most), np.nextafter(np.float32(most), np.float32(1e9))):
+            r = np.zeros(32, np.float32)
+            r[0] = s
+            near = np.float32(np.random.default_rng(e + 200).choice(edge, 10))
+            r[1:11], r[11:21], r[21:31] = near, np.nextafter(near, np.float32(0)), -np.nextafter(near, np.float32(1e9))
+            rows.append(np.ldexp(r, e).astype(np.float32))
+    x = np.stack(rows)
+    same_matrix(M.quantise(torch.from_numpy(x).cuda(), fmt), x)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_blocks_that_hold_no_number(fmt):
+    """A NaN or an infinity makes its block NaN and no other"""
+    x = numbers(5, 160, 3)
+    x[0, 5], x[1, 40], x[2, 159], x[3, 96] = np.nan, np.inf, -np.inf, np.nan
+    m = M.quantise(upload(x), fmt)
+    v = same_matrix(m, x)
+    got = m.read().double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(v)) and np.isnan(got).sum() == 4 * 32
+    assert np.array_equal(got[~np.isnan(got)], v[~np.isnan(v)])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_of_a_checkpoint(fmt):
+    """Row-major codes and scales, as files have them"""
+    x = numbers(70, 161, 8)
+    _, byte, code = O.quantise(x, fmt)
+    if fmt == "e2m1":
+        c = np.pad(code, ((0, 0), (0, 1)), constant_values=9).astype(np.uint8)     # the last half byte is nobody's
+        codes = torch.from_numpy(c[:, 0::2] | (c[:, 1::2] << 4)).cuda()
+    else:
+        codes = torch.from_numpy(code.astype(np.uint8)).cuda().view(torch.float8_e4m3fn)
+    m = M.Mx.of_rows(codes, torch.from_numpy(byte.astype(np.uint8)).cuda(), 161)
+    same_matrix(m, x)
+
+
+# ---- the norm ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,wide,offset", [(1, 4096, 0, 0), (3, 1, 0, 0), (7, 33, 1, 1), (130, 288, 8, 0), (5, 1001, 0, 0), (2, 2049, 3, 2), (3, 14336, 0, 0), (2, 20001, 0, 0)])
+def test_add_norm(fmt, dtype, rows, cols, wide, offset):
+    x, left, w = numbers(rows, cols, 1), numbers(rows, cols, 2), numbers(1, cols, 3)[0]
+    x, w = (torch.from_numpy(t.astype(np.float32)).cuda() for t in (x, w))
+    l = upload(left, dtype, wide, offset)
+    s = (x + l.float()).double().cpu().numpy()                                       # the sum as stored
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + 1e-5) * (0.25 + w.double().cpu().numpy())
+    to = torch.empty_like(x)
+    kept = x.clone()
+    m = M.add_norm(x, l, w, eps=1e-5, w_offset=0.25, format=fmt, x_out=to)
+    assert torch.equal(to.double().cpu(), torch.from_numpy(s)) and torch.equal(x, kept)
+    same_matrix(m, y)
+    m = M.add_norm(x, l, w, eps=1e-5, w_offset=0.25, format=fmt)                     # in place
+    assert torch.equal(x, to)
+    same_matrix(m, y)
+    m = M.add_norm(x, None, w, eps=1e-5, w_offset=0.25, format=fmt)                  # nothing joins
+    assert torch.equal(x, to)
+    same_matrix(m, y)
+
+
+def test_add_norm_of_zeros_and_of_no_numbers():
+    x = torch.zeros(3, 100, device="cuda")
+    x[1, 7], x[2, 9] = float("nan"), float("inf")
+    w = torch.ones(100, device="cuda")
+    got = M.add_norm(x, None, w, eps=1e-5).read().cpu()
+    assert (got[0] == 0).all() and got[1].isnan().all()
+    assert got[2, :32].isnan().all() and (got[2, 32:] == 0).all()                    # inf * 0 in its block, 0 / inf in the others
+
+
+# ---- products ---------------------------------------------------------------------------------------------------------------
+def matrices(rows, n, k, fmt, seed, count=1):
+    """Rows in `fmt` and matrices in 4 bits, made on the host, so that a product is tested by itself; scale bytes of rows that are not there are 255"""
+    g = np.random.default_rng(seed)
+    made = []
+    for r, f in [(rows, fmt)] + [(n, "e2m1")] * count:
+        x = g.standard_normal((r, k)) * np.exp2(g.integers(-3, 4, (r, 1)))
+        _, byte, code = O.quantise(x, f)
+        c = torch.from_numpy(np.pad(code, ((0, 0), (0, k % 2 if f == "e2m1" else 0))).astype(np.uint8))
+        codes = c[:, 0::2] | (c[:, 1::2] << 4) if f == "e2m1" else c.view(torch.float8_e4m3fn)
+        m = M.Mx.of_rows(codes.cuda(), torch.from_numpy(byte.astype(np.uint8)).cuda(), k)
+        tiles = m.scales.view(-1, m.scales.numel() // 512 // -(-r // 128), 32, 4, 4)
+        for lane in range(128):
+            if (r - 1) // 128 * 128 + lane >= r:
+                tiles[-1, :, lane % 32, lane // 32] = 255
+        made.append(m)
+    return made
+
+
+def sum_bound(a, w):
+    """How far fp32 sums of exact products may be off: an instruction adds 32 values or more at a time to the sum, each addition (and each value's alignment) off by less than a unit of the
+    24th bit of what is added up so far, at most sum |a| |w|."""
+    total = np.abs(a) @ np.abs(w).T
+    return (a.shape[1] / 32 + 33) * 2.0 ** -23 * total
+
+
+SIZES = [(1, 1, 1), (1, 128, 128), (2, 33, 32), (3, 127, 31), (15, 129, 33), (16, 256, 256), (17, 300, 129), (33, 64, 384), (64, 260, 500), (65, 128, 640), (128, 129, 1000), (129, 31, 257),
+         (200, 200, 1152), (300, 513, 96), (7, 1000, 4100), (513, 640, 2048), (1000, 777, 300)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,n,k", SIZES)
+def test_linear(fmt, rows, n, k):
+    a, w = matrices(rows, n, k, fmt, rows + n + k)
+    va, vw = O.values(a), O.values(w)
+    want, tol = va @ vw.T, sum_bound(va, vw)
+    got = M.linear(a, w).double().cpu().numpy()
+    assert (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+    room = torch.full((rows, n + 9), 5.0, dtype=torch.bfloat16, device="cuda")
+    M.linear(a, w, out=room[:, 4:4 + n])
+    got = room[:, 4:4 + n].double().cpu().numpy()
+    assert (np.abs(got - want) <= tol + (np.abs(want) + tol) * 2.0 ** -8).all()      # and one rounding to bf16
+    assert (room[:, :4] == 5).all() and (room[:, 4 + n:] == 5).all()
+    M.check_error()
+
+
+ACTS = [("silu", 0.0, 0.0), ("gelu", 0.0, 0.0), ("clamped", 3.0, 1.702), ("relu2", 0.0, 0.0), ("xielu", 0.3, -0.2)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("out_fmt", FORMATS)
+@pytest.mark.parametrize("act,limit,alpha", ACTS)
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (2, 33, 100), (16, 128, 256), (40, 300, 384), (100, 257, 1000), (129, 513, 640), (300, 1000, 513)])
+def test_linear_act(fmt, out_fmt, act, limit, alpha, rows, n, k):
+    gated = act not in M.UNGATED
+    a, *ws = matrices(rows, n, k, fmt, rows + n + k, 2 if gated else 1)
+    va = O.values(a)
+    p = [va @ O.values(w).T for w in ws]
+    y = O.act(act, p[0], p[-1], limit, alpha)
+    m = M.linear_act(a, ws[0] if gated else None, ws[-1], act=act, format=out_fmt, limit=limit, alpha=alpha)
+    M.check_error()
+    cancels = 2.0 ** -23 * np.abs(p[0] * p[-1]) if act == "gelu" else 2.0 ** -21 * np.abs(p[-1]) if act == "xielu" else 2.0 ** -126 * np.abs(p[0]) * (1 + np.abs(p[-1]))
+    near(m, y, cancels, [O.act(act, p[0] + s * sum_bound(va, O.values(ws[0])), p[-1] + t * sum_bound(va, O.values(ws[-1])), limit, alpha) for s in (-1, 1) for t in (-1, 1)])
+
+
+def near(m, y, cancels, around):
+    """m's values are within half a step of y, as far as y itself is known: `around` holds it at the ends of its products' bounds; the activation in fp32 is good to 2^-20 of it, and to
+    `cancels` where it is a difference: gelu's 1 + tanh is off by a unit of tanh near 1 and a rounding, 2^-23 + 2^-24 in all and 0.5 g u times that; xielu's e^u - 1 - u by a unit of e^u - 1 and a
+    rounding, 2^-23 + 2^-24 of |u| at most, times a factor below 2, and so much again for 0.5 u and the sum;
+    a sigmoid below 2^-128, whose e^-g is no number of fp32, is 0, and one below 2^-126 keeps fewer bits: off by 2^-126 of g (1 + u) at most."""
+    off = np.max([np.abs(t - y) for t in around], 0) + np.abs(y) * 2.0 ** -20 + cancels
+    s, rows, cols = O.scales_of(m), m.rows, m.cols
+    blocks = lambda t: np.pad(t, ((0, 0), (0, -cols % 32))).reshape(rows, -1, 32).max(-1)  # noqa: E731
+    lo, hi = blocks(np.abs(y) - off).clip(0), blocks(np.abs(y) + off)
+    most = O.MOST[m.format] * np.exp2(s[:, :lo.shape[1]] - 127.0)
+    assert (lo <= most).all() and ((hi > most / 2) | (s[:, :lo.shape[1]] == 0)).all()      # the smallest power that holds the block
+    assert (s[:, lo.shape[1]:] == 0).all() and not O.codes_of(m)[:, cols:].any()
+    f = np.repeat(np.exp2(s - 127.0), 32, 1)[:, :cols]
+    worst = np.abs(O.values(m) - y) - off - f * O.half_step((np.abs(y) + off) / f, m.format)
+    assert (worst <= 1e-12 * np.abs(y)).all(), worst.max()
+
+
+def test_nan_rows_stay_in_their_rows():
+    a, w = matrices(20, 200, 300, "e4m3", 4)
+    a.scales.view(-1)[(0 * 32 + 3) * 16 + 0] = 255           # row 3, block 0
+    w.scales.view(-1)[(1 * 3 + 2) * 512 + (5 % 32) * 16 + 1] = 255    # row 133, block 9
+    got = M.linear(a, w).cpu()
+    bad = torch.zeros(20, 200, dtype=torch.bool)
+    bad[3], bad[:, 133] = True, True
+    assert torch.equal(got.isnan(), bad)
+
+
+def test_no_rows():
+    w = M.quantise(torch.randn(64, 96, device="cuda"))
+    a = M.quantise(torch.randn(0, 96, device="cuda"), "e4m3")
+    assert a.read().shape == (0, 96) and M.linear(a, w).shape == (0, 64) and M.linear_act(a, w, w).rows == 0
+    assert M.add_norm(torch.randn(0, 96, device="cuda"), None, torch.ones(96, device="cuda"), eps=1e-5).rows == 0
