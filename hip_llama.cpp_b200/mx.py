@@ -32,6 +32,8 @@ class MxStruct(C.Structure):
 MxStruct.__name__ = "tha_mx_t"
 STRUCTS = (MxStruct,)
 
+# the current device, and the number of its current stream; the public calls look around and make an object first, 1 and 3.3 us
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _lib = None
 
@@ -73,23 +75,48 @@ class Mx:
             raise ValueError(f"codes are uint8 (e2m1, two a byte) or float8_e4m3fn, not {codes.dtype}")
         if rows < 0 or not 1 <= cols <= 0x7fffff00 or rows > 0x7fffffff:
             raise ValueError(f"a matrix has rows and at least one column, got {rows} x {cols}")
-        self.format = CODES[codes.dtype]
-        width, count = padded(cols) // (2 if self.format == "e2m1" else 1), -(-rows // TILE) * padded(cols) * TILE // BLOCK
+        format = CODES[codes.dtype]
+        width, count = padded(cols) // (2 if format == "e2m1" else 1), -(-rows // TILE) * padded(cols) * TILE // BLOCK
         if codes.shape != (rows, width) or not codes.is_contiguous() or codes.data_ptr() % 32:
             raise ValueError(f"codes: contiguous [{rows}, {width}] on a 32-byte boundary is needed, got {tuple(codes.shape)}, strides {codes.stride()}")
         if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.numel() != count or scales.device != codes.device or scales.data_ptr() % 16:
             raise ValueError(f"scales: {count} contiguous bytes on {codes.device} and a 16-byte boundary are needed, got {tuple(scales.shape)} {scales.dtype} on {scales.device}")
-        self.codes, self.scales, self.rows, self.cols, self.device = codes, scales, rows, cols, codes.device
-        self.c = MxStruct(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[self.format])
-        self.ref, self.lib = C.byref(self.c), lib()
+        self._codes, self._scales = codes, scales
+        self._bind(codes.data_ptr(), scales.data_ptr(), rows, cols, format, codes.device)
+
+    def _bind(self, codes, scales, rows, cols, format, device):
+        self.rows, self.cols, self.format, self.device = rows, cols, format, device
+        self.c = MxStruct(codes, scales, rows, cols, FORMATS[format])
+        self.ref = C.byref(self.c)
 
     @classmethod
     def empty(cls, rows: int, cols: int, format: str = "e2m1", device="cuda"):
-        """Room for a matrix: what a call fills."""
-        _format(format)
-        width = padded(cols)
-        codes = (torch.empty(rows, width // 2, dtype=torch.uint8, device=device) if format == "e2m1" else torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device))
-        return cls(codes, torch.empty(-(-rows // TILE) * width * TILE // BLOCK, dtype=torch.uint8, device=device), rows, cols)
+        """Room for a matrix: what a call fills.  Codes and scales are one piece of memory; the tensors over them are made when they are asked for."""
+        if format not in FORMATS or rows < 0 or not 1 <= cols <= 0x7fffff00:
+            raise ValueError(f"a matrix of rows and at least one column in e2m1 or e4m3, not {rows} x {cols} in {format!r}")
+        wide = (cols + 127) & -128
+        codes = rows * (wide >> 1 if format == "e2m1" else wide)
+        scales = (codes + 511) & -512
+        room = torch.empty(scales + ((rows + 127) & -128) * (wide >> 5), dtype=torch.uint8, device=device)
+        m = cls.__new__(cls)
+        m._room, m._codes, m._scales = room, None, None
+        at = room.data_ptr()
+        m._bind(at, at + scales, rows, cols, format, room.device)
+        return m
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            width = padded(self.cols) // (2 if self.format == "e2m1" else 1)
+            t = self._room[:self.rows * width].view(self.rows, width)
+            self._codes = t if self.format == "e2m1" else t.view(torch.float8_e4m3fn)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._room[self._room.numel() - -(-self.rows // TILE) * padded(self.cols) * TILE // BLOCK:]
+        return self._scales
 
     @classmethod
     def of_rows(cls, codes, scales, cols: int):
@@ -106,14 +133,9 @@ class Mx:
 
     def read(self, dtype=torch.float32, out=None):
         """The values that the codes stand for (tha_hyb_mx_read), [rows, cols]."""
-        out = _result("out", out, self.rows, self.cols, dtype, self.device)
-        _call(self, "tha_hyb_mx_read", DTYPES[out.dtype], self.ref, out.data_ptr(), _pitch("out", out, self.rows, self.cols, self.device))
+        out, ld = _result("out", out, self.rows, self.cols, dtype, self.device)
+        _call(self.device, "tha_hyb_mx_read", DTYPES[out.dtype], self.ref, out.data_ptr(), ld)
         return out
-
-
-def _format(format):
-    if format not in FORMATS:
-        raise ValueError(f"a format is e2m1 or e4m3, not {format!r}")
 
 
 def _pitch(name, t, rows, cols, device):
@@ -130,12 +152,12 @@ def _floats(name, t, shape, device):
 
 
 def _result(name, out, rows, cols, dtype, device):
+    """(`out` or room for it, its pitch)"""
     if out is None:
         if dtype not in DTYPES:
             raise ValueError(f"results are float32 or bfloat16, not {dtype}")
-        return torch.empty((rows, cols), dtype=dtype, device=device)
-    _pitch(name, out, rows, cols, device)
-    return out
+        return torch.empty((rows, cols), dtype=dtype, device=device), cols
+    return out, _pitch(name, out, rows, cols, device)
 
 
 def _matrix(name, m, rows, cols, format, device):
@@ -147,14 +169,13 @@ def _matrix(name, m, rows, cols, format, device):
     return m
 
 
-def _call(on, name, *args):
-    """A call on the current stream of the device that `on` lies on."""
-    if torch.cuda.current_device() != on.device.index:
-        raise ValueError(f"the tensors are on {on.device}, the current device is cuda:{torch.cuda.current_device()}")
-    library = lib()
-    status = getattr(library.c, name)(_raw_stream(on.device.index), *args)
+def _call(device, name, *args):
+    """A call on the current stream of a device."""
+    if device.type != "cuda" or _current_device() != device.index:
+        raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device() if torch.cuda.is_available() else None}")
+    status = getattr((_lib or lib()).c, name)(_raw_stream(device.index), *args)
     if status:
-        library.check(status, name)
+        _lib.check(status, name)
 
 
 def check_error(device="cuda") -> None:
@@ -166,20 +187,18 @@ def check_error(device="cuda") -> None:
 
 def quantise(x, format: str = "e2m1", out: Mx | None = None) -> Mx:
     """x [rows, cols], fp32 or bf16, rows any pitch apart, as microscaled numbers (tha_hyb_mx_quant)."""
-    _format(format)
     if x.dim() != 2:
         raise ValueError(f"x: [rows, columns] is needed, got {tuple(x.shape)}")
     rows, cols = x.shape
     ldx = _pitch("x", x, rows, cols, x.device)
     out = _matrix("out", out, rows, cols, format, x.device)
-    _call(x, "tha_hyb_mx_quant", DTYPES[x.dtype], x.data_ptr(), ldx, out.ref)
+    _call(x.device, "tha_hyb_mx_quant", DTYPES[x.dtype], x.data_ptr(), ldx, out.ref)
     return out
 
 
 def add_norm(x, left, weight, *, eps: float, w_offset: float = 0.0, format: str = "e4m3", x_out=None, out: Mx | None = None) -> Mx:
     """x + left (fp32 [rows, cols] and fp32 or bf16 of any pitch; left None: x alone) into x_out (None: x itself); its root-mean-square norm, weighted with w_offset + weight,
     as microscaled numbers (tha_hyb_mx_add_norm)."""
-    _format(format)
     if x.dim() != 2:
         raise ValueError(f"x: [rows, columns] is needed, got {tuple(x.shape)}")
     rows, cols = x.shape
@@ -188,7 +207,7 @@ def add_norm(x, left, weight, *, eps: float, w_offset: float = 0.0, format: str 
         _floats(name, t, shape, x.device)
     ldl = 0 if left is None else _pitch("left", left, rows, cols, x.device)
     out = _matrix("out", out, rows, cols, format, x.device)
-    _call(x, "tha_hyb_mx_add_norm", 1 if left is None else DTYPES[left.dtype], x.data_ptr(), None if left is None else left.data_ptr(), ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps,
+    _call(x.device, "tha_hyb_mx_add_norm", 1 if left is None else DTYPES[left.dtype], x.data_ptr(), None if left is None else left.data_ptr(), ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps,
           out.ref)
     return out
 
@@ -197,15 +216,14 @@ def linear(a: Mx, w: Mx, dtype=torch.float32, out=None):
     """a [rows, k] times w [n, k] transposed (tha_hyb_mx_linear): [rows, n], fp32 or bf16.  w is e2m1."""
     if a.device != w.device:
         raise ValueError(f"the rows are on {a.device}, the matrix is on {w.device}")
-    out = _result("out", out, a.rows, w.rows, dtype, a.device)
-    _call(a, "tha_hyb_mx_linear", DTYPES[out.dtype], out.data_ptr(), _pitch("out", out, a.rows, w.rows, a.device), a.ref, w.ref)
+    out, ld = _result("out", out, a.rows, w.rows, dtype, a.device)
+    _call(a.device, "tha_hyb_mx_linear", DTYPES[out.dtype], out.data_ptr(), ld, a.ref, w.ref)
     return out
 
 
 def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = "e4m3", limit: float = 0.0, alpha: float = 0.0, out: Mx | None = None) -> Mx:
     """A feed-forward's input products and activation (tha_hyb_mx_linear_act): act(a gate^T, a up^T) [rows, n] as microscaled numbers.  act: silu, gelu, clamped (limit, alpha), or without a gate
     (None) relu2, xielu (its two stored numbers as limit, alpha)."""
-    _format(format)
     if act not in ACTS:
         raise ValueError(f"act is one of {', '.join(ACTS)}, not {act!r}")
     if (gate is None) != (act in UNGATED):
@@ -213,5 +231,5 @@ def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = 
     if any(m is not None and m.device != a.device for m in (gate, up)):
         raise ValueError(f"the rows are on {a.device}, a matrix is not")
     out = _matrix("out", out, a.rows, up.rows, format, a.device)
-    _call(a, "tha_hyb_mx_linear_act", ACTS[act], a.ref, None if gate is None else gate.ref, up.ref, limit, alpha, out.ref)
+    _call(a.device, "tha_hyb_mx_linear_act", ACTS[act], a.ref, None if gate is None else gate.ref, up.ref, limit, alpha, out.ref)
     return out
