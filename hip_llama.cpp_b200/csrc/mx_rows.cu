@@ -3,9 +3,11 @@
 //   mx_read_kernel      eight values a thread
 //   mx_add_norm_kernel  a block of threads takes a row: x + left, the square sum, the norm, its codes
 // All three are bound by memory: a value is read and written once.
-#include <string.h>
+#include <cuda_fp16.h>
 
+#include "hybrid_ops.cuh"
 #include "mx.cuh"
+#include "workspace.h"
 
 namespace tha {
 
@@ -18,7 +20,7 @@ int mx_refuse(const char* who, const char* why) {
 int mx_check(const tha_mx_t* m, const char* who) {
   if (!m) return mx_refuse(who, "a matrix is NULL");
   if (m->format != THA_MX_E2M1 && m->format != THA_MX_E4M3) return mx_refuse(who, "unknown format");
-  if (m->rows < 0 || m->cols < 1 || m->cols > 0x7fffff00) return mx_refuse(who, "a matrix has at least one column");
+  if (m->rows < 0 || m->cols < 1 || m->cols > MX_MOST_COLS) return mx_refuse(who, "a matrix has at least one column, and 2^30 at most");
   if (m->rows == 0) return THA_STATUS_SUCCESS;
   if (!m->codes || !m->scales) return mx_refuse(who, "codes or scales are NULL");
   if ((reinterpret_cast<uintptr_t>(m->codes) & 31u) || !aligned16(m->scales)) return mx_refuse(who, "codes on a 32-byte and scales on a 16-byte boundary are needed");
@@ -29,131 +31,243 @@ namespace {
 
 constexpr int MR_THREADS = 256;
 constexpr int MR_WARPS = MR_THREADS / 32;
+constexpr int MR_NORM_MOST = 512;                // threads of a row's block at most
+constexpr int MR_N = 4;                           // values of a thread of the norm's at a time
 constexpr int MR_V = 8;                           // values of a lane
-constexpr int MR_SEG = 32 * MR_V;                 // values of a warp
+constexpr int MR_U = 2;                           // such eights of a lane, 256 values apart
+constexpr int MR_SEG = 32 * MR_V * MR_U;          // values of a warp at a time
 
-// `n` values at p as fp32, zeros behind them; vec: p is 16-byte aligned
-__device__ __forceinline__ void mr_load(const float* p, int n, bool vec, float (&v)[MR_V]) {
-  if (vec && n >= MR_V) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
+// four values as fp32, zeros behind the first n; vec: p is on a boundary of four
+__device__ __forceinline__ void mr_load(const float* p, int n, bool vec, float (&v)[MR_N]) {
+  if (vec && n >= MR_N) { hyb_load_vec(p, v); return; }
 #pragma unroll
-  for (int i = 0; i < MR_V; i++) v[i] = i < n ? p[i] : 0.f;
+  for (int i = 0; i < MR_N; i++) v[i] = i < n ? p[i] : 0.f;
 }
-__device__ __forceinline__ void mr_load(const __nv_bfloat16* p, int n, bool vec, float (&v)[MR_V]) {
-  if (vec && n >= MR_V) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const unsigned w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+__device__ __forceinline__ void mr_load(const __nv_bfloat16* p, int n, bool vec, float (&v)[MR_N]) {
+  if (vec && n >= MR_N) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u); v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < MR_V; i++) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+  for (int i = 0; i < MR_N; i++) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
 }
-__device__ __forceinline__ void mr_store(float* p, int n, bool vec, const float (&v)[MR_V]) {
-  if (vec && n >= MR_V) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    return;
-  }
+__device__ __forceinline__ void mr_store(float* p, int n, bool vec, const float (&v)[MR_N]) {
+  if (vec && n >= MR_N) { hyb_store_vec(p, v); return; }
 #pragma unroll
-  for (int i = 0; i < MR_V; i++) if (i < n) p[i] = v[i];
+  for (int i = 0; i < MR_N; i++) if (i < n) p[i] = v[i];
 }
-__device__ __forceinline__ void mr_store(__nv_bfloat16* p, int n, bool vec, const float (&v)[MR_V]) {
-  if (vec && n >= MR_V) {
-    unsigned w[4];
+// sixteen bytes
+__device__ __forceinline__ void mr_store(float* p, const float (&v)[4]) { hyb_store_vec(p, v); }
+__device__ __forceinline__ void mr_store(__nv_bfloat16* p, const float (&v)[8]) {
+  unsigned w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const unsigned*>(&t);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    return;
+  for (int i = 0; i < 4; i++) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const unsigned*>(&t);
   }
-#pragma unroll
-  for (int i = 0; i < MR_V; i++) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The whole warp's 256 values from column `col0` of a row on, a lane's eight in v (zeros behind the row's end), into codes and scales.
+// Four values of a lane at column `col` (a multiple of 4; zeros behind the row's end), eight lanes a block, into codes and, from every eighth lane, the block's scale.  All lanes of the warp.
 template <int FMT>
-__device__ __forceinline__ void mr_codes(const tha_mx_t& out, int row, long long col0, long long padded, const float (&v)[MR_V]) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void mr_codes(const tha_mx_t& out, int row, int col, int padded, const float (&v)[MR_N]) {
   unsigned top = 0;
 #pragma unroll
-  for (int i = 0; i < MR_V; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < MR_N; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(THA_FULL_MASK, top, o));
+  const unsigned byte = mx_scale_byte<FMT>(top);
+  const float inv = mx_inverse(byte);
+  if (col >= padded) return;
+  if (FMT == THA_MX_E2M1) {
+    const unsigned w = mx_e2m1x2(v[0] * inv, v[1] * inv) | mx_e2m1x2(v[2] * inv, v[3] * inv) << 8;
+    *reinterpret_cast<unsigned short*>(static_cast<char*>(out.codes) + (size_t)row * (padded / 2) + col / 2) = (unsigned short)(byte == 255u ? 0u : w);
+  } else {
+    const unsigned w = mx_e4m3x2(v[0] * inv, v[1] * inv) | mx_e4m3x2(v[2] * inv, v[3] * inv) << 16;
+    *reinterpret_cast<unsigned*>(static_cast<char*>(out.codes) + (size_t)row * padded + col) = byte == 255u ? 0u : w;
+  }
+  if (!(threadIdx.x & 7)) out.scales[mx_scale_at(row, col / MX_TILE, padded / MX_TILE) + (col / MX_BLOCK & 3)] = (uint8_t)byte;
+}
+// Eight values of a lane at column `col` (a multiple of 8; zeros behind the row's end), four lanes a block, into codes and, from every fourth lane, the block's scale; top: the bits of
+// the lane's largest |value|.  All lanes of the warp.
+template <int FMT>
+__device__ __forceinline__ void mr_codes(const tha_mx_t& out, int row, int col, int padded, unsigned top, const float (&v)[MR_V]) {
   top = max(top, __shfl_xor_sync(THA_FULL_MASK, top, 1));
   top = max(top, __shfl_xor_sync(THA_FULL_MASK, top, 2));
   const unsigned byte = mx_scale_byte<FMT>(top);
   const float inv = mx_inverse(byte);
-  float y[MR_V];
+  if (col >= padded) return;
+  if (FMT == THA_MX_E2M1) {
+    unsigned w = 0;
 #pragma unroll
-  for (int i = 0; i < MR_V; i++) y[i] = byte == 255u ? 0.f : v[i] * inv;
-  const long long col = col0 + lane * MR_V;
-  if (col < padded) {
-    if (FMT == THA_MX_E2M1) {
-      unsigned w = 0;
-#pragma unroll
-      for (int i = 0; i < 4; i++) w |= mx_e2m1x2(y[2 * i], y[2 * i + 1]) << (8 * i);
-      *reinterpret_cast<unsigned*>(static_cast<char*>(out.codes) + (size_t)row * (padded / 2) + col / 2) = w;
-    } else {
-      uint2 w;
-      w.x = mx_e4m3x2(y[0], y[1]) | mx_e4m3x2(y[2], y[3]) << 16;
-      w.y = mx_e4m3x2(y[4], y[5]) | mx_e4m3x2(y[6], y[7]) << 16;
-      *reinterpret_cast<uint2*>(static_cast<char*>(out.codes) + (size_t)row * padded + col) = w;
-    }
+    for (int i = 0; i < 4; i++) w |= mx_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+    *reinterpret_cast<unsigned*>(static_cast<char*>(out.codes) + (size_t)row * (padded / 2) + col / 2) = byte == 255u ? 0u : w;
+  } else {
+    uint2 w;
+    w.x = mx_e4m3x2(v[0] * inv, v[1] * inv) | mx_e4m3x2(v[2] * inv, v[3] * inv) << 16;
+    w.y = mx_e4m3x2(v[4] * inv, v[5] * inv) | mx_e4m3x2(v[6] * inv, v[7] * inv) << 16;
+    *reinterpret_cast<uint2*>(static_cast<char*>(out.codes) + (size_t)row * padded + col) = byte == 255u ? make_uint2(0u, 0u) : w;
   }
-  unsigned four = 0;                              // lanes 0 and 1: the scales of four blocks each
-#pragma unroll
-  for (int q = 0; q < 4; q++) four |= __shfl_sync(THA_FULL_MASK, byte, (16 * lane + 4 * q) & 31) << (8 * q);
-  const int across = (int)(padded / MX_TILE), t = (int)(col0 / MX_TILE) + lane;
-  if (lane < 2 && t < across) *reinterpret_cast<unsigned*>(out.scales + mx_scale_at(row, t, across)) = four;
+  if (!(threadIdx.x & 3)) out.scales[mx_scale_at(row, col / MX_TILE, padded / MX_TILE) + (col / MX_BLOCK & 3)] = (uint8_t)byte;
 }
+// Eight values as they lie in memory, zeros behind the first n
+__device__ __forceinline__ void mr_fetch(const float* p, int n, bool vec, uint4 (&q)[2]) {
+  if (vec && n >= MR_V) { q[0] = *reinterpret_cast<const uint4*>(p); q[1] = *reinterpret_cast<const uint4*>(p + 4); return; }
+  unsigned t[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) t[i] = i < n ? __float_as_uint(p[i]) : 0u;
+  q[0] = make_uint4(t[0], t[1], t[2], t[3]); q[1] = make_uint4(t[4], t[5], t[6], t[7]);
+}
+__device__ __forceinline__ void mr_fetch(const __nv_bfloat16* p, int n, bool vec, uint4 (&q)[1]) {
+  if (vec && n >= MR_V) { q[0] = *reinterpret_cast<const uint4*>(p); return; }
+  const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+  unsigned t[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) t[i] = (2 * i < n ? h[2 * i] : 0u) | (2 * i + 1 < n ? h[2 * i + 1] : 0u) << 16;
+  q[0] = make_uint4(t[0], t[1], t[2], t[3]);
+}
+__device__ __forceinline__ unsigned mr_values(const uint4 (&q)[2], float (&v)[MR_V]) {
+  const unsigned w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    v[i] = __uint_as_float(w[i]);
+    top = max(top, w[i] & 0x7fffffffu);
+  }
+  return top;
+}
+__device__ __forceinline__ unsigned mr_values(const uint4 (&q)[1], float (&v)[MR_V]) {
+  const unsigned w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+  }
+  return max(top << 16, top & 0xffff0000u);
+}
+
+// A warp's way through the segments of all rows: the next one is `warps` segments further.  One division at its start (one a segment, in 64 bits, and a lane's eight values at a time: 11008 x
+// 4096 values in 57 us).
+struct MrWalk {
+  int row, col, padded, drow, dcol;
+  __device__ __forceinline__ MrWalk(int cols) {
+    padded = (int)mx_padded(cols);
+    const int segs = (padded + MR_SEG - 1) / MR_SEG, w = blockIdx.x * MR_WARPS + (threadIdx.x >> 5), warps = gridDim.x * MR_WARPS;
+    row = w / segs; drow = warps / segs;
+    col = (w - row * segs) * MR_SEG; dcol = (warps - drow * segs) * MR_SEG;
+  }
+  __device__ __forceinline__ void next() {
+    row += drow; col += dcol;
+    if (col >= padded) { col -= (padded + MR_SEG - 1) / MR_SEG * MR_SEG; row++; }
+  }
+};
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(MR_THREADS) mx_quant_kernel(const T* x, long long ldx, const tha_mx_t out, bool vec) {
-  const long long padded = mx_padded(out.cols), segs = (padded + MR_SEG - 1) / MR_SEG;
-  const long long w = (long long)blockIdx.x * MR_WARPS + (threadIdx.x >> 5);
-  if (w >= segs * out.rows) return;
-  const int row = (int)(w / segs);
-  const long long col0 = (w - row * segs) * MR_SEG, col = col0 + (threadIdx.x & 31) * MR_V;
-  float v[MR_V];
-  mr_load(x + row * ldx + col, (int)min((long long)MR_V, max(0ll, out.cols - col)), vec, v);
-  mr_codes<FMT>(out, row, col0, padded, v);
-}
-
-template <int FMT, typename T>
-__global__ void __launch_bounds__(MR_THREADS) mx_read_kernel(const tha_mx_t m, T* x, long long ldx, bool vec) {
-  const long long padded = mx_padded(m.cols), each = (m.cols + MR_V - 1) / MR_V;
-  const long long w = (long long)blockIdx.x * MR_THREADS + threadIdx.x;
-  if (w >= each * m.rows) return;
-  const int row = (int)(w / each);
-  const long long col = (w - row * each) * MR_V;
-  const int across = (int)(padded / MX_TILE);
-  const float scale = mx_scale(m.scales[mx_scale_at(row, (int)(col / MX_TILE), across) + (col / MX_BLOCK & 3)]);
-  float v[MR_V];
-  if (FMT == THA_MX_E2M1) {
-    const unsigned c = *reinterpret_cast<const unsigned*>(static_cast<const char*>(m.codes) + (size_t)row * (padded / 2) + col / 2);
+  hyb_pdl_enter();
+  constexpr int Q = sizeof(T) / 2;                // 16-byte words of eight values
+  const int lane = (threadIdx.x & 31) * MR_V;
+  MrWalk at(out.cols);
+  uint4 now[MR_U][Q], next[MR_U][Q];
+  auto fetch = [&](uint4 (&q)[MR_U][Q]) {
+    const T* p = x + at.row * ldx + at.col + lane;
 #pragma unroll
-    for (int i = 0; i < MR_V; i++) {
-      // 1 bit of mantissa, exponents from 2^0 on, below them steps of a half
-      const unsigned k = c >> (4 * i) & 7u;
-      const float a = k < 2u ? 0.5f * k : __uint_as_float((k >> 1) + 126u << 23 | (k & 1u) << 22);
-      v[i] = (c >> (4 * i) & 8u ? -a : a) * scale;
-    }
-  } else {
-    const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const char*>(m.codes) + (size_t)row * padded + col);
+    for (int u = 0; u < MR_U; u++) mr_fetch(p + u * 32 * MR_V, out.cols - at.col - lane - u * 32 * MR_V, vec, q[u]);
+  };
+  if (at.row < out.rows) fetch(now);
+  while (at.row < out.rows) {
+    const int row = at.row, col = at.col + lane;
+    at.next();
+    if (at.row < out.rows) fetch(next);           // on its way while this one is coded
 #pragma unroll
-    for (int i = 0; i < MR_V; i++) {
-      // 3 bits of mantissa, exponents from 2^-6 on, below them steps of 2^-9; all exponent and mantissa bits set: NaN
-      const unsigned b = (i < 4 ? c.x : c.y) >> (8 * (i & 3)), k = b & 0x7fu;
-      const float a = k < 8u ? k * 0.001953125f : k == 0x7fu ? __uint_as_float(0x7fc00000u) : __uint_as_float((k >> 3) + 120u << 23 | (k & 7u) << 20);
-      v[i] = (b & 0x80u ? -a : a) * scale;
+    for (int u = 0; u < MR_U; u++) {
+      float v[MR_V];
+      const unsigned top = mr_values(now[u], v);
+      mr_codes<FMT>(out, row, col + u * 32 * MR_V, at.padded, top, v);
+#pragma unroll
+      for (int i = 0; i < Q; i++) now[u][i] = next[u][i];
     }
   }
-  mr_store(x + row * ldx + col, (int)min((long long)MR_V, m.cols - col), vec, v);
+}
+
+// two codes as fp16, which holds every number of both formats
+template <int FMT>
+__device__ __forceinline__ float2 mr_pair(unsigned c) {
+  unsigned h;
+  if (FMT == THA_MX_E2M1) asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(c));
+  else asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)c));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// G neighbouring values a lane (16 bytes of fp32 or bf16: a warp's stores lie side by side), MR_SEG of a row a warp
+template <int FMT, typename T>
+__global__ void __launch_bounds__(MR_THREADS) mx_read_kernel(const tha_mx_t m, T* x, long long ldx) {
+  hyb_pdl_enter();
+  constexpr int G = 16 / sizeof(T), U = MR_SEG / (32 * G);
+  const int lane = (threadIdx.x & 31) * G;
+  MrWalk at(m.cols);
+  uint2 now[U] = {}, next[U] = {};
+  unsigned scale[U] = {}, scale_next[U] = {};
+  auto fetch = [&](uint2 (&c)[U], unsigned (&s)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int col = at.col + lane + u * 32 * G;
+      if (col >= m.cols) continue;
+      const char* p = static_cast<const char*>(m.codes) + (size_t)at.row * (FMT == THA_MX_E2M1 ? at.padded / 2 : at.padded) + (FMT == THA_MX_E2M1 ? col / 2 : col);
+      if (FMT == THA_MX_E2M1 && G == 4) c[u].x = *reinterpret_cast<const unsigned short*>(p);
+      else if (FMT == THA_MX_E2M1 || G == 4) c[u].x = *reinterpret_cast<const unsigned*>(p);
+      else c[u] = *reinterpret_cast<const uint2*>(p);
+      s[u] = m.scales[mx_scale_at(at.row, col / MX_TILE, at.padded / MX_TILE) + (col / MX_BLOCK & 3)];
+    }
+  };
+  if (at.row < m.rows) fetch(now, scale);
+  while (at.row < m.rows) {
+    T* p = x + at.row * ldx + at.col + lane;
+    const int left = m.cols - at.col - lane;
+    at.next();
+    if (at.row < m.rows) fetch(next, scale_next);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const float f = mx_scale(scale[u]);
+      float v[G];
+#pragma unroll
+      for (int i = 0; i < G / 2; i++) {
+        const float2 t = mr_pair<FMT>(FMT == THA_MX_E2M1 ? now[u].x >> (8 * i) & 0xffu : (i < 2 ? now[u].x : now[u].y) >> (16 * (i & 1)) & 0xffffu);
+        v[2 * i] = t.x * f; v[2 * i + 1] = t.y * f;
+      }
+      const int n = left - u * 32 * G;
+      if (n >= G) mr_store(p + u * 32 * G, v);
+      else
+#pragma unroll
+        for (int i = 0; i < G; i++) if (i < n) hyb_store(p + u * 32 * G + i, v[i]);
+      now[u] = next[u]; scale[u] = scale_next[u];
+    }
+  }
+}
+// rows on no boundary: one value of each block a lane
+template <int FMT, typename T>
+__global__ void __launch_bounds__(MR_THREADS) mx_read_lanes_kernel(const tha_mx_t m, T* x, long long ldx) {
+  hyb_pdl_enter();
+  const int lane = threadIdx.x & 31;
+  for (MrWalk at(m.cols); at.row < m.rows; at.next()) {
+    const uint8_t* codes = static_cast<const uint8_t*>(m.codes) + (size_t)at.row * (FMT == THA_MX_E2M1 ? at.padded / 2 : at.padded) + (at.col + lane) / (FMT == THA_MX_E2M1 ? 2 : 1);
+    unsigned c[MR_SEG / 32], s[MR_SEG / 32];
+#pragma unroll
+    for (int u = 0; u < MR_SEG / 32; u++) {
+      const int col = at.col + 32 * u;
+      c[u] = s[u] = 0;
+      if (col + lane < m.cols) {
+        c[u] = codes[(FMT == THA_MX_E2M1 ? 16 : 32) * u];
+        s[u] = m.scales[mx_scale_at(at.row, col / MX_TILE, at.padded / MX_TILE) + (u & 3)];
+      }
+    }
+    T* p = x + at.row * ldx + at.col + lane;
+#pragma unroll
+    for (int u = 0; u < MR_SEG / 32; u++)
+      if (at.col + 32 * u + lane < m.cols) hyb_store(p + 32 * u, mr_pair<FMT>(FMT == THA_MX_E2M1 ? c[u] >> (4 * (lane & 1)) & 15u : c[u]).x * mx_scale(s[u]));
+  }
 }
 
 // A number in 64 bits as one of 32 that compares with every number of at most 23 bits as it does itself: cut off, with the last bit set where something was cut. So a code is one rounding.
@@ -162,25 +276,130 @@ __device__ __forceinline__ float mr_odd(double y) {
   return (double)f != y && y == y ? __uint_as_float(__float_as_uint(f) | 1u) : f;
 }
 
+// The norm's sums and products in pairs of fp32 numbers, 48 bits: fp64 costs five conversions a value, at an eighth of the rate of fp32 (2048 x 4096 23 us in fp64, 18 in pairs).
+struct MrSum {
+  float hi = 0.f, lo = 0.f;
+  __device__ __forceinline__ void square(float v) {                    // + v^2
+    const float p = __fmul_rn(v, v), e = __fmaf_rn(v, v, -p), t = __fadd_rn(hi, p), b = __fsub_rn(t, hi);
+    lo = __fadd_rn(lo, __fadd_rn(e, __fadd_rn(__fsub_rn(hi, __fsub_rn(t, b)), __fsub_rn(p, b))));
+    hi = t;
+  }
+};
+// v * (r_hi + r_lo) * (w_offset + w) as a number that compares with every number of at most 23 bits as the product itself does (mr_odd)
+__device__ __forceinline__ float mr_norm(float v, float r_hi, float r_lo, float w_offset, float w) {
+  float g = w, gl = 0.f;
+  if (w_offset != 0.f) {
+    g = __fadd_rn(w_offset, w);
+    const float b = __fsub_rn(g, w_offset);
+    gl = __fadd_rn(__fsub_rn(w_offset, __fsub_rn(g, b)), __fsub_rn(w, b));
+  }
+  const float c = __fmul_rn(r_hi, g), cl = __fmaf_rn(r_hi, gl, __fmaf_rn(r_lo, g, __fmaf_rn(r_hi, g, -c)));
+  const float p = __fmul_rn(v, c), e = __fmaf_rn(v, cl, __fmaf_rn(v, c, -p)), s = __fadd_rn(p, e), rest = __fsub_rn(e, __fsub_rn(s, p));
+  const unsigned u = __float_as_uint(s);
+  const float cut = __uint_as_float(u - ((__float_as_uint(rest) ^ u) >> 31) | 1u);    // cut off towards 0, its last bit set
+  return s == 0.f ? p : rest != 0.f && fabsf(s) < INFINITY ? cut : s;                  // a zero with its sign; rest is NaN with infinities
+}
+
+// A block takes a row, P groups of four values a thread, kept in registers between the two passes.  One warp takes the root.
+template <int FMT, typename T, int P>
+__global__ void __launch_bounds__(MR_NORM_MOST) mx_add_norm_kernel(const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, double inv_cols,
+                                                                   const tha_mx_t out, bool vec, bool vec_left) {
+  hyb_pdl_enter();
+  __shared__ double part[MR_NORM_MOST / 32], whole;
+  __shared__ float2 root;
+  const int row = blockIdx.x, cols = out.cols, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int padded = (int)mx_padded(cols);
+  float v[P][MR_N];
+  MrSum sum;
+  auto there = [&](int i) { return min(MR_N, cols - (int)(threadIdx.x + i * blockDim.x) * MR_N); };    // values of group i, if above 0
+#pragma unroll
+  for (int i = 0; i < P; i++) mr_load(x + (size_t)row * cols + (threadIdx.x + i * blockDim.x) * MR_N, there(i), vec, v[i]);
+  if (left) {
+    float l[P][MR_N];
+#pragma unroll
+    for (int i = 0; i < P; i++) mr_load(left + row * ldl + (threadIdx.x + i * blockDim.x) * MR_N, there(i), vec_left, l[i]);
+#pragma unroll
+    for (int i = 0; i < P; i++)
+#pragma unroll
+      for (int j = 0; j < MR_N; j++) v[i][j] += l[i][j];
+  }
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    mr_store(x_out + (size_t)row * cols + (threadIdx.x + i * blockDim.x) * MR_N, there(i), vec, v[i]);
+#pragma unroll
+    for (int j = 0; j < MR_N; j++) sum.square(v[i][j]);                // values behind the row are 0
+  }
+  double total = (double)sum.hi + sum.lo;
+  auto over_block = [&]() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(THA_FULL_MASK, total, o);
+    if (lane == 0) part[threadIdx.x >> 5] = total;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      total = lane < warps ? part[lane] : 0.0;
+#pragma unroll
+      for (int o = MR_NORM_MOST / 64; o > 0; o >>= 1) total += __shfl_xor_sync(THA_FULL_MASK, total, o);
+      if (lane == 0) {
+        const double m = total * inv_cols + (double)eps;
+        double r;
+        if (m > 0x1p-100 && m < 0x1p100) {         // two steps of Newton's from an fp32 root: 1 / sqrt in fp64 holds the whole block up for longer than its loads
+          r = rsqrtf((float)m);
+          r = r * fma(-0.5 * m * r, r, 1.5);
+          r = r * fma(-0.5 * m * r, r, 1.5);
+        } else {
+          r = 1.0 / sqrt(m);
+        }
+        const float r_hi = (float)r;
+        whole = total;
+        root = make_float2(r_hi, r_hi < INFINITY ? (float)(r - r_hi) : 0.f);
+      }
+    }
+    __syncthreads();
+  };
+  over_block();
+  if (!(whole > 0x1p-60 && whole < 0x1p120)) {     // squares below or above fp32's numbers, or nothing at all: the same answer in the whole block
+    __syncthreads();
+    total = 0.0;
+#pragma unroll
+    for (int i = 0; i < P; i++)
+#pragma unroll
+      for (int j = 0; j < MR_N; j++) total = fma((double)v[i][j], (double)v[i][j], total);
+    over_block();
+  }
+  const float r_hi = root.x, r_lo = root.y;
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const int col = (int)(threadIdx.x + i * blockDim.x) * MR_N, n = there(i);
+    if (col - lane * MR_N >= padded) break;
+    float g[MR_N];
+    mr_load(w + col, n, vec, g);
+#pragma unroll
+    for (int j = 0; j < MR_N; j++) v[i][j] = j < n ? mr_norm(v[i][j], r_hi, r_lo, w_offset, g[j]) : 0.f;
+    mr_codes<FMT>(out, row, col, padded, v[i]);
+  }
+}
+
+// rows of any width: read again where the norm is taken, in fp64
 template <int FMT, typename T>
-__global__ void __launch_bounds__(MR_THREADS) mx_add_norm_kernel(const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t out,
-                                                                 bool vec, bool vec_left) {
+__global__ void __launch_bounds__(MR_THREADS) mx_add_norm_wide_kernel(const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, double inv_cols,
+                                                                 const tha_mx_t out, bool vec, bool vec_left) {
+  hyb_pdl_enter();
   __shared__ double part[MR_WARPS];
   const int row = blockIdx.x, cols = out.cols;
-  const long long padded = mx_padded(cols);
+  const int padded = (int)mx_padded(cols);
   double sum = 0.0;
-  for (long long col = threadIdx.x * MR_V; col < cols; col += MR_THREADS * MR_V) {
-    const int n = (int)min((long long)MR_V, cols - col);
-    float v[MR_V], l[MR_V];
+  for (int col = threadIdx.x * MR_N; col < cols; col += MR_THREADS * MR_N) {
+    const int n = min(MR_N, cols - col);
+    float v[MR_N], l[MR_N];
     mr_load(x + (size_t)row * cols + col, n, vec, v);
     if (left) {
       mr_load(left + row * ldl + col, n, vec_left, l);
 #pragma unroll
-      for (int i = 0; i < MR_V; i++) v[i] += l[i];
+      for (int i = 0; i < MR_N; i++) v[i] += l[i];
     }
     mr_store(x_out + (size_t)row * cols + col, n, vec, v);
 #pragma unroll
-    for (int i = 0; i < MR_V; i++) sum = fma((double)v[i], (double)v[i], sum);
+    for (int i = 0; i < MR_N; i++) sum = fma((double)v[i], (double)v[i], sum);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(THA_FULL_MASK, sum, o);
@@ -189,40 +408,45 @@ __global__ void __launch_bounds__(MR_THREADS) mx_add_norm_kernel(const float* x,
   sum = 0.0;
 #pragma unroll
   for (int i = 0; i < MR_WARPS; i++) sum += part[i];
-  const double r = 1.0 / sqrt(sum / cols + (double)eps);
-  for (long long col0 = (threadIdx.x >> 5) * MR_SEG; col0 < padded; col0 += MR_THREADS * MR_V) {
-    const long long col = col0 + (threadIdx.x & 31) * MR_V;
-    const int n = (int)min((long long)MR_V, max(0ll, cols - col));
-    float v[MR_V], g[MR_V];
+  const double r = 1.0 / sqrt(sum * inv_cols + (double)eps);
+  for (int col0 = (threadIdx.x >> 5) * 32 * MR_N; col0 < padded; col0 += MR_THREADS * MR_N) {
+    const int col = col0 + (threadIdx.x & 31) * MR_N, n = max(0, min(MR_N, cols - col));
+    float v[MR_N], g[MR_N];
     mr_load(x_out + (size_t)row * cols + col, n, vec, v);
     mr_load(w + col, n, vec, g);
 #pragma unroll
-    for (int i = 0; i < MR_V; i++) v[i] = i < n ? mr_odd((double)v[i] * r * ((double)w_offset + (double)g[i])) : 0.f;
-    mr_codes<FMT>(out, row, col0, padded, v);
+    for (int i = 0; i < MR_N; i++) v[i] = i < n ? mr_odd((double)v[i] * r * ((double)w_offset + (double)g[i])) : 0.f;
+    mr_codes<FMT>(out, row, col, padded, v);
   }
 }
 
 bool mr_aligned(const void* p, long long ld, size_t size) { return aligned16(p) && (ld * (long long)size) % 16 == 0; }
 
+// blocks for `rows` rows of `padded` values, a warp a segment: at most eight an SM, whose warps go on to further segments
+unsigned mr_blocks(long long rows, long long padded) {
+  return (unsigned)min((long long)sm_budget() * 8, ((padded + MR_SEG - 1) / MR_SEG * rows + MR_WARPS - 1) / MR_WARPS);
+}
 template <int FMT, typename T>
 int quant_form(cudaStream_t s, const T* x, long long ldx, const tha_mx_t* out) {
-  const long long warps = (mx_padded(out->cols) + MR_SEG - 1) / MR_SEG * out->rows, blocks = (warps + MR_WARPS - 1) / MR_WARPS;
-  if (blocks > 0x7fffffff) return mx_refuse("tha_hyb_mx_quant", "too many values for one call");
-  THA_CUDA_OK(launch(mx_quant_kernel<FMT, T>, dim3((unsigned)blocks), dim3(MR_THREADS), 0, s, false, x, ldx, *out, mr_aligned(x, ldx, sizeof(T))));
+  const bool vec = mr_aligned(x, out->rows > 1 ? ldx : 0, sizeof(T));
+  THA_CUDA_OK(launch(mx_quant_kernel<FMT, T>, dim3(mr_blocks(out->rows, mx_padded(out->cols))), dim3(MR_THREADS), 0, s, pdl_enabled() != 0, x, ldx, *out, vec));
   return THA_STATUS_SUCCESS;
 }
 template <int FMT, typename T>
 int read_form(cudaStream_t s, const tha_mx_t* m, T* x, long long ldx) {
-  const long long threads = ((long long)m->cols + MR_V - 1) / MR_V * m->rows, blocks = (threads + MR_THREADS - 1) / MR_THREADS;
-  if (blocks > 0x7fffffff) return mx_refuse("tha_hyb_mx_read", "too many values for one call");
-  THA_CUDA_OK(launch(mx_read_kernel<FMT, T>, dim3((unsigned)blocks), dim3(MR_THREADS), 0, s, false, *m, x, ldx, mr_aligned(x, ldx, sizeof(T))));
+  const bool vec = mr_aligned(x, m->rows > 1 ? ldx : 0, sizeof(T));
+  THA_CUDA_OK(launch(vec ? mx_read_kernel<FMT, T> : mx_read_lanes_kernel<FMT, T>, dim3(mr_blocks(m->rows, mx_padded(m->cols))), dim3(MR_THREADS), 0, s, pdl_enabled() != 0, *m, x, ldx));
   return THA_STATUS_SUCCESS;
 }
+// Threads of a row's block: many rows leave the SMs full with 256 each, few rows are done sooner by 512.
 template <int FMT, typename T>
 int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t* out) {
-  const bool vec = mr_aligned(x, out->cols, 4) && aligned16(x_out) && aligned16(w);
-  THA_CUDA_OK(launch(mx_add_norm_kernel<FMT, T>, dim3(out->rows), dim3(MR_THREADS), 0, s, false, x, left, ldl, x_out, w, w_offset, eps, *out, vec,
-                     mr_aligned(left, ldl, sizeof(T))));
+  const bool vec = mr_aligned(x, out->rows > 1 ? out->cols : 0, 4) && aligned16(x_out) && aligned16(w), vec_left = mr_aligned(left, out->rows > 1 ? ldl : 0, sizeof(T));
+  const int need = ceil_div(out->cols, MR_N * 32) * 32;                                                       // a thread for four values
+  const int threads = min(need, out->rows > 2 * sm_budget() && need <= 2048 ? 256 : MR_NORM_MOST), p = ceil_div(need, threads);
+  auto k = p <= 1 ? mx_add_norm_kernel<FMT, T, 1> : p <= 2 ? mx_add_norm_kernel<FMT, T, 2> : p <= 4 ? mx_add_norm_kernel<FMT, T, 4> : p <= 8 ? mx_add_norm_kernel<FMT, T, 8>
+           : p <= 16 ? mx_add_norm_kernel<FMT, T, 16> : mx_add_norm_wide_kernel<FMT, T>;
+  THA_CUDA_OK(launch(k, dim3(out->rows), dim3(p <= 16 ? threads : MR_THREADS), 0, s, pdl_enabled() != 0, x, left, ldl, x_out, w, w_offset, eps, 1.0 / out->cols, *out, vec, vec_left));
   return THA_STATUS_SUCCESS;
 }
 
@@ -232,11 +456,11 @@ int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, 
 using namespace tha;
 
 extern "C" size_t tha_hyb_mx_codes_bytes(int format, int rows, int cols) {
-  if ((format != THA_MX_E2M1 && format != THA_MX_E4M3) || rows < 1 || cols < 1 || cols > 0x7fffff00) return 0;
+  if ((format != THA_MX_E2M1 && format != THA_MX_E4M3) || rows < 1 || cols < 1 || cols > MX_MOST_COLS) return 0;
   return (size_t)rows * mx_pitch(format, cols);
 }
 extern "C" size_t tha_hyb_mx_scales_bytes(int rows, int cols) {
-  if (rows < 1 || cols < 1 || cols > 0x7fffff00) return 0;
+  if (rows < 1 || cols < 1 || cols > MX_MOST_COLS) return 0;
   return (((size_t)rows + MX_TILE - 1) / MX_TILE) * (mx_padded(cols) / MX_TILE) * MX_TILE_BYTES;
 }
 

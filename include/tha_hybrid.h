@@ -700,7 +700,7 @@ size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t
 typedef struct {
   void* codes;
   uint8_t* scales;
-  int rows, cols;
+  int rows, cols;       /* cols: 1 .. 2^30 */
   int format;           /* THA_MX_* */
 } tha_mx_t;
 /* bytes of the two arrays; 0: no such matrix */

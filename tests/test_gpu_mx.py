@@ -109,7 +109,8 @@ def test_rows_of_a_checkpoint(fmt):
 # ---- the norm ---------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols,wide,offset", [(1, 4096, 0, 0), (3, 1, 0, 0), (7, 33, 1, 1), (130, 288, 8, 0), (5, 1001, 0, 0), (2, 2049, 3, 2), (3, 14336, 0, 0), (2, 20001, 0, 0)])
+@pytest.mark.parametrize("rows,cols,wide,offset", [(1, 4096, 0, 0), (3, 1, 0, 0), (7, 33, 1, 1), (130, 288, 8, 0), (5, 1001, 0, 0), (2, 2049, 3, 2), (3, 14336, 0, 0), (2, 20001, 0, 0), (2, 32768, 0, 0), (3, 40001, 2, 0),
+                                                   (400, 300, 0, 0), (400, 4104, 1, 0), (700, 8192, 8, 0)])
 def test_add_norm(fmt, dtype, rows, cols, wide, offset):
     x, left, w = numbers(rows, cols, 1), numbers(rows, cols, 2), numbers(1, cols, 3)[0]
     x, w = (torch.from_numpy(t.astype(np.float32)).cuda() for t in (x, w))
@@ -127,6 +128,16 @@ def test_add_norm(fmt, dtype, rows, cols, wide, offset):
     m = M.add_norm(x, None, w, eps=1e-5, w_offset=0.25, format=fmt)                  # nothing joins
     assert torch.equal(x, to)
     same_matrix(m, y)
+
+
+@pytest.mark.parametrize("power", [-90, -60, -20, 40, 70, 100])
+def test_add_norm_at_the_ends_of_fp32(power):
+    """Rows whose squares are no numbers of fp32"""
+    x = np.ldexp(numbers(3, 1000, 5), power).astype(np.float32)
+    w = numbers(1, 1000, 6)[0].astype(np.float32)
+    s = x.astype(np.float64)
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + float(np.float32(1e-30))) * w.astype(np.float64)
+    same_matrix(M.add_norm(torch.from_numpy(x).cuda(), None, torch.from_numpy(w).cuda(), eps=1e-30), y)
 
 
 def test_add_norm_of_zeros_and_of_no_numbers():
