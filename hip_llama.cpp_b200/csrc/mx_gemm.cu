@@ -375,6 +375,9 @@ struct MgpSmem {
   static_assert(NST >= 3 && TOTAL <= TC_SMEM_LIMIT && 256 + NST * SET <= 512, "a stage is too large");
 };
 constexpr int MGP_THREADS = 384;
+// Activation rows of an item: NT, or what is left rounded up; each block has half of them
+template <int NT>
+__device__ __forceinline__ int mgp_width(int left) { return min(NT, (left + 31) & ~31); }
 
 __device__ __forceinline__ void mgp_arrive_leader(uint64_t* bar) {    // the same barrier of the pair's rank 0; what it announces is TMEM and TMA data, never generic memory of this thread
   uint32_t a;
@@ -448,6 +451,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
       int sent = -1;                     // stages that have been asked for, where the producer has given up
       for (int it = pair; it < p.n_items && ok; it += n_pairs) {
         const int tile = it / p.ny, row0 = tile * 256 + rank * TC_BM, n0 = (it - tile * p.ny) * NT;
+        const int half = rank * (mgp_width<NT>(p.N - n0) / 2);
         const int srow = min(row0, (p.M - 1) / MX_TILE * MX_TILE);          // a tile that lies wholly behind the matrix takes the last one's scales: its results go nowhere
         const int xt = (min(NT, p.N - n0) + 127) / 128;                     // tiles of scales that the item's activation rows touch
         for (int i = 0; i < nkb; i++) {
@@ -461,7 +465,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
           tc_mbar_expect_tx(&full[s], p.w_bytes + p.x_bytes + (WT + xt) * some);
           tc_tma_2d(st, &mw0, i * KC, row0, &full[s]);
           if (WT == 2) tc_tma_2d(st + TC_BM * 128, &mw1, i * KC, row0, &full[s]);
-          tc_tma_2d(st + S::W_BYTES, &mx, i * KC, n0 + rank * (NT / 2), &full[s]);
+          tc_tma_2d(st + S::W_BYTES, &mx, i * KC, n0 + half, &full[s]);
           mg_bulk(sw, p.sw0 + mx_scale_at(srow, t0, p.across), some, &full[s]);
           if (WT == 2) mg_bulk(sw + S::SC_BYTES, p.sw1 + mx_scale_at(srow, t0, p.across), some, &full[s]);
           for (int x = 0; x < xt; x++) mg_bulk(sx + x * S::SC_BYTES, p.sx + mx_scale_at(n0 + 128 * x, t0, p.across), some, &full[s]);
@@ -484,6 +488,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
           gb += nkb;
           continue;
         }
+        const uint32_t idesc = p.idesc | (uint32_t)(mgp_width<NT>(p.N - it % p.ny * NT) >> 3) << 17;
         if (n_it >= 1 && !tc_mbar_wait(accfree, (unsigned)(n_it - 1) & 1u, abort_flag)) { ok = false; break; }
         for (int i = 0; i < nkb; i++) {
           const int g = gb + i, s = g % S::NST;
@@ -506,7 +511,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
               const uint32_t at = sf + (uint32_t)(4 * c * (WT + XT));
 #pragma unroll
               for (int w = 0; w < WT; w++)
-                mgp_mma<KIND>(tmem + (uint32_t)(w * NT), adesc + (uint64_t)(1024 * w + 2 * k), bdesc + (uint64_t)(2 * k), p.idesc | (uint32_t)id << 4 | (uint32_t)id << 29, at + 4 * w,
+                mgp_mma<KIND>(tmem + (uint32_t)(w * NT), adesc + (uint64_t)(1024 * w + 2 * k), bdesc + (uint64_t)(2 * k), idesc | (uint32_t)id << 4 | (uint32_t)id << 29, at + 4 * w,
                               at + 4 * WT, (uint32_t)((i | k) != 0));
             }
           }
@@ -550,6 +555,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mgp_arrive_leader(accfree);
+      if (cols <= 0) continue;
       mg_activate<READ>(p, gate, x, row0 + q * 32 + lane < p.M);
 #pragma unroll
       for (int c = 0; c < HC; c += 16)
@@ -657,7 +663,7 @@ int mgp_launch(cudaStream_t s, const MgArgs& a) {
   if (S::WT == 2) THA_TRY_RC(mg_map(KIND, a.W1, TC_BM, &mw1, &wb));
   THA_TRY_RC(mg_map(KIND, a.A, S::NT / 2, &mx, &p.x_bytes));
   p.w_bytes = S::WT * wb;
-  p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, 2 * TC_BM, S::NT);
+  p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, 2 * TC_BM, 0);
   p.ny = ceil_div(p.N, S::NT);
   const long long items = (long long)ceil_div(p.M, 2 * TC_BM) * p.ny;
   if (items > 0x7fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");

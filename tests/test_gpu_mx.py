@@ -176,7 +176,9 @@ def sum_bound(a, w):
 
 
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 33, 32), (3, 127, 31), (15, 129, 33), (16, 256, 256), (17, 300, 129), (33, 64, 384), (64, 260, 500), (65, 128, 640), (128, 129, 1000), (129, 31, 257),
-         (200, 200, 1152), (300, 513, 96), (7, 1000, 4100), (513, 640, 2048), (1000, 777, 300)]
+         (200, 200, 1152), (300, 513, 96), (7, 1000, 4100), (513, 640, 2048), (1000, 777, 300),
+         # pairs: fewer items than pairs; the last round whole, in quarters, in halves; activation rows behind whole tiles of every width
+         (1100, 2600, 160), (1030, 5000, 96), (1024, 6400, 130), (2100, 4900, 64), (900, 3900, 288), (256, 20000, 33)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -201,7 +203,8 @@ ACTS = [("silu", 0.0, 0.0), ("gelu", 0.0, 0.0), ("clamped", 3.0, 1.702), ("relu2
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("out_fmt", FORMATS)
 @pytest.mark.parametrize("act,limit,alpha", ACTS)
-@pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (2, 33, 100), (16, 128, 256), (40, 300, 384), (100, 257, 1000), (129, 513, 640), (300, 1000, 513)])
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (2, 33, 100), (16, 128, 256), (40, 300, 384), (100, 257, 1000), (129, 513, 640), (300, 1000, 513),
+                                      (700, 2100, 160), (513, 4900, 96), (300, 9300, 130), (128, 19000, 64)])
 def test_linear_act(fmt, out_fmt, act, limit, alpha, rows, n, k):
     gated = act not in M.UNGATED
     a, *ws = matrices(rows, n, k, fmt, rows + n + k, 2 if gated else 1)
