@@ -35,22 +35,29 @@ STRUCTS = (MxStruct,)
 # the current device, and the number of its current stream; the public calls look around and make an object first, 1 and 3.3 us
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-_lib = None
+_lib = _c = None
+
+
+def _load():
+    """The library's calls, their arguments' types set."""
+    global _lib, _c
+    _lib = cabi.lib()
+    c, M = _lib.c, C.POINTER(MxStruct)
+    c.tha_hyb_mx_quant.argtypes = [P, I, P, L, M]
+    c.tha_hyb_mx_read.argtypes = [P, I, M, P, L]
+    c.tha_hyb_mx_add_norm.argtypes = [P, I, P, P, L, P, P, F, F, M]
+    c.tha_hyb_mx_linear.argtypes = [P, I, P, L, M, M]
+    c.tha_hyb_mx_linear_act.argtypes = [P, I, M, M, M, F, F, M]
+    for name in ("tha_hyb_mx_codes_bytes", "tha_hyb_mx_scales_bytes"):
+        getattr(c, name).restype = C.c_size_t
+    c.tha_hyb_mx_codes_bytes.argtypes, c.tha_hyb_mx_scales_bytes.argtypes = [I, I, I], [I, I]
+    _c = c
+    return c
 
 
 def lib():
-    global _lib
-    if _lib is None:
-        _lib = cabi.lib()
-        c, M = _lib.c, C.POINTER(MxStruct)
-        c.tha_hyb_mx_quant.argtypes = [P, I, P, L, M]
-        c.tha_hyb_mx_read.argtypes = [P, I, M, P, L]
-        c.tha_hyb_mx_add_norm.argtypes = [P, I, P, P, L, P, P, F, F, M]
-        c.tha_hyb_mx_linear.argtypes = [P, I, P, L, M, M]
-        c.tha_hyb_mx_linear_act.argtypes = [P, I, M, M, M, F, F, M]
-        for name in ("tha_hyb_mx_codes_bytes", "tha_hyb_mx_scales_bytes"):
-            getattr(c, name).restype = C.c_size_t
-        c.tha_hyb_mx_codes_bytes.argtypes, c.tha_hyb_mx_scales_bytes.argtypes = [I, I, I], [I, I]
+    if _c is None:
+        _load()
     return _lib
 
 
@@ -86,8 +93,8 @@ class Mx:
 
     def _bind(self, codes, scales, rows, cols, format, device):
         self.rows, self.cols, self.format, self.device = rows, cols, format, device
-        self.c = MxStruct(codes, scales, rows, cols, FORMATS[format])
-        self.ref = C.byref(self.c)
+        self.c = c = MxStruct(codes, scales, rows, cols, FORMATS[format])
+        self.ref = C.byref(c)
 
     @classmethod
     def empty(cls, rows: int, cols: int, format: str = "e2m1", device="cuda"):
@@ -95,11 +102,10 @@ class Mx:
         if format not in FORMATS or rows < 0 or not 1 <= cols <= MOST_COLS:
             raise ValueError(f"a matrix of rows and at least one column in e2m1 or e4m3, not {rows} x {cols} in {format!r}")
         wide = (cols + 127) & -128
-        codes = rows * (wide >> 1 if format == "e2m1" else wide)
-        scales = (codes + 511) & -512
-        room = torch.empty(scales + ((rows + 127) & -128) * (wide >> 5), dtype=torch.uint8, device=device)
+        scales = (rows * (wide >> 1 if format == "e2m1" else wide) + 511) & -512
         m = cls.__new__(cls)
-        m._room, m._codes, m._scales = room, None, None
+        m._room = room = torch.empty(scales + ((rows + 127) & -128) * (wide >> 5), dtype=torch.uint8, device=device)
+        m._codes = m._scales = None
         at = room.data_ptr()
         m._bind(at, at + scales, rows, cols, format, room.device)
         return m
@@ -133,11 +139,13 @@ class Mx:
 
     def read(self, dtype=torch.float32, out=None):
         """The values that the codes stand for (tha_hyb_mx_read), [rows, cols]."""
-        out, ld = _result("out", out, self.rows, self.cols, dtype, self.device)
-        _call(self.device, "tha_hyb_mx_read", DTYPES[out.dtype], self.ref, out.data_ptr(), ld)
+        out, kind, ld = _result(out, self.rows, self.cols, dtype, self.device)
+        stream = _stream(self.device)
+        _check((_c or _load()).tha_hyb_mx_read(stream, kind, self.ref, out.data_ptr(), ld), "tha_hyb_mx_read")
         return out
 
 
+# What a call costs on the host decides small sizes (7 to 8 us of which the launch is 2): arguments are looked at once, in few steps.
 def _pitch(name, t, rows, cols, device):
     """The row pitch of t [rows, cols], whose columns are neighbours."""
     s = t.stride()
@@ -151,29 +159,36 @@ def _floats(name, t, shape, device):
         raise ValueError(f"{name}: contiguous float32 {list(shape)} on {device} is needed, got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
 
 
-def _result(name, out, rows, cols, dtype, device):
-    """(`out` or room for it, its pitch)"""
-    if out is None:
-        if dtype not in DTYPES:
-            raise ValueError(f"results are float32 or bfloat16, not {dtype}")
-        return torch.empty((rows, cols), dtype=dtype, device=device), cols
-    return out, _pitch(name, out, rows, cols, device)
+def _result(out, rows, cols, dtype, device):
+    """(`out` or room for it, its THA_DT_*, its pitch)"""
+    if out is not None:
+        return out, DTYPES.get(out.dtype), _pitch("out", out, rows, cols, device)
+    kind = DTYPES.get(dtype)
+    if kind is None:
+        raise ValueError(f"results are float32 or bfloat16, not {dtype}")
+    return torch.empty(rows, cols, dtype=dtype, device=device), kind, cols
 
 
-def _matrix(name, m, rows, cols, format, device):
+def _matrix(m, rows, cols, format, device):
     """`m`, or room for a matrix in its place"""
     if m is None:
         return Mx.empty(rows, cols, format, device)
     if (m.rows, m.cols, m.device) != (rows, cols, device):
-        raise ValueError(f"{name}: {rows} x {cols} on {device} is needed, got {m.rows} x {m.cols} on {m.device}")
+        raise ValueError(f"out: {rows} x {cols} on {device} is needed, got {m.rows} x {m.cols} on {m.device}")
+    if format not in FORMATS:
+        raise ValueError(f"a format is e2m1 or e4m3, not {format!r}")
     return m
 
 
-def _call(device, name, *args):
-    """A call on the current stream of a device."""
-    if device.type != "cuda" or _current_device() != device.index:
+def _stream(device):
+    """The current stream of a device that has to be the current one."""
+    index = device.index
+    if index is None or _current_device() != index:
         raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device() if torch.cuda.is_available() else None}")
-    status = getattr((_lib or lib()).c, name)(_raw_stream(device.index), *args)
+    return _raw_stream(index)
+
+
+def _check(status, name):
     if status:
         _lib.check(status, name)
 
@@ -181,55 +196,63 @@ def _call(device, name, *args):
 def check_error(device="cuda") -> None:
     """Waits for the current stream of a device; raises if a kernel on it gave up on a barrier since the last such question (the results of that call are NaN where it was)."""
     torch.cuda.current_stream(device).synchronize()
-    if lib().c.tha_gemm_check_error():
+    if (_c or _load()).tha_gemm_check_error():
         raise cabi.ThaError("a kernel gave up on a barrier of its own")
 
 
 def quantise(x, format: str = "e2m1", out: Mx | None = None) -> Mx:
-    """x [rows, cols], fp32 or bf16, rows any pitch apart, as microscaled numbers (tha_hyb_mx_quant)."""
-    if x.dim() != 2:
-        raise ValueError(f"x: [rows, columns] is needed, got {tuple(x.shape)}")
-    rows, cols = x.shape
-    ldx = _pitch("x", x, rows, cols, x.device)
-    out = _matrix("out", out, rows, cols, format, x.device)
-    _call(x.device, "tha_hyb_mx_quant", DTYPES[x.dtype], x.data_ptr(), ldx, out.ref)
+    """x [rows, cols], fp32 or bf16, rows any pitch apart, as microscaled numbers (tha_hyb_mx_quant).  out: room for them, in its own format."""
+    shape, device = x.shape, x.device
+    if len(shape) != 2:
+        raise ValueError(f"x: [rows, columns] is needed, got {tuple(shape)}")
+    rows, cols = shape
+    ldx = _pitch("x", x, rows, cols, device)
+    out = _matrix(out, rows, cols, format, device)
+    _check((_c or _load()).tha_hyb_mx_quant(_stream(device), DTYPES[x.dtype], x.data_ptr(), ldx, out.ref), "tha_hyb_mx_quant")
     return out
 
 
 def add_norm(x, left, weight, *, eps: float, w_offset: float = 0.0, format: str = "e4m3", x_out=None, out: Mx | None = None) -> Mx:
     """x + left (fp32 [rows, cols] and fp32 or bf16 of any pitch; left None: x alone) into x_out (None: x itself); its root-mean-square norm, weighted with w_offset + weight,
     as microscaled numbers (tha_hyb_mx_add_norm)."""
-    if x.dim() != 2:
-        raise ValueError(f"x: [rows, columns] is needed, got {tuple(x.shape)}")
-    rows, cols = x.shape
-    x_out = x if x_out is None else x_out
-    for name, t, shape in (("x", x, (rows, cols)), ("x_out", x_out, (rows, cols)), ("weight", weight, (cols,))):
-        _floats(name, t, shape, x.device)
-    ldl = 0 if left is None else _pitch("left", left, rows, cols, x.device)
-    out = _matrix("out", out, rows, cols, format, x.device)
-    _call(x.device, "tha_hyb_mx_add_norm", 1 if left is None else DTYPES[left.dtype], x.data_ptr(), None if left is None else left.data_ptr(), ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps,
-          out.ref)
+    shape, device = x.shape, x.device
+    if len(shape) != 2:
+        raise ValueError(f"x: [rows, columns] is needed, got {tuple(shape)}")
+    rows, cols = shape
+    _floats("x", x, shape, device)
+    if x_out is None:
+        x_out = x
+    else:
+        _floats("x_out", x_out, shape, device)
+    _floats("weight", weight, shape[1:], device)
+    kind, at, ldl = 1, None, 0
+    if left is not None:
+        ldl, kind, at = _pitch("left", left, rows, cols, device), DTYPES[left.dtype], left.data_ptr()
+    out = _matrix(out, rows, cols, format, device)
+    _check((_c or _load()).tha_hyb_mx_add_norm(_stream(device), kind, x.data_ptr(), at, ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps, out.ref), "tha_hyb_mx_add_norm")
     return out
 
 
 def linear(a: Mx, w: Mx, dtype=torch.float32, out=None):
     """a [rows, k] times w [n, k] transposed (tha_hyb_mx_linear): [rows, n], fp32 or bf16.  w is e2m1."""
-    if a.device != w.device:
-        raise ValueError(f"the rows are on {a.device}, the matrix is on {w.device}")
-    out, ld = _result("out", out, a.rows, w.rows, dtype, a.device)
-    _call(a.device, "tha_hyb_mx_linear", DTYPES[out.dtype], out.data_ptr(), ld, a.ref, w.ref)
+    device = a.device
+    if device != w.device:
+        raise ValueError(f"the rows are on {device}, the matrix is on {w.device}")
+    out, kind, ld = _result(out, a.rows, w.rows, dtype, device)
+    _check((_c or _load()).tha_hyb_mx_linear(_stream(device), kind, out.data_ptr(), ld, a.ref, w.ref), "tha_hyb_mx_linear")
     return out
 
 
 def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = "e4m3", limit: float = 0.0, alpha: float = 0.0, out: Mx | None = None) -> Mx:
     """A feed-forward's input products and activation (tha_hyb_mx_linear_act): act(a gate^T, a up^T) [rows, n] as microscaled numbers.  act: silu, gelu, clamped (limit, alpha), or without a gate
     (None) relu2, xielu (its two stored numbers as limit, alpha)."""
-    if act not in ACTS:
+    device, kind = a.device, ACTS.get(act)
+    if kind is None:
         raise ValueError(f"act is one of {', '.join(ACTS)}, not {act!r}")
     if (gate is None) != (act in UNGATED):
         raise ValueError(f"{act} {'has no gate' if act in UNGATED else 'needs a gate'}")
-    if any(m is not None and m.device != a.device for m in (gate, up)):
-        raise ValueError(f"the rows are on {a.device}, a matrix is not")
-    out = _matrix("out", out, a.rows, up.rows, format, a.device)
-    _call(a.device, "tha_hyb_mx_linear_act", ACTS[act], a.ref, None if gate is None else gate.ref, up.ref, limit, alpha, out.ref)
+    if up.device != device or (gate is not None and gate.device != device):
+        raise ValueError(f"the rows are on {device}, a matrix is not")
+    out = _matrix(out, a.rows, up.rows, format, device)
+    _check((_c or _load()).tha_hyb_mx_linear_act(_stream(device), kind, a.ref, None if gate is None else gate.ref, up.ref, limit, alpha, out.ref), "tha_hyb_mx_linear_act")
     return out
