@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "tha_hybrid.h"
 
@@ -20,6 +22,18 @@ __host__ __device__ __forceinline__ size_t mx_scale_at(int r, int t, int across)
 }
 int mx_refuse(const char* who, const char* why);
 int mx_check(const tha_mx_t* m, const char* who);   // the matrix by itself
+int mx_error_flag(int** flag);                      // where a kernel that gives up on a barrier says so (tha_gemm_check_error)
+// More shared memory than 48 KB for a kernel's blocks, asked for once a device (0.3 us a call); devices beyond the bits ask every time.
+template <typename K>
+int mx_room(K kernel, int bytes, std::atomic<unsigned long long>* asked) {
+  int dev = 0;
+  THA_CUDA_OK(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (asked->load(std::memory_order_acquire) & bit) return THA_STATUS_SUCCESS;
+  THA_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  asked->fetch_or(bit, std::memory_order_release);
+  return THA_STATUS_SUCCESS;
+}
 
 #ifdef __CUDACC__
 // The scale byte of a block whose largest |value| has the bits `top` (of an fp32 not below 0): with 2^e <= top < 2^(e + 1), the largest number of the format 1.5 * 2^2

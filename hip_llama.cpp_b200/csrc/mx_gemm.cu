@@ -11,16 +11,12 @@
 // A block of threads takes a tile of 128 weight rows (of each of two matrices for a gated activation) and NT activation rows: warp 0 asks for codes (TMA) and scales (bulk copies)
 // into a ring of stages, warp 1 issues copies of scales and MMAs, warps 4-7 read the accumulators out: a thread a weight row, a warp 32 neighbouring results of one activation row.
 // A feed-forward's activation and the quantising of its result happen there: the 32 values of a block are the 32 lanes of a warp.
-#include <atomic>
-
 #include "hybrid_ops.cuh"
 #include "mx.cuh"
 #include "tc_common.cuh"
 #include "workspace.h"
 
 namespace tha {
-
-int gemm_tc_init(int** flag_out);
 
 namespace {
 
@@ -604,18 +600,6 @@ MgForm mg_form(int read, int tiles, int rows, int stages) {
   return {nt, 1};
 }
 
-// The shared memory of a kernel's blocks is asked for once a device (0.3 us a call); devices beyond the bits ask every time.
-template <typename K>
-int mg_room(K kernel, int bytes, std::atomic<unsigned long long>* asked) {
-  int dev = 0;
-  THA_CUDA_OK(cudaGetDevice(&dev));
-  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
-  if (asked->load(std::memory_order_acquire) & bit) return THA_STATUS_SUCCESS;
-  THA_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  asked->fetch_or(bit, std::memory_order_release);
-  return THA_STATUS_SUCCESS;
-}
-
 struct MgArgs { const tha_mx_t *A, *W0, *W1; MgP p; };
 
 template <int KIND, int NT, int READ>
@@ -638,7 +622,7 @@ int mg_launch(cudaStream_t s, const MgArgs& a, int ranks) {
   p.share = ceil_div(stages, p.ranks);
   auto k = mx_gemm_kernel<KIND, NT, READ>;
   static std::atomic<unsigned long long> asked{0};
-  THA_TRY_RC(mg_room(k, S::TOTAL, &asked));
+  THA_TRY_RC(mx_room(k, S::TOTAL, &asked));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3((unsigned)(items * p.ranks)); cfg.blockDim = dim3(MG_THREADS); cfg.dynamicSmemBytes = S::TOTAL; cfg.stream = s;
@@ -671,7 +655,7 @@ int mgp_launch(cudaStream_t s, const MgArgs& a) {
   const int pairs = max(1, sm_budget() / 2);
   auto k = mx_gemm_pair_kernel<KIND, READ>;
   static std::atomic<unsigned long long> asked{0};
-  THA_TRY_RC(mg_room(k, S::TOTAL, &asked));
+  THA_TRY_RC(mx_room(k, S::TOTAL, &asked));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(2u * (unsigned)min((long long)pairs, items)); cfg.blockDim = dim3(MGP_THREADS); cfg.dynamicSmemBytes = S::TOTAL; cfg.stream = s;
@@ -710,11 +694,7 @@ int mg_fill(MgArgs* a, const tha_mx_t* A, const tha_mx_t* W0, const tha_mx_t* W1
   a->p.M = W0->rows; a->p.N = A->rows; a->p.K = A->cols;
   a->p.across = (int)(mx_padded(A->cols) / MX_TILE);
   a->p.sw0 = W0->scales; a->p.sw1 = W1 ? W1->scales : nullptr; a->p.sx = A->scales;
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // allocated by a device's first call, which a capture allows in this mode
-  THA_CUDA_OK(cudaThreadExchangeStreamCaptureMode(&mode));
-  const int st = gemm_tc_init(&a->p.error_flag);
-  THA_CUDA_OK(cudaThreadExchangeStreamCaptureMode(&mode));
-  return st;
+  return mx_error_flag(&a->p.error_flag);
 }
 
 }  // namespace

@@ -110,7 +110,8 @@ def test_rows_of_a_checkpoint(fmt):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols,wide,offset", [(1, 4096, 0, 0), (3, 1, 0, 0), (7, 33, 1, 1), (130, 288, 8, 0), (5, 1001, 0, 0), (2, 2049, 3, 2), (3, 14336, 0, 0), (2, 20001, 0, 0), (2, 32768, 0, 0), (3, 40001, 2, 0),
-                                                   (400, 300, 0, 0), (400, 4104, 1, 0), (700, 8192, 8, 0)])
+                                                   (400, 300, 0, 0), (400, 4104, 1, 0), (700, 8192, 8, 0), (600, 4096, 0, 0), (1300, 1000, 16, 8), (650, 11008, 0, 0),
+                                                   (601, 40, 0, 0), (900, 12, 4, 0)])
 def test_add_norm(fmt, dtype, rows, cols, wide, offset):
     x, left, w = numbers(rows, cols, 1), numbers(rows, cols, 2), numbers(1, cols, 3)[0]
     x, w = (torch.from_numpy(t.astype(np.float32)).cuda() for t in (x, w))
@@ -130,23 +131,27 @@ def test_add_norm(fmt, dtype, rows, cols, wide, offset):
     same_matrix(m, y)
 
 
+@pytest.mark.parametrize("rows", [3, 700])
 @pytest.mark.parametrize("power", [-90, -60, -20, 40, 70, 100])
-def test_add_norm_at_the_ends_of_fp32(power):
-    """Rows whose squares are no numbers of fp32"""
-    x = np.ldexp(numbers(3, 1000, 5), power).astype(np.float32)
+def test_add_norm_at_the_ends_of_fp32(power, rows):
+    """Rows whose squares are no numbers of fp32, some of them between others"""
+    x = numbers(rows, 1000, 5)
+    x[::2] = np.ldexp(x[::2], power)
+    x = x.astype(np.float32)
     w = numbers(1, 1000, 6)[0].astype(np.float32)
     s = x.astype(np.float64)
     y = s / np.sqrt((s * s).mean(-1, keepdims=True) + float(np.float32(1e-30))) * w.astype(np.float64)
     same_matrix(M.add_norm(torch.from_numpy(x).cuda(), None, torch.from_numpy(w).cuda(), eps=1e-30), y)
 
 
-def test_add_norm_of_zeros_and_of_no_numbers():
-    x = torch.zeros(3, 100, device="cuda")
-    x[1, 7], x[2, 9] = float("nan"), float("inf")
+@pytest.mark.parametrize("rows", [3, 900])
+def test_add_norm_of_zeros_and_of_no_numbers(rows):
+    x = torch.zeros(rows, 100, device="cuda")
+    x[1::3, 7], x[2::3, 9] = float("nan"), float("inf")
     w = torch.ones(100, device="cuda")
     got = M.add_norm(x, None, w, eps=1e-5).read().cpu()
-    assert (got[0] == 0).all() and got[1].isnan().all()
-    assert got[2, :32].isnan().all() and (got[2, 32:] == 0).all()                    # inf * 0 in its block, 0 / inf in the others
+    assert (got[0::3] == 0).all() and got[1::3].isnan().all()
+    assert got[2::3, :32].isnan().all() and (got[2::3, 32:] == 0).all()              # inf * 0 in its block, 0 / inf in the others
 
 
 # ---- products ---------------------------------------------------------------------------------------------------------------
