@@ -12,7 +12,7 @@ namespace tha {
 constexpr int MX_BLOCK = 32;      // values under one scale
 constexpr int MX_TILE = 128;      // rows, and values of a row, of a tile of scales
 constexpr int MX_TILE_BYTES = 512;
-constexpr int MX_MOST_COLS = 1 << 30;
+constexpr int MX_MOST = 1 << 30;  // rows, columns
 
 __host__ __device__ __forceinline__ long long mx_padded(int cols) { return ((long long)cols + MX_TILE - 1) / MX_TILE * MX_TILE; }
 __host__ __device__ __forceinline__ long long mx_pitch(int format, int cols) { return format == THA_MX_E2M1 ? mx_padded(cols) / 2 : mx_padded(cols); }

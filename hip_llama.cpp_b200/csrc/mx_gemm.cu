@@ -316,6 +316,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__ 
   }
   if (p.ranks > 1) {
     __syncthreads();
+    if (*((volatile int*)abort_flag)) {              // copies that were under way have landed by now, over the partial tile maybe
+      for (int i = threadIdx.x; i < WT * NT * TC_BM; i += MG_THREADS) part[i] = __uint_as_float(0x7fc00000u);
+      __syncthreads();
+    }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     // this rank's columns of the tile, C neighbours at a time; half of the threads take one such group at a time, a thread a weight row
@@ -616,7 +620,7 @@ int mg_launch(cudaStream_t s, const MgArgs& a, int ranks) {
   p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, TC_BM, NT);
   p.ny = ceil_div(p.N, NT);
   const long long items = (long long)ceil_div(p.M, TC_BM) * p.ny;
-  if (items > 0x7fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");
+  if (items > 0x3fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");
   const int stages = ceil_div(p.across, S::CH);
   p.ranks = ranks;
   p.share = ceil_div(stages, p.ranks);
@@ -650,7 +654,7 @@ int mgp_launch(cudaStream_t s, const MgArgs& a) {
   p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, 2 * TC_BM, 0);
   p.ny = ceil_div(p.N, S::NT);
   const long long items = (long long)ceil_div(p.M, 2 * TC_BM) * p.ny;
-  if (items > 0x7fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");
+  if (items > 0x3fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");
   p.n_items = (int)items;
   const int pairs = max(1, sm_budget() / 2);
   auto k = mx_gemm_pair_kernel<KIND, READ>;

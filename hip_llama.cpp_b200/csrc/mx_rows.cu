@@ -23,7 +23,7 @@ int mx_refuse(const char* who, const char* why) {
 int mx_check(const tha_mx_t* m, const char* who) {
   if (!m) return mx_refuse(who, "a matrix is NULL");
   if (m->format != THA_MX_E2M1 && m->format != THA_MX_E4M3) return mx_refuse(who, "unknown format");
-  if (m->rows < 0 || m->cols < 1 || m->cols > MX_MOST_COLS) return mx_refuse(who, "a matrix has at least one column, and 2^30 at most");
+  if (m->rows < 0 || m->rows > MX_MOST || m->cols < 1 || m->cols > MX_MOST) return mx_refuse(who, "a matrix has at least one column, and 2^30 rows and columns at most");
   if (m->rows == 0) return THA_STATUS_SUCCESS;
   if (!m->codes || !m->scales) return mx_refuse(who, "codes or scales are NULL");
   if ((reinterpret_cast<uintptr_t>(m->codes) & 31u) || !aligned16(m->scales)) return mx_refuse(who, "codes on a 32-byte and scales on a 16-byte boundary are needed");
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(MR_THREADS) mx_read_lanes_kernel(const tha_mx_
 
 // A number in 64 bits as one of 32 that compares with every number of at most 23 bits as it does itself: cut off, with the last bit set where something was cut. So a code is one rounding.
 __device__ __forceinline__ float mr_odd(double y) {
+  if (fabs(y) >= 0x1p128) return (float)y;         // infinite in fp32
   const float f = __double2float_rz(y);
   return (double)f != y && y == y ? __uint_as_float(__float_as_uint(f) | 1u) : f;
 }
@@ -565,11 +566,11 @@ int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, 
 using namespace tha;
 
 extern "C" size_t tha_hyb_mx_codes_bytes(int format, int rows, int cols) {
-  if ((format != THA_MX_E2M1 && format != THA_MX_E4M3) || rows < 1 || cols < 1 || cols > MX_MOST_COLS) return 0;
+  if ((format != THA_MX_E2M1 && format != THA_MX_E4M3) || rows < 1 || rows > MX_MOST || cols < 1 || cols > MX_MOST) return 0;
   return (size_t)rows * mx_pitch(format, cols);
 }
 extern "C" size_t tha_hyb_mx_scales_bytes(int rows, int cols) {
-  if (rows < 1 || cols < 1 || cols > MX_MOST_COLS) return 0;
+  if (rows < 1 || rows > MX_MOST || cols < 1 || cols > MX_MOST) return 0;
   return (((size_t)rows + MX_TILE - 1) / MX_TILE) * (mx_padded(cols) / MX_TILE) * MX_TILE_BYTES;
 }
 

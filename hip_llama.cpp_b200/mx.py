@@ -22,7 +22,7 @@ FORMATS = {"e2m1": 0, "e4m3": 1}                                # THA_MX_*
 CODES = {torch.uint8: "e2m1", torch.float8_e4m3fn: "e4m3"}      # what holds them
 ACTS = {"clamped": 0, "relu2": 1, "gelu": 2, "xielu": 3, "silu": 4}    # THA_ACT_*
 UNGATED = ("relu2", "xielu")
-BLOCK, TILE, MOST_COLS = 32, 128, 1 << 30
+BLOCK, TILE, MOST = 32, 128, 1 << 30
 
 
 class MxStruct(C.Structure):
@@ -80,7 +80,7 @@ class Mx:
     def __init__(self, codes, scales, rows: int, cols: int):
         if codes.dtype not in CODES:
             raise ValueError(f"codes are uint8 (e2m1, two a byte) or float8_e4m3fn, not {codes.dtype}")
-        if rows < 0 or not 1 <= cols <= MOST_COLS or rows > 0x7fffffff:
+        if not 0 <= rows <= MOST or not 1 <= cols <= MOST:
             raise ValueError(f"a matrix has rows and at least one column, got {rows} x {cols}")
         format = CODES[codes.dtype]
         width, count = padded(cols) // (2 if format == "e2m1" else 1), -(-rows // TILE) * padded(cols) * TILE // BLOCK
@@ -99,7 +99,7 @@ class Mx:
     @classmethod
     def empty(cls, rows: int, cols: int, format: str = "e2m1", device="cuda"):
         """Room for a matrix: what a call fills.  Codes and scales are one piece of memory; the tensors over them are made when they are asked for."""
-        if format not in FORMATS or rows < 0 or not 1 <= cols <= MOST_COLS:
+        if format not in FORMATS or not 0 <= rows <= MOST or not 1 <= cols <= MOST:
             raise ValueError(f"a matrix of rows and at least one column in e2m1 or e4m3, not {rows} x {cols} in {format!r}")
         wide = (cols + 127) & -128
         scales = (rows * (wide >> 1 if format == "e2m1" else wide) + 511) & -512

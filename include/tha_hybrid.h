@@ -700,7 +700,7 @@ size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t
 typedef struct {
   void* codes;
   uint8_t* scales;
-  int rows, cols;       /* cols: 1 .. 2^30 */
+  int rows, cols;       /* 0 .. 2^30, 1 .. 2^30 */
   int format;           /* THA_MX_* */
 } tha_mx_t;
 /* bytes of the two arrays; 0: no such matrix */
@@ -714,7 +714,8 @@ int tha_hyb_mx_quant(void* stream, int dtype, const void* x, long long ldx, cons
 /* x (dtype-typed, rows ldx elements apart) = the values that m stands for, code * 2^(c - 127) rounded to dtype (exact but at the ends of its range) */
 int tha_hyb_mx_read(void* stream, int dtype, const tha_mx_t* m, void* x, long long ldx);
 /* A sublayer's result joins the residual stream, whose norm is quantised: x_out = x + left (fp32 [rows, cols] without gaps; x_out may be x; left dtype-typed, rows ldl elements
- * apart, NULL: x_out = x), out = x_out / sqrt(mean(x_out^2) + eps) * (w_offset + w), w [cols].  What is quantised is the norm in 64 bits: a code is one rounding of the norm of x_out as stored. */
+ * apart, NULL: x_out = x), out = x_out / sqrt(mean(x_out^2) + eps) * (w_offset + w), w [cols].  What is quantised is the norm in 64 bits (infinite beyond fp32's
+ * numbers): a code is one rounding of the norm of x_out as stored. */
 int tha_hyb_mx_add_norm(void* stream, int dtype, const float* x, const void* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t* out);
 /* C[m, n] = sum_k A[m, k] W[n, k] (dtype-typed, rows ldc elements apart).  A in either format, W E2M1, as many columns.  Products are exact, sums fp32 on the tensor cores.
  * A kernel that gives up on a barrier (a fault of its pipeline) says so through tha_gemm_check_error (tha_b200.h). */

@@ -254,3 +254,161 @@ def test_no_rows():
     a = M.quantise(torch.randn(0, 96, device="cuda"), "e4m3")
     assert a.read().shape == (0, 96) and M.linear(a, w).shape == (0, 64) and M.linear_act(a, w, w).rows == 0
     assert M.add_norm(torch.randn(0, 96, device="cuda"), None, torch.ones(96, device="cuda"), eps=1e-5).rows == 0
+
+
+# ---- as a layer uses them -----------------------------------------------------------------------------------------------------
+def layer(rows, width, ff, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    return {"x": rand(rows, width), "att": rand(rows, width).bfloat16(), "norm": 1 + 0.1 * rand(width), "wo": M.quantise(rand(width, width) / width ** 0.5),
+            "gate": M.quantise(rand(ff, width) / width ** 0.5), "up": M.quantise(rand(ff, width) / width ** 0.5), "down": M.quantise(rand(width, ff) / ff ** 0.5)}
+
+
+def run_layer(s, fmt="e4m3"):
+    """attention's result -> output product -> residual and norm -> feed-forward -> residual"""
+    x = s["x"].clone()
+    y = M.linear(M.quantise(s["att"], fmt), s["wo"], dtype=torch.bfloat16)
+    a = M.add_norm(x, y, s["norm"], eps=1e-5, format=fmt)
+    h = M.linear_act(a, s["gate"], s["up"], format=fmt)
+    z = M.linear(h, s["down"])
+    last = M.add_norm(x, z, s["norm"], eps=1e-5, format=fmt)
+    return y, a.read(), h.read(), z, x, last.read()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,width,ff", [(1, 288, 768), (17, 512, 1100), (260, 768, 2048), (1100, 512, 2600)])
+def test_a_layer(fmt, rows, width, ff):
+    """Every call's result against 64 bits on what the call ahead of it left"""
+    s = layer(rows, width, ff, rows)
+    y, a, h, z, x, last = (t.double().cpu().numpy() for t in run_layer(s, fmt))
+    att, _, _ = O.quantise(s["att"].double().cpu().numpy(), fmt)
+    wo, gate, up, down = (O.values(s[k]) for k in ("wo", "gate", "up", "down"))
+    assert (np.abs(y - att @ wo.T) <= sum_bound(att, wo) + (np.abs(att @ wo.T) + sum_bound(att, wo)) * 2.0 ** -8).all()
+    first = (s["x"].double().cpu().numpy() + y).astype(np.float32).astype(np.float64)
+    norm = lambda t: t / np.sqrt((t * t).mean(-1, keepdims=True) + 1e-5) * s["norm"].double().cpu().numpy()  # noqa: E731
+    assert np.array_equal(a, O.quantise(norm(first), fmt)[0])
+    assert (np.abs(z - h @ down.T) <= sum_bound(h, down)).all()
+    assert np.array_equal(x, (first + z).astype(np.float32).astype(np.float64)) and np.array_equal(last, O.quantise(norm(x), fmt)[0])
+    g, u = a @ gate.T, a @ up.T
+    want = O.act("silu", g, u, 0, 0)
+    # a value is off by half a step at most, 2^-4 (8 bits) or 1/4 (4 bits) of it or as much of the smallest normal number under its block's scale, which is below 2 / M of the block's largest
+    top = np.repeat(np.pad(np.abs(want), ((0, 0), (0, -ff % 32))).reshape(rows, -1, 32).max(-1), 32, 1)[:, :ff]
+    half, least = (2.0 ** -4, 2.0 ** -6 / 448) if fmt == "e4m3" else (0.25, 1 / 6)
+    assert (np.abs(h - want) <= 1.01 * half * np.maximum(np.abs(want), 2 * least * top) + 1e-5 * top).all()
+
+
+def test_captured_layers_share_nothing():
+    """Two captured layers on streams of their own, replayed at once and again with other inputs, as the same calls one by one"""
+    cases = [layer(5, 512, 1100, 1), layer(700, 512, 2600, 2)]
+    graphs, outs = [], []
+    for s in cases:
+        run_layer(s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run_layer(s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(3):
+        for s in cases:
+            s["att"].copy_(torch.randn_like(s["att"], dtype=torch.float32))
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for s, o in zip(cases, outs):
+            for got, want in zip(o, run_layer(s)):
+                assert torch.equal(got, want)
+    M.check_error()
+
+
+def test_first_calls_of_a_process_captured():
+    """What the library keeps for a device is made inside the capture"""
+    import subprocess
+    import sys
+    code = ("import sys; sys.path.insert(0, 'tests')\nimport torch\nfrom pkgload import load_pkg\nM = load_pkg('mx')\n"
+            "x = torch.randn(700, 4096, device='cuda'); w = torch.ones(4096, device='cuda'); k = torch.randn(2600, 4096, device='cuda')\ntorch.cuda.synchronize()\n"
+            "g = torch.cuda.CUDAGraph()\nwith torch.cuda.graph(g):\n    q = M.quantise(k); a = M.add_norm(x, None, w, eps=1e-5); y = M.linear(a, q); h = M.linear_act(a, q, q)\n"
+            "g.replay(); torch.cuda.synchronize()\nassert torch.equal(y, M.linear(M.add_norm(x, None, w, eps=1e-5), M.quantise(k)))\n"
+            "assert torch.equal(h.read(), M.linear_act(a, q, q).read())\nM.check_error(); print('fine')\n")
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_threads_and_streams():
+    """Four threads on streams of their own make calls of different forms at once"""
+    import threading
+    cases = [layer(*c) for c in ((1, 512, 1100, 1), (33, 512, 1100, 2), (300, 768, 2048, 3), (900, 512, 2600, 4))]
+    want = [run_layer(s) for s in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got = run_layer(cases[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not bad and not any(t.is_alive() for t in threads)
+    M.check_error()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (33, 130), (129, 513), (700, 4096)])
+def test_nothing_else_is_written(fmt, rows, cols):
+    """Memory around a matrix, and the scale bytes of rows behind its last one, stay as they were"""
+    size = M.Mx.empty(rows, cols, fmt)
+    nc, ns = size.codes.numel(), size.scales.numel()
+    room = torch.full((512 + nc + 1024 + ns + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+    a, b = 512, (512 + nc + 1023) // 512 * 512
+    codes = room[a:a + nc].view(rows, -1)
+    m = M.Mx(codes if fmt == "e2m1" else codes.view(torch.float8_e4m3fn), room[b:b + ns], rows, cols)
+    x = torch.randn(rows, cols, device="cuda")
+    one, up = M.quantise(torch.randn(rows, 64, device="cuda"), "e4m3"), M.quantise(torch.randn(cols, 64, device="cuda"))
+
+    def around():
+        t = room.clone()
+        t[a:a + nc] = 0xA5
+        s = t[b:b + ns].view(-1, ns // 512 // -(-rows // 128), 32, 4, 4)
+        for r in range(rows - (rows - 1) // 128 * 128):
+            s[-1, :, r % 32, r // 32] = 0xA5
+        s[:-1] = 0xA5
+        return bool((t == 0xA5).all())
+
+    for call in (lambda: M.quantise(x, out=m), lambda: M.add_norm(x, None, torch.ones(cols, device="cuda"), eps=1e-5, out=m), lambda: M.linear_act(one, None, up, act="relu2", out=m),
+                 lambda: M.linear_act(one, up, up, out=m)):
+        room.fill_(0xA5)
+        call()
+        assert around()
+        assert not O.codes_of(m)[:, cols:].any() and (O.scales_of(m)[:, -(-cols // 32):] == 0).all()
+
+
+def test_long_rows():
+    """Offsets beyond 32 bits: a matrix of more than 2^31 codes, and results of more than 2^31 elements"""
+    rows, cols = 70000, 33000
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-1], x[0, :5], x[35000, 7] = torch.randn(cols, device="cuda").bfloat16(), 2.0, -3.0
+    for fmt in FORMATS:
+        m = M.quantise(x, fmt)
+        back = m.read(torch.bfloat16)
+        want = O.quantise(x[[0, 35000, rows - 1]].double().cpu().numpy(), fmt)[0]
+        assert np.array_equal(back[[0, 35000, rows - 1]].double().cpu().numpy(), want)
+        assert int((back != 0).sum()) == int((torch.from_numpy(want) != 0).sum())
+        del m, back
+    del x
+    a, w = matrices(70000, 31000, 32, "e4m3", 1)
+    got = M.linear(a, w, dtype=torch.bfloat16)
+    pick = [0, 1, 34999, 69998, 69999]
+    va, vw = O.values(a)[pick], O.values(w)
+    want = va @ vw.T
+    assert (np.abs(got[pick].double().cpu().numpy() - want) <= sum_bound(va, vw) + (np.abs(want) + sum_bound(va, vw)) * 2.0 ** -8).all()

@@ -60,7 +60,7 @@ def test_sizes_of_no_matrix():
     assert c.tha_hyb_mx_scales_bytes(0, 5) == c.tha_hyb_mx_scales_bytes(5, 0) == 0
 
 
-BAD = [dict(format="e5m2"), dict(cols=0), dict(cols=-3), dict(rows=-1), dict(codes=16), dict(scales=1032), dict(codes=-BASE), dict(scales=-BASE), dict(cols=(1 << 30) + 1)]
+BAD = [dict(format="e5m2"), dict(cols=0), dict(cols=-3), dict(rows=-1), dict(codes=16), dict(scales=1032), dict(codes=-BASE), dict(scales=-BASE), dict(cols=(1 << 30) + 1), dict(rows=(1 << 30) + 1)]
 
 
 @pytest.mark.parametrize("bad", BAD)
