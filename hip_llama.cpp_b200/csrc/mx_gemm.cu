@@ -45,7 +45,7 @@ struct MgSmem {
   static constexpr int W_BYTES = WT * TC_BM * 128, X_BYTES = NT * 128;
   static constexpr int SW_BYTES = CH * MX_TILE_BYTES, SX_BYTES = CH * MX_TILE_BYTES;   // of one matrix, of one row tile
   static constexpr int STAGE = (W_BYTES + X_BYTES + WT * SW_BYTES + XT * SX_BYTES + 1023) / 1024 * 1024;
-  static constexpr int ROOM = STAGE <= 36 * 1024 ? 110 * 1024 : 220 * 1024;             // two blocks an SM, or one
+  static constexpr int ROOM = STAGE <= 37 * 1024 ? 111 * 1024 : 220 * 1024;             // two blocks an SM, or one
   static constexpr int NST = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
   static constexpr int ACC_COLS = WT * NT;
   static constexpr int SET = CH * 4 * (WT + XT);                      // TMEM columns of a stage's scales
@@ -53,7 +53,8 @@ struct MgSmem {
   static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int TOTAL = NST * STAGE + 1024 + (2 * NST + 2) * 8 + 64;
   static_assert(NST * STAGE >= ACC_COLS * TC_BM * 4, "the partial tile lies over the ring");
-  static_assert(COLS <= (ROOM <= 110 * 1024 ? 256 : 512) && TOTAL <= TC_SMEM_LIMIT && NST >= 3, "a stage is too large");
+  static_assert(ROOM > 111 * 1024 || 2 * (TOTAL + 1024) <= 228 * 1024, "two blocks an SM");
+  static_assert(COLS <= (ROOM <= 111 * 1024 ? 256 : 512) && TOTAL <= TC_SMEM_LIMIT && NST >= 3, "a stage is too large");
 };
 
 __device__ __forceinline__ void mg_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -588,9 +589,10 @@ int mg_map(int kind, const tha_mx_t* m, int box_rows, CUtensorMap* out, int* byt
 //   192 rows x [12288, 4096] e4m3: 288 tiles of 64 14.4, pairs 16.5; 256 rows, 384 tiles 24.6, pairs 17.4      e2m1 10.6 / 11.9, 17.1 / 12.5
 //   gated [2 x 4096, 4096]: 256 rows, 128 tiles 19.2, pairs 21.9; [2 x 12288, 4096]: 64 rows, 96 tiles 20.6, pairs 24.9; 128 rows, 192 tiles 38.2, pairs 26.0
 // Tiles of 128 rows were between the two or behind both everywhere (256 rows x [4096, 4096]: 64 11.1, 128 12.1, pairs 15.0), 32 rows take 5 % less time than 64 with so few.
-// The blocks of a cluster share a tile's stages: up to 8, 4 or 2 of them while the SMs hold them, where there are stages enough to share:
+// The blocks of a cluster share a tile's stages: 8, 4, 3 or 2 of them while the SMs hold them, where there are stages enough to share:
 //   1 row x [4096, 11008], 86 stages, at 1 / 2 / 4 / 8 blocks 22.1 / 14.0 / 9.6 / 8.5;  [4096, 4096], 32 stages 9.7 / 7.4 / 5.8 / 5.8;  [2048, 2048], 16 stages 5.9 / 5.2 / 4.4 / 4.2;
 //   16 rows x [1024, 1024], 8 stages 3.6 / 4.3 / 3.9 / 3.8;  128 rows x [4096, 4096] 11.9 / 10.5 / 9.3;  16 rows x [12288, 4096] 10.7 / 9.9 / 13.9
+//   16 rows x [2 x 11008, 4096] 20.2 / 15.6 / (3) 14.0;
 //   a gated one's blocks share the activation, too: 16 rows x [2 x 1024, 1024] - / 5.5 / 4.7 / 4.8
 // Clusters have to fit the SMs of a GPC together: seven eighths of the places are counted (96 tiles x 3 blocks on 296 places: 15.7 where 2 take 9.9).
 struct MgForm { int nt, ranks; };                  // nt 0: pairs
@@ -599,7 +601,7 @@ MgForm mg_form(int read, int tiles, int rows, int stages) {
   const int places = read == MG_GATED && nt == 64 ? sms : 2 * sms;
   const long long items = (long long)tiles * ceil_div(rows, nt);
   if (items > places) return {rows > 64 ? 0 : nt, 1};
-  for (int ranks = stages >= 64 || (read == MG_GATED && nt == 16 && stages >= 16) ? 8 : 4; ranks > 1; ranks >>= 1)
+  for (int ranks = stages >= 64 || (read == MG_GATED && nt == 16 && stages >= 16) ? 8 : 4; ranks > 1; ranks = ranks == 8 ? 4 : ranks - 1)
     if (stages >= (read == MG_GATED ? 8 : 16) && items * ranks * 8 <= (long long)places * 7) return {nt, ranks};
   return {nt, 1};
 }
