@@ -222,6 +222,23 @@ def test_linear_act(fmt, out_fmt, act, limit, alpha, rows, n, k):
     near(m, y, cancels, [O.act(act, p[0] + s * sum_bound(va, O.values(ws[0])), p[-1] + t * sum_bound(va, O.values(ws[-1])), limit, alpha) for s in (-1, 1) for t in (-1, 1)])
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "clamped"])
+@pytest.mark.parametrize("power", [20, 45, 55])
+@pytest.mark.parametrize("rows,n", [(3, 300), (600, 9300)])
+def test_large_gates(act, power, rows, n):
+    """Gates whose cube, in gelu, is no number of fp32, and whose sigmoid is 1 or 0"""
+    a, gate, up = matrices(rows, n, 64, "e4m3", power, 2)
+    gate.scales.add_(torch.where(gate.scales < 255, torch.tensor(power, dtype=torch.uint8, device="cuda"), torch.tensor(0, dtype=torch.uint8, device="cuda")))
+    va, vg, vu = O.values(a), O.values(gate), O.values(up)
+    g, u = va @ vg.T, va @ vu.T
+    m = M.linear_act(a, gate, up, act=act, limit=5.0, alpha=1.5)
+    M.check_error()
+    y = O.act(act, g, u, 5.0, 1.5)
+    assert np.isfinite(y).all() and np.isfinite(O.values(m)).all()
+    cancels = 2.0 ** -23 * np.abs(g * u) if act == "gelu" else 2.0 ** -126 * np.abs(g) * (1 + np.abs(u))
+    near(m, y, cancels, [O.act(act, g + s * sum_bound(va, vg), u + t * sum_bound(va, vu), 5.0, 1.5) for s in (-1, 1) for t in (-1, 1)])
+
+
 def near(m, y, cancels, around):
     """m's values are within half a step of y, as far as y itself is known: `around` holds it at the ends of its products' bounds; the activation in fp32 is good to 2^-20 of it, and to
     `cancels` where it is a difference: gelu's 1 + tanh is off by a unit of tanh near 1 and a rounding, 2^-23 + 2^-24 in all and 0.5 g u times that; xielu's e^u - 1 - u by a unit of e^u - 1 and a
@@ -239,13 +256,18 @@ def near(m, y, cancels, around):
     assert (worst <= 1e-12 * np.abs(y)).all(), worst.max()
 
 
-def test_nan_rows_stay_in_their_rows():
-    a, w = matrices(20, 200, 300, "e4m3", 4)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,n", [(20, 200), (100, 200), (1100, 2600)])
+def test_nan_rows_stay_in_their_rows(fmt, rows, n):
+    a, w = matrices(rows, n, 300, fmt, 4)
     a.scales.view(-1)[(0 * 32 + 3) * 16 + 0] = 255           # row 3, block 0
     w.scales.view(-1)[(1 * 3 + 2) * 512 + (5 % 32) * 16 + 1] = 255    # row 133, block 9
     got = M.linear(a, w).cpu()
-    bad = torch.zeros(20, 200, dtype=torch.bool)
+    bad = torch.zeros(rows, n, dtype=torch.bool)
     bad[3], bad[:, 133] = True, True
+    assert torch.equal(got.isnan(), bad)
+    got = M.linear_act(a, w, w).read().cpu()                 # a block of the result is NaN as a whole
+    bad[:, 128:160] = True
     assert torch.equal(got.isnan(), bad)
 
 
