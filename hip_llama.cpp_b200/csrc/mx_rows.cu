@@ -1,10 +1,10 @@
 // Rows into microscaled numbers and back, and the norm that ends in them (tha_mx_t).
-//   mx_quant_kernel          a warp takes 512 consecutive values of a row at a time: a lane eight and eight of them, four lanes a block, whose largest |value| is a maximum of bit patterns
+//   mx_quant_kernel          a warp takes 512 consecutive values of a row at a time: two or four lanes a block, whose largest |value| is a maximum of bit patterns
 //   mx_read_kernel           16 bytes of results a lane (mx_read_lanes_kernel: rows on no boundary)
 //   mx_add_norm_kernel       a block of threads takes a row: x + left, the square sum in fp64, the norm, its codes
 //   mx_add_norm_ring_kernel  the same for many wide rows, which come through a ring; mx_add_norm_wide_kernel: rows beyond what registers hold
-// A value is read and written once: bound by memory, quantising at 4.3 TB/s (11008 x 4096 bf16 to 4 bits 26.6 us) to 6.1 (fp32 to 8 bits 37.0), reading back at 4.7 (4 bits to bf16 24.2) and
-// 5.1 (8 bits to fp32 44.3); where values are 16 bits or less the instructions for each, 8 to 10, are as many as the SMs issue meanwhile.
+// A value is read and written once: bound by memory, quantising at 5.4 TB/s (11008 x 4096 bf16 to 4 bits 21.2 us) to 6.1 (fp32 to 8 bits 37.0), reading back at 4.7 (4 bits to bf16 24.2) and
+// 5.1 (8 bits to fp32 44.3); where values are 16 bits or less the instructions for each are as many as the SMs issue meanwhile.
 #include <cuda_fp16.h>
 
 #include "hybrid_ops.cuh"
@@ -46,8 +46,7 @@ constexpr int MR_WARPS = MR_THREADS / 32;
 constexpr int MR_NORM_MOST = 512;                // threads of a row's block at most
 constexpr int MR_N = 4;                           // values of a thread of the norm's at a time
 constexpr int MR_V = 8;                           // values of a lane
-constexpr int MR_U = 2;                           // such eights of a lane, 256 values apart
-constexpr int MR_SEG = 32 * MR_V * MR_U;          // values of a warp at a time
+constexpr int MR_SEG = 512;                       // values of a warp at a time
 
 // four values as fp32, zeros behind the first n; vec: p is on a boundary of four
 __device__ __forceinline__ void mr_load(const float* p, int n, bool vec, float (&v)[MR_N]) {
@@ -123,7 +122,7 @@ __device__ __forceinline__ void mr_codes(const tha_mx_t& out, int row, int col, 
   }
   if (!(threadIdx.x & 3)) out.scales[mx_scale_at(row, col / MX_TILE, padded / MX_TILE) + (col / MX_BLOCK & 3)] = (uint8_t)byte;
 }
-// Eight values as they lie in memory, zeros behind the first n
+// Eight values as they lie in memory, zeros behind the first n; bf16 on a boundary: sixteen
 __device__ __forceinline__ void mr_fetch(const float* p, int n, bool vec, uint4 (&q)[2]) {
   if (vec && n >= MR_V) { q[0] = *reinterpret_cast<const uint4*>(p); q[1] = *reinterpret_cast<const uint4*>(p + 4); return; }
   unsigned t[8];
@@ -131,13 +130,19 @@ __device__ __forceinline__ void mr_fetch(const float* p, int n, bool vec, uint4 
   for (int i = 0; i < 8; i++) t[i] = i < n ? __float_as_uint(p[i]) : 0u;
   q[0] = make_uint4(t[0], t[1], t[2], t[3]); q[1] = make_uint4(t[4], t[5], t[6], t[7]);
 }
-__device__ __forceinline__ void mr_fetch(const __nv_bfloat16* p, int n, bool vec, uint4 (&q)[1]) {
-  if (vec && n >= MR_V) { q[0] = *reinterpret_cast<const uint4*>(p); return; }
+__device__ __forceinline__ void mr_fetch(const __nv_bfloat16* p, int n, uint4 (&q)[1]) {
   const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
   unsigned t[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) t[i] = (2 * i < n ? h[2 * i] : 0u) | (2 * i + 1 < n ? h[2 * i + 1] : 0u) << 16;
   q[0] = make_uint4(t[0], t[1], t[2], t[3]);
+}
+__device__ __forceinline__ void mr_fetch(const __nv_bfloat16* p, int n, uint4 (&q)[2]) {
+  uint4 h[1];
+  if (n >= MR_V) q[0] = *reinterpret_cast<const uint4*>(p);
+  else { mr_fetch(p, n, h); q[0] = h[0]; }
+  if (n >= 2 * MR_V) q[1] = *reinterpret_cast<const uint4*>(p + MR_V);
+  else { mr_fetch(p + MR_V, n - MR_V, h); q[1] = h[0]; }
 }
 __device__ __forceinline__ unsigned mr_values(const uint4 (&q)[2], float (&v)[MR_V]) {
   const unsigned w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
@@ -160,6 +165,35 @@ __device__ __forceinline__ unsigned mr_values(const uint4 (&q)[1], float (&v)[MR
   }
   return max(top << 16, top & 0xffff0000u);
 }
+__device__ __forceinline__ unsigned mr_mul2(unsigned a, unsigned b) {   // two products of bf16
+  const __nv_bfloat162 t = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const unsigned*>(&t);
+}
+// The same for sixteen values of bf16, two lanes a block: maxima and scaling two at a time (a power of two times a bf16 is one; what underflows has the code 0)
+template <int FMT>
+__device__ __forceinline__ void mr_codes(const tha_mx_t& out, int row, int col, int padded, const uint4 (&q)[2]) {
+  const unsigned w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+  top = __vmaxu2(top, __shfl_xor_sync(THA_FULL_MASK, top, 1));
+  const unsigned byte = mx_scale_byte<FMT>(max(top << 16, top & 0xffff0000u));
+  const unsigned inv = byte == 255u ? 0u : (254u - byte) * 0x00800080u;    // 1 / scale, twice
+  if (col >= padded) return;
+  unsigned c[FMT == THA_MX_E2M1 ? 2 : 4] = {};
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const unsigned y = mr_mul2(w[i], inv);
+    const float a = __uint_as_float(y << 16), b = __uint_as_float(y & 0xffff0000u);
+    if (FMT == THA_MX_E2M1) c[i >> 2] |= mx_e2m1x2(a, b) << (8 * (i & 3));
+    else c[i >> 1] |= mx_e4m3x2(a, b) << (16 * (i & 1));
+  }
+#pragma unroll
+  for (int i = 0; i < (FMT == THA_MX_E2M1 ? 2 : 4); i++) c[i] = byte == 255u ? 0u : c[i];
+  if (FMT == THA_MX_E2M1) *reinterpret_cast<uint2*>(static_cast<char*>(out.codes) + (size_t)row * (padded / 2) + col / 2) = make_uint2(c[0], c[1]);
+  else *reinterpret_cast<uint4*>(static_cast<char*>(out.codes) + (size_t)row * padded + col) = make_uint4(c[0], c[1], c[FMT == THA_MX_E2M1 ? 0 : 2], c[FMT == THA_MX_E2M1 ? 0 : 3]);
+  if (!(threadIdx.x & 1)) out.scales[mx_scale_at(row, col / MX_TILE, padded / MX_TILE) + (col / MX_BLOCK & 3)] = (uint8_t)byte;
+}
 
 // A warp's way through the segments of all rows: the next one is `warps` segments further.  One division at its start (one a segment, in 64 bits, and a lane's eight values at a time: 11008 x
 // 4096 values in 57 us).
@@ -177,17 +211,23 @@ struct MrWalk {
   }
 };
 
-template <int FMT, typename T>
+// V values of a lane at a time.  bf16 on 16-byte boundaries: sixteen, two instructions for a pair (11008 x 4096 to 4 bits 21.2 us, eight 26.6); rows on no boundary, value by value: eight
+// (4000 x 4097 16.4 us, sixteen 23.0)
+template <int FMT, typename T, int V>
 __global__ void __launch_bounds__(MR_THREADS) mx_quant_kernel(const T* x, long long ldx, const tha_mx_t out, bool vec) {
   hyb_pdl_enter();
-  constexpr int Q = sizeof(T) / 2;                // 16-byte words of eight values
-  const int lane = (threadIdx.x & 31) * MR_V;
+  constexpr int U = MR_SEG / (32 * V), Q = V * sizeof(T) / 16;
+  const int lane = (threadIdx.x & 31) * V;
   MrWalk at(out.cols);
-  uint4 now[MR_U][Q], next[MR_U][Q];
-  auto fetch = [&](uint4 (&q)[MR_U][Q]) {
+  uint4 now[U][Q], next[U][Q];
+  auto fetch = [&](uint4 (&q)[U][Q]) {
     const T* p = x + at.row * ldx + at.col + lane;
 #pragma unroll
-    for (int u = 0; u < MR_U; u++) mr_fetch(p + u * 32 * MR_V, out.cols - at.col - lane - u * 32 * MR_V, vec, q[u]);
+    for (int u = 0; u < U; u++) {
+      const int n = out.cols - at.col - lane - u * 32 * V;
+      if constexpr (sizeof(T) == 2) mr_fetch(p + u * 32 * V, n, q[u]);
+      else mr_fetch(p + u * 32 * V, n, vec, q[u]);
+    }
   };
   if (at.row < out.rows) fetch(now);
   while (at.row < out.rows) {
@@ -195,10 +235,14 @@ __global__ void __launch_bounds__(MR_THREADS) mx_quant_kernel(const T* x, long l
     at.next();
     if (at.row < out.rows) fetch(next);           // on its way while this one is coded
 #pragma unroll
-    for (int u = 0; u < MR_U; u++) {
-      float v[MR_V];
-      const unsigned top = mr_values(now[u], v);
-      mr_codes<FMT>(out, row, col + u * 32 * MR_V, at.padded, top, v);
+    for (int u = 0; u < U; u++) {
+      if constexpr (V == 16) {
+        mr_codes<FMT>(out, row, col + u * 32 * V, at.padded, now[u]);
+      } else {
+        float v[MR_V];
+        const unsigned top = mr_values(now[u], v);
+        mr_codes<FMT>(out, row, col + u * 32 * V, at.padded, top, v);
+      }
 #pragma unroll
       for (int i = 0; i < Q; i++) now[u][i] = next[u][i];
     }
@@ -517,7 +561,8 @@ unsigned mr_blocks(long long rows, long long padded) {
 template <int FMT, typename T>
 int quant_form(cudaStream_t s, const T* x, long long ldx, const tha_mx_t* out) {
   const bool vec = mr_aligned(x, out->rows > 1 ? ldx : 0, sizeof(T));
-  THA_CUDA_OK(launch(mx_quant_kernel<FMT, T>, dim3(mr_blocks(out->rows, mx_padded(out->cols))), dim3(MR_THREADS), 0, s, pdl_enabled() != 0, x, ldx, *out, vec));
+  auto k = sizeof(T) == 2 && vec ? mx_quant_kernel<FMT, T, sizeof(T) == 2 ? 16 : 8> : mx_quant_kernel<FMT, T, 8>;
+  THA_CUDA_OK(launch(k, dim3(mr_blocks(out->rows, mx_padded(out->cols))), dim3(MR_THREADS), 0, s, pdl_enabled() != 0, x, ldx, *out, vec));
   return THA_STATUS_SUCCESS;
 }
 template <int FMT, typename T>

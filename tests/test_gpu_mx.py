@@ -77,7 +77,12 @@ def test_every_binade_and_border(fmt):
             r[1:11], r[11:21], r[21:31] = near, np.nextafter(near, np.float32(0)), -np.nextafter(near, np.float32(1e9))
             rows.append(np.ldexp(r, e).astype(np.float32))
     x = np.stack(rows)
-    same_matrix(M.quantise(torch.from_numpy(x).cuda(), fmt), x)
+    for dtype in DTYPES:                                     # one block a row, and all in a row
+        for t in (torch.from_numpy(x).cuda().to(dtype), torch.from_numpy(x).cuda().to(dtype).view(1, -1)):
+            m = M.quantise(t, fmt)
+            v = torch.from_numpy(same_matrix(m, t.double().cpu().numpy()))
+            assert torch.equal(m.read().double().cpu(), v.float().double())
+            assert torch.equal(m.read(torch.bfloat16).double().cpu(), v.float().bfloat16().double())
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
