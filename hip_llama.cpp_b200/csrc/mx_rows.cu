@@ -302,27 +302,27 @@ __global__ void __launch_bounds__(MR_THREADS) mx_read_kernel(const tha_mx_t m, T
     }
   }
 }
-// rows on no boundary: one value of each block a lane
+// rows on no boundary: one value of each block a lane, the scales of four blocks in a word
 template <int FMT, typename T>
 __global__ void __launch_bounds__(MR_THREADS) mx_read_lanes_kernel(const tha_mx_t m, T* x, long long ldx) {
   hyb_pdl_enter();
+  constexpr int B = MR_SEG / MX_BLOCK, STEP = FMT == THA_MX_E2M1 ? MX_BLOCK / 2 : MX_BLOCK;      // blocks of a segment, bytes of a block
   const int lane = threadIdx.x & 31;
   for (MrWalk at(m.cols); at.row < m.rows; at.next()) {
     const uint8_t* codes = static_cast<const uint8_t*>(m.codes) + (size_t)at.row * (FMT == THA_MX_E2M1 ? at.padded / 2 : at.padded) + (at.col + lane) / (FMT == THA_MX_E2M1 ? 2 : 1);
-    unsigned c[MR_SEG / 32], s[MR_SEG / 32];
+    const int across = at.padded / MX_TILE, left = m.cols - at.col - lane, tiles = across - at.col / MX_TILE;
+    const uint8_t* scales = m.scales + mx_scale_at(at.row, at.col / MX_TILE, across);
+    unsigned c[B], s[B / 4];
 #pragma unroll
-    for (int u = 0; u < MR_SEG / 32; u++) {
-      const int col = at.col + 32 * u;
-      c[u] = s[u] = 0;
-      if (col + lane < m.cols) {
-        c[u] = codes[(FMT == THA_MX_E2M1 ? 16 : 32) * u];
-        s[u] = m.scales[mx_scale_at(at.row, col / MX_TILE, at.padded / MX_TILE) + (u & 3)];
-      }
-    }
+    for (int u = 0; u < B; u++) c[u] = 32 * u < left ? codes[STEP * u] : 0u;
+#pragma unroll
+    for (int k = 0; k < B / 4; k++) s[k] = k < tiles ? *reinterpret_cast<const unsigned*>(scales + k * MX_TILE_BYTES) : 0u;
     T* p = x + at.row * ldx + at.col + lane;
 #pragma unroll
-    for (int u = 0; u < MR_SEG / 32; u++)
-      if (at.col + 32 * u + lane < m.cols) hyb_store(p + 32 * u, mr_pair<FMT>(FMT == THA_MX_E2M1 ? c[u] >> (4 * (lane & 1)) & 15u : c[u]).x * mx_scale(s[u]));
+    for (int u = 0; u < B; u++) {
+      const float f = mx_scale(s[u >> 2] >> (8 * (u & 3)) & 0xffu);
+      if (32 * u < left) hyb_store(p + 32 * u, mr_pair<FMT>(FMT == THA_MX_E2M1 ? c[u] >> (4 * (lane & 1)) & 15u : c[u]).x * f);
+    }
   }
 }
 
