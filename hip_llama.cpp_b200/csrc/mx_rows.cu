@@ -267,15 +267,17 @@ __global__ void __launch_bounds__(MR_THREADS) mx_read_kernel(const tha_mx_t m, T
   uint2 now[U] = {}, next[U] = {};
   unsigned scale[U] = {}, scale_next[U] = {};
   auto fetch = [&](uint2 (&c)[U], unsigned (&s)[U]) {
+    const int col = at.col + lane, left = m.cols - col;
+    const char* codes = static_cast<const char*>(m.codes) + (size_t)at.row * (FMT == THA_MX_E2M1 ? at.padded / 2 : at.padded) + (FMT == THA_MX_E2M1 ? col / 2 : col);
+    const uint8_t* scales = m.scales + mx_scale_at(at.row, col / MX_TILE, at.padded / MX_TILE) + (col / MX_BLOCK & 3);
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int col = at.col + lane + u * 32 * G;
-      if (col >= m.cols) continue;
-      const char* p = static_cast<const char*>(m.codes) + (size_t)at.row * (FMT == THA_MX_E2M1 ? at.padded / 2 : at.padded) + (FMT == THA_MX_E2M1 ? col / 2 : col);
+      if (u * 32 * G >= left) continue;
+      const char* p = codes + u * 32 * G / (FMT == THA_MX_E2M1 ? 2 : 1);
       if (FMT == THA_MX_E2M1 && G == 4) c[u].x = *reinterpret_cast<const unsigned short*>(p);
       else if (FMT == THA_MX_E2M1 || G == 4) c[u].x = *reinterpret_cast<const unsigned*>(p);
       else c[u] = *reinterpret_cast<const uint2*>(p);
-      s[u] = m.scales[mx_scale_at(at.row, col / MX_TILE, at.padded / MX_TILE) + (col / MX_BLOCK & 3)];
+      s[u] = scales[u * (32 * G / MX_TILE) * MX_TILE_BYTES];
     }
   };
   if (at.row < m.rows) fetch(now, scale);
