@@ -365,7 +365,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__ 
 // A pair (cta_group::2) takes 256 weight rows (of each of two matrices for a gated activation) x NT activation rows: each block has 128 of the weight rows and half of the activation rows
 // in its shared memory, an MMA reads both halves, and each block's TMEM gets 128 lanes of results.  Persistent: 74 pairs walk the items with running counters.  The accumulators take
 // 256 of TMEM's 512 columns and scales the others, so there is one set of them: eight warps fetch an item's sums into registers, 128 a thread, and hand the columns back before they do
-// anything with them; activation, quantising and stores run behind the next item's MMAs.  2048 rows x [12288, 4096] e4m3 80 us with codes of uniform random bytes (2.6 PFLOP/s), 98 with those
+// anything with them; activation, quantising and stores run behind the next item's MMAs.  2048 rows x [12288, 4096] e4m3 80 us with random codes of one sign (2.6 PFLOP/s), 97 with those
 // of normal numbers, 3333 rows x [11008, 4096] e2m1 68 and 75, 2048 rows x [2 x 11008, 4096] with silu 132 and 165: bound by power (960 to 1000 W at 1475 MHz), the tensor pipe at 54 to 65 % of
 // the cycles, some 43 bytes a cycle and SM from L2.
 // Scales: a block's TMEM holds those of its own weight rows and of all NT activation rows.  NT is a multiple of 128, so that an item's scales start with a tile of them: an MMA's scale

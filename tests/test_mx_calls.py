@@ -113,3 +113,25 @@ def test_the_binding_refuses():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_devices(monkeypatch):
+    x, w = torch.zeros(4, 96), torch.ones(96)
+    m = M.Mx.empty(4, 96, "e4m3", "cpu")
+    for call in (lambda: M.quantise(x), lambda: M.add_norm(x, None, w, eps=1e-5), lambda: m.read(), lambda: M.linear(m, M.Mx.empty(5, 96, device="cpu"))):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+    monkeypatch.setattr(M, "_current_device", lambda: 1)
+    with pytest.raises(ValueError, match="current device"):
+        M._stream(torch.device("cuda", 0))
+    monkeypatch.setattr(M, "_raw_stream", lambda index: 100 + index)
+    assert M._stream(torch.device("cuda", 1)) == 101
+
+
+def test_room_is_one_piece():
+    """The tensors over a matrix that a call made lie where the call wrote"""
+    for rows, cols, fmt in ((3, 70, "e2m1"), (130, 300, "e4m3"), (0, 5, "e2m1")):
+        m = M.Mx.empty(rows, cols, fmt, "cpu")
+        again = M.Mx(m.codes, m.scales, rows, cols)
+        assert rows == 0 or (again.c.codes, again.c.scales) == (m.c.codes, m.c.scales)
+        assert again.format == fmt and m.codes is m.codes and m.scales is m.scales
