@@ -27,7 +27,7 @@ enum { MG_F8 = 0, MG_F4 = 1 };                     // kind::mxf8f6f4, kind::mxf4
 enum { MG_PLAIN = 0, MG_UNGATED = 1, MG_GATED = 2 };
 
 struct MgP {
-  int M, N, K;                                     // weight rows, activation rows, values of a row
+  int M, N;                                        // weight rows, activation rows
   int ny, n_items;                                 // tiles of activation rows, items in all (pairs of blocks)
   int across;                                      // tiles of 128 values along k
   int ranks, share;                                // blocks of a cluster that share a tile, stages of each
@@ -702,7 +702,7 @@ int mg_check(const tha_mx_t* A, const tha_mx_t* W, const char* who) {
 }
 int mg_fill(MgArgs* a, const tha_mx_t* A, const tha_mx_t* W0, const tha_mx_t* W1) {
   a->A = A; a->W0 = W0; a->W1 = W1;
-  a->p.M = W0->rows; a->p.N = A->rows; a->p.K = A->cols;
+  a->p.M = W0->rows; a->p.N = A->rows;
   a->p.across = (int)(mx_padded(A->cols) / MX_TILE);
   a->p.sw0 = W0->scales; a->p.sw1 = W1 ? W1->scales : nullptr; a->p.sx = A->scales;
   return mx_error_flag(&a->p.error_flag);

@@ -593,9 +593,8 @@ int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, 
   const int need = ceil_div(out->cols, MR_N * 32) * 32;                                                       // a thread for four values
   const size_t stage = (size_t)out->cols * (4 + (left ? sizeof(T) : 0));
   if (vec && vec_left && (out->cols * sizeof(T)) % 16 == 0 && out->rows >= 2 * sm_budget() && need >= 1024 && need <= 6 * MR_NORM_MOST && 2 * stage <= 208 * 1024) {
-    const int threads = min(need, MR_NORM_MOST), p = ceil_div(need, threads);
+    const int threads = MR_NORM_MOST, p = ceil_div(need, threads);
     const int stages = (int)min((size_t)MR_RING_MOST, (p <= 2 && 2 * stage <= 104 * 1024 ? 104 * 1024 : 208 * 1024) / stage);
-    if (p <= 1) return ring_form<FMT, T, 1>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
     if (p <= 2) return ring_form<FMT, T, 2>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
     if (p <= 4) return ring_form<FMT, T, 4>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
     return ring_form<FMT, T, 6>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
