@@ -77,6 +77,8 @@ class Mx:
     """A matrix of rows x cols microscaled numbers.  codes: uint8 [rows, padded(cols) / 2] (e2m1, two a byte, the first in the low half) or float8_e4m3fn [rows, padded(cols)], what is padding 0;
     scales: uint8 in the order of `tiles`, 255: NaN."""
 
+    _codes = _scales = None                                     # until they are asked for, where a call made room
+
     def __init__(self, codes, scales, rows: int, cols: int):
         if codes.dtype not in CODES:
             raise ValueError(f"codes are uint8 (e2m1, two a byte) or float8_e4m3fn, not {codes.dtype}")
@@ -89,25 +91,22 @@ class Mx:
         if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.numel() != count or scales.device != codes.device or scales.data_ptr() % 16:
             raise ValueError(f"scales: {count} contiguous bytes on {codes.device} and a 16-byte boundary are needed, got {tuple(scales.shape)} {scales.dtype} on {scales.device}")
         self._codes, self._scales = codes, scales
-        self._bind(codes.data_ptr(), scales.data_ptr(), rows, cols, format, codes.device)
-
-    def _bind(self, codes, scales, rows, cols, format, device):
-        self.rows, self.cols, self.format, self.device = rows, cols, format, device
-        self.c = c = MxStruct(codes, scales, rows, cols, FORMATS[format])
-        self.ref = C.byref(c)
+        self.rows, self.cols, self.format, self.device = rows, cols, format, codes.device
+        self.c = MxStruct(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[format])
 
     @classmethod
     def empty(cls, rows: int, cols: int, format: str = "e2m1", device="cuda"):
         """Room for a matrix: what a call fills.  Codes and scales are one piece of memory; the tensors over them are made when they are asked for."""
-        if format not in FORMATS or not 0 <= rows <= MOST or not 1 <= cols <= MOST:
+        kind = FORMATS.get(format)
+        if kind is None or not 0 <= rows <= MOST or not 1 <= cols <= MOST:
             raise ValueError(f"a matrix of rows and at least one column in e2m1 or e4m3, not {rows} x {cols} in {format!r}")
         wide = (cols + 127) & -128
-        scales = (rows * (wide >> 1 if format == "e2m1" else wide) + 511) & -512
+        scales = (rows * (wide if kind else wide >> 1) + 511) & -512
         m = cls.__new__(cls)
         m._room = room = torch.empty(scales + ((rows + 127) & -128) * (wide >> 5), dtype=torch.uint8, device=device)
-        m._codes = m._scales = None
         at = room.data_ptr()
-        m._bind(at, at + scales, rows, cols, format, room.device)
+        m.rows, m.cols, m.format, m.device = rows, cols, format, room.device
+        m.c = MxStruct(at, at + scales, rows, cols, kind)
         return m
 
     @property
@@ -140,8 +139,9 @@ class Mx:
     def read(self, dtype=torch.float32, out=None):
         """The values that the codes stand for (tha_hyb_mx_read), [rows, cols]."""
         out, kind, ld = _result(out, self.rows, self.cols, dtype, self.device)
-        stream = _stream(self.device)
-        _check((_c or _load()).tha_hyb_mx_read(stream, kind, self.ref, out.data_ptr(), ld), "tha_hyb_mx_read")
+        status = (_c or _load()).tha_hyb_mx_read(_stream(self.device), kind, self.c, out.data_ptr(), ld)
+        if status:
+            _lib.check(status, "tha_hyb_mx_read")
         return out
 
 
@@ -170,9 +170,7 @@ def _result(out, rows, cols, dtype, device):
 
 
 def _matrix(m, rows, cols, format, device):
-    """`m`, or room for a matrix in its place"""
-    if m is None:
-        return Mx.empty(rows, cols, format, device)
+    """`m`, which has to have this size"""
     if (m.rows, m.cols, m.device) != (rows, cols, device):
         raise ValueError(f"out: {rows} x {cols} on {device} is needed, got {m.rows} x {m.cols} on {m.device}")
     if format not in FORMATS:
@@ -186,11 +184,6 @@ def _stream(device):
     if index is None or _current_device() != index:
         raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device() if torch.cuda.is_available() else None}")
     return _raw_stream(index)
-
-
-def _check(status, name):
-    if status:
-        _lib.check(status, name)
 
 
 def check_error(device="cuda") -> None:
@@ -207,8 +200,10 @@ def quantise(x, format: str = "e2m1", out: Mx | None = None) -> Mx:
         raise ValueError(f"x: [rows, columns] is needed, got {tuple(shape)}")
     rows, cols = shape
     ldx = _pitch("x", x, rows, cols, device)
-    out = _matrix(out, rows, cols, format, device)
-    _check((_c or _load()).tha_hyb_mx_quant(_stream(device), DTYPES[x.dtype], x.data_ptr(), ldx, out.ref), "tha_hyb_mx_quant")
+    out = Mx.empty(rows, cols, format, device) if out is None else _matrix(out, rows, cols, format, device)
+    status = (_c or _load()).tha_hyb_mx_quant(_stream(device), DTYPES[x.dtype], x.data_ptr(), ldx, out.c)
+    if status:
+        _lib.check(status, "tha_hyb_mx_quant")
     return out
 
 
@@ -228,8 +223,10 @@ def add_norm(x, left, weight, *, eps: float, w_offset: float = 0.0, format: str 
     kind, at, ldl = 1, None, 0
     if left is not None:
         ldl, kind, at = _pitch("left", left, rows, cols, device), DTYPES[left.dtype], left.data_ptr()
-    out = _matrix(out, rows, cols, format, device)
-    _check((_c or _load()).tha_hyb_mx_add_norm(_stream(device), kind, x.data_ptr(), at, ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps, out.ref), "tha_hyb_mx_add_norm")
+    out = Mx.empty(rows, cols, format, device) if out is None else _matrix(out, rows, cols, format, device)
+    status = (_c or _load()).tha_hyb_mx_add_norm(_stream(device), kind, x.data_ptr(), at, ldl, x_out.data_ptr(), weight.data_ptr(), w_offset, eps, out.c)
+    if status:
+        _lib.check(status, "tha_hyb_mx_add_norm")
     return out
 
 
@@ -239,7 +236,9 @@ def linear(a: Mx, w: Mx, dtype=torch.float32, out=None):
     if device != w.device:
         raise ValueError(f"the rows are on {device}, the matrix is on {w.device}")
     out, kind, ld = _result(out, a.rows, w.rows, dtype, device)
-    _check((_c or _load()).tha_hyb_mx_linear(_stream(device), kind, out.data_ptr(), ld, a.ref, w.ref), "tha_hyb_mx_linear")
+    status = (_c or _load()).tha_hyb_mx_linear(_stream(device), kind, out.data_ptr(), ld, a.c, w.c)
+    if status:
+        _lib.check(status, "tha_hyb_mx_linear")
     return out
 
 
@@ -253,6 +252,8 @@ def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = 
         raise ValueError(f"{act} {'has no gate' if act in UNGATED else 'needs a gate'}")
     if up.device != device or (gate is not None and gate.device != device):
         raise ValueError(f"the rows are on {device}, a matrix is not")
-    out = _matrix(out, a.rows, up.rows, format, device)
-    _check((_c or _load()).tha_hyb_mx_linear_act(_stream(device), kind, a.ref, None if gate is None else gate.ref, up.ref, limit, alpha, out.ref), "tha_hyb_mx_linear_act")
+    out = Mx.empty(a.rows, up.rows, format, device) if out is None else _matrix(out, a.rows, up.rows, format, device)
+    status = (_c or _load()).tha_hyb_mx_linear_act(_stream(device), kind, a.c, None if gate is None else gate.c, up.c, limit, alpha, out.c)
+    if status:
+        _lib.check(status, "tha_hyb_mx_linear_act")
     return out
