@@ -43,7 +43,7 @@ namespace {
 
 constexpr int MR_THREADS = 256;
 constexpr int MR_WARPS = MR_THREADS / 32;
-constexpr int MR_NORM_MOST = 512;                // threads of a row's block at most
+constexpr int MR_NORM_MOST = 512;                // threads of a row's block at most, twice that with few values each
 constexpr int MR_N = 4;                           // values of a thread of the norm's at a time
 constexpr int MR_V = 8;                           // values of a lane
 constexpr int MR_SEG = 512;                       // values of a warp at a time
@@ -388,10 +388,10 @@ __device__ __forceinline__ void mr_norm_codes(const tha_mx_t& out, int row, int 
 
 // A block takes a row, P groups of four values a thread, kept in registers between the two passes.
 template <int FMT, typename T, int P>
-__global__ void __launch_bounds__(MR_NORM_MOST) mx_add_norm_kernel(const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, double inv_cols,
+__global__ void __launch_bounds__(P <= 4 ? 2 * MR_NORM_MOST : MR_NORM_MOST) mx_add_norm_kernel(const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, double inv_cols,
                                                                    const tha_mx_t out, bool vec, bool vec_left) {
   hyb_pdl_enter();
-  __shared__ double part[MR_NORM_MOST / 32];
+  __shared__ double part[32];
   const int row = blockIdx.x, cols = out.cols, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int padded = (int)mx_padded(cols);
   float v[P][MR_N];
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(MR_NORM_MOST) mx_add_norm_kernel(const float* 
   __syncthreads();
   total = lane < warps ? part[lane] : 0.0;
 #pragma unroll
-  for (int o = MR_NORM_MOST / 64; o > 0; o >>= 1) total += __shfl_xor_sync(THA_FULL_MASK, total, o);
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(THA_FULL_MASK, total, o);
   const double r = __shfl_sync(THA_FULL_MASK, mr_root(total * inv_cols + (double)eps), 0);
 #pragma unroll
   for (int i = 0; i < P; i++) {
@@ -586,7 +586,8 @@ int ring_form(cudaStream_t s, const float* x, const T* left, long long ldl, floa
 }
 // The ring for wide rows that are many and fit it twice; else a block a row.  us, a block a row / ring: 2048 x 4096 with bf16 28.7 / 25.1, fp32 23.9 / 25.0; 1000 x 8192 bf16 42 / 26;
 // 1000 x 11008 bf16 58 / 35; 300 x 11008 fp32 18.9 / 16.9; 8000 x 2048 bf16 42 / 53; 4000 x 1024 fp32 13.0 / 19.7.
-// Threads of a row's block: many rows leave the SMs full with 256 each, few rows are done sooner by 512.
+// Threads of a row's block: few rows are done the sooner the more there are (1 x 4096 with 128, 256, 512, 1024: 6.6, 4.1, 2.9, 2.6; 64 x 11008 with 256, 512, 1024: 15.6, 9.1, 6.7), many fill the
+// SMs with 256 (2000 x 2048 fp32 13.6, 12.3, 13.5 with 128, 256, 512).
 template <int FMT, typename T>
 int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t* out) {
   const bool vec = mr_aligned(x, out->rows > 1 ? out->cols : 0, 4) && aligned16(x_out) && aligned16(w), vec_left = mr_aligned(left, out->rows > 1 ? ldl : 0, sizeof(T));
@@ -599,7 +600,7 @@ int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, 
     if (p <= 4) return ring_form<FMT, T, 4>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
     return ring_form<FMT, T, 6>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
   }
-  const int threads = min(need, out->rows > 2 * sm_budget() && need <= 2048 ? 256 : MR_NORM_MOST), p = ceil_div(need, threads);
+  const int threads = min(need, out->rows > 4 * sm_budget() && need <= 1024 ? 256 : need <= 8 * MR_NORM_MOST ? 2 * MR_NORM_MOST : MR_NORM_MOST), p = ceil_div(need, threads);
   auto k = p <= 1 ? mx_add_norm_kernel<FMT, T, 1> : p <= 2 ? mx_add_norm_kernel<FMT, T, 2> : p <= 4 ? mx_add_norm_kernel<FMT, T, 4> : p <= 8 ? mx_add_norm_kernel<FMT, T, 8>
            : p <= 16 ? mx_add_norm_kernel<FMT, T, 16> : mx_add_norm_wide_kernel<FMT, T>;
   THA_CUDA_OK(launch(k, dim3(out->rows), dim3(p <= 16 ? threads : MR_THREADS), 0, s, pdl_enabled() != 0, x, left, ldl, x_out, w, w_offset, eps, 1.0 / out->cols, *out, vec, vec_left));
