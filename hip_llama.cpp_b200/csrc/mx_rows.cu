@@ -601,7 +601,7 @@ int add_norm_form(cudaStream_t s, const float* x, const T* left, long long ldl, 
     return ring_form<FMT, T, 6>(s, x, left, ldl, x_out, w, w_offset, eps, out, threads, stages, stage);
   }
   const int threads = min(need, out->rows > 4 * sm_budget() && need <= 1024 ? 256 : need <= 8 * MR_NORM_MOST ? 2 * MR_NORM_MOST : MR_NORM_MOST), p = ceil_div(need, threads);
-  auto k = p <= 1 ? mx_add_norm_kernel<FMT, T, 1> : p <= 2 ? mx_add_norm_kernel<FMT, T, 2> : p <= 4 ? mx_add_norm_kernel<FMT, T, 4> : p <= 8 ? mx_add_norm_kernel<FMT, T, 8>
+  auto k = p <= 1 ? mx_add_norm_kernel<FMT, T, 1> : p <= 2 ? mx_add_norm_kernel<FMT, T, 2> : p <= 4 ? mx_add_norm_kernel<FMT, T, 4>
            : p <= 16 ? mx_add_norm_kernel<FMT, T, 16> : mx_add_norm_wide_kernel<FMT, T>;
   THA_CUDA_OK(launch(k, dim3(out->rows), dim3(p <= 16 ? threads : MR_THREADS), 0, s, pdl_enabled() != 0, x, left, ldl, x_out, w, w_offset, eps, 1.0 / out->cols, *out, vec, vec_left));
   return THA_STATUS_SUCCESS;
