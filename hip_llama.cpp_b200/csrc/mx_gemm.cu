@@ -125,14 +125,21 @@ __device__ __forceinline__ float mg_sigmoid(float z) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + more));
   return r;
 }
-// hyb_act_value, its gated ones by the sigmoid above: 0.5 (1 + tanh t) is the sigmoid of 2 t
+// x, at most and at least a limit, as fminf and fmaxf have them but for what is no number: that stays none
+__device__ __forceinline__ float mg_most(float x, float limit) { return x > limit ? limit : x; }
+__device__ __forceinline__ float mg_least(float x, float limit) { return x < limit ? limit : x; }
+// hyb_act_value, its gated ones by the sigmoid above: 0.5 (1 + tanh t) is the sigmoid of 2 t.  Every one of them keeps NaN: of a block that is none, of a sum that a kernel gave up.
 template <int ACT>
 __device__ __forceinline__ float mg_act_value(float g, float u, float limit, float alpha) {
   if (ACT == THA_ACT_SILU_GLU) return g * mg_sigmoid(g) * u;
   if (ACT == THA_ACT_GELU_TANH_GLU) return g * mg_sigmoid(1.5957691216057308f * (g + 0.044715f * g * g * g)) * u;
   if (ACT == THA_ACT_GLU_CLAMPED) {
-    const float gc = fminf(g, limit);
-    return gc * mg_sigmoid(alpha * gc) * (fminf(fmaxf(u, -limit), limit) + 1.0f);
+    const float gc = mg_most(g, limit);
+    return gc * mg_sigmoid(alpha * gc) * (mg_most(mg_least(u, -limit), limit) + 1.0f);
+  }
+  if (ACT == THA_ACT_RELU2) {
+    const float t = mg_least(u, 0.f);
+    return t * t;
   }
   return hyb_act_value(ACT, g, u, limit, alpha);
 }

@@ -439,3 +439,28 @@ def test_long_rows():
     va, vw = O.values(a)[pick], O.values(w)
     want = va @ vw.T
     assert (np.abs(got[pick].double().cpu().numpy() - want) <= sum_bound(va, vw) + (np.abs(want) + sum_bound(va, vw)) * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("act,limit,alpha", ACTS)
+@pytest.mark.parametrize("where", ["rows", "gate", "up"])
+@pytest.mark.parametrize("rows,n,k", [(20, 200, 300), (20, 200, 4100), (1100, 2600, 300)])
+def test_nan_passes_every_activation(fmt, act, limit, alpha, where, rows, n, k):
+    """One block, clusters, pairs: what is no number in the rows or in a matrix is none in the result, and changes nothing else"""
+    gated = act not in M.UNGATED
+    if where == "gate" and not gated:
+        where = "up"
+    a, *ws = matrices(rows, n, k, fmt, 4, 2 if gated else 1)
+    call = lambda: M.linear_act(a, ws[0] if gated else None, ws[-1], act=act, limit=limit, alpha=alpha).read().cpu()  # noqa: E731
+    clean = call()
+    bad = torch.zeros(rows, n, dtype=torch.bool)
+    if where == "rows":
+        a.scales.view(-1)[(0 * 32 + 3) * 16 + 0] = 255       # row 3, block 0
+        bad[3] = True
+    else:
+        w, across = ws[0 if where == "gate" else -1], -(-k // 128)
+        w.scales.view(-1)[(1 * across + 2) * 512 + (5 % 32) * 16 + 1] = 255    # row 133, block 9
+        bad[:, 128:160] = True                               # a block of the result is NaN as a whole
+    got = call()
+    assert not clean.isnan().any() and torch.equal(got.isnan(), bad) and torch.equal(got[~bad], clean[~bad])
+    M.check_error()
