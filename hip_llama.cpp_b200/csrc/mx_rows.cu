@@ -350,16 +350,20 @@ __device__ __forceinline__ double mr_root(double m) {
 // The norm of four values of a lane, (v r) (w_offset + w), into codes.  All lanes of the warp.
 // In fp32 the norm is off by less than 2^-21 of itself (four roundings, a fifth with the scale); where scale and codes are the same for 1 - 2^-21 and 1 + 2^-21 of it, as for all but one value in
 // some ten thousand, they are the norm's.  Else, or where fp32 ends, the warp takes its values in fp64.  (Every value in fp64, or in pairs of fp32 numbers: 2048 x 4096 29 and 27.5 us.)
+// Where fp32 ends: r (w_offset + w) may be no number of it, or one of few bits, though the norm is an ordinary number.  Beyond its end y is infinite or NaN, and the block goes by fp64.  Below 2^-126,
+// with r above 2^-60, w_offset + w is below 2^-66 and the norm, as |v| r is at most the root of 2^30 columns, below 2^-51: a code of 0 in a block whose largest value is above 2^-31.  Blocks below
+// that go by fp64, but for those whose values are all 0.
 template <int FMT>
 __device__ __forceinline__ void mr_norm_codes(const tha_mx_t& out, int row, int col, int padded, int n, const float (&v)[MR_N], const float (&w)[MR_N], float w_offset, double r) {
   const float rf = (float)r;
   float y[MR_N];
-  unsigned top = 0;
+  unsigned top = 0, some = 0;
 #pragma unroll
   for (int i = 0; i < MR_N; i++) {
     y[i] = v[i] * (rf * (w_offset + w[i]));
     if (n < MR_N && i >= n) y[i] = 0.f;           // behind the row, whatever the root is
     top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+    some |= __float_as_uint(v[i]);
   }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(THA_FULL_MASK, top, o));
@@ -371,18 +375,17 @@ __device__ __forceinline__ void mr_norm_codes(const tha_mx_t& out, int row, int 
     const float f = k ? hi : lo;
     c[k] = FMT == THA_MX_E2M1 ? mx_e2m1x2(y[0] * f, y[1] * f) | mx_e2m1x2(y[2] * f, y[3] * f) << 8 : mx_e4m3x2(y[0] * f, y[1] * f) | mx_e4m3x2(y[2] * f, y[3] * f) << 16;
   }
-  // the scale changes behind a fraction of 1.5 or 1.75: sure where top is more than 8 units from that; below 2^-101 fp32 has not the bits
-  const bool sure = byte == 255u || top == 0u || (c[0] == c[1] && (top - (FMT == THA_MX_E2M1 ? 0x400000u : 0x600000u) + 8u & 0x7fffffu) > 16u && top > 0x0d000000u);
-  if (!__all_sync(THA_FULL_MASK, sure && rf > 0x1p-100f && rf < 0x1p100f)) {
+  // the scale changes behind a fraction of 1.5 or 1.75: sure where top is more than 8 units from that, above 2^-31 and more than 16 units from fp32's end
+  const bool sure = (top | some << 1) == 0u || (c[0] == c[1] && (top - (FMT == THA_MX_E2M1 ? 0x400000u : 0x600000u) + 8u & 0x7fffffu) > 16u && top - 0x30000000u < 0x7f7ffff0u - 0x30000000u);
+  if (!__all_sync(THA_FULL_MASK, sure && rf > 0x1p-60f && rf < 0x1p100f)) {
 #pragma unroll
     for (int i = 0; i < MR_N; i++) y[i] = i < n ? mr_odd((double)v[i] * r * ((double)w_offset + (double)w[i])) : 0.f;
     mr_codes<FMT>(out, row, col, padded, y);
     return;
   }
   if (col >= padded) return;
-  const unsigned code = byte == 255u ? 0u : c[0];
-  if (FMT == THA_MX_E2M1) *reinterpret_cast<unsigned short*>(static_cast<char*>(out.codes) + (size_t)row * (padded / 2) + col / 2) = (unsigned short)code;
-  else *reinterpret_cast<unsigned*>(static_cast<char*>(out.codes) + (size_t)row * padded + col) = code;
+  if (FMT == THA_MX_E2M1) *reinterpret_cast<unsigned short*>(static_cast<char*>(out.codes) + (size_t)row * (padded / 2) + col / 2) = (unsigned short)c[0];
+  else *reinterpret_cast<unsigned*>(static_cast<char*>(out.codes) + (size_t)row * padded + col) = c[0];
   if (!(threadIdx.x & 7)) out.scales[mx_scale_at(row, col / MX_TILE, padded / MX_TILE) + (col / MX_BLOCK & 3)] = (uint8_t)byte;
 }
 

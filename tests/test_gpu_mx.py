@@ -464,3 +464,52 @@ def test_nan_passes_every_activation(fmt, act, limit, alpha, where, rows, n, k):
     got = call()
     assert not clean.isnan().any() and torch.equal(got.isnan(), bad) and torch.equal(got[~bad], clean[~bad])
     M.check_error()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("power,weight,w_offset", [(95, -50, 0.0), (90, -40, 0.0), (95, -60, 0.0), (70, -70, 0.0), (-60, 80, 0.0), (-40, 120, 0.0), (20, -120, 0.0), (0, 122, 2.0 ** 127),
+                                                   (30, 0, 1.0)])
+@pytest.mark.parametrize("rows,cols", [(3, 300), (700, 1000), (600, 4096), (310, 11008), (2, 40001)])
+def test_add_norm_with_weights_far_from_one(fmt, power, weight, w_offset, rows, cols):
+    """Roots times weights that are no numbers of fp32, or have few bits there, where the norm is an ordinary one: a block a row, the ring, wide rows.  Some weights, with their offset, are 0."""
+    x = numbers(rows, cols, 5)
+    x[::2] = np.ldexp(x[::2], power)
+    if w_offset == 2.0 ** 127:
+        x[:, 0], x[:, 1:] = 2.0 ** 40, x[:, 1:] * 2.0 ** -30      # the norm of most is small
+    x = x.astype(np.float32)
+    w = np.ldexp(numbers(1, cols, 6)[0], weight).astype(np.float32)
+    w[::7] = -w_offset
+    s = x.astype(np.float64)
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + float(np.float32(1e-30))) * (w_offset + w.astype(np.float64))
+    y[np.abs(y) >= 2.0 ** 128] = np.inf
+    same_matrix(M.add_norm(torch.from_numpy(x).cuda(), None, torch.from_numpy(w).cuda(), eps=1e-30, w_offset=w_offset, format=fmt), y)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols", [(3, 300), (700, 1000), (600, 4096)])
+def test_add_norm_with_weights_beyond_fp32(fmt, rows, cols):
+    """A weight and its offset whose sum is no number of fp32, on small values: numbers; on large ones: infinite, the block NaN"""
+    x = np.full((rows, cols), 2.0 ** -40, np.float32)
+    x[:, 0], x[1, 33:] = 2.0 ** 20, 2.0 ** 20
+    w = np.full(cols, 3e38, np.float32)
+    w_offset = float(np.float32(3e38))
+    s = x.astype(np.float64)
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + float(np.float32(1e-5))) * (w_offset + w.astype(np.float64))
+    y[np.abs(y) >= 2.0 ** 128] = np.inf
+    assert np.isinf(y[0, 0]) and np.isfinite(y[0, 32:]).all() and (y[0, 32:] != 0).all() and np.isinf(y[1, 40])
+    same_matrix(M.add_norm(torch.from_numpy(x).cuda(), None, torch.from_numpy(w).cuda(), eps=1e-5, w_offset=w_offset, format=fmt), y)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("power,weight", [(55, -80), (58, -70), (40, -100), (-30, -60)])
+@pytest.mark.parametrize("rows,cols", [(3, 300), (700, 1000), (600, 4096)])
+def test_add_norm_with_small_weights_among_others(fmt, power, weight, rows, cols):
+    """Weights of whole blocks, and of single columns in others, far below those beside them; blocks of zeros of either sign"""
+    x = np.ldexp(numbers(rows, cols, 7), power).astype(np.float32)
+    x[:, 96:128] = np.copysign(0.0, np.random.default_rng(8).standard_normal((rows, 32)))
+    w = numbers(1, cols, 9)[0]
+    w[32:64], w[64:96:2], w[128::3] = np.ldexp(w[32:64], weight), np.ldexp(w[64:96:2], weight), np.ldexp(w[128::3], weight)
+    w = w.astype(np.float32)
+    s = x.astype(np.float64)
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + float(np.float32(1e-30))) * w.astype(np.float64)
+    same_matrix(M.add_norm(torch.from_numpy(x).cuda(), None, torch.from_numpy(w).cuda(), eps=1e-30, format=fmt), y)
