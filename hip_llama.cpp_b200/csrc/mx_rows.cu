@@ -48,11 +48,11 @@ constexpr int MR_N = 4;                           // values of a thread of the n
 constexpr int MR_V = 8;                           // values of a lane
 constexpr int MR_SEG = 512;                       // values of a warp at a time
 
-// four values as fp32, zeros behind the first n; vec: p is on a boundary of four
-__device__ __forceinline__ void mr_load(const float* p, int n, bool vec, float (&v)[MR_N]) {
+// four values as fp32, zeros (`none`) behind the first n; vec: p is on a boundary of four
+__device__ __forceinline__ void mr_load(const float* p, int n, bool vec, float (&v)[MR_N], float none = 0.f) {
   if (vec && n >= MR_N) { hyb_load_vec(p, v); return; }
 #pragma unroll
-  for (int i = 0; i < MR_N; i++) v[i] = i < n ? p[i] : 0.f;
+  for (int i = 0; i < MR_N; i++) v[i] = i < n ? p[i] : none;
 }
 __device__ __forceinline__ void mr_load(const __nv_bfloat16* p, int n, bool vec, float (&v)[MR_N]) {
   if (vec && n >= MR_N) {
@@ -470,16 +470,18 @@ mx_add_norm_ring_kernel(const float* x, const T* left, long long ldl, float* x_o
 #pragma unroll
   for (int i = 0; i < P; i++) mr_load(w + col_of(i), cols - col_of(i), true, g[i]);
   int n = 0;
+  bool ok = true;                                 // a thread that has given up a wait waits and reads no more: its values are NaN from then on and, through the sums, its rows' codes
   for (long long row = blockIdx.x; row < out.rows; row += gridDim.x, n++) {
     const int s = n % stages;
-    const bool ok = tc_mbar_wait(&full[s], (unsigned)(n / stages) & 1u, &abort_flag);
+    ok = ok && tc_mbar_wait(&full[s], (unsigned)(n / stages) & 1u, &abort_flag);
+    const float none = ok ? 0.f : __uint_as_float(0x7fc00000u);
     const unsigned char* at = ring + (size_t)s * (x_bytes + l_bytes);
     float v[P][MR_N];
     double total = 0.0;
 #pragma unroll
     for (int i = 0; i < P; i++) {
       const int col = col_of(i);
-      mr_load(reinterpret_cast<const float*>(at) + col, ok ? cols - col : 0, true, v[i]);
+      mr_load(reinterpret_cast<const float*>(at) + col, ok ? cols - col : 0, true, v[i], none);
       if (l_bytes) {
         float l[MR_N];
         mr_load(reinterpret_cast<const T*>(at + x_bytes) + col, ok ? cols - col : 0, true, l);
@@ -489,7 +491,6 @@ mx_add_norm_ring_kernel(const float* x, const T* left, long long ldl, float* x_o
 #pragma unroll
       for (int j = 0; j < MR_N; j++) total = fma((double)v[i][j], (double)v[i][j], total);        // values behind the row are 0
     }
-    if (!ok) total = __longlong_as_double(0x7ff8000000000000ll);         // given up: the row's codes say NaN
     double* p = part[n & 1];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(THA_FULL_MASK, total, o);
@@ -498,7 +499,7 @@ mx_add_norm_ring_kernel(const float* x, const T* left, long long ldl, float* x_o
     total = lane < warps ? p[lane] : 0.0;
 #pragma unroll
     for (int o = MR_NORM_MOST / 64; o > 0; o >>= 1) total += __shfl_xor_sync(THA_FULL_MASK, total, o);
-    if (threadIdx.x == 0 && row + (long long)stages * gridDim.x < out.rows) ask(s, row + (long long)stages * gridDim.x);
+    if (threadIdx.x == 0 && ok && row + (long long)stages * gridDim.x < out.rows) ask(s, row + (long long)stages * gridDim.x);
 #pragma unroll
     for (int i = 0; i < P; i++) mr_store(x_out + (size_t)row * cols + col_of(i), cols - col_of(i), true, v[i]);
     const double r = __shfl_sync(THA_FULL_MASK, mr_root(total * inv_cols + (double)eps), 0);

@@ -708,7 +708,8 @@ size_t tha_hyb_mx_codes_bytes(int format, int rows, int cols);
 size_t tha_hyb_mx_scales_bytes(int rows, int cols);
 
 /* The calls below write rows, cols and format as `out` gives them and fail when these do not fit the other arguments.  Inputs and results do not overlap, but for x and x_out.  No rows: nothing is done.
- * No call needs scratch, and all may be captured. */
+ * No call needs scratch, and all may be captured.  A kernel that gives up on a barrier of its own (a fault of its pipeline) leaves NaN in the results concerned, x_out among them, and says so through
+ * tha_gemm_check_error (tha_b200.h). */
 /* out = x [out->rows, out->cols], dtype-typed, rows ldx elements apart */
 int tha_hyb_mx_quant(void* stream, int dtype, const void* x, long long ldx, const tha_mx_t* out);
 /* x (dtype-typed, rows ldx elements apart) = the values that m stands for, code * 2^(c - 127) rounded to dtype (exact but at the ends of its range) */
@@ -717,8 +718,7 @@ int tha_hyb_mx_read(void* stream, int dtype, const tha_mx_t* m, void* x, long lo
  * apart, NULL: x_out = x), out = x_out / sqrt(mean(x_out^2) + eps) * (w_offset + w), w [cols].  What is quantised is the norm in 64 bits (infinite beyond fp32's
  * numbers): a code is one rounding of the norm of x_out as stored. */
 int tha_hyb_mx_add_norm(void* stream, int dtype, const float* x, const void* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t* out);
-/* C[m, n] = sum_k A[m, k] W[n, k] (dtype-typed, rows ldc elements apart).  A in either format, W E2M1, as many columns.  Products are exact, sums fp32 on the tensor cores.
- * A kernel that gives up on a barrier (a fault of its pipeline) says so through tha_gemm_check_error (tha_b200.h). */
+/* C[m, n] = sum_k A[m, k] W[n, k] (dtype-typed, rows ldc elements apart).  A in either format, W E2M1, as many columns.  Products are exact, sums fp32 on the tensor cores. */
 int tha_hyb_mx_linear(void* stream, int dtype, void* C, long long ldc, const tha_mx_t* A, const tha_mx_t* W);
 /* The input products of a feed-forward with its activation: out [A->rows, W_up->rows] = act of A . W_gate^T and A . W_up^T (THA_ACT_* but for THA_ACT_POLYNORM; W_gate NULL for the ungated ones;
  * limit, alpha as in tha_hyb_ff_act), quantised from fp32 where the products are read out.  out->cols is W_up->rows. */

@@ -1,6 +1,7 @@
 """What the calls over microscaled numbers refuse, and the layout that their binding makes: no GPU."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -135,3 +136,21 @@ def test_room_is_one_piece():
         again = M.Mx(m.codes, m.scales, rows, cols)
         assert rows == 0 or (again.c.codes, again.c.scales) == (m.c.codes, m.c.scales)
         assert again.format == fmt and m.codes is m.codes and m.scales is m.scales
+
+
+def source(name, kernel):
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(os.path.dirname(M.__file__), "csrc", name)).read())
+    text = text[text.index(kernel + "("):]
+    return text[:text.index("\n}\n")]
+
+
+def test_a_norm_whose_wait_gives_up_leaves_no_number():
+    """No wait of the ring runs out in a sound pipeline, so this is read from its source: a thread that has given up waits and reads no more and has NaN for its values, which go into the row's sum,
+    and so into root and codes, and into x_out; nothing more is asked for, and what is under way lands ahead of the block's end."""
+    k = source("mx_rows.cu", "mx_add_norm_ring_kernel")
+    rows = k[k.index("bool ok = true;"):]
+    order = [rows.index(t) for t in ("ok = ok && tc_mbar_wait(&full[s]", "const float none = ok ? 0.f : __uint_as_float(0x7fc00000u);", "ok ? cols - col : 0, true, v[i], none);", "total = fma(", "__syncthreads();",
+                                     "if (threadIdx.x == 0 && ok && row", "ask(s", "mr_store(x_out", "mr_norm_codes<FMT>", "if (threadIdx.x == 0 && abort_flag) {", "tc_drain(full, stages, asked);")]
+    assert order == sorted(order) and rows.count("tc_mbar_wait") == rows.count("mr_store(x_out") == len(re.findall(r"\bask\(", rows)) == len(re.findall(r"\bok = ", rows)) - 1 == 1
+    load = source("mx_rows.cu", "void mr_load")
+    assert "float none = 0.f" in load and "v[i] = i < n ? p[i] : none;" in load
