@@ -360,8 +360,7 @@ __device__ __forceinline__ void mr_norm_codes(const tha_mx_t& out, int row, int 
   unsigned top = 0, some = 0;
 #pragma unroll
   for (int i = 0; i < MR_N; i++) {
-    y[i] = v[i] * (rf * (w_offset + w[i]));
-    if (n < MR_N && i >= n) y[i] = 0.f;           // behind the row, whatever the root is
+    y[i] = v[i] * (rf * (w_offset + w[i]));       // behind the row 0, as v is, or NaN: by fp64
     top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
     some |= __float_as_uint(v[i]);
   }
