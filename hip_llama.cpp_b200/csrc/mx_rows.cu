@@ -347,7 +347,7 @@ __device__ __forceinline__ double mr_root(double m) {
   return r * fma(-0.5 * m * r, r, 1.5);
 }
 
-// The norm of four values of a lane, (v r) (w_offset + w), into codes.  All lanes of the warp.
+// The norm of four values of a lane, (v r) (w_offset + w), into codes; behind the row's n values v is 0 and w -w_offset.  All lanes of the warp.
 // In fp32 the norm is off by less than 2^-21 of itself (four roundings, a fifth with the scale); where scale and codes are the same for 1 - 2^-21 and 1 + 2^-21 of it, as for all but one value in
 // some ten thousand, they are the norm's.  Else, or where fp32 ends, the warp takes its values in fp64.  (Every value in fp64, or in pairs of fp32 numbers: 2048 x 4096 29 and 27.5 us.)
 // Where fp32 ends: r (w_offset + w) may be no number of it, or one of few bits, though the norm is an ordinary number.  Beyond its end y is infinite or NaN, and the block goes by fp64.  Below 2^-126,
@@ -360,7 +360,7 @@ __device__ __forceinline__ void mr_norm_codes(const tha_mx_t& out, int row, int 
   unsigned top = 0, some = 0;
 #pragma unroll
   for (int i = 0; i < MR_N; i++) {
-    y[i] = v[i] * (rf * (w_offset + w[i]));       // behind the row 0, as v is, or NaN: by fp64
+    y[i] = v[i] * (rf * (w_offset + w[i]));       // behind the row 0 times 0, whose code is 0 (that of 0 times less is not), or NaN: by fp64
     top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
     some |= __float_as_uint(v[i]);
   }
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(P <= 4 ? 2 * MR_NORM_MOST : MR_NORM_MOST) mx_a
     const int col = (int)(threadIdx.x + i * blockDim.x) * MR_N, n = there(i);
     if (col - lane * MR_N >= padded) break;
     float g[MR_N];
-    mr_load(w + col, n, vec, g);
+    mr_load(w + col, n, vec, g, -w_offset);
     mr_norm_codes<FMT>(out, row, col, padded, n, v[i], g, w_offset, r);
   }
 }
@@ -467,7 +467,7 @@ mx_add_norm_ring_kernel(const float* x, const T* left, long long ldl, float* x_o
   float g[P][MR_N];
   auto col_of = [&](int i) { return (int)(threadIdx.x + i * blockDim.x) * MR_N; };                 // cols is a multiple of 4
 #pragma unroll
-  for (int i = 0; i < P; i++) mr_load(w + col_of(i), cols - col_of(i), true, g[i]);
+  for (int i = 0; i < P; i++) mr_load(w + col_of(i), cols - col_of(i), true, g[i], -w_offset);
   int n = 0;
   bool ok = true;                                 // a thread that has given up a wait waits and reads no more: its values are NaN from then on and, through the sums, its rows' codes
   for (long long row = blockIdx.x; row < out.rows; row += gridDim.x, n++) {

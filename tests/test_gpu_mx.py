@@ -513,3 +513,17 @@ def test_add_norm_with_small_weights_among_others(fmt, power, weight, rows, cols
     s = x.astype(np.float64)
     y = s / np.sqrt((s * s).mean(-1, keepdims=True) + float(np.float32(1e-30))) * w.astype(np.float64)
     same_matrix(M.add_norm(torch.from_numpy(x).cuda(), None, torch.from_numpy(w).cuda(), eps=1e-30, format=fmt), y)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 301), (700, 1000), (600, 4100), (310, 11012), (2, 40001)])
+def test_add_norm_with_an_offset_below_zero(fmt, dtype, rows, cols):
+    """What pads a row has codes of 0, not those of -0; zeros among the values keep their sign"""
+    x, left, w = numbers(rows, cols, 1), numbers(rows, cols, 2), numbers(1, cols, 3)[0]
+    x[:, 64:96], left[:, 64:96] = -0.0, -0.0
+    x, w = (torch.from_numpy(t.astype(np.float32)).cuda() for t in (x, w))
+    l = upload(left, dtype)
+    s = (x + l.float()).double().cpu().numpy()
+    y = s / np.sqrt((s * s).mean(-1, keepdims=True) + 1e-5) * (-8.5 + w.double().cpu().numpy())
+    same_matrix(M.add_norm(x, l, w, eps=1e-5, w_offset=-8.5, format=fmt), y)
