@@ -160,11 +160,12 @@ __device__ __forceinline__ void mg_activate(const MgP& p, const float (&g)[G], f
     else mg_act<THA_ACT_GLU_CLAMPED>(g, x, there, p.limit, p.alpha);
   }
 }
-// C results of activation rows n .. (`count` of them there) and weight row `row`, a warp's rows neighbours from a multiple of 32 on.  All lanes of the warp.
+// C results of activation rows n .. (`count` of them there) and weight row `row`, a warp's rows neighbours from a multiple of 32 on.  All lanes of the warp, which leave together: what follows
+// may be for a whole warp (tcgen05.ld, the cluster's barrier).
 template <int READ, int C>
 __device__ __forceinline__ void mg_store(const MgP& p, long long padded, int n, int count, int row, float (&x)[C]) {
   if (READ == MG_PLAIN) {
-    if (row >= p.M) return;
+    if (row >= p.M) count = 0;
     if (p.bf16) {
       __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + (size_t)n * p.ldo + row;
 #pragma unroll
@@ -181,6 +182,7 @@ __device__ __forceinline__ void mg_store(const MgP& p, long long padded, int n, 
   } else {
     mg_store_blocks<THA_MX_E4M3>(p.y, n, count, row, padded, x);
   }
+  __syncwarp();
 }
 
 // ranks > 1: the blocks of a cluster take a share of the tile's stages each, leave their partial tiles in shared memory and sum each other's, ranks in ascending order.

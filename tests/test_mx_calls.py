@@ -154,3 +154,14 @@ def test_a_norm_whose_wait_gives_up_leaves_no_number():
     assert order == sorted(order) and rows.count("tc_mbar_wait") == rows.count("mr_store(x_out") == len(re.findall(r"\bask\(", rows)) == len(re.findall(r"\bok = ", rows)) - 1 == 1
     load = source("mx_rows.cu", "void mr_load")
     assert "float none = 0.f" in load and "v[i] = i < n ? p[i] : none;" in load
+
+
+def test_lanes_without_a_weight_row_stay_with_their_warp():
+    """A store of results ends with its whole warp: behind it come tcgen05.ld and barrier.cluster, which take a warp as one.  Read from the source, as lanes that leave early usually meet again."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(os.path.dirname(M.__file__), "csrc", "mx_gemm.cu")).read())
+    store = text[text.index("void mg_store("):]
+    store = store[:store.index("\n}\n")]
+    assert "return" not in store and store.rstrip().endswith("__syncwarp();")
+    for kernel in ("mx_gemm_kernel", "mx_gemm_pair_kernel"):
+        k = source("mx_gemm.cu", kernel)
+        assert "mg_store<READ>" in k and "mg_store_blocks" not in k
