@@ -188,8 +188,10 @@ def _stream(device):
 
 def check_error(device="cuda") -> None:
     """Waits for the current stream of a device; raises if a kernel on it gave up on a barrier since the last such question (the results of that call are NaN where it was)."""
-    torch.cuda.current_stream(device).synchronize()
-    if (_c or _load()).tha_gemm_check_error():
+    with torch.cuda.device(device):                             # whose kernels the library is asked about
+        torch.cuda.current_stream().synchronize()
+        gave_up = (_c or _load()).tha_gemm_check_error()
+    if gave_up:
         raise cabi.ThaError("a kernel gave up on a barrier of its own")
 
 

@@ -165,3 +165,36 @@ def test_lanes_without_a_weight_row_stay_with_their_warp():
     for kernel in ("mx_gemm_kernel", "mx_gemm_pair_kernel"):
         k = source("mx_gemm.cu", kernel)
         assert "mg_store<READ>" in k and "mg_store_blocks" not in k
+
+
+def test_the_error_of_another_device(monkeypatch):
+    """check_error asks about the device that it is given, current or not, and leaves the current one as it was"""
+    import contextlib
+    current, asked, waited = [0], [], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], torch.device(d).index if torch.device(d).index is not None else current[0]
+        yield
+        current[0] = before
+
+    class Stream:
+        def __init__(self, d):
+            self.d = current[0] if d is None else torch.device(d).index
+
+        def synchronize(self):
+            waited.append(self.d)
+
+    class Calls:
+        def tha_gemm_check_error(self):
+            asked.append(current[0])
+            return current[0]
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: Stream(d))
+    monkeypatch.setattr(M, "_c", Calls())
+    M.check_error("cuda:0")
+    with pytest.raises(M.cabi.ThaError):
+        M.check_error("cuda:1")
+    M.check_error()
+    assert asked == waited == [0, 1, 0] and current == [0]
