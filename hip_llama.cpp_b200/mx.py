@@ -22,6 +22,7 @@ FORMATS = {"e2m1": 0, "e4m3": 1}                                # THA_MX_*
 CODES = {torch.uint8: "e2m1", torch.float8_e4m3fn: "e4m3"}      # what holds them
 ACTS = {"clamped": 0, "relu2": 1, "gelu": 2, "xielu": 3, "silu": 4}    # THA_ACT_*
 UNGATED = ("relu2", "xielu")
+WITH_NUMBERS = ("clamped", "xielu")                             # that take limit and alpha
 BLOCK, TILE, MOST = 32, 128, 1 << 30
 
 
@@ -244,7 +245,8 @@ def linear(a: Mx, w: Mx, dtype=torch.float32, out=None):
     return out
 
 
-def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = "e4m3", limit: float = 0.0, alpha: float = 0.0, out: Mx | None = None) -> Mx:
+def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = "e4m3", limit: float | None = None, alpha: float | None = None,
+               out: Mx | None = None) -> Mx:
     """A feed-forward's input products and activation (tha_hyb_mx_linear_act): act(a gate^T, a up^T) [rows, n] as microscaled numbers.  act: silu, gelu, clamped (limit, alpha), or without a gate
     (None) relu2, xielu (its two stored numbers as limit, alpha)."""
     device, kind = a.device, ACTS.get(act)
@@ -252,6 +254,10 @@ def linear_act(a: Mx, gate: Mx | None, up: Mx, act: str = "silu", format: str = 
         raise ValueError(f"act is one of {', '.join(ACTS)}, not {act!r}")
     if (gate is None) != (act in UNGATED):
         raise ValueError(f"{act} {'has no gate' if act in UNGATED else 'needs a gate'}")
+    if limit is None or alpha is None:
+        if act in WITH_NUMBERS:
+            raise ValueError(f"{act} needs limit and alpha")
+        limit = alpha = 0.0
     if up.device != device or (gate is not None and gate.device != device):
         raise ValueError(f"the rows are on {device}, a matrix is not")
     out = Mx.empty(a.rows, up.rows, format, device) if out is None else _matrix(out, a.rows, up.rows, format, device)

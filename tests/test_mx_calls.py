@@ -198,3 +198,17 @@ def test_the_error_of_another_device(monkeypatch):
         M.check_error("cuda:1")
     M.check_error()
     assert asked == waited == [0, 1, 0] and current == [0]
+
+
+def test_activations_that_take_numbers_are_given_them():
+    """clamped without a limit would clamp at 0"""
+    a, w = M.Mx.empty(4, 96, "e4m3", "cpu"), M.Mx.empty(200, 96, device="cpu")
+    for act, gate in (("clamped", w), ("xielu", None)):
+        for numbers in ({}, {"limit": 7.0}, {"alpha": 1.702}):
+            with pytest.raises(ValueError, match="limit and alpha"):
+                M.linear_act(a, gate, w, act=act, **numbers)
+        with pytest.raises(ValueError, match="current device"):         # taken, but for where it is
+            M.linear_act(a, gate, w, act=act, limit=7.0, alpha=1.702)
+    for act, gate in (("silu", w), ("gelu", w), ("relu2", None)):
+        with pytest.raises(ValueError, match="current device"):
+            M.linear_act(a, gate, w, act=act)
