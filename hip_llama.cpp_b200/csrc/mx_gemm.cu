@@ -635,8 +635,7 @@ int mg_launch(cudaStream_t s, const MgArgs& a, int ranks) {
   p.w_bytes = S::WT * wb;
   p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, TC_BM, NT);
   p.ny = ceil_div(p.N, NT);
-  const long long items = (long long)ceil_div(p.M, TC_BM) * p.ny;
-  if (items > 0x3fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");
+  const long long items = (long long)ceil_div(p.M, TC_BM) * p.ny;      // 2^23 at most: mg_form sends no more here than the SMs have places for, or 64 activation rows
   const int stages = ceil_div(p.across, S::CH);
   p.ranks = ranks;
   p.share = ceil_div(stages, p.ranks);
@@ -669,16 +668,14 @@ int mgp_launch(cudaStream_t s, const MgArgs& a) {
   p.w_bytes = S::WT * wb;
   p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, 2 * TC_BM, 0);
   p.ny = ceil_div(p.N, S::NT);
-  const long long items = (long long)ceil_div(p.M, 2 * TC_BM) * p.ny;
-  if (items > 0x3fffffff) return mx_refuse("tha_hyb_mx_linear", "too many results for one call");
-  p.n_items = (int)items;
+  p.n_items = ceil_div(p.M, 2 * TC_BM) * p.ny;
   const int pairs = max(1, sm_budget() / 2);
   auto k = mx_gemm_pair_kernel<KIND, READ>;
   static std::atomic<unsigned long long> asked{0};
   THA_TRY_RC(mx_room(k, S::TOTAL, &asked));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(2u * (unsigned)min((long long)pairs, items)); cfg.blockDim = dim3(MGP_THREADS); cfg.dynamicSmemBytes = S::TOTAL; cfg.stream = s;
+  cfg.gridDim = dim3(2u * (unsigned)min(pairs, p.n_items)); cfg.blockDim = dim3(MGP_THREADS); cfg.dynamicSmemBytes = S::TOTAL; cfg.stream = s;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -709,7 +706,8 @@ int mg_check(const tha_mx_t* A, const tha_mx_t* W, const char* who) {
   if (A->cols != W->cols) return mx_refuse(who, "rows and matrix have different columns");
   return THA_STATUS_SUCCESS;
 }
-int mg_fill(MgArgs* a, const tha_mx_t* A, const tha_mx_t* W0, const tha_mx_t* W1) {
+int mg_fill(MgArgs* a, const tha_mx_t* A, const tha_mx_t* W0, const tha_mx_t* W1, const char* who) {
+  if ((long long)ceil_div(W0->rows, 2 * TC_BM) * ceil_div(A->rows, W1 ? 128 : 256) > 0x3fffffff) return mx_refuse(who, "too many results for one call");   // items of pairs are counted in 31 bits
   a->A = A; a->W0 = W0; a->W1 = W1;
   a->p.M = W0->rows; a->p.N = A->rows;
   a->p.across = (int)(mx_padded(A->cols) / MX_TILE);
@@ -730,7 +728,7 @@ extern "C" int tha_hyb_mx_linear(void* stream, int dtype, void* C, long long ldc
   if (!C) return mx_refuse(who, "C is NULL");
   if (ldc < W->rows && A->rows > 1) return mx_refuse(who, "a row pitch below the row");
   MgArgs a = {};
-  THA_TRY_RC(mg_fill(&a, A, W, nullptr));
+  THA_TRY_RC(mg_fill(&a, A, W, nullptr, who));
   a.p.out = C; a.p.ldo = ldc; a.p.bf16 = dtype == THA_DT_BF16;
   return mg_run<MG_PLAIN>((cudaStream_t)stream, a);
 }
@@ -754,7 +752,7 @@ extern "C" int tha_hyb_mx_linear_act(void* stream, int act, const tha_mx_t* A, c
     alpha = 0.5f + fmaxf(q, 0.f) + log1pf(expf(-fabsf(q)));
   }
   MgArgs a = {};
-  THA_TRY_RC(mg_fill(&a, A, gated ? W_gate : W_up, gated ? W_up : nullptr));
+  THA_TRY_RC(mg_fill(&a, A, gated ? W_gate : W_up, gated ? W_up : nullptr, who));
   a.p.y = *out; a.p.act = act; a.p.limit = limit; a.p.alpha = alpha;
   return gated ? mg_run<MG_GATED>((cudaStream_t)stream, a) : mg_run<MG_UNGATED>((cudaStream_t)stream, a);
 }

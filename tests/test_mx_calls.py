@@ -212,3 +212,11 @@ def test_activations_that_take_numbers_are_given_them():
     for act, gate in (("silu", w), ("gelu", w), ("relu2", None)):
         with pytest.raises(ValueError, match="current device"):
             M.linear_act(a, gate, w, act=act)
+
+
+def test_more_results_than_a_call_counts():
+    """Refused under the call's own name, ahead of anything that is asked of a device"""
+    rows, w = C.byref(struct(rows=1 << 30)), C.byref(struct(format="e2m1", rows=1 << 30))
+    assert "too many" in refused("tha_hyb_mx_linear", 1, BASE, 1 << 30, rows, w)
+    y = C.byref(struct(rows=1 << 30, cols=1 << 30))
+    assert "too many" in refused("tha_hyb_mx_linear_act", 4, rows, w, w, 0.0, 0.0, y) and "too many" in refused("tha_hyb_mx_linear_act", 1, rows, None, w, 0.0, 0.0, y)
