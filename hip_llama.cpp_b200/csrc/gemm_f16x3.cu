@@ -62,14 +62,6 @@ struct X3Smem {
   static_assert(TOTAL <= TC_SMEM_LIMIT, "shared memory overflow");
 };
 
-__device__ __forceinline__ void x3_arrive_leader(uint64_t* bar) {   // the same barrier of the pair's rank 0.  What it announces is TMEM and TMA data, never generic memory of this thread
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc_smem_u32(bar)));
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
-}
-__device__ __forceinline__ void x3_commit(uint64_t* bar) {   // to both CTAs
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tc_smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
 // kind::f16 with fp16 operands, fp32 accumulate, M = 256 over the pair, N = 128
 constexpr uint32_t X3_IDESC = (1u << 4) | ((uint32_t)(X3_NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 __device__ __forceinline__ void x3_mma(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t accumulate) {
@@ -213,7 +205,7 @@ gemm_f16x3_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant
               for (int i = 0; i < w.nkb; i++) {
                 const int g = gb + i, s = g % S::SX;
                 if (!tc_mbar_wait(&xfull[s], (g / S::SX) & 1u, abort_flag)) { ok = false; break; }
-                x3_arrive_leader(&xpeer[s]);
+                tc_pair_arrive(&xpeer[s]);
               }
               gb += w.nkb;
               continue;
@@ -237,10 +229,10 @@ gemm_f16x3_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant
                   x3_mma(dc, ah + 8 * k, xl + (uint64_t)(2 * k), 1u);
                   x3_mma(d, ah + 8 * k, xh + (uint64_t)(2 * k), (uint32_t)((i - i0 | k) != 0));
                 }
-                x3_commit(&aempty[sa]);
-                x3_commit(&xempty[s]);
+                tc_pair_commit(&aempty[sa]);
+                tc_pair_commit(&xempty[s]);
               }
-              if (ok) x3_commit(&accum[buf]);
+              if (ok) tc_pair_commit(&accum[buf]);
             }
             gb += w.nkb;
           }
@@ -252,7 +244,7 @@ gemm_f16x3_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant
       if (warp == 0 && tc_elect()) tc_drain(wfull, S::SW, sent < 0 ? gb : sent);
       if (warp == 3 && tc_elect()) tc_drain(xfull, S::SX, sent < 0 ? gb : sent);
       if (warp == 1 && rank == 0 && tc_elect()) {
-        x3_commit(mmadone);
+        tc_pair_commit(mmadone);
         tc_drain(mmadone, 1, 1);
       }
     }
@@ -326,7 +318,7 @@ gemm_f16x3_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) x3_arrive_leader(&aready[sa]);
+          if (lane == 0) tc_pair_arrive(&aready[sa]);
         }
         if (pass == 0 && (__hisinf(__low2half(top)) || __hisinf(__high2half(top)))) *bad_rows = 1;
         gb += w.nkb;
@@ -363,7 +355,7 @@ gemm_f16x3_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) x3_arrive_leader(part == 0 ? corrfree : &mainfree[buf]);
+            if (lane == 0) tc_pair_arrive(part == 0 ? corrfree : &mainfree[buf]);
           }
         }
         if (ok) ok = tc_mbar_wait_warp(&rowready[par], (unsigned)(n_it >> 2) & 1u, abort_flag);

@@ -67,10 +67,6 @@ __device__ __forceinline__ void q8i_mma(uint32_t tmem_d, uint64_t adesc, uint64_
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void q8i_bulk(void* dst, const void* src, unsigned bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void q8i_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void q8i_ld(uint32_t taddr, uint32_t (&v)[16]) { tc_tmem_ld16(taddr, v); }
 __device__ __forceinline__ void q8i_ld(uint32_t taddr, uint32_t (&v)[8]) {
@@ -208,7 +204,7 @@ gemm_q8i_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__
           if (n > GPS) n = GPS;
           tc_mbar_expect_tx(&xfull[xr], n * xbytes);
           const float* src = p.xsT + (size_t)((w.slot0 + j) << gps_sh) * p.ldxs + w.n0;
-          for (int g = 0; g < n; g++) q8i_bulk(xs_sm + ((xr << gps_sh) + g) * NT, src + (size_t)g * p.ldxs, xbytes, &xfull[xr]);
+          for (int g = 0; g < n; g++) tc_bulk(xs_sm + ((xr << gps_sh) + g) * NT, src + (size_t)g * p.ldxs, xbytes, &xfull[xr]);
           if (++xr == nxs) xr = 0;
           if (++s == nring) s = 0;
         };

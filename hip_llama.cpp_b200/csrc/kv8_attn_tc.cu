@@ -161,10 +161,6 @@ __global__ void __launch_bounds__(2 * DT) kv8_stage_kernel(tha_attn_t a, tha_row
       if (!kt_stage_part<DT, FMT>(a, rows, kv, min_rows, i, staged, scales)) return;
   }
 }
-__device__ __forceinline__ void kt_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
-}
 
 // grid (kv_heads, tiles of pairs * splits)
 template <int DT, int FMT, bool SPLIT, bool MORE, typename T>
@@ -531,10 +527,10 @@ __global__ void __launch_bounds__(kt_threads(SPLIT, DT), 3 - kt_groups(SPLIT, DT
           sent[side]++;
 #pragma unroll
           for (int hf = 0; hf < 2; hf++) {
-            if (side == 0) kt_bulk(&s_scales[jl % KT_SCALES][hf], scales + from[hf], 16, &full[0][at]);
+            if (side == 0) tc_bulk(&s_scales[jl % KT_SCALES][hf], scales + from[hf], 16, &full[0][at]);
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
-              kt_bulk(KVs + (side * SLOTS + at) * TILE + kb * (KT_KEYS * 128) + hf * (32 * 128), staged + from[hf] * kt_part(DT) + (side * KB + kb) * (32 * 128), 32 * 128, &full[side][at]);
+              tc_bulk(KVs + (side * SLOTS + at) * TILE + kb * (KT_KEYS * 128) + hf * (32 * 128), staged + from[hf] * kt_part(DT) + (side * KB + kb) * (32 * 128), 32 * 128, &full[side][at]);
           }
         }
         if (++at == SLOTS) { at = 0; turn++; }

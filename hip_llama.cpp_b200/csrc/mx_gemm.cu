@@ -42,15 +42,14 @@ struct MgP {
 template <int KIND, int NT, int READ>
 struct MgSmem {
   static constexpr int WT = READ == MG_GATED ? 2 : 1;                 // weight matrices
-  static constexpr int XT = (NT + 127) / 128;                         // scale tiles of the activation rows
   static constexpr int CH = KIND == MG_F4 ? 2 : 1;                    // scale tiles along k in a stage (128 bytes of a row of codes)
   static constexpr int W_BYTES = WT * TC_BM * 128, X_BYTES = NT * 128;
-  static constexpr int SW_BYTES = CH * MX_TILE_BYTES, SX_BYTES = CH * MX_TILE_BYTES;   // of one matrix, of one row tile
-  static constexpr int STAGE = (W_BYTES + X_BYTES + WT * SW_BYTES + XT * SX_BYTES + 1023) / 1024 * 1024;
+  static constexpr int SC_BYTES = CH * MX_TILE_BYTES;                 // scales of one matrix; of the activation rows, which lie in one tile
+  static constexpr int STAGE = (W_BYTES + X_BYTES + (WT + 1) * SC_BYTES + 1023) / 1024 * 1024;
   static constexpr int ROOM = STAGE <= 37 * 1024 ? 111 * 1024 : 220 * 1024;             // two blocks an SM, or one
   static constexpr int NST = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
   static constexpr int ACC_COLS = WT * NT;
-  static constexpr int SET = CH * 4 * (WT + XT);                      // TMEM columns of a stage's scales
+  static constexpr int SET = CH * 4 * (WT + 1);                       // TMEM columns of a stage's scales
   static constexpr int COLS = ACC_COLS + NST * SET;
   static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int TOTAL = NST * STAGE + 1024 + (2 * NST + 2) * 8 + 64;
@@ -59,10 +58,6 @@ struct MgSmem {
   static_assert(COLS <= (ROOM <= 111 * 1024 ? 256 : 512) && TOTAL <= TC_SMEM_LIMIT && NST >= 3, "a stage is too large");
 };
 
-__device__ __forceinline__ void mg_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void mg_prefetch(const CUtensorMap* map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
 }
@@ -83,8 +78,8 @@ __device__ __forceinline__ void mg_mma(uint32_t d, uint64_t a, uint64_t b, uint3
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
 }
 // Block-scaled instruction descriptor: formats of A and B, N / 8, scales as powers of two, M / 16.  Which of a scale word's four bytes an instruction takes is in bits 4-5 (B), 29-30 (A).
-uint32_t mg_idesc(int kind, int fa, int fb, int rows, int nt) {
-  const uint32_t a = kind == MG_F4 ? 1u : fa == THA_MX_E2M1 ? 5u : 0u, b = kind == MG_F4 ? 1u : fb == THA_MX_E2M1 ? 5u : 0u;
+uint32_t mg_idesc(int kind, int rows, int nt) {
+  const uint32_t a = kind == MG_F4 ? 1u : 5u, b = kind == MG_F4 ? 1u : 0u;       // E2M1 x E2M1; E2M1 x E4M3
   return a << 7 | b << 10 | (uint32_t)(nt >> 3) << 17 | 1u << 23 | (uint32_t)(rows >> 4) << 24;
 }
 
@@ -239,16 +234,14 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__ 
         const int t0 = (kb0 + i) * CH, chunks = min(CH, p.across - t0);              // scale tiles of this stage: one in an odd matrix's last stage
         unsigned char* st = smem + s * S::STAGE;
         unsigned char* sw = st + S::W_BYTES + S::X_BYTES;
-        unsigned char* sx = sw + WT * S::SW_BYTES;
         const uint32_t some = (uint32_t)(chunks * MX_TILE_BYTES);
-        tc_mbar_expect_tx(&full[s], p.w_bytes + p.x_bytes + (WT + S::XT) * some);
+        tc_mbar_expect_tx(&full[s], p.w_bytes + p.x_bytes + (WT + 1) * some);
         tc_tma_2d(st, &mw0, (kb0 + i) * (KIND == MG_F4 ? KB / 2 : KB), row0, &full[s]);
         if (WT == 2) tc_tma_2d(st + TC_BM * 128, &mw1, (kb0 + i) * (KIND == MG_F4 ? KB / 2 : KB), row0, &full[s]);
         tc_tma_2d(st + S::W_BYTES, &mx, (kb0 + i) * (KIND == MG_F4 ? KB / 2 : KB), n0, &full[s]);
-        mg_bulk(sw, p.sw0 + mx_scale_at(row0, t0, p.across), some, &full[s]);
-        if (WT == 2) mg_bulk(sw + S::SW_BYTES, p.sw1 + mx_scale_at(row0, t0, p.across), some, &full[s]);
-#pragma unroll
-        for (int x = 0; x < S::XT; x++) mg_bulk(sx + x * S::SX_BYTES, p.sx + mx_scale_at((n0 & ~127) + 128 * x, t0, p.across), some, &full[s]);
+        tc_bulk(sw, p.sw0 + mx_scale_at(row0, t0, p.across), some, &full[s]);
+        if (WT == 2) tc_bulk(sw + S::SC_BYTES, p.sw1 + mx_scale_at(row0, t0, p.across), some, &full[s]);
+        tc_bulk(sw + WT * S::SC_BYTES, p.sx + mx_scale_at(n0 & ~127, t0, p.across), some, &full[s]);
       }
     }
   } else if (warp == 1) {
@@ -260,21 +253,19 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__ 
         if (!tc_mbar_wait(&full[s], (i / S::NST) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const int chunks = min(CH, p.across - (kb0 + i) * CH);
-        const uint32_t st = tc_smem_u32(smem + s * S::STAGE), sw = st + S::W_BYTES + S::X_BYTES, sx = sw + WT * S::SW_BYTES;
+        const uint32_t st = tc_smem_u32(smem + s * S::STAGE), sc = st + S::W_BYTES + S::X_BYTES;
         // a stage has TMEM columns of its own for its scales: the MMAs that read their last contents have completed when the stage was filled again
         const uint32_t sf = tmem_sf + (uint32_t)(s * S::SET);
         for (int c = 0; c < chunks; c++) {
 #pragma unroll
-          for (int w = 0; w < WT; w++) mg_copy_scales(sf + (uint32_t)(4 * (c * (WT + S::XT) + w)), sw + (uint32_t)(w * S::SW_BYTES + c * MX_TILE_BYTES));
-#pragma unroll
-          for (int x = 0; x < S::XT; x++) mg_copy_scales(sf + (uint32_t)(4 * (c * (WT + S::XT) + WT + x)), sx + (uint32_t)(x * S::SX_BYTES + c * MX_TILE_BYTES));
+          for (int t = 0; t <= WT; t++) mg_copy_scales(sf + (uint32_t)(4 * (c * (WT + 1) + t)), sc + (uint32_t)(t * S::SC_BYTES + c * MX_TILE_BYTES));   // the matrices', the activation rows'
         }
         const uint64_t adesc = tc_smem_desc(st), bdesc = tc_smem_desc(st + S::W_BYTES);
 #pragma unroll
         for (int k = 0; k < 4; k++) {                // 32 bytes of codes each: 2 descriptor units
           const int c = KIND == MG_F4 ? k >> 1 : 0, id = KIND == MG_F4 ? 2 * (k & 1) : k;
           if (c < chunks) {
-            const uint32_t at = sf + (uint32_t)(4 * c * (WT + S::XT));
+            const uint32_t at = sf + (uint32_t)(4 * c * (WT + 1));
 #pragma unroll
             for (int w = 0; w < WT; w++)
               mg_mma<KIND>(tmem + (uint32_t)(w * NT), adesc + (uint64_t)(1024 * w + 2 * k), bdesc + (uint64_t)(2 * k), p.idesc | (uint32_t)id << 4 | (uint32_t)id << 29, at + 4 * w,
@@ -394,14 +385,6 @@ constexpr int MGP_THREADS = 384;
 template <int NT>
 __device__ __forceinline__ int mgp_width(int left) { return min(NT, (left + 31) & ~31); }
 
-__device__ __forceinline__ void mgp_arrive_leader(uint64_t* bar) {    // the same barrier of the pair's rank 0; what it announces is TMEM and TMA data, never generic memory of this thread
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc_smem_u32(bar)));
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
-}
-__device__ __forceinline__ void mgp_commit(uint64_t* bar) {           // to both blocks
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tc_smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
 __device__ __forceinline__ void mgp_copy_scales(uint32_t taddr, uint32_t saddr) {   // in both blocks, each from its own shared memory
   uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
@@ -481,9 +464,9 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
           tc_tma_2d(st, &mw0, i * KC, row0, &full[s]);
           if (WT == 2) tc_tma_2d(st + TC_BM * 128, &mw1, i * KC, row0, &full[s]);
           tc_tma_2d(st + S::W_BYTES, &mx, i * KC, n0 + half, &full[s]);
-          mg_bulk(sw, p.sw0 + mx_scale_at(srow, t0, p.across), some, &full[s]);
-          if (WT == 2) mg_bulk(sw + S::SC_BYTES, p.sw1 + mx_scale_at(srow, t0, p.across), some, &full[s]);
-          for (int x = 0; x < xt; x++) mg_bulk(sx + x * S::SC_BYTES, p.sx + mx_scale_at(n0 + 128 * x, t0, p.across), some, &full[s]);
+          tc_bulk(sw, p.sw0 + mx_scale_at(srow, t0, p.across), some, &full[s]);
+          if (WT == 2) tc_bulk(sw + S::SC_BYTES, p.sw1 + mx_scale_at(srow, t0, p.across), some, &full[s]);
+          for (int x = 0; x < xt; x++) tc_bulk(sx + x * S::SC_BYTES, p.sx + mx_scale_at(n0 + 128 * x, t0, p.across), some, &full[s]);
         }
         gb += nkb;
       }
@@ -498,7 +481,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
           for (int i = 0; i < nkb; i++) {
             const int g = gb + i, s = g % S::NST;
             if (!tc_mbar_wait(&full[s], (g / S::NST) & 1u, abort_flag)) { ok = false; break; }
-            mgp_arrive_leader(&peer[s]);
+            tc_pair_arrive(&peer[s]);
           }
           gb += nkb;
           continue;
@@ -530,13 +513,13 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
                               at + 4 * WT, (uint32_t)((i | k) != 0));
             }
           }
-          mgp_commit(&empty[s]);
+          tc_pair_commit(&empty[s]);
         }
-        if (ok) mgp_commit(accum);
+        if (ok) tc_pair_commit(accum);
         gb += nkb;
       }
       if (!ok && rank == 0) {            // MMAs that have been issued end ahead of the blocks
-        mgp_commit(mmadone);
+        tc_pair_commit(mmadone);
         tc_drain(mmadone, 1, 1);
       }
     }
@@ -569,7 +552,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mgp_arrive_leader(accfree);
+      if (lane == 0) tc_pair_arrive(accfree);
       if (cols <= 0) continue;
       mg_activate<READ>(p, gate, x, row0 + q * 32 + lane < p.M);
 #pragma unroll
@@ -633,7 +616,7 @@ int mg_launch(cudaStream_t s, const MgArgs& a, int ranks) {
   if (S::WT == 2) THA_TRY_RC(mg_map(KIND, a.W1, TC_BM, &mw1, &wb));
   THA_TRY_RC(mg_map(KIND, a.A, NT, &mx, &p.x_bytes));
   p.w_bytes = S::WT * wb;
-  p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, TC_BM, NT);
+  p.idesc = mg_idesc(KIND, TC_BM, NT);
   p.ny = ceil_div(p.N, NT);
   const long long items = (long long)ceil_div(p.M, TC_BM) * p.ny;      // 2^23 at most: mg_form sends no more here than the SMs have places for, or 64 activation rows
   const int stages = ceil_div(p.across, S::CH);
@@ -666,7 +649,7 @@ int mgp_launch(cudaStream_t s, const MgArgs& a) {
   if (S::WT == 2) THA_TRY_RC(mg_map(KIND, a.W1, TC_BM, &mw1, &wb));
   THA_TRY_RC(mg_map(KIND, a.A, S::NT / 2, &mx, &p.x_bytes));
   p.w_bytes = S::WT * wb;
-  p.idesc = mg_idesc(KIND, a.W0->format, a.A->format, 2 * TC_BM, 0);
+  p.idesc = mg_idesc(KIND, 2 * TC_BM, 0);
   p.ny = ceil_div(p.N, S::NT);
   p.n_items = ceil_div(p.M, 2 * TC_BM) * p.ny;
   const int pairs = max(1, sm_budget() / 2);

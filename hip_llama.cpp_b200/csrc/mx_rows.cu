@@ -335,10 +335,6 @@ __device__ __forceinline__ float mr_odd(double y) {
   return (double)f != y && y == y ? __uint_as_float(__float_as_uint(f) | 1u) : f;
 }
 
-__device__ __forceinline__ void mr_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(tc_smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar)) : "memory");
-}
 // 1 / sqrt(m): two steps of Newton's from an fp32 root (1 / sqrt in fp64 holds a block up for longer than its loads)
 __device__ __forceinline__ double mr_root(double m) {
   if (!(m > 0x1p-100 && m < 0x1p100)) return 1.0 / sqrt(m);
@@ -459,8 +455,8 @@ mx_add_norm_ring_kernel(const float* x, const T* left, long long ldl, float* x_o
     asked++;
     unsigned char* at = ring + (size_t)s * (x_bytes + l_bytes);
     tc_mbar_expect_tx(&full[s], x_bytes + l_bytes);
-    mr_bulk(at, x + row * cols, x_bytes, &full[s]);
-    if (l_bytes) mr_bulk(at + x_bytes, left + row * ldl, l_bytes, &full[s]);
+    tc_bulk(at, x + row * cols, x_bytes, &full[s]);
+    if (l_bytes) tc_bulk(at + x_bytes, left + row * ldl, l_bytes, &full[s]);
   };
   if (threadIdx.x == 0)
     for (int s = 0; s < stages && blockIdx.x + (long long)s * gridDim.x < out.rows; s++) ask(s, blockIdx.x + (long long)s * gridDim.x);
