@@ -527,3 +527,77 @@ def test_add_norm_with_an_offset_below_zero(fmt, dtype, rows, cols):
     s = (x + l.float()).double().cpu().numpy()
     y = s / np.sqrt((s * s).mean(-1, keepdims=True) + 1e-5) * (-8.5 + w.double().cpu().numpy())
     same_matrix(M.add_norm(x, l, w, eps=1e-5, w_offset=-8.5, format=fmt), y)
+
+
+# ---- pairs of blocks at the edges of their items; sums -------------------------------------------------------------------------
+# Matrices of 61 tiles of 128 rows, so that tiles of 64 activation rows would be more than the SMs have places for.  An item is 256 weight rows x 256 activation rows (128 with a gate): what is left
+# of the activation rows is rounded up to 32 and touches one tile of 128 scales or two; 20 and 128 rows in the last item leave its second block without any; 384 columns are three tiles
+# of 128 values, an odd number, of which 4-bit stages take two.
+LEFT, EDGE_N, EDGE_K = [1, 31, 32, 33, 127, 128, 129], [7700, 7808], 384
+
+
+@pytest.fixture(scope="module")
+def edge():
+    made = {}
+
+    def of(n, fmt):
+        if (n, fmt) not in made:
+            a, gate, up = matrices(256 + 129, n, EDGE_K, fmt, n, 2)
+            made[n, fmt] = (a, gate, up, O.values(a), O.values(gate), O.values(up))
+        return made[n, fmt]
+    return of
+
+
+def first_rows(a, rows):
+    """The first rows of a matrix, in memory of their own, scale bytes behind them 255"""
+    m = M.Mx.empty(rows, a.cols, a.format)
+    m.codes.view(torch.uint8).copy_(a.codes.view(torch.uint8)[:rows])
+    m.scales.copy_(a.scales.view(-1)[:m.scales.numel()])
+    tiles = m.scales.view(-1, m.scales.numel() // 512 // -(-rows // 128), 32, 4, 4)
+    for lane in range(128):
+        if (rows - 1) // 128 * 128 + lane >= rows:
+            tiles[-1, :, lane % 32, lane // 32] = 255
+    return m
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n", EDGE_N)
+@pytest.mark.parametrize("left", LEFT)
+def test_pairs_at_the_edges_of_their_items(fmt, n, left, edge):
+    a, gate, up, va, vg, vu = edge(n, fmt)
+    rows = 256 + left
+    got = M.linear(first_rows(a, rows), up).double().cpu().numpy()
+    assert (np.abs(got - va[:rows] @ vu.T) <= sum_bound(va[:rows], vu)).all()
+    rows = 128 + left
+    m = M.linear_act(first_rows(a, rows), gate, up)
+    g, u, bg, bu = va[:rows] @ vg.T, va[:rows] @ vu.T, sum_bound(va[:rows], vg), sum_bound(va[:rows], vu)
+    near(m, O.act("silu", g, u, 0, 0), 2.0 ** -126 * np.abs(g) * (1 + np.abs(u)), [O.act("silu", g + s * bg, u + t * bu, 0, 0) for s in (-1, 1) for t in (-1, 1)])
+    M.check_error()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,n,k", [(1, 128, 1000), (20, 260, 4100), (70, 300, 5900), (1100, 2600, 5900)])
+@pytest.mark.parametrize("sign", ["one", "both"])
+def test_sums_of_whole_numbers_are_exact(fmt, rows, n, k, sign):
+    """Products are whole numbers, and |a| |w| adds up to less than 2^24: every sum on the way, in any order, is a number of fp32, and an accumulator with fewer bits would show.  8-bit rows
+    are up to 448 under a scale of 1, 4-bit rows up to 6 under a scale of 128 or of 1: in 5900 columns of one sign 2^22 to 2^24, odd sums among them."""
+    g = np.random.default_rng(k + rows)
+    whole = np.array([1, 2, 3, 4, 6])
+    w = np.where(g.random((n, k)) < 0.6, 6, g.choice(whole, (n, k)))
+    w[g.random((n, k)) < 0.1] = 0
+    if fmt == "e4m3":
+        wide = np.array([v for v in O.levels(fmt) if v >= 1 and v == int(v)]).astype(int)
+        a = np.where(g.random((rows, k)) < 0.8, g.choice(wide[wide >= 256], (rows, k)), g.choice(wide, (rows, k)))
+    else:
+        a = g.choice(whole, (rows, k)) * np.where(np.repeat(g.random((rows, -(-k // 32))) < 0.7, 32, 1)[:, :k], 128, 1)
+    if sign == "both":
+        a, w = a * g.choice([-1, 1], (rows, k)), w * g.choice([-1, 1], (n, k))
+    total = np.abs(a).astype(float) @ np.abs(w).astype(float).T
+    assert total.max() < 2 ** 24 and (k < 5900 or total.max() > 2 ** 22)
+    x, y = torch.from_numpy(a.astype(np.float32)).cuda(), torch.from_numpy(w.astype(np.float32)).cuda()
+    ma, mw = M.quantise(x, fmt), M.quantise(y)
+    assert torch.equal(ma.read(), x) and torch.equal(mw.read(), y)                   # no code is rounded
+    want = a.astype(float) @ w.astype(float).T                                       # exact: all below 2^53
+    assert (want % 2 != 0).any()
+    assert np.array_equal(M.linear(ma, mw).double().cpu().numpy(), want)
+    M.check_error()
