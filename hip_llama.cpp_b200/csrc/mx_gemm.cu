@@ -155,12 +155,12 @@ __device__ __forceinline__ void mg_activate(const MgP& p, const float (&g)[G], f
     else mg_act<THA_ACT_GLU_CLAMPED>(g, x, there, p.limit, p.alpha);
   }
 }
-// C results of activation rows n .. (`count` of them there) and weight row `row`, a warp's rows neighbours from a multiple of 32 on.  All lanes of the warp, which leave together: what follows
-// may be for a whole warp (tcgen05.ld, the cluster's barrier).
+// C results of activation rows n .. (`count` of them there) and weight row `row`, a warp's rows neighbours from a multiple of 32 on.  All lanes of the warp, which may leave one
+// by one: what follows for the whole of it (tcgen05.ld, the cluster's barrier) has a __syncwarp ahead.
 template <int READ, int C>
 __device__ __forceinline__ void mg_store(const MgP& p, long long padded, int n, int count, int row, float (&x)[C]) {
   if (READ == MG_PLAIN) {
-    if (row >= p.M) count = 0;
+    if (row >= p.M) return;
     if (p.bf16) {
       __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + (size_t)n * p.ldo + row;
 #pragma unroll
@@ -177,7 +177,6 @@ __device__ __forceinline__ void mg_store(const MgP& p, long long padded, int n, 
   } else {
     mg_store_blocks<THA_MX_E4M3>(p.y, n, count, row, padded, x);
   }
-  __syncwarp();
 }
 
 // ranks > 1: the blocks of a cluster take a share of the tile's stages each, leave their partial tiles in shared memory and sum each other's, ranks in ascending order.
@@ -308,6 +307,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__ 
       if (p.ranks == 1) {
         mg_activate<READ>(p, gate, x, row0 + r < p.M);
         mg_store<READ>(p, padded, n0 + c, cols - c, row0 + r, x);
+        __syncwarp();
       } else {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -349,6 +349,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_constant__ 
       }
       mg_activate<READ>(p, sum[0], sum[WT - 1], row0 + r < p.M);
       mg_store<READ>(p, padded, n0 + c, cols - c, row0 + r, sum[WT - 1]);
+      __syncwarp();
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // a block's shared memory stays until every rank has read it
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -558,6 +559,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap mw0, const __grid_consta
 #pragma unroll
       for (int c = 0; c < HC; c += 16)
         if (c < cols) mg_store<READ>(p, padded, n0 + c, cols - c, row0 + q * 32 + lane, *reinterpret_cast<float(*)[16]>(x + c));
+      __syncwarp();
     }
   }
   tc_fence_before();

@@ -157,14 +157,16 @@ def test_a_norm_whose_wait_gives_up_leaves_no_number():
 
 
 def test_lanes_without_a_weight_row_stay_with_their_warp():
-    """A store of results ends with its whole warp: behind it come tcgen05.ld and barrier.cluster, which take a warp as one.  Read from the source, as lanes that leave early usually meet again."""
-    text = re.sub(r"//[^\n]*", "", open(os.path.join(os.path.dirname(M.__file__), "csrc", "mx_gemm.cu")).read())
-    store = text[text.index("void mg_store("):]
-    store = store[:store.index("\n}\n")]
-    assert "return" not in store and store.rstrip().endswith("__syncwarp();")
+    """Lanes may leave a store of results one by one; between it and whatever takes a warp as one (tcgen05.ld, barrier.cluster) stands a __syncwarp.  Read from the source, as lanes that leave early
+    usually meet again."""
+    stores = 0
     for kernel in ("mx_gemm_kernel", "mx_gemm_pair_kernel"):
         k = source("mx_gemm.cu", kernel)
-        assert "mg_store<READ>" in k and "mg_store_blocks" not in k
+        assert "mg_store_blocks" not in k
+        for m in re.finditer(r"mg_store<READ>\([^;]*;", k):
+            assert re.match(r"\s*__syncwarp\(\);", k[m.end():]), k[m.start():m.end() + 80]
+            stores += 1
+    assert stores == 3
 
 
 def test_the_error_of_another_device(monkeypatch):
