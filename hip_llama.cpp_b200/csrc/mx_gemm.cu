@@ -2,7 +2,9 @@
 //
 //   C[n, m] = sum_k A[n, k] W[m, k],   A [N, K] rows in 8 or 4 bits, W [M, K] in 4 bits, scales powers of two for each 32 values of a row
 //
-// tcgen05.mma multiplies codes, which are exact, and the two scales of a block of k, which are powers of two, and sums in fp32 in TMEM.  Which kind goes by A's format:
+// tcgen05.mma multiplies codes, which are exact, and the two scales of a block of k, which are powers of two, and sums in fp32 in TMEM.  Sums that 24 bits hold are exact; others are cut off
+// at each instruction, so that rows of one sign come out low: of sum |a| |w|, 8-bit rows of 1024 / 4096 / 11008 / 32768 columns are off by 4e-8 / 1.9e-7 / 8.3e-7 / 6.8e-6 (a product in plain
+// fp32 by 3e-8 / 7e-8 / 1.4e-7 / 4.7e-7), less where a cluster's blocks share the columns (32768: 1.8e-7); with signs at random 2e-9 at most.  Which kind goes by A's format:
 //   E4M3 x E2M1   kind::mxf8f6f4, 32 values of k an instruction; 4-bit codes lie in shared memory as 8 bytes of codes and 8 of nothing for each 16, which TMA makes of the packed rows
 //   E2M1 x E2M1   kind::mxf4, 64 values of k an instruction, codes packed
 // Weight rows are the instruction's M (128 TMEM lanes), activation rows its N.  Scales lie in TMEM too: a tile of 128 rows and 4 blocks (512 bytes, as tha_mx_t keeps them) becomes

@@ -692,7 +692,7 @@ size_t tha_hyb_kv8_attn_scratch(int dtype, const tha_attn_t* a, const tha_rows_t
 
 /* A matrix whose rows are cut into blocks of 32 values.  A block has one scale, the power of two 2^(c - 127) kept as the byte c: the smallest from 0 on at which no
  * value of the block exceeds the format's largest number M (6, 448).  A value's code is the format's number nearest to value / scale, ties to even.  A block that holds a NaN or an infinity gets
- * c = 255, which stands for NaN, and codes of 0: all of it reads as NaN.
+ * c = 255, which stands for NaN, and codes of 0: all of it reads as NaN.  (The OCP specification's own way to a scale takes the exponent of the largest value alone and cuts values off at M.)
  * Rows are padded to P = cols rounded up to a multiple of 128.  codes [rows][P / 2 bytes (E2M1: two values a byte, the first in the low half) or P bytes (E4M3)], on a 32-byte boundary.
  * scales: in tiles of 128 rows and 4 blocks, [rows rounded up to 128 / 128][P / 128][row % 32][row / 32 % 4][block % 4], 512 bytes a tile, on a 16-byte boundary: the order in which the
  * tensor cores take them.  What is padding in a row has codes of 0 and scales other than 255 (0 from the calls below); scale bytes of rows behind the last one may hold
@@ -716,9 +716,10 @@ int tha_hyb_mx_quant(void* stream, int dtype, const void* x, long long ldx, cons
 int tha_hyb_mx_read(void* stream, int dtype, const tha_mx_t* m, void* x, long long ldx);
 /* A sublayer's result joins the residual stream, whose norm is quantised: x_out = x + left (fp32 [rows, cols] without gaps; x_out may be x; left dtype-typed, rows ldl elements
  * apart, NULL: x_out = x), out = x_out / sqrt(mean(x_out^2) + eps) * (w_offset + w), w [cols].  What is quantised is the norm in 64 bits (infinite beyond fp32's
- * numbers): a code is one rounding of the norm of x_out as stored. */
+ * numbers): a code is one rounding of the norm of x_out as stored.  eps is not below 0. */
 int tha_hyb_mx_add_norm(void* stream, int dtype, const float* x, const void* left, long long ldl, float* x_out, const float* w, float w_offset, float eps, const tha_mx_t* out);
-/* C[m, n] = sum_k A[m, k] W[n, k] (dtype-typed, rows ldc elements apart).  A in either format, W E2M1, as many columns.  Products are exact, sums fp32 on the tensor cores. */
+/* C[m, n] = sum_k A[m, k] W[n, k] (dtype-typed, rows ldc elements apart).  A in either format, W E2M1, as many columns.  Products are exact.  Sums are fp32 on the tensor cores, which
+ * cut off where others round: exact as long as 24 bits hold them, else off by at most (columns / 32 + 33) 2^-23 of sum_k |A| |W|. */
 int tha_hyb_mx_linear(void* stream, int dtype, void* C, long long ldc, const tha_mx_t* A, const tha_mx_t* W);
 /* The input products of a feed-forward with its activation: out [A->rows, W_up->rows] = act of A . W_gate^T and A . W_up^T (THA_ACT_* but for THA_ACT_POLYNORM; W_gate NULL for the ungated ones;
  * limit, alpha as in tha_hyb_ff_act), quantised from fp32 where the products are read out.  out->cols is W_up->rows. */
