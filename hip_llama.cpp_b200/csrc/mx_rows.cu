@@ -651,6 +651,7 @@ extern "C" int tha_hyb_mx_add_norm(void* stream, int dtype, const float* x, cons
   if (out->rows == 0) return THA_STATUS_SUCCESS;
   if (!x || !x_out || !w) return mx_refuse(who, "x, x_out or w is NULL");
   if (left && ldl < out->cols && out->rows > 1) return mx_refuse(who, "a row pitch below the row");
+  if (!(eps >= 0.f)) return mx_refuse(who, "eps is below 0");       // a root above 1 / rms, which the norm's way through fp32 counts on not to meet
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == THA_DT_F32)
     return out->format == THA_MX_E2M1 ? add_norm_form<THA_MX_E2M1>(s, x, (const float*)left, ldl, x_out, w, w_offset, eps, out)

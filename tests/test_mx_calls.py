@@ -222,3 +222,9 @@ def test_more_results_than_a_call_counts():
     assert "too many" in refused("tha_hyb_mx_linear", 1, BASE, 1 << 30, rows, w)
     y = C.byref(struct(rows=1 << 30, cols=1 << 30))
     assert "too many" in refused("tha_hyb_mx_linear_act", 4, rows, w, w, 0.0, 0.0, y) and "too many" in refused("tha_hyb_mx_linear_act", 1, rows, None, w, 0.0, 0.0, y)
+
+
+def test_eps_below_zero():
+    a = C.byref(struct())
+    for eps in (-1e-5, float("nan"), -float("inf")):
+        assert "eps" in refused("tha_hyb_mx_add_norm", 1, BASE, BASE, 96, BASE, BASE, 0.0, eps, a)
